@@ -561,6 +561,87 @@ int nsosx_moe_sparse_decode(const nsosx_linear_view* up_views,
                             void* workspace, void* out, int out_dtype, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Scored expert routing with its gradients, and int8 experts.  No counterpart in the
+ * reference, whose router is nsosx_moe_route and whose weights are ternary or float.
+ * ------------------------------------------------------------------------- */
+
+/* Routing by scores.  Per row, with x the logits (f32 or bf16, row stride logits_stride
+ * elements):
+ *   s = softmax(x), or 1 / (1 + exp(-x)) where sigmoid != 0;
+ *   c = s + bias[e] (bias f32 [E]) or, with bias NULL, s;
+ *   with groups > 1 (equal runs of E / groups experts) a group's score is the sum of its
+ *   group_best (1 or 2) largest c, and the group_keep best groups stay;
+ *   the k largest c of the groups that stay are chosen (selected, in that order);
+ *   weights[r, i] = s of choice i, divided by the sum over the row's choices where renorm != 0,
+ *   times scale.  The bias takes part in the choice only.
+ * Choices are those of the values in 64 bits, ties to the lower index (groups too); with
+ * neither a bias nor two values a group the order of c is that of x.  An expert whose logit
+ * (or c) is -inf is not available: a row with fewer than k available experts gets -1 and weight
+ * 0 for the rest.  A row with a NaN score gets the first k experts and NaN weights.
+ *   valid_rows uint8 [rows] or NULL: a row whose byte is 0 is padding (as nsosx_moe_route's):
+ *   weights 0, selected and slot_of -1, no slots.
+ *   weights f32 [rows, k]; selected int32 [rows, k].
+ *   counts int32 [E]; offsets int32 [E+1]; perm int32 [rows*k] (slot -> row, expert-major,
+ *   rows ascending; -1 past offsets[E]); slot_of int32 [rows, k].
+ *   workspace: int32, nsosx_moe_route_scored_workspace(rows, E) elements.
+ * counts, offsets, perm, slot_of and workspace all NULL: weights and selected only.
+ * E <= 512, k <= 16, k <= group_keep * E / groups, groups <= 16 dividing E, rows * k < 2^31. */
+int64_t nsosx_moe_route_scored_workspace(int rows, int experts);
+int nsosx_moe_route_scored(const void* logits, int logits_dtype, int64_t logits_stride,
+                           const uint8_t* valid_rows, const float* bias, int rows, int experts,
+                           int k, int sigmoid, int groups, int group_keep, int group_best,
+                           int renorm, float scale, float* weights, int32_t* selected,
+                           int32_t* counts, int32_t* offsets, int32_t* perm, int32_t* slot_of,
+                           int32_t* workspace, void* stream);
+
+/* Gradient of the logits from that of nsosx_moe_route_scored's weights (the choice itself and
+ * the bias have none): selected int32 [rows, k] as the forward left it (-1 or an index past E
+ * adds nothing, an expert named twice gets both), dweights f32 [rows, k]; dlogits [rows, E]
+ * contiguous in logits_dtype, every element written (a padding row's with zeros). */
+int nsosx_moe_route_scored_backward(const void* logits, int logits_dtype, int64_t logits_stride,
+                                    const int32_t* selected, const float* dweights, int rows,
+                                    int experts, int k, int sigmoid, int renorm, float scale,
+                                    void* dlogits, void* stream);
+
+/* out[r] = sum_i expert_out[slot_of[r, i]] * weights[r, i], i ascending, f32 sums; a slot
+ * outside [0, slots) adds nothing.  expert_out [slots, dim] (in_dtype), out [rows, dim]
+ * (out_dtype), which must not overlap; any number of experts, k <= 16. */
+int nsosx_moe_combine_topk(const void* expert_out, int in_dtype, const int32_t* slot_of,
+                           const float* weights, int rows, int slots, int k, int dim, void* out,
+                           int out_dtype, void* stream);
+
+/* Its gradients: dexpert[slot_of[r, i]] = weights[r, i] * dout[r] (expert_dtype) and
+ * dweights[r, i] = <dout[r], expert_out[slot_of[r, i]]> (f32; 0 for a slot outside
+ * [0, slots)).  perm (int32 [slots], the routing's) or NULL: rows of dexpert whose perm is -1
+ * are written as zeros; with NULL the rows that no slot_of names are left as they were.  No
+ * slot may be named twice; dexpert must not overlap an input. */
+int nsosx_moe_combine_topk_backward(const void* dout, int dout_dtype, const void* expert_out,
+                                    int expert_dtype, const int32_t* slot_of,
+                                    const float* weights, const int32_t* perm, int rows,
+                                    int slots, int k, int dim, void* dexpert, float* dweights,
+                                    void* stream);
+
+/* Product of int8 codes and int8 weights with a scale per token and per output:
+ *   y[m, n] = float(sum_k q[m, k] * w[n, k]) * act_scale[m] * w_scale[n] (+ bias[n])
+ * (exact int32 sums, then each step rounded to f32, no fma).  q int8 [M, K] and act_scale f32
+ * [M] as nsosx_quantize_act_i8 leaves them (w and w_scale too: it quantizes a weight
+ * matrix's rows); w int8 [N, K]; w_scale, bias (or NULL) f32 [N]; y [M, N] f32 or bf16.
+ * Any M, N and K <= 131071, any alignment (16-byte aligned rows are the fast ones). */
+int nsosx_int8_gemm(const int8_t* q, const float* act_scale, const int8_t* w,
+                    const float* w_scale, const float* bias, int M, int K, int N, void* y,
+                    int y_dtype, void* stream);
+
+/* nsosx_int8_gemm for the row segments of routed experts: slot s of expert e (offsets[e] <= s
+ * < offsets[e+1], device int32 [experts + 1]) multiplies row perm[s] of q (row s with perm
+ * NULL) with w[e]; then, where squared_relu != 0, max(v, 0)^2.  w int8 [experts, N, K];
+ * w_scale, bias (or NULL) f32 [experts, N]; q int8 [q_rows, K], act_scale f32 [q_rows]; y
+ * [slots, N], whose rows past offsets[experts] are left as they were.  experts <= 1024. */
+int nsosx_grouped_int8_gemm(const int8_t* q, const float* act_scale, int q_rows, const int8_t* w,
+                            const float* w_scale, const float* bias, const int32_t* offsets,
+                            const int32_t* perm, int slots, int experts, int K, int N,
+                            int squared_relu, void* y, int y_dtype, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Row norms of the hybrid block and the decode conv ring.
  * ------------------------------------------------------------------------- */
 

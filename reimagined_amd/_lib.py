@@ -84,6 +84,17 @@ SIGNATURES = {
     "nsosx_moe_sparse_decode_workspace": (_i64, [_i, _i, _i, _i]),
     "nsosx_moe_sparse_decode": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp,
                                      _vp, _i, _vp]),
+    "nsosx_moe_route_scored_workspace": (_i64, [_i, _i]),
+    "nsosx_moe_route_scored": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f,
+                                    _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "nsosx_moe_route_scored_backward": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp,
+                                             _vp]),
+    "nsosx_moe_combine_topk": (_i, [_vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _i, _vp]),
+    "nsosx_moe_combine_topk_backward": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _vp,
+                                             _vp, _vp]),
+    "nsosx_int8_gemm": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _vp]),
+    "nsosx_grouped_int8_gemm": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i,
+                                     _vp, _i, _vp]),
     "nsosx_sha256_hex": (_i, [_vp, ctypes.c_uint64, _vp]),
 }
 

@@ -1,0 +1,201 @@
+// The weighted sum of a routed row's expert outputs by its k weights, and its gradients, on
+// gfx950: out[r] = sum_i w[r, i] y[slot(r, i)] in rank order, any number of experts.
+#include "common.hpp"
+
+namespace nsosx {
+
+constexpr int kTopkMax = 16;
+
+template <int V, int DT>
+__device__ __forceinline__ void row_load(const void* p, int64_t at, int n, float (&v)[V]) {
+    if constexpr (V == 8) {
+        load8<DT>(p, at, v);
+    } else {
+        v[0] = n > 0 ? load_act<DT>(p, at) : 0.0f;
+    }
+}
+
+template <int V, int DT>
+__device__ __forceinline__ void row_store(void* p, int64_t at, const float (&v)[V]) {
+    if constexpr (V == 8 && DT == NSOSX_F32) {
+        float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
+        d[0] = make_float4(v[0], v[1], v[2], v[3]);
+        d[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else if constexpr (V == 8) {
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) =
+            make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                       pack_bf16x2(v[6], v[7]));
+    } else {
+        store_act<DT>(p, at, v[0]);
+    }
+}
+
+// A wave per 64 V elements of a row.
+template <int IDT, int ODT, int V>
+__global__ __launch_bounds__(256) void combine_topk_kernel(const void* __restrict__ expert_out,
+                                                           const int32_t* __restrict__ slot_of,
+                                                           const float* __restrict__ weights,
+                                                           int rows, int slots, int k, int dim,
+                                                           int pieces, void* __restrict__ out) {
+    const int64_t task = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (task >= (int64_t)rows * pieces) return;
+    const int64_t r = task / pieces;
+    const int d = ((int)(task - r * pieces) * 64 + (threadIdx.x & 63)) * V;
+    if (d >= dim) return;
+    float acc[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = 0.0f;
+    for (int i = 0; i < k; ++i) {
+        const int s = slot_of[r * k + i];
+        if (s < 0 || s >= slots) continue;
+        const float w = weights[r * k + i];
+        float v[V];
+        row_load<V, IDT>(expert_out, (int64_t)s * dim + d, 1, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] = __fmaf_rn(v[j], w, acc[j]);
+    }
+    row_store<V, ODT>(out, r * dim + d, acc);
+}
+
+// A workgroup of WPR waves per row: the waves take the row's pieces in turn, each holds its
+// part of the k dot products, and the parts are added in wave order.
+template <int DDT, int EDT, int V>
+__global__ __launch_bounds__(256) void combine_topk_bwd_kernel(const void* __restrict__ dout,
+                                                               const void* __restrict__ expert_out,
+                                                               const int32_t* __restrict__ slot_of,
+                                                               const float* __restrict__ weights,
+                                                               int rows, int slots, int k, int dim,
+                                                               void* __restrict__ dexpert,
+                                                               float* __restrict__ dweights) {
+    __shared__ float s_dot[4][kTopkMax];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int waves = blockDim.x >> 6;
+    const int64_t r = blockIdx.x;
+    for (int i = 0; i < k; ++i) {
+        const int s = slot_of[r * k + i];
+        const bool real = s >= 0 && s < slots;
+        float dot = 0.0f;
+        if (real) {
+            const float w = weights[r * k + i];
+            for (int d = (wave * 64 + lane) * V; d < dim; d += waves * 64 * V) {
+                float g[V], v[V];
+                row_load<V, DDT>(dout, r * dim + d, 1, g);
+                row_load<V, EDT>(expert_out, (int64_t)s * dim + d, 1, v);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    dot = __fmaf_rn(g[j], v[j], dot);
+                    g[j] = g[j] * w;
+                }
+                row_store<V, EDT>(dexpert, (int64_t)s * dim + d, g);
+            }
+        }
+        dot = wave_sum(dot);
+        if (lane == 0) s_dot[wave][i] = dot;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < k) {
+        float sum = s_dot[0][threadIdx.x];
+        for (int w = 1; w < waves; ++w) sum += s_dot[w][threadIdx.x];
+        dweights[r * k + threadIdx.x] = sum;
+    }
+}
+
+// Rows of dexpert whose slot no row holds (perm < 0): zero.
+template <int EDT>
+__global__ __launch_bounds__(256) void combine_topk_zero_kernel(const int32_t* __restrict__ perm,
+                                                                int slots, int dim,
+                                                                void* __restrict__ dexpert) {
+    const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    const int lane = threadIdx.x & 63;
+    const int64_t s0 = (int64_t)wave * 64;
+    if (s0 >= slots) return;
+    uint64_t empty = __ballot(s0 + lane < slots && perm[s0 + lane] < 0);
+    for (; empty; empty &= empty - 1) {
+        const int64_t row = s0 + __builtin_ctzll(empty);
+        for (int d = lane; d < dim; d += kWave) store_act<EDT>(dexpert, row * dim + d, 0.0f);
+    }
+}
+
+static bool vector_rows(int dim, const void* a, const void* b, const void* c) {
+    return dim % 8 == 0 && ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) |
+                             reinterpret_cast<uintptr_t>(c)) & 15) == 0;
+}
+
+}  // namespace nsosx
+
+using namespace nsosx;
+
+extern "C" int nsosx_moe_combine_topk(const void* expert_out, int in_dtype, const int32_t* slot_of,
+                                      const float* weights, int rows, int slots, int k, int dim,
+                                      void* out, int out_dtype, void* stream) {
+    if (!expert_out || !slot_of || !weights || !out)
+        return fail(NSOSX_ERR_INVALID, "moe_combine_topk: null pointer");
+    if (rows <= 0 || slots <= 0 || k <= 0 || k > kTopkMax || dim <= 0)
+        return fail(NSOSX_ERR_INVALID, "moe_combine_topk: need positive sizes and k <= 16");
+    if (!valid_dtype(in_dtype) || !valid_dtype(out_dtype))
+        return fail(NSOSX_ERR_INVALID, "moe_combine_topk: bad dtype");
+    if (overlaps(out, (int64_t)rows * dim * (out_dtype == NSOSX_F32 ? 4 : 2), expert_out,
+                 (int64_t)slots * dim * (in_dtype == NSOSX_F32 ? 4 : 2)))
+        return fail(NSOSX_ERR_INVALID, "moe_combine_topk: out overlaps expert_out");
+    const bool v8 = vector_rows(dim, expert_out, out, nullptr);
+    const int pieces = (dim - 1) / (v8 ? 512 : 64) + 1;
+    const int64_t grid = ((int64_t)rows * pieces + 3) / 4;
+    if (grid > 0x7fffffffLL) return fail(NSOSX_ERR_OVERFLOW, "moe_combine_topk: rows * dim too large");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+#define NSOSX_CT(I, O)                                                                              \
+    if (v8) hipLaunchKernelGGL((combine_topk_kernel<I, O, 8>), dim3((unsigned)grid), dim3(256), 0,  \
+                               st, expert_out, slot_of, weights, rows, slots, k, dim, pieces, out); \
+    else hipLaunchKernelGGL((combine_topk_kernel<I, O, 1>), dim3((unsigned)grid), dim3(256), 0, st, \
+                            expert_out, slot_of, weights, rows, slots, k, dim, pieces, out);
+    if (in_dtype == NSOSX_F32) {
+        if (out_dtype == NSOSX_F32) { NSOSX_CT(NSOSX_F32, NSOSX_F32) } else { NSOSX_CT(NSOSX_F32, NSOSX_BF16) }
+    } else {
+        if (out_dtype == NSOSX_F32) { NSOSX_CT(NSOSX_BF16, NSOSX_F32) } else { NSOSX_CT(NSOSX_BF16, NSOSX_BF16) }
+    }
+#undef NSOSX_CT
+    return check_launch("moe_combine_topk");
+}
+
+extern "C" int nsosx_moe_combine_topk_backward(const void* dout, int dout_dtype,
+                                               const void* expert_out, int expert_dtype,
+                                               const int32_t* slot_of, const float* weights,
+                                               const int32_t* perm, int rows, int slots, int k,
+                                               int dim, void* dexpert, float* dweights,
+                                               void* stream) {
+    if (!dout || !expert_out || !slot_of || !weights || !dexpert || !dweights)
+        return fail(NSOSX_ERR_INVALID, "moe_combine_topk_backward: null pointer");
+    if (rows <= 0 || slots <= 0 || k <= 0 || k > kTopkMax || dim <= 0)
+        return fail(NSOSX_ERR_INVALID, "moe_combine_topk_backward: need positive sizes and k <= 16");
+    if (!valid_dtype(dout_dtype) || !valid_dtype(expert_dtype))
+        return fail(NSOSX_ERR_INVALID, "moe_combine_topk_backward: bad dtype");
+    const int64_t db = (int64_t)rows * dim * (dout_dtype == NSOSX_F32 ? 4 : 2);
+    const int64_t eb = (int64_t)slots * dim * (expert_dtype == NSOSX_F32 ? 4 : 2);
+    if (overlaps(dexpert, eb, expert_out, eb) || overlaps(dexpert, eb, dout, db))
+        return fail(NSOSX_ERR_INVALID, "moe_combine_topk_backward: dexpert overlaps an input");
+    const bool v8 = vector_rows(dim, dout, expert_out, dexpert);
+    const int per = v8 ? 512 : 64;
+    const dim3 block(64 * (dim > 2 * per ? 4 : dim > per ? 2 : 1));
+    hipStream_t st = static_cast<hipStream_t>(stream);
+#define NSOSX_CB(D, E)                                                                             \
+    if (v8) hipLaunchKernelGGL((combine_topk_bwd_kernel<D, E, 8>), dim3(rows), block, 0, st, dout, \
+                               expert_out, slot_of, weights, rows, slots, k, dim, dexpert, dweights); \
+    else hipLaunchKernelGGL((combine_topk_bwd_kernel<D, E, 1>), dim3(rows), block, 0, st, dout,    \
+                            expert_out, slot_of, weights, rows, slots, k, dim, dexpert, dweights);
+    if (dout_dtype == NSOSX_F32) {
+        if (expert_dtype == NSOSX_F32) { NSOSX_CB(NSOSX_F32, NSOSX_F32) } else { NSOSX_CB(NSOSX_F32, NSOSX_BF16) }
+    } else {
+        if (expert_dtype == NSOSX_F32) { NSOSX_CB(NSOSX_BF16, NSOSX_F32) } else { NSOSX_CB(NSOSX_BF16, NSOSX_BF16) }
+    }
+#undef NSOSX_CB
+    if (perm) {
+        const dim3 grid((slots - 1) / 256 + 1);
+        if (expert_dtype == NSOSX_F32)
+            hipLaunchKernelGGL(combine_topk_zero_kernel<NSOSX_F32>, grid, dim3(256), 0, st, perm, slots,
+                               dim, dexpert);
+        else
+            hipLaunchKernelGGL(combine_topk_zero_kernel<NSOSX_BF16>, grid, dim3(256), 0, st, perm,
+                               slots, dim, dexpert);
+    }
+    return check_launch("moe_combine_topk_backward");
+}

@@ -725,6 +725,187 @@ def moe_combine(expert_out, slot_of, selected, weights, out_dtype=torch.float32)
     return out
 
 
+# ---- scored routing and int8 experts ----------------------------------------------
+
+def _on(fn: str, device, **tensors) -> None:
+    """Contiguous tensors of one device, which has to be the current one (whose stream the call
+    goes to): (tensor, dtype or None, shape or None) each; a None tensor is skipped."""
+    for name, (t, dtype, shape) in tensors.items():
+        if t is None:
+            continue
+        _dev(t, name, dtype)
+        if t.device != device:
+            raise ValueError(f"{fn}: {name} must be on {device}, got {t.device}")
+        if shape is not None and t.shape != tuple(shape):
+            raise ValueError(f"{fn}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if device.index != torch.cuda.current_device():
+        raise ValueError(f"{fn}: the tensors' device {device} must be the current one")
+
+
+def _logit_rows(fn: str, logits: torch.Tensor) -> int:
+    """Checks router logits [rows, E] (a column slice of a wider tensor is fine); row stride."""
+    if not logits.is_cuda:
+        raise ValueError("logits must be a device tensor")
+    if logits.dim() != 2 or 0 in logits.shape:
+        raise ValueError(f"{fn}: logits must be [rows, experts], got {tuple(logits.shape)}")
+    _dt(logits)
+    rows, e = logits.shape
+    if (e > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < e):
+        raise ValueError(f"{fn}: logits need unit column stride and rows that do not overlap")
+    return logits.stride(0) if rows > 1 else e
+
+
+def _score_mode(fn: str, score: str) -> int:
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(f"{fn}: score must be 'softmax' or 'sigmoid', got {score!r}")
+    return int(score == "sigmoid")
+
+
+def moe_route_scored(logits: torch.Tensor, k: int, score: str = "softmax", bias=None,
+                     groups: int = 1, group_keep: int | None = None, group_best: int = 2,
+                     renorm: bool = True, scale: float = 1.0, valid_rows=None,
+                     select_only: bool = False) -> dict:
+    """Routing by softmax or sigmoid scores, with a balance bias [E] that takes part in the
+    choice only, group-limited choice (the group_keep best of `groups` equal runs of experts by
+    the sum of their group_best largest values), top-k <= 16 of up to 512 experts and weights
+    renormalised over the choice and scaled (nsosx_moe_route_scored).
+
+    logits f32 or bf16 [rows, E].  -> weights f32 [rows, k], selected int32 [rows, k], and,
+    unless select_only, counts [E], offsets [E+1], perm [rows*k] (-1 past offsets[E]) and
+    slot_of [rows, k] for grouped_int8_gemm and moe_combine_topk.  valid_rows as moe_route."""
+    fn = "moe_route_scored"
+    stride = _logit_rows(fn, logits)
+    rows, e = logits.shape
+    sig = _score_mode(fn, score)
+    dev = logits.device
+    mask = valid_rows_mask(valid_rows, rows, dev)
+    _on(fn, dev, bias=(bias, torch.float32, (e,)), valid_rows=(mask, torch.uint8, None))
+    if not 0 < k <= e:
+        raise ValueError(f"{fn}: need 0 < k <= {e} experts, got {k}")
+    keep = groups if group_keep is None else group_keep
+    shape = (rows, k)
+    out = {"weights": torch.empty(shape, dtype=torch.float32, device=dev),
+           "selected": torch.empty(shape, dtype=torch.int32, device=dev)}
+    ws = None
+    if not select_only:
+        i32 = dict(dtype=torch.int32, device=dev)
+        out.update(counts=torch.empty(e, **i32), offsets=torch.empty(e + 1, **i32),
+                   perm=torch.empty(rows * k, **i32), slot_of=torch.empty(shape, **i32))
+        ws = torch.empty(max(1, int(lib().nsosx_moe_route_scored_workspace(rows, e))), **i32)
+    call("nsosx_moe_route_scored", _p(logits), _dt(logits), stride, _p(mask), _p(bias), rows, e, k,
+         sig, groups, keep, group_best, int(renorm), float(scale), _p(out["weights"]),
+         _p(out["selected"]), _p(out.get("counts")), _p(out.get("offsets")), _p(out.get("perm")),
+         _p(out.get("slot_of")), _p(ws), _stream())
+    return out
+
+
+def moe_route_scored_backward(logits: torch.Tensor, selected: torch.Tensor, dweights: torch.Tensor,
+                              score: str = "softmax", renorm: bool = True,
+                              scale: float = 1.0) -> torch.Tensor:
+    """Gradient of moe_route_scored's logits [rows, E] (their dtype) from that of its weights
+    (nsosx_moe_route_scored_backward); the balance bias has none."""
+    fn = "moe_route_scored_backward"
+    stride = _logit_rows(fn, logits)
+    rows, e = logits.shape
+    if selected.dim() != 2 or selected.shape[0] != rows or selected.shape[1] < 1:
+        raise ValueError(f"{fn}: selected must be [rows, k], got {tuple(selected.shape)}")
+    k = selected.shape[1]
+    sig = _score_mode(fn, score)
+    _on(fn, logits.device, selected=(selected, torch.int32, None),
+        dweights=(dweights, torch.float32, (rows, k)))
+    out = torch.empty((rows, e), dtype=logits.dtype, device=logits.device)
+    call("nsosx_moe_route_scored_backward", _p(logits), _dt(logits), stride, _p(selected),
+         _p(dweights), rows, e, k, sig, int(renorm), float(scale), _p(out), _stream())
+    return out
+
+
+def _combine_shapes(fn, expert_out, slot_of, weights):
+    if expert_out.dim() != 2 or slot_of.dim() != 2 or 0 in expert_out.shape or 0 in slot_of.shape:
+        raise ValueError(f"{fn}: expert_out must be [slots, dim] and slot_of [rows, k]")
+    _dt(expert_out)
+    _on(fn, expert_out.device, expert_out=(expert_out, None, None),
+        slot_of=(slot_of, torch.int32, None), weights=(weights, torch.float32, slot_of.shape))
+    return (*slot_of.shape, *expert_out.shape)
+
+
+def moe_combine_topk(expert_out: torch.Tensor, slot_of: torch.Tensor, weights: torch.Tensor,
+                     out_dtype=torch.float32) -> torch.Tensor:
+    """out[r] = sum_i weights[r, i] * expert_out[slot_of[r, i]] (nsosx_moe_combine_topk): the
+    combine of moe_route_scored's weights [rows, k]; slot -1 adds nothing."""
+    fn = "moe_combine_topk"
+    rows, k, slots, dim = _combine_shapes(fn, expert_out, slot_of, weights)
+    if out_dtype not in _DT:
+        raise ValueError(f"{fn}: out_dtype must be float32 or bfloat16")
+    out = torch.empty((rows, dim), dtype=out_dtype, device=expert_out.device)
+    call("nsosx_moe_combine_topk", _p(expert_out), _dt(expert_out), _p(slot_of), _p(weights), rows,
+         slots, k, dim, _p(out), _DT[out_dtype], _stream())
+    return out
+
+
+def moe_combine_topk_backward(dout: torch.Tensor, expert_out: torch.Tensor, slot_of: torch.Tensor,
+                              weights: torch.Tensor, perm=None) -> tuple:
+    """Gradients of moe_combine_topk -> (dexpert_out [slots, dim] in expert_out's dtype, dweights
+    f32 [rows, k]).  Rows of expert_out that no row holds get zeros: those with perm -1 where the
+    routing's perm is given, else all are cleared first."""
+    fn = "moe_combine_topk_backward"
+    rows, k, slots, dim = _combine_shapes(fn, expert_out, slot_of, weights)
+    _dt(dout)
+    _on(fn, expert_out.device, dout=(dout, None, (rows, dim)), perm=(perm, torch.int32, (slots,)))
+    de = torch.empty_like(expert_out) if perm is not None else torch.zeros_like(expert_out)
+    dw = torch.empty((rows, k), dtype=torch.float32, device=expert_out.device)
+    call("nsosx_moe_combine_topk_backward", _p(dout), _dt(dout), _p(expert_out), _dt(expert_out),
+         _p(slot_of), _p(weights), _p(perm), rows, slots, k, dim, _p(de), _p(dw), _stream())
+    return de, dw
+
+
+def int8_gemm(q: torch.Tensor, act_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+              bias=None, out_dtype=torch.float32) -> torch.Tensor:
+    """y = (q @ w^T) * act_scale[:, None] * w_scale (+ bias) (nsosx_int8_gemm): int8 codes q
+    [M, K] and weights w [N, K], a scale per token and per output, both as
+    quantize_activations_bitnet gives them; y [M, N] f32 or bf16."""
+    fn = "int8_gemm"
+    if q.dim() != 2 or w.dim() != 2 or q.shape[1] != w.shape[1] or 0 in q.shape or 0 in w.shape:
+        raise ValueError(f"{fn}: q [M, K] and w [N, K] must agree in K, got {tuple(q.shape)} and "
+                         f"{tuple(w.shape)}")
+    (m, k), n = q.shape, w.shape[0]
+    _on(fn, q.device, q=(q, torch.int8, None), act_scale=(act_scale, torch.float32, (m,)),
+        w=(w, torch.int8, None), w_scale=(w_scale, torch.float32, (n,)),
+        bias=(bias, torch.float32, (n,)))
+    if out_dtype not in _DT:
+        raise ValueError(f"{fn}: out_dtype must be float32 or bfloat16")
+    y = torch.empty((m, n), dtype=out_dtype, device=q.device)
+    call("nsosx_int8_gemm", _p(q), _p(act_scale), _p(w), _p(w_scale), _p(bias), m, k, n, _p(y),
+         _DT[out_dtype], _stream())
+    return y
+
+
+def grouped_int8_gemm(q: torch.Tensor, act_scale: torch.Tensor, w: torch.Tensor,
+                      w_scale: torch.Tensor, offsets: torch.Tensor, perm=None, bias=None,
+                      squared_relu: bool = False, out_dtype=torch.float32) -> torch.Tensor:
+    """int8_gemm of every expert's rows (nsosx_grouped_int8_gemm): w [E, N, K], w_scale and bias
+    [E, N], the segments offsets [E+1] and, where q holds the unrouted rows, the slots' rows
+    perm (else q is in slot order).  -> y [slots, N]; rows past offsets[E] are not written."""
+    fn = "grouped_int8_gemm"
+    if q.dim() != 2 or w.dim() != 3 or q.shape[1] != w.shape[2] or 0 in q.shape or 0 in w.shape:
+        raise ValueError(f"{fn}: q [rows, K] and w [E, N, K] must agree in K, got "
+                         f"{tuple(q.shape)} and {tuple(w.shape)}")
+    (rows, k), (e, n) = q.shape, w.shape[:2]
+    slots = rows if perm is None else perm.numel()
+    if slots == 0:
+        raise ValueError(f"{fn}: perm must hold the slots' rows")
+    _on(fn, q.device, q=(q, torch.int8, None), act_scale=(act_scale, torch.float32, (rows,)),
+        w=(w, torch.int8, None), w_scale=(w_scale, torch.float32, (e, n)),
+        offsets=(offsets, torch.int32, (e + 1,)), perm=(perm, torch.int32, (slots,)),
+        bias=(bias, torch.float32, (e, n)))
+    if out_dtype not in _DT:
+        raise ValueError(f"{fn}: out_dtype must be float32 or bfloat16")
+    y = torch.empty((slots, n), dtype=out_dtype, device=q.device)
+    call("nsosx_grouped_int8_gemm", _p(q), _p(act_scale), rows, _p(w), _p(w_scale), _p(bias),
+         _p(offsets), _p(perm), slots, e, k, n, int(squared_relu), _p(y), _DT[out_dtype],
+         _stream())
+    return y
+
+
 # ---- row norms of the hybrid block and the decode conv ring -----------------
 
 def rmsnorm_gated(y: torch.Tensor, z=None, gamma=None, eps: float = 1e-5,

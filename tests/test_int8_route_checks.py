@@ -1,0 +1,134 @@
+"""Refusals of scored routing, the top-k combine and the int8 products (CPU only): the wrappers
+on CPU tensors, the C entries on placeholder addresses that no check dereferences."""
+import pytest
+import torch
+
+from reimagined_amd import _lib, ops
+
+P = 1 << 20  # a placeholder address, never dereferenced
+
+
+def refused(fn, *args, status=1):
+    lib = _lib.lib()
+    assert getattr(lib, fn)(*args) == status, lib.nsosx_last_error().decode()
+    return lib.nsosx_last_error().decode()
+
+
+def route(logits=P, dt=0, stride=64, rows=4, e=64, k=2, groups=1, keep=1, best=1, w=P, sel=P, c=P, o=P,
+          perm=P, slot=P, ws=P):
+    return (logits, dt, stride, None, None, rows, e, k, 0, groups, keep, best, 1, 1.0, w, sel, c, o, perm,
+            slot, ws, None)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(logits=None), "null"), (dict(w=None), "null"), (dict(sel=None), "null"),
+    (dict(c=None), "null"), (dict(perm=None), "null"), (dict(ws=None), "null"),
+    (dict(dt=2), "dtype"), (dict(rows=0), "rows > 0"), (dict(e=0, stride=1), "E <= 512"),
+    (dict(e=513, stride=513), "E <= 512"), (dict(k=0), "0 < k"), (dict(k=17), "k <= 16"),
+    (dict(e=4, k=5), "k <= E"), (dict(stride=63), "stride"), (dict(groups=0), "groups"),
+    (dict(groups=17), "groups"), (dict(groups=3), "groups"), (dict(groups=4, keep=0), "groups"),
+    (dict(groups=4, keep=5), "groups"), (dict(groups=4, keep=2, best=3), "groups"),
+    (dict(e=16, groups=8, keep=1, k=3, stride=16), "kept groups"),
+])
+def test_route_refusals(kw, text):
+    assert text in refused("nsosx_moe_route_scored", *route(**kw))
+
+
+def test_route_overflow():
+    assert "too large" in refused("nsosx_moe_route_scored", *route(rows=2**31 - 1, k=2), status=2)
+
+
+def test_route_workspace():
+    lib = _lib.lib()
+    assert lib.nsosx_moe_route_scored_workspace(0, 8) == 0
+    assert lib.nsosx_moe_route_scored_workspace(8, 513) == 0
+    assert lib.nsosx_moe_route_scored_workspace(1, 8) == 8
+    for rows in (1, 65, 5000, 100000):
+        assert lib.nsosx_moe_route_scored_workspace(rows, 256) >= 256 * ((rows + 63) // 64)
+
+
+@pytest.mark.parametrize("args,text", [
+    ((None, 0, 8, P, P, 1, 8, 2, 0, 1, 1.0, P, None), "null"),
+    ((P, 3, 8, P, P, 1, 8, 2, 0, 1, 1.0, P, None), "dtype"),
+    ((P, 0, 7, P, P, 1, 8, 2, 0, 1, 1.0, P, None), "stride"),
+    ((P, 0, 8, P, P, 1, 8, 9, 0, 1, 1.0, P, None), "k <= E"),
+    ((P, 0, 8, P, P, 0, 8, 2, 0, 1, 1.0, P, None), "rows"),
+])
+def test_route_backward_refusals(args, text):
+    assert text in refused("nsosx_moe_route_scored_backward", *args)
+
+
+@pytest.mark.parametrize("args,text", [
+    ((None, 0, P, P, 4, 8, 2, 16, 2 * P, 0, None), "null"),
+    ((P, 2, P, P, 4, 8, 2, 16, 2 * P, 0, None), "dtype"),
+    ((P, 0, P, P, 4, 8, 17, 16, 2 * P, 0, None), "k <= 16"),
+    ((P, 0, P, P, 4, 0, 2, 16, 2 * P, 0, None), "positive"),
+    ((P, 0, P, P, 4, 8, 2, 16, P + 64, 0, None), "overlaps"),
+])
+def test_combine_refusals(args, text):
+    assert text in refused("nsosx_moe_combine_topk", *args)
+
+
+@pytest.mark.parametrize("args,text", [
+    ((P, 0, None, 0, P, P, None, 4, 8, 2, 16, 2 * P, P, None), "null"),
+    ((P, 0, P, 5, P, P, None, 4, 8, 2, 16, 2 * P, P, None), "dtype"),
+    ((P, 0, P, 0, P, P, None, 4, 8, 0, 16, 2 * P, P, None), "k <= 16"),
+    ((P, 0, 4 * P, 0, P, P, None, 4, 8, 2, 16, P, P, None), "overlaps"),
+    ((4 * P, 0, P, 0, P, P, None, 4, 8, 2, 16, P, P, None), "overlaps"),
+])
+def test_combine_backward_refusals(args, text):
+    assert text in refused("nsosx_moe_combine_topk_backward", *args)
+
+
+@pytest.mark.parametrize("args,text,status", [
+    ((None, P, P, P, None, 1, 16, 16, P, 0, None), "null", 1),
+    ((P, P, P, None, None, 1, 16, 16, P, 0, None), "null", 1),
+    ((P, P, P, P, None, 0, 16, 16, P, 0, None), "positive", 1),
+    ((P, P, P, P, None, 1, 0, 16, P, 0, None), "positive", 1),
+    ((P, P, P, P, None, 1, 16, 16, P, 2, None), "dtype", 1),
+    ((P, P, P, P, None, 1, 131072, 16, P, 0, None), "131071", 2),
+    ((P, P, P, P, None, 2**31 - 1, 16, 2**31 - 1, P, 0, None), "too large", 2),
+])
+def test_int8_refusals(args, text, status):
+    assert text in refused("nsosx_int8_gemm", *args, status=status)
+
+
+@pytest.mark.parametrize("args,text,status", [
+    ((P, P, 4, None, P, None, P, None, 4, 2, 16, 16, 0, P, 0, None), "null", 1),
+    ((P, P, 4, P, P, None, None, None, 4, 2, 16, 16, 0, P, 0, None), "null", 1),
+    ((P, P, 4, P, P, None, P, None, 4, 0, 16, 16, 0, P, 0, None), "positive", 1),
+    ((P, P, 4, P, P, None, P, None, 4, 1025, 16, 16, 0, P, 0, None), "1024", 1),
+    ((P, P, 3, P, P, None, P, None, 4, 2, 16, 16, 0, P, 0, None), "every slot", 1),
+    ((P, P, 4, P, P, None, P, None, 4, 2, 16, 16, 0, P, 7, None), "dtype", 1),
+    ((P, P, 4, P, P, None, P, None, 4, 2, 200000, 16, 0, P, 0, None), "131071", 2),
+    ((P, P, 4, P, P, None, P, P, 2**31 - 1, 2, 16, 2**31 - 1, 0, P, 0, None), "too large", 2),
+])
+def test_grouped_int8_refusals(args, text, status):
+    assert text in refused("nsosx_grouped_int8_gemm", *args, status=status)
+
+
+I8, F, I32 = torch.int8, torch.float32, torch.int32
+
+
+@pytest.mark.parametrize("fn,text", [
+    (lambda: ops.moe_route_scored(torch.zeros(4, 8), 2), "device tensor"),
+    (lambda: ops.moe_route_scored_backward(torch.zeros(4, 8), torch.zeros(4, 2, dtype=I32), torch.zeros(4, 2)),
+     "device tensor"),
+    (lambda: ops.moe_combine_topk(torch.zeros(8, 4), torch.zeros(4, 2, dtype=I32), torch.zeros(4, 2)),
+     "device tensor"),
+    (lambda: ops.moe_combine_topk(torch.zeros(8), torch.zeros(4, 2, dtype=I32), torch.zeros(4, 2)),
+     "expert_out"),
+    (lambda: ops.int8_gemm(torch.zeros(4, 8, dtype=I8), torch.zeros(4), torch.zeros(3, 8, dtype=I8),
+                           torch.zeros(3)), "device tensor"),
+    (lambda: ops.int8_gemm(torch.zeros(4, 8, dtype=I8), torch.zeros(4), torch.zeros(3, 9, dtype=I8),
+                           torch.zeros(3)), "agree in K"),
+    (lambda: ops.grouped_int8_gemm(torch.zeros(4, 8, dtype=I8), torch.zeros(4),
+                                   torch.zeros(2, 3, 9, dtype=I8), torch.zeros(2, 3),
+                                   torch.zeros(3, dtype=I32)), "agree in K"),
+    (lambda: ops.grouped_int8_gemm(torch.zeros(0, 8, dtype=I8), torch.zeros(0),
+                                   torch.zeros(2, 3, 8, dtype=I8), torch.zeros(2, 3),
+                                   torch.zeros(3, dtype=I32)), "agree in K"),
+])
+def test_wrapper_refusals_on_cpu_tensors(fn, text):
+    with pytest.raises(ValueError, match=text):
+        fn()
