@@ -5,98 +5,192 @@
 #include "int8_tiles.hpp"
 
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 namespace nsosx {
 
+// The tiles of a kernel: kN outputs x kM tokens a workgroup.
+template <int NT, int MT, int W, int D, bool ALIGNED>
+struct Split {
+    static constexpr int kN = 16 * NT, kM = 16 * MT, kThreads = 64 * W;
+    static constexpr int kBand = 8, kWavesPerSimd = 1;
+    static constexpr int kSmem = i8_split_smem<NT, MT, W, D>();
+    template <int YDT>
+    static __device__ __forceinline__ void run(const I8Problem& pb, const I8Rows& rows, int n0, int m0,
+                                               void* y, char* smem) {
+        i8_split_tile<YDT, NT, MT, W, D, ALIGNED>(pb, rows, n0, m0, y, smem);
+    }
+};
+
+template <int NWN, int NWM, int TM>
+struct Staged {  // any alignment
+    static constexpr int kN = 64 * NWN, kM = 32 * TM * NWM, kThreads = 64 * NWN * NWM;
+    static constexpr int kBand = 8, kWavesPerSimd = 1;
+    static constexpr int kSmem = i8_tile_smem<NWN, NWM, TM>();
+    template <int YDT>
+    static __device__ __forceinline__ void run(const I8Problem& pb, const I8Rows& rows, int n0, int m0,
+                                               void* y, char* smem) {
+        i8_tile<YDT, NWN, NWM, TM>(pb, rows, n0, m0, y, smem);
+    }
+};
+
+template <int NWN, int NWM, int TM, int BAND, int WPS>
+struct Wide {  // 16-byte aligned rows
+    static constexpr int kN = 64 * NWN, kM = 32 * TM * NWM, kThreads = 64 * NWN * NWM;
+    static constexpr int kBand = BAND, kWavesPerSimd = WPS;
+    static constexpr int kSmem = i8_tile_smem<NWN, NWM, TM>();
+    template <int YDT>
+    static __device__ __forceinline__ void run(const I8Problem& pb, const I8Rows& rows, int n0, int m0,
+                                               void* y, char* smem) {
+        i8_wide_tile<YDT, NWN, NWM, TM>(pb, rows, n0, m0, y, smem);
+    }
+};
+
+template <bool A> using Split16x16 = Split<1, 1, 8, 4, A>;
+template <bool A> using Split16x64 = Split<1, 4, 8, 3, A>;
+template <bool A> using Split32x64 = Split<2, 4, 4, 3, A>;
+template <bool A> using Split64x64 = Split<4, 4, 4, 4, A>;
+using Block128 = Wide<2, 2, 2, 8, 2>;
+using Block256 = Wide<4, 2, 4, 4, 1>;
+using Any128 = Staged<2, 2, 2>;
+
 // ---- one weight matrix ------------------------------------------------------
 
-template <int YDT, int MT>
-__global__ __launch_bounds__(kSkinnyThreads) void i8_skinny_kernel(I8Problem pb, I8Rows rows,
-                                                                   void* __restrict__ y) {
-    extern __shared__ __align__(16) char smem_i8[];
-    const int ntn = (pb.N + 15) / 16;
-    const int nt = blockIdx.x % ntn, mt = blockIdx.x / ntn;
-    i8_skinny_tile<YDT, MT>(pb, rows, nt * 16, mt * 16 * MT, y,
-                            reinterpret_cast<int32_t*>(smem_i8));
-}
-
-template <int YDT, int NWN, int NWM, int TM>
-__global__ __launch_bounds__(64 * NWN * NWM) void i8_tile_kernel(I8Problem pb, I8Rows rows,
-                                                                void* __restrict__ y) {
-    extern __shared__ __align__(16) char smem_i8[];
-    constexpr int BN = 64 * NWN, BM = 32 * TM * NWM;
+template <class T, int YDT>
+__global__ __launch_bounds__(T::kThreads, T::kWavesPerSimd) void i8_gemm_kernel(I8Problem pb, I8Rows rows,
+                                                                              void* __restrict__ y) {
+    extern __shared__ __align__(1024) char smem_i8[];
     int nt, mt;
-    i8_tile_order(blockIdx.x, (pb.N + BN - 1) / BN, (rows.count + BM - 1) / BM, nt, mt);
-    i8_tile<YDT, NWN, NWM, TM>(pb, rows, nt * BN, mt * BM, y, smem_i8);
+    i8_tile_order<T::kBand>(blockIdx.x, (pb.N + T::kN - 1) / T::kN, (rows.count + T::kM - 1) / T::kM, nt, mt);
+    T::template run<YDT>(pb, rows, nt * T::kN, mt * T::kM, y, smem_i8);
 }
 
 // ---- the experts' segments ----------------------------------------------------
 
-template <int YDT, int MT>
-__global__ __launch_bounds__(kSkinnyThreads) void i8_grouped_skinny_kernel(I8Group gp,
-                                                                           void* __restrict__ y) {
-    extern __shared__ __align__(16) char smem_i8[];
-    const int ntn = (gp.N + 15) / 16;
-    const int nt = blockIdx.x % ntn, e = blockIdx.x / ntn;
-    I8Problem pb;
-    I8Rows rows;
-    if (!i8_segment(gp, e, pb, rows)) return;
-    for (int m0 = 0; m0 < rows.count; m0 += 16 * MT) {
-        i8_skinny_tile<YDT, MT>(pb, rows, nt * 16, m0, y, reinterpret_cast<int32_t*>(smem_i8));
-        __syncthreads();  // the partial sums are read before the next tile's are written
-    }
-}
-
-template <int YDT, int NWN, int NWM, int TM>
-__global__ __launch_bounds__(64 * NWN * NWM) void i8_grouped_tile_kernel(I8Group gp,
-                                                                        void* __restrict__ y) {
-    extern __shared__ __align__(16) char smem_i8[];
-    constexpr int BN = 64 * NWN, BM = 32 * TM * NWM;
-    const int ntn = (gp.N + BN - 1) / BN;
+// One row tile of one segment a workgroup.
+template <class T, int YDT>
+__global__ __launch_bounds__(T::kThreads, T::kWavesPerSimd) void i8_grouped_kernel(I8Group gp,
+                                                                                 void* __restrict__ y) {
+    extern __shared__ __align__(1024) char smem_i8[];
+    const int ntn = (gp.N + T::kN - 1) / T::kN;
     const int nt = blockIdx.x % ntn;
     int e, m0;
-    if (!i8_find_segment<BM>(gp, blockIdx.x / ntn, e, m0)) return;
+    if (!i8_find_segment<T::kM>(gp, blockIdx.x / ntn, e, m0)) return;
     I8Problem pb;
     I8Rows rows;
     if (!i8_segment(gp, e, pb, rows)) return;
-    i8_tile<YDT, NWN, NWM, TM>(pb, rows, nt * BN, m0, y, smem_i8);
+    T::template run<YDT>(pb, rows, nt * T::kN, m0, y, smem_i8);
 }
 
 // ---- launches -------------------------------------------------------------------
 
-template <int YDT, int MT>
-static void launch_skinny_t(const I8Problem& pb, const I8Rows& rows, void* y, hipStream_t st) {
-    const int64_t grid = (int64_t)((pb.N + 15) / 16) * ((rows.count + 16 * MT - 1) / (16 * MT));
-    hipLaunchKernelGGL((i8_skinny_kernel<YDT, MT>), dim3((unsigned)grid), dim3(kSkinnyThreads),
-                       i8_skinny_smem(MT), st, pb, rows, y);
+template <class T, int YDT>
+static void launch_gemm_t(const I8Problem& pb, const I8Rows& rows, void* y, hipStream_t st) {
+    const int64_t grid = (int64_t)((pb.N - 1) / T::kN + 1) * ((rows.count - 1) / T::kM + 1);
+    hipLaunchKernelGGL((i8_gemm_kernel<T, YDT>), dim3((unsigned)grid), dim3(T::kThreads), T::kSmem, st,
+                       pb, rows, y);
+}
+
+template <class T, int YDT>
+static void launch_grouped_t(const I8Group& gp, void* y, hipStream_t st) {
+    // every expert's last tile may be partial, and a tile holds at least one row
+    const int64_t mtiles = std::min<int64_t>(gp.slots, gp.slots / T::kM + gp.experts);
+    const int64_t grid = (int64_t)((gp.N - 1) / T::kN + 1) * mtiles;
+    hipLaunchKernelGGL((i8_grouped_kernel<T, YDT>), dim3((unsigned)grid), dim3(T::kThreads), T::kSmem,
+                       st, gp, y);
+}
+
+// Which tile takes a shape: the estimated time of each in us, fitted to a sweep of K 512 .. 8192,
+// N 768 .. 8192 and 1 .. 4096 rows with the weights from HBM (within 9 % of the measured times on
+// average, and the choice within 1 % of the best one's time, 15 % at most): a fixed part and one
+// per round of 256 tiles, both linear in K.  A round is a whole one where a compute unit holds one
+// workgroup.  Measured, us (16 x 16 / 16 x 64 / 32 x 64 / 64 x 64 / 128 x 128 / 256 x 256):
+//   K 4096, N 4096:    1 row   5.1 /  5.9 /  6.8 / 10.0 / 21   / 47
+//                     64 rows 10.7 / 11.1 /  9.6 / 12.5 / 23   / 49
+//                    200 rows    - / 29   / 16.8 / 14.1 / 23   / 51
+//                   1024 rows    - /  -   / 52   / 48   / 27   / 52
+//                   4096 rows    - /  -   /  -   /  -   / 75   / 69
+// Rows that do not start on 16 bytes go through registers on the way to LDS, which costs every
+// tile about a quarter, and have no 256 x 256 one (2048 x 2009 -> 5125 on 128 x 128: 55 us).
+constexpr int64_t kI8MaxTiles = 1 << 24;  // of 128 x 128: 256 threads each, less than 2^32
+
+enum class I8Tile { k16x16, k16x64, k32x64, k64x64, k128x128, k256x256 };
+
+template <class Tiles>
+static I8Tile choose_tile(int K, bool aligned, Tiles tiles) {
+    const double k = K / 1024.0;
+    auto part = [](double t) { return std::max(1.0, t / 256); };
+    auto whole = [](double t) { return std::max(1.0, std::ceil(t / 256)); };
+    const double cost[] = {
+        2.8 - 0.2 * k + part(tiles(16, 16)) * 0.63 * k,
+        1.7 - 0.65 * k + part(tiles(16, 64)) * (1.26 + 1.52 * k),
+        2.6 - 0.4 * k + whole(tiles(32, 64)) * (0.6 + 1.66 * k),
+        1.0 - 0.5 * k + whole(tiles(64, 64)) * (3.25 + 2.43 * k),
+        2.7 + 0.8 * k + part(tiles(128, 128)) * (1.2 + 4.2 * k),
+        whole(tiles(256, 256)) * (8.0 + 15.3 * k),
+    };
+    // a launch holds less than 2^32 threads (tiles of 16 rows: 512 each): the larger ones always do
+    const bool fits[] = {tiles(16, 16) < 4e6, tiles(16, 64) < 4e6, tiles(32, 64) < 8e6,
+                         tiles(64, 64) < 8e6, true, aligned};
+    int best = 4;
+    for (int i = 0; i < 6; ++i)
+        if (fits[i] && cost[i] < cost[best]) best = i;
+    return static_cast<I8Tile>(best);
+}
+
+template <int YDT, bool A>
+static void launch_int8_t(const I8Problem& pb, const I8Rows& rows, void* y, hipStream_t st) {
+    auto tiles = [&](int n, int m) {
+        return (double)((pb.N - 1) / n + 1) * ((rows.count - 1) / m + 1);
+    };
+    switch (choose_tile(pb.K, A, tiles)) {
+        case I8Tile::k16x16: return launch_gemm_t<Split16x16<A>, YDT>(pb, rows, y, st);
+        case I8Tile::k16x64: return launch_gemm_t<Split16x64<A>, YDT>(pb, rows, y, st);
+        case I8Tile::k32x64: return launch_gemm_t<Split32x64<A>, YDT>(pb, rows, y, st);
+        case I8Tile::k64x64: return launch_gemm_t<Split64x64<A>, YDT>(pb, rows, y, st);
+        case I8Tile::k128x128:
+            return launch_gemm_t<std::conditional_t<A, Block128, Any128>, YDT>(pb, rows, y, st);
+        case I8Tile::k256x256:
+            if constexpr (A) launch_gemm_t<Block256, YDT>(pb, rows, y, st);
+    }
+}
+
+template <int YDT, bool A>
+static void launch_grouped_a(const I8Group& gp, void* y, hipStream_t st) {
+    // the experts' row counts are on the device: each expert's last tile is taken as three quarters
+    // of a tile more than its share
+    auto tiles = [&](int n, int m) {
+        return (double)((gp.N - 1) / n + 1) *
+               std::min<double>(gp.slots, std::ceil((double)gp.slots / m + 0.75 * gp.experts));
+    };
+    switch (choose_tile(gp.K, A, tiles)) {
+        case I8Tile::k16x16: return launch_grouped_t<Split16x16<A>, YDT>(gp, y, st);
+        case I8Tile::k16x64: return launch_grouped_t<Split16x64<A>, YDT>(gp, y, st);
+        case I8Tile::k32x64: return launch_grouped_t<Split32x64<A>, YDT>(gp, y, st);
+        case I8Tile::k64x64: return launch_grouped_t<Split64x64<A>, YDT>(gp, y, st);
+        case I8Tile::k128x128:
+            return launch_grouped_t<std::conditional_t<A, Block128, Any128>, YDT>(gp, y, st);
+        case I8Tile::k256x256:
+            if constexpr (A) launch_grouped_t<Block256, YDT>(gp, y, st);
+    }
+}
+
+// rows that all start on 16 bytes
+static bool aligned_rows(int K, const void* a, const void* b) {
+    return K % 16 == 0 && ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0;
 }
 
 template <int YDT>
 static void launch_int8(const I8Problem& pb, const I8Rows& rows, void* y, hipStream_t st) {
-    if (rows.count <= 128) {
-        if (rows.count <= 16) launch_skinny_t<YDT, 1>(pb, rows, y, st);
-        else if (rows.count <= 32) launch_skinny_t<YDT, 2>(pb, rows, y, st);
-        else launch_skinny_t<YDT, 4>(pb, rows, y, st);
-        return;
-    }
-    const int64_t grid = (int64_t)((pb.N + 127) / 128) * ((rows.count + 127) / 128);
-    hipLaunchKernelGGL((i8_tile_kernel<YDT, 2, 2, 2>), dim3((unsigned)grid), dim3(256),
-                       (i8_tile_smem<2, 2, 2>()), st, pb, rows, y);
+    if (aligned_rows(pb.K, pb.w, rows.q)) launch_int8_t<YDT, true>(pb, rows, y, st);
+    else launch_int8_t<YDT, false>(pb, rows, y, st);
 }
 
 template <int YDT>
 static void launch_grouped(const I8Group& gp, void* y, hipStream_t st) {
-    if (gp.slots <= 64 * (int64_t)gp.experts) {
-        const int64_t grid = (int64_t)((gp.N + 15) / 16) * gp.experts;
-        hipLaunchKernelGGL((i8_grouped_skinny_kernel<YDT, 2>), dim3((unsigned)grid),
-                           dim3(kSkinnyThreads), i8_skinny_smem(2), st, gp, y);
-        return;
-    }
-    // every expert's last tile may be partial; a tile holds at least one row
-    const int64_t mtiles = std::min<int64_t>(gp.slots, gp.slots / 128 + gp.experts);
-    const int64_t grid = (int64_t)((gp.N + 127) / 128) * mtiles;
-    hipLaunchKernelGGL((i8_grouped_tile_kernel<YDT, 2, 2, 2>), dim3((unsigned)grid), dim3(256),
-                       (i8_tile_smem<2, 2, 2>()), st, gp, y);
+    if (aligned_rows(gp.K, gp.w, gp.q)) launch_grouped_a<YDT, true>(gp, y, st);
+    else launch_grouped_a<YDT, false>(gp, y, st);
 }
 
 }  // namespace nsosx
@@ -112,7 +206,7 @@ extern "C" int nsosx_int8_gemm(const int8_t* q, const float* act_scale, const in
         return fail(NSOSX_ERR_INVALID, "int8_gemm: M, K and N must be positive");
     if (!valid_dtype(y_dtype)) return fail(NSOSX_ERR_INVALID, "int8_gemm: bad dtype");
     if (K > kI8MaxK) return fail(NSOSX_ERR_OVERFLOW, "int8_gemm: K past the int32 sums (131071)");
-    if (((int64_t)N + 15) / 16 * (((int64_t)M + 15) / 16) > 0x7fffffffLL)
+    if (((int64_t)N + 127) / 128 * (((int64_t)M + 127) / 128) >= kI8MaxTiles)
         return fail(NSOSX_ERR_OVERFLOW, "int8_gemm: M * N too large");
     const I8Problem pb{w, w_scale, bias, N, K, 0};
     const I8Rows rows{q, act_scale, nullptr, 0, M, M};
@@ -137,7 +231,7 @@ extern "C" int nsosx_grouped_int8_gemm(const int8_t* q, const float* act_scale, 
     if (!valid_dtype(y_dtype)) return fail(NSOSX_ERR_INVALID, "grouped_int8_gemm: bad dtype");
     if (K > kI8MaxK)
         return fail(NSOSX_ERR_OVERFLOW, "grouped_int8_gemm: K past the int32 sums (131071)");
-    if (((int64_t)N + 15) / 16 * ((int64_t)slots / 16 + experts) > 0x7fffffffLL)
+    if (((int64_t)N + 127) / 128 * ((int64_t)slots / 128 + experts) >= kI8MaxTiles)
         return fail(NSOSX_ERR_OVERFLOW, "grouped_int8_gemm: slots * N too large");
     const I8Group gp{w, w_scale, bias, q, act_scale, offsets, perm, q_rows, slots, experts, N, K,
                      squared_relu != 0};

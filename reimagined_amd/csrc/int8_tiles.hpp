@@ -98,14 +98,32 @@ __device__ __forceinline__ i8x16 load16(const int8_t* p) {
     return i8x16{(int)v.x, (int)v.y, (int)v.z, (int)v.w};
 }
 
-// Bytes k .. k + 15 of a row, zeros past K.
+// Bytes k .. k + 15 of a row, zeros past K: one load that ends with the row at the latest, its
+// bytes moved down.  (A byte at a time, each load waits for the one before: 77 x 2009 -> 5125 took
+// 28 us.)  Only a row shorter than 16 bytes goes byte by byte.
 __device__ __forceinline__ i8x16 load16_tail(const int8_t* row, int k, int K) {
-    if (k + 16 <= K) return load16(row + k);
-    uint32_t d[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (k + i < K) d[i / 4] |= (uint32_t)(uint8_t)row[k + i] << (8 * (i % 4));
-    return i8x16{(int)d[0], (int)d[1], (int)d[2], (int)d[3]};
+    uint64_t lo = 0, hi = 0;
+    if (K < 16) {
+        for (int i = 0; k + i < K; ++i) {
+            const uint64_t b = (uint8_t)row[k + i];
+            if (i < 8) lo |= b << (8 * i);
+            else hi |= b << (8 * (i - 8));
+        }
+    } else {
+        const int at = min(k, K - 16), move = k - at;
+        const i8x16 v = load16(row + at);
+        lo = (uint32_t)v.x | ((uint64_t)(uint32_t)v.y << 32);
+        hi = (uint32_t)v.z | ((uint64_t)(uint32_t)v.w << 32);
+        if (move >= 8) {
+            lo = hi;
+            hi = 0;
+        }
+        const int bits = 8 * (move & 7);
+        lo = (lo >> bits) | (bits ? hi << (64 - bits) : 0);
+        hi >>= bits;
+        if (move >= 16) lo = hi = 0;
+    }
+    return i8x16{(int)(uint32_t)lo, (int)(lo >> 32), (int)(uint32_t)hi, (int)(hi >> 32)};
 }
 
 // The affine of one output.  Rounded at the conversion, both products and the sum.
@@ -118,91 +136,164 @@ __device__ __forceinline__ float i8_affine(int acc, float as, float ws, float bi
     return v;
 }
 
-// ===========================================================================
-// Few rows: a workgroup owns 16 outputs x 16 MT tokens and its eight waves split K.  Every
-// wave runs v_mfma_i32_16x16x64_i8 on fragments straight from memory (lane l: row l % 16, the
-// 16 bytes of K quarter l / 16), so a 64-deep step reads 64 contiguous bytes of 16 weight
-// rows; the partial sums meet in LDS.  What bounds it is the read of the weights.
-// ===========================================================================
-constexpr int kSkinnyWaves = 8;
-constexpr int kSkinnyThreads = 64 * kSkinnyWaves;
+// Outputs n .. n + 3 of token m (of the segment) from their sums.
+template <int YDT>
+__device__ __forceinline__ void i8_store4(const I8Problem& pb, const I8Rows& rows, int n, int m,
+                                          const i8x16& sum, void* __restrict__ y) {
+    if (m >= rows.count || n >= pb.N) return;
+    const int64_t orow = rows.begin + m;
+    const float as = rows.act_scale[i8_source(rows, (int)orow)];
+    float o[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const int at = min(n + c, pb.N - 1);
+        o[c] = i8_affine(sum[c], as, pb.w_scale[at], pb.bias ? pb.bias[at] : 0.0f, pb.sqrelu);
+    }
+    const int64_t at = orow * pb.N + n;
+    constexpr int kSize = YDT == NSOSX_F32 ? 4 : 2;
+    char* dst = static_cast<char*>(y) + at * kSize;
+    if (n + 4 <= pb.N && (reinterpret_cast<uintptr_t>(dst) & (4 * kSize - 1)) == 0) {
+        if constexpr (YDT == NSOSX_F32)
+            *reinterpret_cast<float4*>(dst) = make_float4(o[0], o[1], o[2], o[3]);
+        else
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+        return;
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        if (n + c < pb.N) store_act<YDT>(y, at + c, o[c]);
+}
 
-constexpr int i8_skinny_smem(int mt) { return kSkinnyWaves * mt * 256 * 4; }
+// ===========================================================================
+// Few tiles: a workgroup owns 16 NT outputs x 16 MT tokens, and its W waves each take a part of K
+// for the whole tile, with v_mfma_i32_16x16x64_i8.  A wave has its own ring of D slots in LDS, a
+// 64-deep block of the tile's 16 (NT + MT) rows each, so that nothing waits for another wave until
+// the end, where the partial sums are added in LDS.
+//
+// The way through LDS is there for the loads: four neighbouring lanes fetch the 64 bytes of one
+// row, which the vector cache serves at 60 bytes a clock, where lanes in the operand's order
+// (neighbours on different rows) get 16.  A fragment's row r has its 16-byte chunk c in place
+// c ^ (r / 4), so that the 16 lanes that read one chunk of 16 rows meet 64 different banks.  LDS
+// moves 64 bytes a clock, written and read, and that bounds a tile: 32 (NT + MT) bytes a step of K.
+// ===========================================================================
+template <int NT, int MT, int W, int D>
+constexpr int i8_split_smem() {
+    const int ring = W * D * (NT + MT) * 1024, sums = W > 1 ? W * NT * MT * 1024 : 0;
+    return ring > sums ? ring : sums;
+}
 
-template <int YDT, int MT>
-__device__ __forceinline__ void i8_skinny_tile(const I8Problem& pb, const I8Rows& rows, int n0,
-                                               int m0, void* __restrict__ y,
-                                               int32_t* __restrict__ s_part) {
-    constexpr int U = MT >= 4 ? 4 : 8;  // steps whose loads are in flight together
+template <int YDT, int NT, int MT, int W, int D, bool ALIGNED>
+__device__ __forceinline__ void i8_split_tile(const I8Problem& pb, const I8Rows& rows, int n0, int m0,
+                                              void* __restrict__ y, char* __restrict__ smem) {
+    constexpr int F = NT + MT;  // fragments (16 rows x 64 bytes) of a block
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    char* ring = smem + wave * (D * F * 1024);
+    // this lane's row and chunk of every fragment, as fetched
+    const int fr = lane >> 2, fc = ((lane & 3) ^ (fr >> 2)) * 16;
+    const int8_t* src[F];
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+        // rows past N or the segment re-read its last one; their outputs are not stored
+        const int64_t row =
+            f < NT ? min(n0 + 16 * f + fr, pb.N - 1)
+                   : i8_source(rows, rows.begin + min(m0 + 16 * (f - NT) + fr, rows.count - 1));
+        src[f] = (f < NT ? pb.w : rows.q) + row * pb.K;
+    }
+    // as read: row r, K quarter g
     const int r = lane & 15, g = lane >> 4;
-    // rows past N or the segment re-read its last one; their outputs are not stored
-    const int8_t* wrow = pb.w + (int64_t)min(n0 + r, pb.N - 1) * pb.K + 16 * g;
-    const int8_t* xrow[MT];
+    const int at = r * 64 + ((g ^ (r >> 2)) << 4);
+    i8x16 acc[NT][MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
-        xrow[t] = rows.q + (int64_t)i8_source(rows, rows.begin + min(m0 + 16 * t + r, rows.count - 1)) *
-                               pb.K + 16 * g;
-    i8x16 acc[MT];
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = i8x16{0, 0, 0, 0};
-    const int steps = pb.K / 64;
-    const int s0 = steps * wave / kSkinnyWaves, s1 = steps * (wave + 1) / kSkinnyWaves;
-    int s = s0;
-    for (; s + U <= s1; s += U) {
-        i8x16 a[U], b[U][MT];
+        for (int t = 0; t < MT; ++t) acc[n][t] = i8x16{0, 0, 0, 0};
+    i8x16 fa[F];
+    auto read = [&](int slot) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            a[u] = load16(wrow + (int64_t)(s + u) * 64);
+        for (int f = 0; f < F; ++f) fa[f] = *reinterpret_cast<const i8x16*>(ring + (slot * F + f) * 1024 + at);
+    };
+    auto mul = [&] {
 #pragma unroll
-            for (int t = 0; t < MT; ++t) b[u][t] = load16(xrow[t] + (int64_t)(s + u) * 64);
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                acc[n][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[n], fa[NT + t], acc[n][t], 0, 0, 0);
+    };
+    const int full = pb.K / 64, blocks = (pb.K + 63) / 64;
+    const int b0 = (int)((int64_t)blocks * wave / W), b1 = (int)((int64_t)blocks * (wave + 1) / W);
+    const int e1 = min(b1, full);  // this wave's whole blocks: b0 .. e1 - 1
+    if constexpr (ALIGNED) {
+        auto issue = [&](int b, int slot) {
+#pragma unroll
+            for (int f = 0; f < F; ++f)
+                __builtin_amdgcn_global_load_lds(
+                    (const __attribute__((address_space(1))) void*)(src[f] + b * 64 + fc),
+                    (__attribute__((address_space(3))) void*)(ring + (slot * F + f) * 1024), 16, 0, 0);
+        };
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+            if (b0 + d < e1) issue(b0 + d, d);
+        int slot = 0;
+        for (int b = b0; b < e1; ++b) {
+            if (b + D <= e1)  // D blocks are in flight: the oldest has landed
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * F) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            read(slot);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot is read before it is filled
+            if (b + D < e1) issue(b + D, slot);
+            mul();
+            slot = slot + 1 == D ? 0 : slot + 1;
         }
+    } else {
+        // through registers: the next block's loads lie under this one's products
+        i8x16 reg[F];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int f = 0; f < F; ++f)
+            if (b0 < e1) reg[f] = load16(src[f] + b0 * 64 + fc);
+        for (int b = b0; b < e1; ++b) {
+#pragma unroll
+            for (int f = 0; f < F; ++f) *reinterpret_cast<i8x16*>(ring + f * 1024 + lane * 16) = reg[f];
+            if (b + 1 < e1)
+#pragma unroll
+                for (int f = 0; f < F; ++f) reg[f] = load16(src[f] + (b + 1) * 64 + fc);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            read(0);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            mul();
+        }
+    }
+    if (b1 > full && b0 < b1) {  // the last block is not whole (every slot of the ring is free)
+#pragma unroll
+        for (int f = 0; f < F; ++f)
+            *reinterpret_cast<i8x16*>(ring + f * 1024 + lane * 16) = load16_tail(src[f], full * 64 + fc, pb.K);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        read(0);
+        mul();
+    }
+    // accumulator c of lane l: output n0 + 16 n + 4 (l / 16) + c, token m0 + 16 t + l % 16
+    if constexpr (W > 1) {
+        __syncthreads();  // every wave is done with its ring
+        char* part = smem + wave * (NT * MT * 1024) + lane * 16;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) *reinterpret_cast<i8x16*>(part + (n * MT + t) * 1024) = acc[n][t];
+        __syncthreads();
+        for (int i = wave; i < NT * MT; i += W) {  // the waves share the 16 x 16 tiles out
+            i8x16 sum = {0, 0, 0, 0};
+#pragma unroll
+            for (int p = 0; p < W; ++p)
+                sum += *reinterpret_cast<const i8x16*>(smem + (p * NT * MT + i) * 1024 + lane * 16);
+            i8_store4<YDT>(pb, rows, n0 + 16 * (i / MT) + 4 * g, m0 + 16 * (i % MT) + r, sum, y);
+        }
+    } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int t = 0; t < MT; ++t)
-                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u], b[u][t], acc[t], 0, 0, 0);
-    }
-    for (; s < s1; ++s) {
-        const i8x16 a = load16(wrow + (int64_t)s * 64);
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, load16(xrow[t] + (int64_t)s * 64),
-                                                           acc[t], 0, 0, 0);
-    }
-    if (wave == kSkinnyWaves - 1 && steps * 64 < pb.K) {
-        const int k = steps * 64 + 16 * g;
-        const i8x16 a = load16_tail(wrow - 16 * g, k, pb.K);
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                a, load16_tail(xrow[t] - 16 * g, k, pb.K), acc[t], 0, 0, 0);
-    }
-    // accumulator c of lane l: output n0 + 4 (l / 16) + c, token m0 + 16 t + l % 16
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-        *reinterpret_cast<int4*>(s_part + ((wave * MT + t) * 64 + lane) * 4) =
-            make_int4(acc[t].x, acc[t].y, acc[t].z, acc[t].w);
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * MT; i += kSkinnyThreads) {
-        const int t = i >> 6, l = i & 63;
-        const int m = m0 + 16 * t + (l & 15), n = n0 + 4 * (l >> 4);
-        if (m >= rows.count || n >= pb.N) continue;
-        int sum[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int w = 0; w < kSkinnyWaves; ++w) {
-            const int4 v = *reinterpret_cast<const int4*>(s_part + ((w * MT + t) * 64 + l) * 4);
-            sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
-        }
-        const int64_t orow = rows.begin + m;
-        const float as = rows.act_scale[i8_source(rows, (int)orow)];
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            if (n + c < pb.N)
-                store_act<YDT>(y, orow * pb.N + n + c,
-                               i8_affine(sum[c], as, pb.w_scale[n + c],
-                                         pb.bias ? pb.bias[n + c] : 0.0f, pb.sqrelu));
+                i8_store4<YDT>(pb, rows, n0 + 16 * n + 4 * g, m0 + 16 * t + r, acc[n][t], y);
     }
 }
 
@@ -218,11 +309,18 @@ constexpr int kI8BK = 128;
 template <int NWN, int NWM, int TM>
 constexpr int i8_tile_smem() { return 2 * (64 * NWN + 32 * TM * NWM) * kI8BK; }
 
+// Linear workgroup id -> tile.  Consecutive ids go round-robin to the 8 XCDs; each XCD takes a
+// contiguous run of tiles, in bands of GM row tiles, rows fastest, so that the tiles in flight
+// on an XCD share both operands in its L2 (128 x 128 tiles of 4096 x 4096 x 8192: 168 us with the
+// outputs fastest, 150 in bands of 8).
+template <int GM>
 __device__ __forceinline__ void i8_tile_order(int L, int ntn, int ntm, int& nt, int& mt) {
     const int total = ntn * ntm, per = total / 8;
     const int t = L < per * 8 ? (L % 8) * per + L / 8 : L;
-    nt = t % ntn;
-    mt = t / ntn;
+    const int band = t / (GM * ntn), first = band * GM, size = min(GM, ntm - first);
+    const int in = t - first * ntn;
+    mt = first + in % size;
+    nt = in / size;
 }
 
 template <int YDT, int NWN, int NWM, int TM>
@@ -377,6 +475,113 @@ __device__ __forceinline__ void i8_tile(const I8Problem& pb, const I8Rows& rows,
             if (kt + 2 < KT) fetch(kt + 2);
         }
         __syncthreads();
+    }
+    i8_epilogue<YDT, NWN, NWM, TM>(pb, rows, n0, m0, y, smem, acc);
+}
+
+// The same tile with its stages brought straight into LDS (global_load_lds, 16 bytes a lane: the
+// rows have to start on 16 bytes), and the last quarter of a stage multiplied after the barrier
+// that frees its buffer, so that the barrier's wait and the first reads of the next stage lie
+// under matrix instructions.  256 x 256 blocks of eight waves, 4096 x 4096 x 8192: 127 .. 137 us,
+// 2.0 .. 2.16 POP/s (128 x 128 blocks 147 .. 154, through registers 186 .. 194); matrix instructions
+// alone reach 3.1 POP/s on such data.  LDS bounds it: 192 KB read and 64 KB written a stage at 64
+// bytes a clock.  64-deep stages in rings of three or four, and 256 x 128 blocks of four waves, two
+// a compute unit, were no faster at any size (138 -> 142 .. 159 us).  At K 1024 the stores show, which
+// all compute units make at once (8192 x 1024 x 4096: 46 us, 13 of them 67 MB of outputs).
+template <int YDT, int NWN, int NWM, int TM>
+__device__ __forceinline__ void i8_wide_tile(const I8Problem& pb, const I8Rows& rows, int n0, int m0,
+                                             void* __restrict__ y, char* smem) {
+    constexpr int kWaves = NWN * NWM, BN = 64 * NWN, BM = 32 * TM * NWM;
+    constexpr int kStage = (BN + BM) * kI8BK, kLoads = (BN + BM) / 8 / kWaves;
+    static_assert(BN / 8 % kWaves == 0 && BM / 8 % kWaves == 0, "whole loads");
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wn = wave % NWN, wm = wave / NWN;
+    const int g = lane >> 5, li = lane & 31;
+    // load i of a wave fills rows 8 (i kWaves + wave) .. + 7 of the stage (weights, then tokens)
+    const int8_t* src[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int row = (i * kWaves + wave) * 8 + (lane >> 3);
+        const int c = (lane & 7) ^ ((row >> 1) & 7);
+        // rows past N or the segment re-read its last one; their outputs are not stored
+        src[i] = (i * kWaves * 8 < BN
+                      ? pb.w + (int64_t)min(n0 + row, pb.N - 1) * pb.K
+                      : rows.q + (int64_t)i8_source(rows, rows.begin + min(m0 + row - BN, rows.count - 1)) * pb.K) +
+                 c * 16;
+    }
+    auto stage_at = [&](int kt, int i) { return smem + (kt & 1) * kStage + (i * kWaves + wave) * 1024; };
+    auto issue = [&](int kt) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)(src[i] + kt * kI8BK),
+                (__attribute__((address_space(3))) void*)stage_at(kt, i), 16, 0, 0);
+    };
+    i32x16 acc[2][TM];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < TM; ++b) acc[a][b] = i32x16{};
+    const int sw = (li >> 1) & 7;
+    const int wrow = (64 * wn + li) * kI8BK, xrow = (BN + 32 * TM * wm + li) * kI8BK;
+    i8x16 fa[2][2], fb[2][TM];
+    auto read = [&](int kt, int ks, int p) {
+        const char* st = smem + (kt & 1) * kStage;
+        const int slot = ((2 * ks + g) ^ sw) * 16;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) fa[p][n] = *reinterpret_cast<const i8x16*>(st + wrow + n * 4096 + slot);
+#pragma unroll
+        for (int t = 0; t < TM; ++t) fb[p][t] = *reinterpret_cast<const i8x16*>(st + xrow + t * 4096 + slot);
+    };
+    auto mul = [&](int p) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int t = 0; t < TM; ++t)
+                acc[n][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[p][n], fb[p][t], acc[n][t], 0, 0, 0);
+    };
+    // this wave's loads have landed and its reads are done; behind the barrier, everyone's
+    auto meet = [&] {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    const int KT = pb.K / kI8BK;
+    if (KT > 0) {
+        issue(0);
+        meet();
+        if (KT > 1) issue(1);
+        read(0, 0, 0);
+    }
+    for (int kt = 0; kt < KT; ++kt) {
+        read(kt, 1, 1);
+        mul(0);
+        read(kt, 2, 0);
+        mul(1);
+        read(kt, 3, 1);
+        mul(0);
+        meet();
+        if (kt + 2 < KT) issue(kt + 2);
+        if (kt + 1 < KT) read(kt + 1, 0, 0);
+        mul(1);
+    }
+    if (KT * kI8BK < pb.K) {
+        // the last stage is not whole: through registers, zeros past K.  (Every wave has read every
+        // stage into registers before the last barrier: both buffers are free.)
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int row = (i * kWaves + wave) * 8 + (lane >> 3);
+            const int c = ((lane & 7) ^ ((row >> 1) & 7)) * 16;
+            *reinterpret_cast<i8x16*>(stage_at(KT, i) + lane * 16) =
+                load16_tail(src[i] - c, KT * kI8BK + c, pb.K);
+        }
+        meet();
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            read(KT, ks, 0);
+            mul(0);
+        }
     }
     i8_epilogue<YDT, NWN, NWM, TM>(pb, rows, n0, m0, y, smem, acc);
 }
