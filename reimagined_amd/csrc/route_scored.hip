@@ -21,7 +21,8 @@ struct RouteScored {
     int32_t* offsets;        // [E + 1]
     int32_t* perm;           // [rows * k]
     int32_t* slot_of;        // [rows, k]
-    int32_t* block_counts;   // workspace [E, blocks]
+    int32_t* block_counts;   // workspace [E, blocks], or [blocks, E] where by_block
+    int by_block;
 };
 
 // ---- sixteen lanes per row -----------------------------------------------------
@@ -38,15 +39,8 @@ template <int N>
 __device__ __forceinline__ float ror16(float v) {
     return __uint_as_float(ror16<N>(__float_as_uint(v)));
 }
-template <int N>
-__device__ __forceinline__ double ror16(double v) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint64_t lo = ror16<N>((uint32_t)u), hi = ror16<N>((uint32_t)(u >> 32));
-    return __builtin_bit_cast(double, lo | (hi << 32));
-}
-
-template <typename T>
-__device__ __forceinline__ T larger(T a, T b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
 
 template <typename T>
 __device__ __forceinline__ T row_max(T v) {
@@ -67,145 +61,490 @@ __device__ __forceinline__ bool row_any(bool p) {
 }
 
 // The two largest of a row from each lane's two largest (a >= b).
-template <typename T, int N>
-__device__ __forceinline__ void merge2(T& a, T& b) {
-    const T oa = ror16<N>(a), ob = ror16<N>(b);
-    b = larger(a < oa ? a : oa, larger(b, ob));
+template <int N>
+__device__ __forceinline__ void merge2(float& a, float& b) {
+    const float oa = ror16<N>(a), ob = ror16<N>(b);
+    b = larger(fminf(a, oa), larger(b, ob));
     a = larger(a, oa);
+}
+
+// This lane's values of a row of E floats: expert 16 v + l, -inf past E or where the row is not
+// live.  (Every load is made, from the last expert where there is none: a branch around each
+// would wait for each.)
+template <int V, int DT>
+__device__ __forceinline__ void row_values(const void* x, int64_t base, int E, bool live, float (&c)[V]) {
+    const int l = threadIdx.x & 15;
+#pragma unroll
+    for (int v = 0; v < V; ++v) c[v] = load_act<DT>(x, base + min(16 * v + l, E - 1));
+#pragma unroll
+    for (int v = 0; v < V; ++v) c[v] = live && 16 * v + l < E ? c[v] : -INFINITY;
 }
 
 // Score of group `q` (its best one or two values in c; unavailable experts, -inf, add nothing),
 // the same in every lane of the row; -inf where no expert of it is available.
-template <typename T, int V>
-__device__ __forceinline__ T group_score(const T (&c)[V], int q, int size, int best) {
-    const T none = -(T)INFINITY;
+template <int V>
+__device__ __forceinline__ float group_score(const float (&c)[V], int q, int size, int best) {
+    const float none = -INFINITY;
     const int l = threadIdx.x & 15;
-    T a = none, b = none;
+    float a = none, b = none;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         if (16 * v + 15 < q * size || 16 * v >= (q + 1) * size) continue;
         const int e = 16 * v + l;
-        const T x = e >= q * size && e < (q + 1) * size ? c[v] : none;
-        b = larger(b, a < x ? a : x);
+        const float x = e >= q * size && e < (q + 1) * size ? c[v] : none;
+        b = larger(b, fminf(a, x));
         a = larger(a, x);
     }
-    merge2<T, 8>(a, b);
-    merge2<T, 4>(a, b);
-    merge2<T, 2>(a, b);
-    merge2<T, 1>(a, b);
+    merge2<8>(a, b);
+    merge2<4>(a, b);
+    merge2<2>(a, b);
+    merge2<1>(a, b);
     return best == 2 && b > none ? a + b : a;
 }
 
-template <int N, typename T>
-__device__ __forceinline__ void outranked(T s, int l, int& rank) {
-    const T o = ror16<N>(s);
+template <int N>
+__device__ __forceinline__ void outranked(float s, int l, int& rank) {
+    const float o = ror16<N>(s);
     const int ol = ror16<N>(l);
     rank += o > s || (o == s && ol < l) ? 1 : 0;
 }
 
-// Bit q of the result: group q is one of the `keep` best (ties to the lower group).
-template <typename T, int V>
-__device__ __forceinline__ uint32_t kept_groups(const T (&c)[V], const RouteScored& p) {
-    const int l = threadIdx.x & 15;
-    const int size = p.E / p.groups;
-    T s = -(T)INFINITY;
-    for (int q = 0; q < p.groups; ++q) {
-        const T v = group_score<T, V>(c, q, size, p.best);
-        if (l == q) s = v;
-    }
+// Rank of lane l's value among the row's 16 (ties to the lower index).
+__device__ __forceinline__ int row_rank(float s, int index) {
     int rank = 0;
-    outranked<1>(s, l, rank); outranked<2>(s, l, rank); outranked<3>(s, l, rank);
-    outranked<4>(s, l, rank); outranked<5>(s, l, rank); outranked<6>(s, l, rank);
-    outranked<7>(s, l, rank); outranked<8>(s, l, rank); outranked<9>(s, l, rank);
-    outranked<10>(s, l, rank); outranked<11>(s, l, rank); outranked<12>(s, l, rank);
-    outranked<13>(s, l, rank); outranked<14>(s, l, rank); outranked<15>(s, l, rank);
-    const bool in = l < p.groups && rank < p.keep;
-    return (uint32_t)(__ballot(in) >> (threadIdx.x & 48)) & 0xFFFFu;
+    outranked<1>(s, index, rank); outranked<2>(s, index, rank); outranked<3>(s, index, rank);
+    outranked<4>(s, index, rank); outranked<5>(s, index, rank); outranked<6>(s, index, rank);
+    outranked<7>(s, index, rank); outranked<8>(s, index, rank); outranked<9>(s, index, rank);
+    outranked<10>(s, index, rank); outranked<11>(s, index, rank); outranked<12>(s, index, rank);
+    outranked<13>(s, index, rank); outranked<14>(s, index, rank); outranked<15>(s, index, rank);
+    return rank;
 }
 
-// The scores' sum and maximum of a softmax row, in T (unavailable experts are -inf).
-template <typename T, int V>
-__device__ __forceinline__ void softmax_stats(const T (&x)[V], T& mx, T& sum) {
+// Up to 8 groups of 16 VS experts each (VS values of every lane): the score of group l / 2 in lane
+// l.  Each step exchanges halves (lanes 8 apart take groups 0 .. 3 or 4 .. 7, and so on), so that 8
+// groups cost 8 merges where a reduction each costs 32 (16384 rows of 256 experts in 8 groups:
+// 18.9 -> @@ us with the rest of the choice).
+template <int CTRL>
+__device__ __forceinline__ float lane_move(float v) {
+    return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(v), CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ void join2(float& a, float& b, float oa, float ob) {
+    b = larger(fminf(a, oa), larger(b, ob));
+    a = larger(a, oa);
+}
+template <int CTRL, int N>
+__device__ __forceinline__ void exchange_halves(float (&a)[8], float (&b)[8], bool upper) {
+#pragma unroll
+    for (int q = 0; q < N / 2; ++q) {
+        const float a0 = a[q], a1 = a[q + N / 2], b0 = b[q], b1 = b[q + N / 2];
+        const float oa = lane_move<CTRL>(upper ? a0 : a1), ob = lane_move<CTRL>(upper ? b0 : b1);
+        a[q] = upper ? a1 : a0;
+        b[q] = upper ? b1 : b0;
+        join2(a[q], b[q], oa, ob);
+    }
+}
+template <int VS, int V>
+__device__ __forceinline__ float group_scores(const float (&c)[V], int best) {
+    const float none = -INFINITY;
+    const int l = threadIdx.x & 15;
+    float a[8], b[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        a[q] = b[q] = none;
+#pragma unroll
+        for (int v = q * VS; v < (q + 1) * VS && v < V; ++v) {
+            b[q] = larger(b[q], fminf(a[q], c[v]));
+            a[q] = larger(a[q], c[v]);
+        }
+    }
+    exchange_halves<0x128, 8>(a, b, l & 8);  // lane l ^ 8
+    exchange_halves<0x141, 4>(a, b, l & 4);  // lane l ^ 7
+    exchange_halves<0x1B, 2>(a, b, l & 2);   // lane l ^ 3
+    join2(a[0], b[0], lane_move<0xB1>(a[0]), lane_move<0xB1>(b[0]));  // lane l ^ 1
+    return best == 2 && b[0] > none ? a[0] + b[0] : a[0];
+}
+
+__device__ __forceinline__ float row_min(float v) { return -row_max(-v); }
+
+// Bit q of the result: group q is one of the `keep` best (ties to the lower group).  gap: what
+// the worst group that stays has over the best one that goes.
+template <int V>
+__device__ __forceinline__ uint32_t kept_groups(const float (&c)[V], const RouteScored& p, float& gap) {
+    const float none = -INFINITY;
+    const int l = threadIdx.x & 15;
+    const int size = p.E / p.groups;
+    float s = none;
+    int group = l;  // whose score s is
+    const int values = size % 16 == 0 && p.groups <= 8 ? size / 16 : 0;
+    if (values == 1 || values == 2 || values == 4 || values == 8) {
+        s = values == 1 ? group_scores<1>(c, p.best) : values == 2 ? group_scores<2>(c, p.best)
+            : values == 4 ? group_scores<4>(c, p.best) : group_scores<8>(c, p.best);
+        group = l >> 1;
+        if (l & 1) s = none;  // (each score once)
+    } else {
+        for (int q = 0; q < p.groups; ++q) {
+            const float v = group_score<V>(c, q, size, p.best);
+            if (l == q) s = v;
+        }
+    }
+    // (an odd lane, which has no group, ranks behind the group of its neighbour)
+    const int rank = row_rank(s, values ? l : group);
+    bool in = group < p.groups && rank < p.keep;
+    uint32_t kept = 0;
+    if (values == 1 || values == 2 || values == 4 || values == 8) {
+        in = in && !(l & 1);
+        const uint32_t bits = (uint32_t)(__ballot(in) >> (threadIdx.x & 48)) & 0xFFFFu;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) kept |= ((bits >> (2 * q)) & 1u) << q;
+    } else {
+        kept = (uint32_t)(__ballot(in) >> (threadIdx.x & 48)) & 0xFFFFu;
+    }
+    gap = row_min(in ? s : INFINITY) - row_max(in ? none : s);
+    return kept;
+}
+
+// exp(x) to a unit in 64 bits: x = n ln 2 + r with |r| <= ln 2 / 2, the Taylor sum of exp(r) to
+// r^13 (the next term is below 2^-57), times 2^n.
+__device__ __forceinline__ double exp_of(double x) {
+    x = fmin(fmax(x, -800.0), 800.0);  // 0 and infinity past either end
+    const double n = rint(x * 0x1.71547652b82fep+0);
+    double r = fma(-n, 0x1.62e42fefa39efp-1, x);
+    r = fma(-n, 0x1.abc9e3b39803fp-56, r);
+    double p = 1.0 / 6227020800.0;
+    p = fma(p, r, 1.0 / 479001600.0);
+    p = fma(p, r, 1.0 / 39916800.0);
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return ldexp(p, (int)n);
+}
+
+// The maximum and the scores' sum of a softmax row (unavailable experts are -inf).
+template <int V>
+__device__ __forceinline__ void softmax_stats(const float (&x)[V], float& mx, float& sum) {
     mx = x[0];
 #pragma unroll
-    for (int v = 1; v < V; ++v) mx = larger(mx, x[v]);
+    for (int v = 1; v < V; ++v) mx = fmaxf(mx, x[v]);
     mx = row_max(mx);
-    sum = 0;
+    sum = 0.0f;
 #pragma unroll
-    for (int v = 0; v < V; ++v) sum += x[v] == -(T)INFINITY ? (T)0 : exp(x[v] - mx);  // a NaN stays
+    for (int v = 0; v < V; ++v) sum += x[v] == -INFINITY ? 0.0f : expf(x[v] - mx);  // a NaN stays
     sum = row_sum(sum);
 }
 
-// The row's choice values in 64 bits, then k rounds of a row maximum: expert index of choice
-// l in lane l (-1 where no expert is left).
-template <int V, int DT>
-__device__ __forceinline__ int select_row(const RouteScored& p, int64_t row, bool live, bool& bad) {
-    const double none = -(double)INFINITY;
+// -inf for the experts of the groups that go (bit q of kept: group q stays).
+template <int V>
+__device__ __forceinline__ void close_groups(const RouteScored& p, uint32_t kept, float (&c)[V]) {
+    const int size = p.E / p.groups;
     const int l = threadIdx.x & 15;
-    double c[V];
-    bool nan = false;
+    int group = l / size, left = l % size;  // of expert 16 v + l, without a division each
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int e = 16 * v + l;
-        c[v] = live && e < p.E ? (double)load_act<DT>(p.logits, row * p.stride + e) : none;
-        nan |= c[v] != c[v];
+        if (!((kept >> group) & 1)) c[v] = -INFINITY;
+        left += 16;
+        while (left >= size) {
+            left -= size;
+            ++group;
+        }
     }
-    if (p.sigmoid) {
-        if (p.bias || (p.groups > 1 && p.best == 2)) {
+}
+
+// The choice by 32-bit scores, with a proof that it is the one of 64 bits: every value becomes a
+// 32-bit key, its distance from a point below the row's largest in fixed point (2 for scores, 32
+// for logits that are compared as they are) above the complement of its index, each lane sorts its
+// keys, and k + 1 rounds take the largest of the row's 16 first ones.  The choice stands where the
+// fixed-point values of neighbours in that order differ by more than the scores' error.  Where
+// they do not (about 2 of 10^4 rows of 256 sigmoid scores with a bias), where groups lie too close
+// together, values outside the window or a NaN in the row, the whole wave chooses for the row in 64
+// bits (select_wave).  bfloat16 logits compared as they are make exact keys.
+//
+// Errors: a sigmoid by exp2 and reciprocal of one unit each is off by s (1 - s) (|x| 2^-24 + 2^-23)
+// + s 1.5 2^-23 at most, below 1.7 2^-23; a softmax score by p (|x - max| 2^-23 + (V + 8) 2^-24),
+// below 2^-18 (p |x - max| <= 0.37); the sum with the bias by 2^-24 of the value.
+// Batcher's odd-even merge sort, descending, of N keys from LO.
+template <int A, int B, int V>
+__device__ __forceinline__ void order_pair(uint32_t (&key)[V]) {
+    const uint32_t a = key[A], b = key[B];
+    key[A] = a > b ? a : b;
+    key[B] = a > b ? b : a;
+}
+template <int I, int END, int R, int V>
+__device__ __forceinline__ void order_pairs(uint32_t (&key)[V]) {
+    if constexpr (I + R < END) {
+        order_pair<I, I + R>(key);
+        order_pairs<I + 2 * R, END, R>(key);
+    }
+}
+template <int LO, int N, int R, int V>
+__device__ __forceinline__ void merge_keys(uint32_t (&key)[V]) {
+    if constexpr (2 * R < N) {
+        merge_keys<LO, N, 2 * R>(key);
+        merge_keys<LO + R, N, 2 * R>(key);
+        order_pairs<LO + R, LO + N, R>(key);
+    } else {
+        order_pair<LO, LO + R>(key);
+    }
+}
+template <int LO, int N, int V>
+__device__ __forceinline__ void sort_keys(uint32_t (&key)[V]) {
+    if constexpr (N > 1) {
+        sort_keys<LO, N / 2>(key);
+        sort_keys<LO + N / 2, N / 2>(key);
+        merge_keys<LO, N, 1>(key);
+    }
+}
+
+// Expert index of choice l in lane l (-1: none), where `sure`.
+template <int V, int DT>
+__device__ __forceinline__ int select_fast(const RouteScored& p, int64_t row, bool live, bool& sure) {
+    constexpr int IB = V == 2 ? 5 : V == 4 ? 6 : V == 8 ? 7 : V == 16 ? 8 : 9;  // bits of an index
+    constexpr int NB = 32 - IB;
+    constexpr uint32_t kIndex = (1u << IB) - 1;
+    const float none = -INFINITY;
+    const int l = threadIdx.x & 15;
+    const bool scored = p.bias || (p.groups > 1 && p.best == 2);
+    float c[V], b[V];
+    bool odd = false;  // a NaN, or an infinite logit of a softmax
+    row_values<V, DT>(p.logits, row * p.stride, p.E, live, c);
+    if (p.bias) row_values<V, NSOSX_F32>(p.bias, 0, p.E, true, b);
+    float err = 0.0f;
+    if (!p.sigmoid) {
+        float mx = c[0];
 #pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (c[v] > none) c[v] = 1.0 / (1.0 + exp(-c[v]));
+        for (int v = 1; v < V; ++v) mx = fmaxf(mx, c[v]);
+        mx = row_max(mx);
+        odd |= mx == INFINITY;
+        if (scored) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) sum += c[v] == none ? 0.0f : __expf(c[v] - mx);
+            const float inv = __builtin_amdgcn_rcpf(row_sum(sum));
+#pragma unroll
+            for (int v = 0; v < V; ++v) c[v] = c[v] == none ? none : __expf(c[v] - mx) * inv;
+            err = 0x1p-18f;
+        }
+    } else if (scored) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            c[v] = c[v] == none ? none : __builtin_amdgcn_rcpf(1.0f + __expf(-c[v]));
+        err = 0x1p-22f;
+    }
+    if (p.bias) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) c[v] = c[v] == none ? none : c[v] + b[v];
+    }
+    float mx = none;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        odd |= c[v] != c[v];
+        mx = fmaxf(mx, c[v]);
+    }
+    mx = row_max(mx);
+    odd |= mx == INFINITY;
+    if (scored) err += 0x1p-23f * fabsf(mx);
+    bool ok = true;
+    if (p.groups > 1) {
+        float gap;
+        const uint32_t kept = kept_groups<V>(c, p, gap);
+        ok = err == 0.0f || gap > 6.0f * err;  // two errors a group, the sums' rounding one more
+        close_groups<V>(p, kept, c);
+    }
+    uint32_t key[V];
+    uint32_t apart = 1;  // by how much fixed-point neighbours have to differ
+    constexpr bool kExact = DT == NSOSX_BF16;
+    const bool exact = kExact && !scored;
+    if (exact) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            // (adding +0 turns -0 into +0: equal values make equal keys)
+            const uint32_t u = __float_as_uint(c[v] + 0.0f) >> 16;
+            const uint32_t o = u & 0x8000u ? ~u & 0xFFFFu : u | 0x8000u;
+            key[v] = c[v] == none ? 0u : (o << 16) | (0xFFFFu - (16 * v + l));
         }
     } else {
-        double mx, sum;
-        softmax_stats<double, V>(c, mx, sum);
-        nan |= mx == (double)INFINITY;
-        if (p.bias || (p.groups > 1 && p.best == 2)) {
+        const float scale = scored ? (float)(1u << (NB - 1)) : (float)(1u << (NB - 5));
+        const float base = mx - (scored ? 2.0f : 32.0f);
+        const float top = (float)(1u << NB) - (NB > 24 ? (float)(1u << (NB - 24)) : 1.0f);
 #pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (c[v] > none) c[v] = exp(c[v] - mx) / sum;
+        for (int v = 0; v < V; ++v) {
+            const float t = fminf(fmaxf((c[v] - base) * scale, 0.0f), top);
+            key[v] = c[v] == none ? 0u : ((uint32_t)t << IB) | (kIndex - (16 * v + l));
+        }
+        // both values' errors, the difference's and the product's rounding, the truncation
+        if (scored) apart = (uint32_t)fminf(2.0f * err * scale, 1e9f) + (1u << (NB > 24 ? NB - 23 : 1)) + 2;
+    }
+    sort_keys<0, V>(key);
+    auto take = [&] {  // the row's largest key, out of its lane's list
+        const uint32_t m = row_max(key[0]);
+        if (key[0] == m) {  // (as selects, the compiler made this a search through the array)
+#pragma unroll
+            for (int v = 0; v + 1 < V; ++v) key[v] = key[v + 1];
+            key[V - 1] = 0;
+        }
+        return m;
+    };
+    uint32_t mine = 0, before = 0;  // choice l's key, in lane l
+    for (int i = 0; i <= p.k; ++i) {
+        const uint32_t m = row_max(key[0]);
+        // (the key behind the last choice only has to be apart from it)
+        ok = ok && (exact || ((i == 0 || (before >> IB) >= (m >> IB) + apart) &&
+                              (i == p.k || (m >> IB) != 0)));
+        before = m;
+        if (l == i && i < p.k) mine = m;
+        if (key[0] == m) {  // (as selects, the compiler made this a search through the array)
+#pragma unroll
+            for (int v = 0; v + 1 < V; ++v) key[v] = key[v + 1];
+            key[V - 1] = 0;
+        }
+    }
+    sure = !live || (ok && !row_any(odd));
+    if (!live || mine == 0) return -1;
+    return exact ? (int)(0xFFFFu - (mine & 0xFFFFu)) : (int)(kIndex - (mine & kIndex));
+}
+
+// Step O of a reduction over a wave: a rotation within the 16-lane rows for 1 .. 8, the rows
+// exchanged for 16 and 32.
+template <int O>
+__device__ __forceinline__ uint32_t wave_move(uint32_t v) {
+    if constexpr (O < 16) {
+        return ror16<O>(v);
+    } else if constexpr (O == 16) {
+        const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return threadIdx.x & 16 ? p[0] : p[1];
+    } else {
+        const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return threadIdx.x & 32 ? p[0] : p[1];
+    }
+}
+template <int O>
+__device__ __forceinline__ double wave_move(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint64_t lo = wave_move<O>((uint32_t)u), hi = wave_move<O>((uint32_t)(u >> 32));
+    return __builtin_bit_cast(double, lo | (hi << 32));
+}
+template <int O = 32>
+__device__ __forceinline__ double wave_max(double v) {
+    v = fmax(v, wave_move<O>(v));
+    if constexpr (O > 1) v = wave_max<O / 2>(v);
+    return v;
+}
+template <int O = 32>
+__device__ __forceinline__ double wave_sum(double v) {
+    v += wave_move<O>(v);
+    if constexpr (O > 1) v = wave_sum<O / 2>(v);
+    return v;
+}
+template <int O = 32>
+__device__ __forceinline__ void wave_max2(double& a, double& b) {
+    const double oa = wave_move<O>(a), ob = wave_move<O>(b);
+    b = fmax(fmin(a, oa), fmax(b, ob));
+    a = fmax(a, oa);
+    if constexpr (O > 1) wave_max2<O / 2>(a, b);
+}
+
+// One row (the same in every lane) chosen by a whole wave in 64 bits, expert 64 v + lane in value v:
+// choice i in every lane whose number mod 16 is i (-1 where no expert is left).  bad: the row
+// holds a NaN, or an infinite logit that its softmax cannot take.
+template <int V, int DT>
+__device__ __forceinline__ int select_wave(const RouteScored& p, int64_t row, bool& bad) {
+    constexpr int W = V > 4 ? V / 4 : 1;
+    const double none = -(double)INFINITY;
+    const int lane = threadIdx.x & 63;
+    const bool scored = p.bias || (p.groups > 1 && p.best == 2);
+    double c[W];
+    bool nan = false;
+#pragma unroll
+    for (int v = 0; v < W; ++v) {
+        const int e = 64 * v + lane;
+        const float x = load_act<DT>(p.logits, row * p.stride + min(e, p.E - 1));
+        nan |= x != x;
+        c[v] = e < p.E ? (double)x : none;
+    }
+    if (p.sigmoid) {
+        if (scored) {
+#pragma unroll
+            for (int v = 0; v < W; ++v)
+                if (c[v] > none) c[v] = 1.0 / (1.0 + exp_of(-c[v]));
+        }
+    } else {
+        double mx = c[0], sum = 0.0;
+#pragma unroll
+        for (int v = 1; v < W; ++v) mx = fmax(mx, c[v]);
+        mx = wave_max(mx);
+        nan |= mx == (double)INFINITY;
+        if (scored) {
+#pragma unroll
+            for (int v = 0; v < W; ++v) {
+                if (c[v] > none) c[v] = exp_of(c[v] - mx);
+                sum += c[v] > none ? c[v] : 0.0;
+            }
+            sum = wave_sum(sum);
+#pragma unroll
+            for (int v = 0; v < W; ++v)
+                if (c[v] > none) c[v] = c[v] / sum;
         }
     }
     if (p.bias) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int e = 16 * v + l;
-            if (e < p.E && c[v] > none) c[v] += (double)p.bias[e];
+        for (int v = 0; v < W; ++v) {
+            const float b = p.bias[min(64 * v + lane, p.E - 1)];
+            if (c[v] > none) c[v] += (double)b;
             nan |= c[v] != c[v];
         }
     }
-    bad = row_any(nan);
+    bad = __any(nan);
     if (p.groups > 1) {
-        const uint32_t kept = kept_groups<double, V>(c, p);
         const int size = p.E / p.groups;
+        double s = none;  // lane q's: the score of group q
+        for (int q = 0; q < p.groups; ++q) {
+            double a = none, b = none;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int e = 16 * v + l;
+            for (int v = 0; v < W; ++v) {
+                const int e = 64 * v + lane;
+                const double x = e >= q * size && e < (q + 1) * size ? c[v] : none;
+                b = fmax(b, fmin(a, x));
+                a = fmax(a, x);
+            }
+            wave_max2(a, b);
+            if (lane == q) s = p.best == 2 && b > none ? a + b : a;
+        }
+        int rank = 0;
+        for (int q = 0; q < p.groups; ++q) {
+            const double o = __shfl(s, q, kWave);
+            rank += o > s || (o == s && q < lane) ? 1 : 0;
+        }
+        const uint64_t kept = __ballot(lane < p.groups && rank < p.keep);
+#pragma unroll
+        for (int v = 0; v < W; ++v) {
+            const int e = 64 * v + lane;
             if (e < p.E && !((kept >> (e / size)) & 1)) c[v] = none;
         }
     }
     int mine = -1;
     for (int i = 0; i < p.k; ++i) {
-        double bv = none;
-        int be = 0x7fffffff;
+        double top = c[0];
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-            if (c[v] > bv) {  // ties keep the lower index
-                bv = c[v];
-                be = 16 * v + l;
-            }
-#define NSOSX_STEP(N)                                                   \
-    {                                                                   \
-        const double ov = ror16<N>(bv);                                 \
-        const int oe = ror16<N>(be);                                    \
-        if (ov > bv || (ov == bv && oe < be)) { bv = ov; be = oe; }     \
-    }
-        NSOSX_STEP(8) NSOSX_STEP(4) NSOSX_STEP(2) NSOSX_STEP(1)
-#undef NSOSX_STEP
+        for (int v = 1; v < W; ++v) top = fmax(top, c[v]);
+        top = wave_max(top);
+        int e = -1;  // the lowest index of that value
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-            if (be == 16 * v + l) c[v] = none;
-        if (l == i) mine = bv > none ? be : -1;
+        for (int v = W - 1; v >= 0; --v) {
+            const uint64_t at = __ballot(c[v] == top);
+            e = at ? 64 * v + __builtin_ctzll(at) : e;
+        }
+        if (!(top > none)) e = -1;
+#pragma unroll
+        for (int v = 0; v < W; ++v)
+            if (e == 64 * v + lane) c[v] = none;
+        if ((lane & 15) == i) mine = e;
     }
     return mine;
 }
@@ -224,12 +563,8 @@ __device__ __forceinline__ float row_weight(const RouteScored& p, int64_t row, b
             t = x > 0.0f ? 1.0f / (1.0f + expf(-x)) : expf(x) / (1.0f + expf(x));
         } else {
             float all[V], mx, sum;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const int e = 16 * v + l;
-                all[v] = live && e < p.E ? load_act<DT>(p.logits, row * p.stride + e) : none;
-            }
-            softmax_stats<float, V>(all, mx, sum);
+            row_values<V, DT>(p.logits, row * p.stride, p.E, live, all);
+            softmax_stats<V>(all, mx, sum);
             t = expf(x - mx) / sum;
         }
         return mine >= 0 ? t * p.scale : 0.0f;
@@ -244,23 +579,35 @@ __device__ __forceinline__ float row_weight(const RouteScored& p, int64_t row, b
     return mine >= 0 ? t / sum * p.scale : 0.0f;
 }
 
-// Exclusive scan of counts [E] into s_off [E + 1] by the first wave of a workgroup.
+// Inclusive scan over a wave.
+__device__ __forceinline__ int wave_scan(int v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        const int u = __shfl_up(v, o, kWave);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+
+// Exclusive scan of counts [E] into s_off [E + 1] by the first wave of a workgroup: each lane
+// takes a run of 8, all loads at once.
 __device__ __forceinline__ void scan_counts(const int32_t* counts, int E, int32_t* s_off) {
     if (threadIdx.x >= kWave) return;
-    const int lane = threadIdx.x;
-    int carry = 0;
-    for (int e0 = 0; e0 < E; e0 += kWave) {
-        const int c = e0 + lane < E ? counts[e0 + lane] : 0;
-        int upto = c;
+    const int first = threadIdx.x * 8;
+    int c[8], sum = 0;
 #pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const int v = __shfl_up(upto, o, kWave);
-            if (lane >= o) upto += v;
-        }
-        if (e0 + lane < E) s_off[e0 + lane] = carry + upto - c;
-        carry += __builtin_amdgcn_readlane(upto, kWave - 1);
+    for (int i = 0; i < 8; ++i) c[i] = first + i < E ? counts[first + i] : 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += c[i];
+    int at = wave_scan(sum) - sum;
+    static_assert(kScoredMaxExperts == 8 * kWave, "a wave's runs hold every expert");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (first + i <= E) s_off[first + i] = at;
+        at += c[i];
     }
-    if (lane == 0) s_off[E] = carry;
+    if (E == kScoredMaxExperts && threadIdx.x == kWave - 1) s_off[E] = at;
 }
 
 // A workgroup of 16 RB threads routes RB rows, ranks them per expert through 64-bit row masks
@@ -276,11 +623,21 @@ __global__ __launch_bounds__(V > 16 ? 512 : 1024) void route_scored_kernel(Route
         for (int e = threadIdx.x; e < p.E; e += blockDim.x) s_mask[e] = 0;
         __syncthreads();
     }
-    const bool live = row < p.rows && (!p.valid || p.valid[row] != 0);
-    bool bad;
-    int mine = select_row<V, DT>(p, row, live, bad);
+    const int in = min(row, p.rows - 1);  // a row to read, past the last one too
+    const bool live = row < p.rows && (!p.valid || p.valid[in] != 0);
+    bool bad = false, sure;
+    int mine = select_fast<V, DT>(p, in, live, sure);
+    for (uint64_t left = __ballot(!sure && l == 0); left; left &= left - 1) {
+        const int first = __builtin_ctzll(left);
+        bool wrong;
+        const int c = select_wave<V, DT>(p, __builtin_amdgcn_readlane(in, first), wrong);
+        if ((int)(threadIdx.x & 48) == first) {
+            mine = c;
+            bad = wrong;
+        }
+    }
     if (live && bad) mine = l < p.k ? l : -1;  // a NaN score: the first k experts, weights NaN
-    float w = row_weight<V, DT>(p, row, live, mine);
+    float w = row_weight<V, DT>(p, in, live, mine);
     if (live && bad) w = NAN;
     const bool entry = row < p.rows && l < p.k;
     const int64_t at = (int64_t)row * p.k + l;
@@ -296,7 +653,8 @@ __global__ __launch_bounds__(V > 16 ? 512 : 1024) void route_scored_kernel(Route
     if (gridDim.x > 1) {
         if (entry) p.slot_of[at] = rank;  // the rank within the block, until the placement
         for (int e = threadIdx.x; e < p.E; e += blockDim.x)
-            p.block_counts[(int64_t)e * gridDim.x + blockIdx.x] = __popcll(s_mask[e]);
+            p.block_counts[p.by_block ? (int64_t)blockIdx.x * p.E + e : (int64_t)e * gridDim.x + blockIdx.x] =
+                __popcll(s_mask[e]);
         return;
     }
     for (int e = threadIdx.x; e < p.E; e += blockDim.x) p.counts[e] = s_cnt[e] = __popcll(s_mask[e]);
@@ -313,7 +671,8 @@ __global__ __launch_bounds__(V > 16 ? 512 : 1024) void route_scored_kernel(Route
     for (int i = total + threadIdx.x; i < p.rows * p.k; i += blockDim.x) p.perm[i] = -1;
 }
 
-// Per expert (a wave each): the exclusive scan of its counts over the blocks, in place.
+// Per expert (a wave each): the exclusive scan of its counts over the blocks, in place, 256 blocks
+// at a time.
 __global__ __launch_bounds__(256) void route_scored_scan_kernel(int32_t* __restrict__ block_counts,
                                                                 int blocks, int E,
                                                                 int32_t* __restrict__ counts) {
@@ -322,37 +681,89 @@ __global__ __launch_bounds__(256) void route_scored_scan_kernel(int32_t* __restr
     const int lane = threadIdx.x & 63;
     int32_t* row = block_counts + (int64_t)e * blocks;
     int carry = 0;
-    for (int b0 = 0; b0 < blocks; b0 += kWave) {
-        const int c = b0 + lane < blocks ? row[b0 + lane] : 0;
-        int upto = c;
+    for (int b0 = 0; b0 < blocks; b0 += 4 * kWave) {
+        const int b = b0 + 4 * lane;
+        int c[4];
 #pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const int v = __shfl_up(upto, o, kWave);
-            if (lane >= o) upto += v;
+        for (int i = 0; i < 4; ++i) c[i] = b + i < blocks ? row[b + i] : 0;
+        const int sum = c[0] + c[1] + c[2] + c[3];
+        const int upto = wave_scan(sum);
+        int at = carry + upto - sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (b + i < blocks) row[b + i] = at;
+            at += c[i];
         }
-        if (b0 + lane < blocks) row[b0 + lane] = carry + upto - c;
         carry += __builtin_amdgcn_readlane(upto, kWave - 1);
     }
     if (lane == 0) counts[e] = carry;
 }
 
 // Ranks within a block -> slots.
+__device__ __forceinline__ void place_entry(const RouteScored& p, const int32_t* s_off, int64_t i,
+                                            int row, int e, int rank) {
+    if (e >= 0) {
+        p.slot_of[i] = s_off[e] + rank;
+        p.perm[s_off[e] + rank] = row;
+    }
+    if (i >= s_off[p.E]) p.perm[i] = -1;
+}
+
 __global__ __launch_bounds__(256) void route_scored_place_kernel(RouteScored p, int blocks,
                                                                  int block_rows) {
     __shared__ int32_t s_off[kScoredMaxExperts + 1];
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const bool entry = i < (int64_t)p.rows * p.k;
+    const int row = entry ? (int)(i / p.k) : 0, e = entry ? p.selected[i] : -1;
+    const int rank =
+        e >= 0 ? p.block_counts[(int64_t)e * blocks + row / block_rows] + p.slot_of[i] : -1;
     scan_counts(p.counts, p.E, s_off);
     __syncthreads();
     if (blockIdx.x == 0)
-        for (int e = threadIdx.x; e <= p.E; e += blockDim.x) p.offsets[e] = s_off[e];
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (int64_t)p.rows * p.k) return;
-    const int row = (int)(i / p.k), e = p.selected[i];
-    if (e >= 0) {
-        const int s = s_off[e] + p.block_counts[(int64_t)e * blocks + row / block_rows] + p.slot_of[i];
-        p.slot_of[i] = s;
-        p.perm[s] = row;
+        for (int j = threadIdx.x; j <= p.E; j += blockDim.x) p.offsets[j] = s_off[j];
+    if (entry) place_entry(p, s_off, i, row, e, rank);
+}
+
+// The same with the scans over the blocks, for few counts (kScoredPlaceCounts): a workgroup for each
+// block of rows, which sums every expert's counts, and those before its own block, by itself (4096
+// rows of 60 experts: @@ us less than the two launches).
+constexpr int kScoredPlaceCounts = 16384;
+
+__global__ __launch_bounds__(256) void route_scored_scan_place_kernel(RouteScored p, int blocks,
+                                                                      int block_rows) {
+    __shared__ int32_t s_off[kScoredMaxExperts + 1], s_all[kScoredMaxExperts], s_before[kScoredMaxExperts];
+    const int tid = threadIdx.x;
+    // as many threads an expert as there are, a run of the blocks each
+    const int parts = max(256 / p.E, 1);
+    for (int e = tid; e < p.E; e += 256) s_all[e] = s_before[e] = 0;
+    __syncthreads();
+    for (int t = tid; t < p.E * parts; t += 256) {
+        const int part = t / p.E, e = t - part * p.E;
+        const int32_t* column = p.block_counts + e;
+        const int b0 = blocks * part / parts, b1 = blocks * (part + 1) / parts;
+        int before = 0, all = 0;
+#pragma unroll 16
+        for (int b = b0; b < b1; ++b) {
+            const int v = column[b * p.E];
+            all += v;
+            before += b < (int)blockIdx.x ? v : 0;
+        }
+        atomicAdd(&s_all[e], all);  // (whole numbers: in any order)
+        atomicAdd(&s_before[e], before);
     }
-    if (i >= s_off[p.E]) p.perm[i] = -1;
+    __syncthreads();
+    scan_counts(s_all, p.E, s_off);
+    __syncthreads();
+    if (blockIdx.x == 0) {
+        for (int j = tid; j <= p.E; j += 256) p.offsets[j] = s_off[j];
+        for (int j = tid; j < p.E; j += 256) p.counts[j] = s_all[j];
+    }
+    const int64_t first = (int64_t)blockIdx.x * block_rows * p.k;
+    const int64_t end = min(first + (int64_t)block_rows * p.k, (int64_t)p.rows * p.k);
+    for (int64_t i = first + tid; i < end; i += 256) {
+        const int e = p.selected[i];
+        place_entry(p, s_off, i, (int)(i / p.k), e, e >= 0 ? s_before[e] + p.slot_of[i] : -1);
+    }
 }
 
 // ---- gradient ---------------------------------------------------------------------
@@ -381,7 +792,7 @@ __global__ __launch_bounds__(256) void route_scored_bwd_kernel(RouteScoredBwd p)
     const bool live = row < p.rows;
     for (int i = threadIdx.x; i < 16 * p.E; i += 256) s_g[i] = 0.0f;
     __syncthreads();
-    const int64_t base = (int64_t)row * p.stride;
+    const int64_t base = (int64_t)min(row, p.rows - 1) * p.stride;
     const int64_t at = (int64_t)row * p.k + l;
     int e = live && l < p.k ? p.selected[at] : -1;
     if (e >= p.E) e = -1;
@@ -392,10 +803,8 @@ __global__ __launch_bounds__(256) void route_scored_bwd_kernel(RouteScoredBwd p)
     float mx = none, sum = 1.0f, dot = 0.0f;
     float all[V];
     if (dense) {
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-            all[v] = live && 16 * v + l < p.E ? load_act<DT>(p.logits, base + 16 * v + l) : none;
-        softmax_stats<float, V>(all, mx, sum);
+        row_values<V, DT>(p.logits, base, p.E, live, all);
+        softmax_stats<V>(all, mx, sum);
         dot = row_sum(e < 0 || x == none ? 0.0f : g * (expf(x - mx) / sum));
     } else if (p.renorm) {
         const float m = row_max(x);
@@ -484,7 +893,8 @@ extern "C" int nsosx_moe_route_scored(const void* logits, int logits_dtype, int6
     const int blocks = (rows - 1) / rb + 1;
     RouteScored p{logits, logits_stride, valid_rows, bias, rows, experts, k, sigmoid != 0,
                   group_keep == groups ? 1 : groups, group_keep, group_best, renorm != 0, scale,
-                  weights, selected, counts, offsets, perm, slot_of, workspace};
+                  weights, selected, counts, offsets, perm, slot_of, workspace,
+                  (int64_t)blocks * experts <= kScoredPlaceCounts};
     hipStream_t st = static_cast<hipStream_t>(stream);
 #define NSOSX_RS(V)                                                                             \
     do {                                                                                        \
@@ -497,7 +907,9 @@ extern "C" int nsosx_moe_route_scored(const void* logits, int logits_dtype, int6
     } while (0)
     NSOSX_SCORED_V(experts, NSOSX_RS);
 #undef NSOSX_RS
-    if (!select_only && blocks > 1) {
+    if (!select_only && blocks > 1 && p.by_block) {
+        hipLaunchKernelGGL(route_scored_scan_place_kernel, dim3(blocks), dim3(256), 0, st, p, blocks, rb);
+    } else if (!select_only && blocks > 1) {
         hipLaunchKernelGGL(route_scored_scan_kernel, dim3((experts + 3) / 4), dim3(256), 0, st,
                            workspace, blocks, experts, counts);
         const int64_t entries = (int64_t)rows * k;

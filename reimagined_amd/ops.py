@@ -727,19 +727,28 @@ def moe_combine(expert_out, slot_of, selected, weights, out_dtype=torch.float32)
 
 # ---- scored routing and int8 experts ----------------------------------------------
 
-def _on(fn: str, device, **tensors) -> None:
-    """Contiguous tensors of one device, which has to be the current one (whose stream the call
-    goes to): (tensor, dtype or None, shape or None) each; a None tensor is skipped."""
-    for name, (t, dtype, shape) in tensors.items():
-        if t is None:
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _on(fn: str, dev: int, *tensors) -> None:
+    """Checks (name, tensor or None, dtype or None, shape or None) each: contiguous tensors of
+    device `dev`, which has to be the current one (whose stream the call goes to)."""
+    for name, t, dtype, shape in tensors:
+        # (one line where all is well: a decode step runs this on every call)
+        if t is None or (t.get_device() == dev >= 0 and t.is_contiguous() and
+                         (dtype is None or t.dtype == dtype) and
+                         (shape is None or t.shape == shape)):
             continue
         _dev(t, name, dtype)
-        if t.device != device:
-            raise ValueError(f"{fn}: {name} must be on {device}, got {t.device}")
-        if shape is not None and t.shape != tuple(shape):
-            raise ValueError(f"{fn}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"{fn}: the tensors' device {device} must be the current one")
+        if t.get_device() != dev:
+            raise ValueError(f"{fn}: {name} must be on device {dev}, got {t.device}")
+        raise ValueError(f"{fn}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if _current_device() != dev:
+        raise ValueError(f"{fn}: the tensors' device {dev} must be the current one")
+
+
+def _stream_on(dev: int):
+    return _stream() if _raw_stream is None else _raw_stream(dev)
 
 
 def _logit_rows(fn: str, logits: torch.Tensor) -> int:
@@ -779,24 +788,29 @@ def moe_route_scored(logits: torch.Tensor, k: int, score: str = "softmax", bias=
     sig = _score_mode(fn, score)
     dev = logits.device
     mask = valid_rows_mask(valid_rows, rows, dev)
-    _on(fn, dev, bias=(bias, torch.float32, (e,)), valid_rows=(mask, torch.uint8, None))
+    _on(fn, logits.get_device(), ("bias", bias, torch.float32, (e,)),
+        ("valid_rows", mask, torch.uint8, None))
     if not 0 < k <= e:
         raise ValueError(f"{fn}: need 0 < k <= {e} experts, got {k}")
     keep = groups if group_keep is None else group_keep
-    shape = (rows, k)
-    out = {"weights": torch.empty(shape, dtype=torch.float32, device=dev),
-           "selected": torch.empty(shape, dtype=torch.int32, device=dev)}
-    ws = None
-    if not select_only:
-        i32 = dict(dtype=torch.int32, device=dev)
-        out.update(counts=torch.empty(e, **i32), offsets=torch.empty(e + 1, **i32),
-                   perm=torch.empty(rows * k, **i32), slot_of=torch.empty(shape, **i32))
-        ws = torch.empty(max(1, int(lib().nsosx_moe_route_scored_workspace(rows, e))), **i32)
+    # the int32 outputs (and the workspace behind them) are pieces of one buffer
+    n = rows * k
+    w = torch.empty((rows, k), dtype=torch.float32, device=dev)
+    if select_only:
+        sel = torch.empty((rows, k), dtype=torch.int32, device=dev)
+        call("nsosx_moe_route_scored", _p(logits), _dt(logits), stride, _p(mask), _p(bias), rows, e,
+             k, sig, groups, keep, group_best, int(renorm), float(scale), _p(w), _p(sel), None,
+             None, None, None, None, _stream_on(logits.get_device()))
+        return {"weights": w, "selected": sel}
+    ws = max(1, int(lib().nsosx_moe_route_scored_workspace(rows, e)))
+    buf = torch.empty(3 * n + 2 * e + 1 + ws, dtype=torch.int32, device=dev)
+    sel, slot_of, perm, counts, offsets, ws = buf.split((n, n, n, e, e + 1, ws))
+    sel, slot_of = sel.view(rows, k), slot_of.view(rows, k)
     call("nsosx_moe_route_scored", _p(logits), _dt(logits), stride, _p(mask), _p(bias), rows, e, k,
-         sig, groups, keep, group_best, int(renorm), float(scale), _p(out["weights"]),
-         _p(out["selected"]), _p(out.get("counts")), _p(out.get("offsets")), _p(out.get("perm")),
-         _p(out.get("slot_of")), _p(ws), _stream())
-    return out
+         sig, groups, keep, group_best, int(renorm), float(scale), _p(w), _p(sel), _p(counts),
+         _p(offsets), _p(perm), _p(slot_of), _p(ws), _stream_on(logits.get_device()))
+    return {"weights": w, "selected": sel, "counts": counts, "offsets": offsets, "perm": perm,
+            "slot_of": slot_of}
 
 
 def moe_route_scored_backward(logits: torch.Tensor, selected: torch.Tensor, dweights: torch.Tensor,
@@ -811,20 +825,20 @@ def moe_route_scored_backward(logits: torch.Tensor, selected: torch.Tensor, dwei
         raise ValueError(f"{fn}: selected must be [rows, k], got {tuple(selected.shape)}")
     k = selected.shape[1]
     sig = _score_mode(fn, score)
-    _on(fn, logits.device, selected=(selected, torch.int32, None),
-        dweights=(dweights, torch.float32, (rows, k)))
-    out = torch.empty((rows, e), dtype=logits.dtype, device=logits.device)
+    dev = logits.get_device()
+    _on(fn, dev, ("selected", selected, torch.int32, None),
+        ("dweights", dweights, torch.float32, (rows, k)))
+    out = logits.new_empty((rows, e))
     call("nsosx_moe_route_scored_backward", _p(logits), _dt(logits), stride, _p(selected),
-         _p(dweights), rows, e, k, sig, int(renorm), float(scale), _p(out), _stream())
+         _p(dweights), rows, e, k, sig, int(renorm), float(scale), _p(out), _stream_on(dev))
     return out
 
 
 def _combine_shapes(fn, expert_out, slot_of, weights):
     if expert_out.dim() != 2 or slot_of.dim() != 2 or 0 in expert_out.shape or 0 in slot_of.shape:
         raise ValueError(f"{fn}: expert_out must be [slots, dim] and slot_of [rows, k]")
-    _dt(expert_out)
-    _on(fn, expert_out.device, expert_out=(expert_out, None, None),
-        slot_of=(slot_of, torch.int32, None), weights=(weights, torch.float32, slot_of.shape))
+    _on(fn, expert_out.get_device(), ("expert_out", expert_out, None, None),
+        ("slot_of", slot_of, torch.int32, None), ("weights", weights, torch.float32, slot_of.shape))
     return (*slot_of.shape, *expert_out.shape)
 
 
@@ -836,9 +850,9 @@ def moe_combine_topk(expert_out: torch.Tensor, slot_of: torch.Tensor, weights: t
     rows, k, slots, dim = _combine_shapes(fn, expert_out, slot_of, weights)
     if out_dtype not in _DT:
         raise ValueError(f"{fn}: out_dtype must be float32 or bfloat16")
-    out = torch.empty((rows, dim), dtype=out_dtype, device=expert_out.device)
+    out = expert_out.new_empty((rows, dim), dtype=out_dtype)
     call("nsosx_moe_combine_topk", _p(expert_out), _dt(expert_out), _p(slot_of), _p(weights), rows,
-         slots, k, dim, _p(out), _DT[out_dtype], _stream())
+         slots, k, dim, _p(out), _DT[out_dtype], _stream_on(expert_out.get_device()))
     return out
 
 
@@ -849,12 +863,12 @@ def moe_combine_topk_backward(dout: torch.Tensor, expert_out: torch.Tensor, slot
     routing's perm is given, else all are cleared first."""
     fn = "moe_combine_topk_backward"
     rows, k, slots, dim = _combine_shapes(fn, expert_out, slot_of, weights)
-    _dt(dout)
-    _on(fn, expert_out.device, dout=(dout, None, (rows, dim)), perm=(perm, torch.int32, (slots,)))
+    dev = expert_out.get_device()
+    _on(fn, dev, ("dout", dout, None, (rows, dim)), ("perm", perm, torch.int32, (slots,)))
     de = torch.empty_like(expert_out) if perm is not None else torch.zeros_like(expert_out)
-    dw = torch.empty((rows, k), dtype=torch.float32, device=expert_out.device)
+    dw = weights.new_empty((rows, k))
     call("nsosx_moe_combine_topk_backward", _p(dout), _dt(dout), _p(expert_out), _dt(expert_out),
-         _p(slot_of), _p(weights), _p(perm), rows, slots, k, dim, _p(de), _p(dw), _stream())
+         _p(slot_of), _p(weights), _p(perm), rows, slots, k, dim, _p(de), _p(dw), _stream_on(dev))
     return de, dw
 
 
@@ -864,18 +878,20 @@ def int8_gemm(q: torch.Tensor, act_scale: torch.Tensor, w: torch.Tensor, w_scale
     [M, K] and weights w [N, K], a scale per token and per output, both as
     quantize_activations_bitnet gives them; y [M, N] f32 or bf16."""
     fn = "int8_gemm"
-    if q.dim() != 2 or w.dim() != 2 or q.shape[1] != w.shape[1] or 0 in q.shape or 0 in w.shape:
+    if q.dim() != 2 or w.dim() != 2 or q.shape[1] != w.shape[1] or not (q.numel() and w.numel()):
         raise ValueError(f"{fn}: q [M, K] and w [N, K] must agree in K, got {tuple(q.shape)} and "
                          f"{tuple(w.shape)}")
-    (m, k), n = q.shape, w.shape[0]
-    _on(fn, q.device, q=(q, torch.int8, None), act_scale=(act_scale, torch.float32, (m,)),
-        w=(w, torch.int8, None), w_scale=(w_scale, torch.float32, (n,)),
-        bias=(bias, torch.float32, (n,)))
+    m, k = q.shape
+    n = w.shape[0]
+    dev = q.get_device()
+    _on(fn, dev, ("q", q, torch.int8, None), ("act_scale", act_scale, torch.float32, (m,)),
+        ("w", w, torch.int8, None), ("w_scale", w_scale, torch.float32, (n,)),
+        ("bias", bias, torch.float32, (n,)))
     if out_dtype not in _DT:
         raise ValueError(f"{fn}: out_dtype must be float32 or bfloat16")
-    y = torch.empty((m, n), dtype=out_dtype, device=q.device)
+    y = q.new_empty((m, n), dtype=out_dtype)
     call("nsosx_int8_gemm", _p(q), _p(act_scale), _p(w), _p(w_scale), _p(bias), m, k, n, _p(y),
-         _DT[out_dtype], _stream())
+         _DT[out_dtype], _stream_on(dev))
     return y
 
 
@@ -886,23 +902,25 @@ def grouped_int8_gemm(q: torch.Tensor, act_scale: torch.Tensor, w: torch.Tensor,
     [E, N], the segments offsets [E+1] and, where q holds the unrouted rows, the slots' rows
     perm (else q is in slot order).  -> y [slots, N]; rows past offsets[E] are not written."""
     fn = "grouped_int8_gemm"
-    if q.dim() != 2 or w.dim() != 3 or q.shape[1] != w.shape[2] or 0 in q.shape or 0 in w.shape:
+    if q.dim() != 2 or w.dim() != 3 or q.shape[1] != w.shape[2] or not (q.numel() and w.numel()):
         raise ValueError(f"{fn}: q [rows, K] and w [E, N, K] must agree in K, got "
                          f"{tuple(q.shape)} and {tuple(w.shape)}")
-    (rows, k), (e, n) = q.shape, w.shape[:2]
+    rows, k = q.shape
+    e, n, _ = w.shape
     slots = rows if perm is None else perm.numel()
     if slots == 0:
         raise ValueError(f"{fn}: perm must hold the slots' rows")
-    _on(fn, q.device, q=(q, torch.int8, None), act_scale=(act_scale, torch.float32, (rows,)),
-        w=(w, torch.int8, None), w_scale=(w_scale, torch.float32, (e, n)),
-        offsets=(offsets, torch.int32, (e + 1,)), perm=(perm, torch.int32, (slots,)),
-        bias=(bias, torch.float32, (e, n)))
+    dev = q.get_device()
+    _on(fn, dev, ("q", q, torch.int8, None), ("act_scale", act_scale, torch.float32, (rows,)),
+        ("w", w, torch.int8, None), ("w_scale", w_scale, torch.float32, (e, n)),
+        ("offsets", offsets, torch.int32, (e + 1,)), ("perm", perm, torch.int32, (slots,)),
+        ("bias", bias, torch.float32, (e, n)))
     if out_dtype not in _DT:
         raise ValueError(f"{fn}: out_dtype must be float32 or bfloat16")
-    y = torch.empty((slots, n), dtype=out_dtype, device=q.device)
+    y = q.new_empty((slots, n), dtype=out_dtype)
     call("nsosx_grouped_int8_gemm", _p(q), _p(act_scale), rows, _p(w), _p(w_scale), _p(bias),
          _p(offsets), _p(perm), slots, e, k, n, int(squared_relu), _p(y), _DT[out_dtype],
-         _stream())
+         _stream_on(dev))
     return y
 
 
