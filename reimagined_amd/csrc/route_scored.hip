@@ -784,13 +784,20 @@ struct RouteScoredBwd {
     void* dlogits;  // [rows, E], contiguous
 };
 
+// Whether another choice of the row, N lanes on, names the same expert (N up to 8 meets every pair).
+template <int N>
+__device__ __forceinline__ void same_expert(int e, bool& twice) {
+    twice |= e >= 0 && ror16<N>(e) == e;
+}
+
 template <int V, int DT>
 __global__ __launch_bounds__(256) void route_scored_bwd_kernel(RouteScoredBwd p) {
-    extern __shared__ float s_g[];  // [16, E]
+    extern __shared__ __align__(16) float s_g[];  // [16, E]
     const int l = threadIdx.x & 15, rl = threadIdx.x >> 4;
     const int row = blockIdx.x * 16 + rl;
     const bool live = row < p.rows;
-    for (int i = threadIdx.x; i < 16 * p.E; i += 256) s_g[i] = 0.0f;
+    for (int i = threadIdx.x; i < 4 * p.E; i += 256)
+        reinterpret_cast<float4*>(s_g)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     __syncthreads();
     const int64_t base = (int64_t)min(row, p.rows - 1) * p.stride;
     const int64_t at = (int64_t)row * p.k + l;
@@ -820,19 +827,47 @@ __global__ __launch_bounds__(256) void route_scored_bwd_kernel(RouteScoredBwd p)
         const float s = x > 0.0f ? 1.0f / (1.0f + expf(-x)) : expf(x) / (1.0f + expf(x));
         g = g * s * (1.0f / (1.0f + expf(x)));
     }
-    // one lane after the other, so that an expert named twice adds both
-    for (int i = 0; i < p.k; ++i)
-        if (l == i && e >= 0) s_g[rl * p.E + e] += g;
-    __syncthreads();
-    if (!live) return;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const int j = 16 * v + l;
-        if (j >= p.E) continue;
-        float d = s_g[rl * p.E + j];
-        if (dense) d = all[v] == none ? 0.0f : (expf(all[v] - mx) / sum) * (d - dot);
-        store_act<DT>(p.dlogits, (int64_t)row * p.E + j, d);
+    // An expert named twice gets both, one lane after the other (the order is the same each time); a
+    // wave without one, every routing's, stores at once.
+    bool twice = false;
+    same_expert<1>(e, twice); same_expert<2>(e, twice); same_expert<3>(e, twice); same_expert<4>(e, twice);
+    same_expert<5>(e, twice); same_expert<6>(e, twice); same_expert<7>(e, twice); same_expert<8>(e, twice);
+    if (__any(twice)) {
+        for (int i = 0; i < p.k; ++i)
+            if (l == i && e >= 0) s_g[rl * p.E + e] += g;
+    } else if (e >= 0) {
+        s_g[rl * p.E + e] = g;
     }
+    if (dense) {
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int j = 16 * v + l;
+            if (j < p.E) {
+                const float d = s_g[rl * p.E + j];
+                s_g[rl * p.E + j] = all[v] == none ? 0.0f : (expf(all[v] - mx) / sum) * (d - dot);
+            }
+        }
+    }
+    __syncthreads();
+    // the workgroup's rows lie behind each other: out in 16-byte pieces
+    const int64_t first = (int64_t)blockIdx.x * 16 * p.E;
+    const int count = min(16, p.rows - (int)blockIdx.x * 16) * p.E;
+    constexpr int kPiece = DT == NSOSX_F32 ? 4 : 8;
+    const int pieces = (reinterpret_cast<uintptr_t>(p.dlogits) & 15) == 0 ? count / kPiece : 0;
+    for (int i = threadIdx.x; i < pieces; i += 256) {
+        const float4 a = *reinterpret_cast<const float4*>(s_g + i * kPiece);
+        if constexpr (DT == NSOSX_F32) {
+            *reinterpret_cast<float4*>(static_cast<float*>(p.dlogits) + first + i * kPiece) = a;
+        } else {
+            const float4 b = *reinterpret_cast<const float4*>(s_g + i * kPiece + 4);
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dlogits) + first + i * kPiece) =
+                make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y),
+                           pack_bf16x2(b.z, b.w));
+        }
+    }
+    for (int i = pieces * kPiece + threadIdx.x; i < count; i += 256)
+        store_act<DT>(p.dlogits, first + i, s_g[i]);
 }
 
 static int scored_block_rows(int rows, int E) {
