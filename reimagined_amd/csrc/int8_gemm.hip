@@ -15,6 +15,7 @@ template <int NT, int MT, int W, int D, bool ALIGNED>
 struct Split {
     static constexpr int kN = 16 * NT, kM = 16 * MT, kThreads = 64 * W;
     static constexpr int kBand = 8, kWavesPerSimd = 1;
+    static constexpr bool kRuns = false;
     static constexpr int kSmem = i8_split_smem<NT, MT, W, D>();
     template <int YDT>
     static __device__ __forceinline__ void run(const I8Problem& pb, const I8Rows& rows, int n0, int m0,
@@ -27,6 +28,7 @@ template <int NWN, int NWM, int TM>
 struct Staged {  // any alignment
     static constexpr int kN = 64 * NWN, kM = 32 * TM * NWM, kThreads = 64 * NWN * NWM;
     static constexpr int kBand = 8, kWavesPerSimd = 1;
+    static constexpr bool kRuns = true;
     static constexpr int kSmem = i8_tile_smem<NWN, NWM, TM>();
     template <int YDT>
     static __device__ __forceinline__ void run(const I8Problem& pb, const I8Rows& rows, int n0, int m0,
@@ -39,6 +41,7 @@ template <int NWN, int NWM, int TM, int BAND, int WPS>
 struct Wide {  // 16-byte aligned rows
     static constexpr int kN = 64 * NWN, kM = 32 * TM * NWM, kThreads = 64 * NWN * NWM;
     static constexpr int kBand = BAND, kWavesPerSimd = WPS;
+    static constexpr bool kRuns = true;
     static constexpr int kSmem = i8_tile_smem<NWN, NWM, TM>();
     template <int YDT>
     static __device__ __forceinline__ void run(const I8Problem& pb, const I8Rows& rows, int n0, int m0,
@@ -68,15 +71,25 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesPerSimd) void i8_gemm_kernel(
 
 // ---- the experts' segments ----------------------------------------------------
 
-// One row tile of one segment a workgroup.
+// One row tile of one segment a workgroup.  Outputs are fastest, so that where their tiles divide
+// by the 8 XCDs, each XCD reads an eighth of every expert's weights.  Where they do not, and an
+// expert has more than one row tile to share its weights, the large tiles are dealt to the XCDs in
+// contiguous runs, as those of one matrix, so that they are read by one or two (8192 rows to 8 of 128 experts of 2048 -> 768, 128 x 128 tiles: 169
+// us, and 200 with outputs fastest; to 2 of 8 experts of 1024 -> 4096: 112 and 105).  The launch
+// holds as many workgroups as there can be tiles; those past the real ones end here.
 template <class T, int YDT>
 __global__ __launch_bounds__(T::kThreads, T::kWavesPerSimd) void i8_grouped_kernel(I8Group gp,
                                                                                  void* __restrict__ y) {
     extern __shared__ __align__(1024) char smem_i8[];
     const int ntn = (gp.N + T::kN - 1) / T::kN;
-    const int nt = blockIdx.x % ntn;
+    int nt = blockIdx.x % ntn, mt = blockIdx.x / ntn;
+    if (T::kRuns && ntn % 8 != 0 && gp.slots > (int64_t)T::kM * gp.experts) {
+        const int total = i8_all_tiles<T::kM>(gp);
+        if (mt >= total) return;
+        i8_tile_order<T::kBand>(blockIdx.x, ntn, total, nt, mt);
+    }
     int e, m0;
-    if (!i8_find_segment<T::kM>(gp, blockIdx.x / ntn, e, m0)) return;
+    if (!i8_find_segment<T::kM>(gp, mt, e, m0)) return;
     I8Problem pb;
     I8Rows rows;
     if (!i8_segment(gp, e, pb, rows)) return;
@@ -128,7 +141,7 @@ static I8Tile choose_tile(int K, bool aligned, Tiles tiles) {
         2.6 - 0.4 * k + whole(tiles(32, 64)) * (0.6 + 1.66 * k),
         1.0 - 0.5 * k + whole(tiles(64, 64)) * (3.25 + 2.43 * k),
         2.7 + 0.8 * k + part(tiles(128, 128)) * (1.2 + 4.2 * k),
-        whole(tiles(256, 256)) * (8.0 + 15.3 * k),
+        whole(tiles(256, 256)) * (6.8 + 14.7 * k),
     };
     // a launch holds less than 2^32 threads (tiles of 16 rows: 512 each): the larger ones always do
     const bool fits[] = {tiles(16, 16) < 4e6, tiles(16, 64) < 4e6, tiles(32, 64) < 8e6,

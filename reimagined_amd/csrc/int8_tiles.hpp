@@ -60,25 +60,40 @@ __device__ __forceinline__ bool i8_segment(const I8Group& gp, int e, I8Problem& 
     return true;
 }
 
-// Row tile `tile` of the experts' segments in order (ceil(rows / BM) tiles each): its expert
-// and first row.  A wave counts 64 experts' tiles at a time.
+// Row tiles of expert j's segment.
+template <int BM>
+__device__ __forceinline__ int i8_row_tiles(const I8Group& gp, int j) {
+    if (j >= gp.experts) return 0;
+    const int n = min(max(gp.offsets[j + 1], 0), gp.slots) - min(max(gp.offsets[j], 0), gp.slots);
+    return n > 0 ? (n + BM - 1) / BM : 0;
+}
+
+__device__ __forceinline__ int i8_wave_scan(int v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        const int u = __shfl_up(v, o, kWave);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+
+// All segments' row tiles.
+template <int BM>
+__device__ __forceinline__ int i8_all_tiles(const I8Group& gp) {
+    int total = 0;
+    for (int e0 = 0; e0 < gp.experts; e0 += kWave)
+        total += wave_sum_i32(i8_row_tiles<BM>(gp, e0 + (threadIdx.x & 63)));
+    return __builtin_amdgcn_readfirstlane(total);
+}
+
+// Row tile `tile` of the segments in order: its expert and first row.  A wave counts 64 experts at
+// a time.
 template <int BM>
 __device__ __forceinline__ bool i8_find_segment(const I8Group& gp, int tile, int& e, int& m0) {
-    const int lane = threadIdx.x & 63;
     for (int e0 = 0; e0 < gp.experts; e0 += kWave) {
-        const int j = e0 + lane;
-        int tiles = 0;
-        if (j < gp.experts) {
-            const int b = min(max(gp.offsets[j], 0), gp.slots);
-            const int n = min(max(gp.offsets[j + 1], 0), gp.slots) - b;
-            tiles = n > 0 ? (n + BM - 1) / BM : 0;
-        }
-        int upto = tiles;
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const int v = __shfl_up(upto, o, kWave);
-            if (lane >= o) upto += v;
-        }
+        const int tiles = i8_row_tiles<BM>(gp, e0 + (threadIdx.x & 63));
+        const int upto = i8_wave_scan(tiles);
         const uint64_t past = __ballot(tile < upto);
         if (past) {
             const int l = __builtin_ctzll(past);
@@ -127,9 +142,11 @@ __device__ __forceinline__ i8x16 load16_tail(const int8_t* row, int k, int K) {
 }
 
 // The affine of one output.  Rounded at the conversion, both products and the sum.
-__device__ __forceinline__ float i8_affine(int acc, float as, float ws, float bias, int sqrelu) {
-    float v = __fadd_rn(__fmul_rn(__fmul_rn(static_cast<float>(acc), as), ws), bias);
-    if (sqrelu) {
+template <bool BIAS, bool SQRELU>
+__device__ __forceinline__ float i8_affine(int acc, float as, float ws, float bias) {
+    float v = __fmul_rn(__fmul_rn(static_cast<float>(acc), as), ws);
+    if (BIAS) v = __fadd_rn(v, bias);
+    if (SQRELU) {
         v = v < 0.0f ? 0.0f : v;  // a NaN stays
         v = __fmul_rn(v, v);
     }
@@ -147,7 +164,11 @@ __device__ __forceinline__ void i8_store4(const I8Problem& pb, const I8Rows& row
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const int at = min(n + c, pb.N - 1);
-        o[c] = i8_affine(sum[c], as, pb.w_scale[at], pb.bias ? pb.bias[at] : 0.0f, pb.sqrelu);
+        const float ws = pb.w_scale[at];
+        const float v = pb.bias ? i8_affine<true, false>(sum[c], as, ws, pb.bias[at])
+                                : i8_affine<false, false>(sum[c], as, ws, 0.0f);
+        const float h = v < 0.0f ? 0.0f : v;
+        o[c] = pb.sqrelu ? __fmul_rn(h, h) : v;
     }
     const int64_t at = orow * pb.N + n;
     constexpr int kSize = YDT == NSOSX_F32 ? 4 : 2;
@@ -306,8 +327,28 @@ __device__ __forceinline__ void i8_split_tile(const I8Problem& pb, const I8Rows&
 // ===========================================================================
 constexpr int kI8BK = 128;
 
+// Two stages, and behind them the tile's scales and biases per output and scales per token, there
+// from the start: fetched in the epilogue, they are two memory round trips of every tile.
 template <int NWN, int NWM, int TM>
-constexpr int i8_tile_smem() { return 2 * (64 * NWN + 32 * TM * NWM) * kI8BK; }
+constexpr int i8_stages_smem() { return 2 * (64 * NWN + 32 * TM * NWM) * kI8BK; }
+template <int NWN, int NWM, int TM>
+constexpr int i8_tile_smem() {
+    return i8_stages_smem<NWN, NWM, TM>() + (2 * 64 * NWN + 32 * TM * NWM) * 4;
+}
+
+template <int NWN, int NWM, int TM>
+__device__ __forceinline__ void i8_stage_scales(const I8Problem& pb, const I8Rows& rows, int n0, int m0,
+                                                char* smem) {
+    constexpr int kThreads = 64 * NWN * NWM, BN = 64 * NWN, BM = 32 * TM * NWM;
+    float* s_scale = reinterpret_cast<float*>(smem + i8_stages_smem<NWN, NWM, TM>());
+    for (int i = threadIdx.x; i < BN; i += kThreads) {
+        const int n = min(n0 + i, pb.N - 1);
+        s_scale[i] = pb.w_scale[n];
+        if (pb.bias) s_scale[BN + i] = pb.bias[n];
+    }
+    for (int i = threadIdx.x; i < BM; i += kThreads)
+        s_scale[2 * BN + i] = rows.act_scale[i8_source(rows, rows.begin + min(m0 + i, rows.count - 1))];
+}
 
 // Linear workgroup id -> tile.  Consecutive ids go round-robin to the 8 XCDs; each XCD takes a
 // contiguous run of tiles, in bands of GM row tiles, rows fastest, so that the tiles in flight
@@ -323,47 +364,53 @@ __device__ __forceinline__ void i8_tile_order(int L, int ntn, int ntm, int& nt, 
     nt = in / size;
 }
 
-template <int YDT, int NWN, int NWM, int TM>
-__device__ __forceinline__ void i8_epilogue(const I8Problem& pb, const I8Rows& rows, int n0, int m0,
+template <int YDT, int NWN, int NWM, int TM, bool BIAS, bool SQRELU>
+__device__ __forceinline__ void i8_epilogue_as(const I8Problem& pb, const I8Rows& rows, int n0, int m0,
                                             void* __restrict__ y, char* smem,
                                             const i32x16 (&acc)[2][TM]) {
-    constexpr int kThreads = 64 * NWN * NWM, kSize = YDT == NSOSX_F32 ? 4 : 2;
+    constexpr int kSize = YDT == NSOSX_F32 ? 4 : 2;
     constexpr int kRow = 64 * kSize, kSlice = 32 * kRow, kChunks = kRow / 16;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wn = wave % NWN, wm = wave / NWN;
     const int g = lane >> 5, li = lane & 31;
-    float* s_scale = reinterpret_cast<float*>(smem + NWN * NWM * kSlice);
-    float* s_bias = s_scale + 64 * NWN;
+    const float* s_scale = reinterpret_cast<const float*>(smem + i8_stages_smem<NWN, NWM, TM>());
+    const float* s_bias = s_scale + 64 * NWN;
+    const float* s_act = s_bias + 64 * NWN;
+    float as[TM];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) as[t] = s_act[32 * (wm * TM + t) + li];
     __syncthreads();  // every wave is done with the stages
-    for (int i = tid; i < 64 * NWN; i += kThreads) {
-        const int n = min(n0 + i, pb.N - 1);
-        s_scale[i] = pb.w_scale[n];
-        s_bias[i] = pb.bias ? pb.bias[n] : 0.0f;
-    }
-    __syncthreads();
     char* slice = smem + wave * kSlice;
+    // 16-byte chunk c of row r sits in place c ^ swizzle(r): two rows of 128 bytes, or one of 256, are
+    // all the banks
+    auto swizzle = [](int row) { return YDT == NSOSX_F32 ? row & 15 : (row >> 1) & 7; };
     const int nw = n0 + 64 * wn;
     const bool whole = nw + 64 <= pb.N && pb.N % (16 / kSize) == 0 &&
                        (reinterpret_cast<uintptr_t>(y) & 15) == 0;
+    // the scales and biases of this lane's outputs, once for all TM tiles (a ds_read_b128 takes 16
+    // clocks however many lanes share an address; read for each tile they were most of the epilogue)
+    float4 sc[8], bs[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        sc[c] = *reinterpret_cast<const float4*>(s_scale + 64 * wn + 8 * c + 4 * g);
+        bs[c] = BIAS ? *reinterpret_cast<const float4*>(s_bias + 64 * wn + 8 * c + 4 * g) : float4{};
+    }
 #pragma unroll
     for (int t = 0; t < TM; ++t) {
         const int mt = m0 + 32 * (wm * TM + t);
         if (mt >= rows.count) break;
-        const float as = rows.act_scale[i8_source(rows, rows.begin + min(mt + li, rows.count - 1))];
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4) {
                 const int at = 32 * nb + 8 * q4 + 4 * g;  // of the wave's 64 outputs
-                const float4 sc = *reinterpret_cast<const float4*>(s_scale + 64 * wn + at);
-                const float4 bs = *reinterpret_cast<const float4*>(s_bias + 64 * wn + at);
+                const float4 s4 = sc[4 * nb + q4], b4 = bs[4 * nb + q4];
                 const i32x16& a = acc[nb][t];
-                const float o0 = i8_affine(a[4 * q4], as, sc.x, bs.x, pb.sqrelu);
-                const float o1 = i8_affine(a[4 * q4 + 1], as, sc.y, bs.y, pb.sqrelu);
-                const float o2 = i8_affine(a[4 * q4 + 2], as, sc.z, bs.z, pb.sqrelu);
-                const float o3 = i8_affine(a[4 * q4 + 3], as, sc.w, bs.w, pb.sqrelu);
-                const int chunk = at * kSize / 16;
-                char* dst = slice + li * kRow + ((chunk ^ (li & (kChunks - 1))) << 4);
+                const float o0 = i8_affine<BIAS, SQRELU>(a[4 * q4], as[t], s4.x, b4.x);
+                const float o1 = i8_affine<BIAS, SQRELU>(a[4 * q4 + 1], as[t], s4.y, b4.y);
+                const float o2 = i8_affine<BIAS, SQRELU>(a[4 * q4 + 2], as[t], s4.z, b4.z);
+                const float o3 = i8_affine<BIAS, SQRELU>(a[4 * q4 + 3], as[t], s4.w, b4.w);
+                char* dst = slice + li * kRow + ((at * kSize / 16 ^ swizzle(li)) << 4);
                 if constexpr (YDT == NSOSX_F32)
                     *reinterpret_cast<float4*>(dst) = make_float4(o0, o1, o2, o3);
                 else
@@ -378,7 +425,7 @@ __device__ __forceinline__ void i8_epilogue(const I8Problem& pb, const I8Rows& r
             for (int i = 0; i < 32 * kChunks / 64; ++i) {
                 const int row = i * (64 / kChunks) + lane / kChunks;
                 const u32x4 v = *reinterpret_cast<const u32x4*>(
-                    slice + row * kRow + ((c ^ (row & (kChunks - 1))) << 4));
+                    slice + row * kRow + ((c ^ swizzle(row)) << 4));
                 if (mt + row < rows.count)
                     __builtin_nontemporal_store(
                         v, reinterpret_cast<u32x4*>(static_cast<char*>(y) +
@@ -389,7 +436,7 @@ __device__ __forceinline__ void i8_epilogue(const I8Problem& pb, const I8Rows& r
             const int last = min(32, rows.count - mt);
             for (int row = 0; row < last; ++row) {
                 const char* src = slice + row * kRow +
-                                  ((((lane * kSize) / 16) ^ (row & (kChunks - 1))) << 4) +
+                                  ((((lane * kSize) / 16) ^ swizzle(row)) << 4) +
                                   (lane * kSize) % 16;
                 if (nw + lane < pb.N) {
                     const int64_t at = (int64_t)(rows.begin + mt + row) * pb.N + nw + lane;
@@ -401,6 +448,21 @@ __device__ __forceinline__ void i8_epilogue(const I8Problem& pb, const I8Rows& r
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the next tile's writes
+    }
+}
+
+// (The branch on bias and activation is out here: inside, every output formed both and chose, and
+// the epilogue's 9 operations an output, where 4 do, were 7 us of a 256 x 256 tile.)
+template <int YDT, int NWN, int NWM, int TM>
+__device__ __forceinline__ void i8_epilogue(const I8Problem& pb, const I8Rows& rows, int n0, int m0,
+                                            void* __restrict__ y, char* smem,
+                                            const i32x16 (&acc)[2][TM]) {
+    if (pb.sqrelu) {
+        if (pb.bias) i8_epilogue_as<YDT, NWN, NWM, TM, true, true>(pb, rows, n0, m0, y, smem, acc);
+        else i8_epilogue_as<YDT, NWN, NWM, TM, false, true>(pb, rows, n0, m0, y, smem, acc);
+    } else {
+        if (pb.bias) i8_epilogue_as<YDT, NWN, NWM, TM, true, false>(pb, rows, n0, m0, y, smem, acc);
+        else i8_epilogue_as<YDT, NWN, NWM, TM, false, false>(pb, rows, n0, m0, y, smem, acc);
     }
 }
 
@@ -447,6 +509,7 @@ __device__ __forceinline__ void i8_tile(const I8Problem& pb, const I8Rows& rows,
 #pragma unroll
         for (int b = 0; b < TM; ++b) acc[a][b] = i32x16{};
     fetch(0);
+    i8_stage_scales<NWN, NWM, TM>(pb, rows, n0, m0, smem);
     put(0);
     if (KT > 1) fetch(1);
     __syncthreads();
@@ -548,23 +611,30 @@ __device__ __forceinline__ void i8_wide_tile(const I8Problem& pb, const I8Rows& 
         asm volatile("" ::: "memory");
     };
     const int KT = pb.K / kI8BK;
+    // a wave without outputs loads and meets with the others, and leaves the rest to them
+    const bool busy = m0 + 32 * TM * wm < rows.count && n0 + 64 * wn < pb.N;
+    if (KT > 0) issue(0);
+    i8_stage_scales<NWN, NWM, TM>(pb, rows, n0, m0, smem);
     if (KT > 0) {
-        issue(0);
         meet();
         if (KT > 1) issue(1);
-        read(0, 0, 0);
+        if (busy) read(0, 0, 0);
     }
     for (int kt = 0; kt < KT; ++kt) {
-        read(kt, 1, 1);
-        mul(0);
-        read(kt, 2, 0);
-        mul(1);
-        read(kt, 3, 1);
-        mul(0);
+        if (busy) {
+            read(kt, 1, 1);
+            mul(0);
+            read(kt, 2, 0);
+            mul(1);
+            read(kt, 3, 1);
+            mul(0);
+        }
         meet();
         if (kt + 2 < KT) issue(kt + 2);
-        if (kt + 1 < KT) read(kt + 1, 0, 0);
-        mul(1);
+        if (busy) {
+            if (kt + 1 < KT) read(kt + 1, 0, 0);
+            mul(1);
+        }
     }
     if (KT * kI8BK < pb.K) {
         // the last stage is not whole: through registers, zeros past K.  (Every wave has read every
