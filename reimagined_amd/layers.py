@@ -8,6 +8,11 @@
   MoEFFN             MoERouter::forward from logits + JambaBlock::forward_moe
                      (src/jamba.cpp:3692-3973, 8140-8319): device routing,
                      grouped ternary GEMMs, squared ReLU, weighted combine
+  Int8Linear         a linear layer on int8 weights with a scale per output channel, for
+                     layers that ternary weights cost too much and float ones too long
+  Int8MoEFFN         the routed feed-forward with int8 experts behind a scored router
+                     (softmax or sigmoid scores, balance bias, expert groups), and the
+                     gradients that train that router
   HybridBlock        JambaBlock::forward (src/jamba.cpp:3158-3375) for a Mamba
                      core and an MoE feed-forward: block norms, residual adds
 
@@ -322,6 +327,94 @@ class MoEFFN:
         return {"out": out, "weights": b["weights"], "selected": b["selected"], "workspace": ws}
 
 
+def quantize_weights_i8(w, device="cuda") -> tuple:
+    """A float weight matrix [N, K] (or [E, N, K]) as int8 codes and a scale per output channel:
+    w's rows through the activation quantizer (absmax over the row, 127 steps to each side)."""
+    t = torch.as_tensor(np.ascontiguousarray(w, np.float32) if isinstance(w, np.ndarray) else w,
+                        dtype=torch.float32).to(device).contiguous()
+    if t.dim() < 2 or not t.numel():
+        raise ValueError("quantize_weights_i8: w must be [outputs, inputs] or [experts, outputs, inputs]")
+    q, s = ops.quantize_activations_bitnet(t.view(-1, t.shape[-1]))
+    return q.view(t.shape), s.view(t.shape[:-1])
+
+
+class Int8Linear:
+    """y = x @ w^T (+ bias) with int8 weights, a scale per output channel, and int8 activations, a
+    scale per token: the quantizer of BitLinear, then the int8 product.
+
+    rms_input: BitLinear's RMS_PERI input norm (eps 1e-6), off by default."""
+
+    def __init__(self, w_float, device="cuda", bias=None, rms_input: bool = False):
+        self.w, self.w_scale = quantize_weights_i8(w_float, device)
+        if self.w.dim() != 2:
+            raise ValueError("Int8Linear: w must be [outputs, inputs]")
+        self.out_features, self.in_features = self.w.shape
+        self.bias = None if bias is None else torch.as_tensor(bias, dtype=torch.float32).to(device)
+        self.rms_input = rms_input
+
+    def forward(self, x: torch.Tensor, out_dtype=None) -> torch.Tensor:
+        q, s = ops.quantize_activations_bitnet(x, rms_input=self.rms_input)
+        return ops.int8_gemm(q, s, self.w, self.w_scale, bias=self.bias, out_dtype=out_dtype or x.dtype)
+
+
+class Int8MoEFFN:
+    """Routed feed-forward with int8 experts: scored routing, int8 codes of the rows, per expert
+    up -> squared ReLU -> int8 codes -> down, and the combine by the routing's weights.
+
+    w_up [E, d_ff, d_model], w_down [E, d_model, d_ff] (arrays, tensors or lists of matrices);
+    score, groups, group_keep, group_best, renorm, scale as ops.moe_route_scored, balance_bias
+    [E] its bias (a device tensor that a training loop may update between steps).  A drop-in for
+    MoEFFN in HybridBlock(moe=...).  Nothing is kept between calls but the weights."""
+
+    def __init__(self, w_up, w_down, device="cuda", k: int = 2, score: str = "softmax",
+                 balance_bias=None, groups: int = 1, group_keep: int | None = None,
+                 group_best: int = 2, renorm: bool = True, scale: float = 1.0,
+                 rms_input: bool = True, hidden_dtype=torch.float32):
+        stack = lambda w: np.stack([np.asarray(m, np.float32) for m in w]) if isinstance(w, list) else w
+        self.up, self.up_scale = quantize_weights_i8(stack(w_up), device)
+        self.down, self.down_scale = quantize_weights_i8(stack(w_down), device)
+        self.experts, self.d_ff, self.d_model = self.up.shape
+        if tuple(self.down.shape) != (self.experts, self.d_model, self.d_ff):
+            raise ValueError("Int8MoEFFN: w_up [E, d_ff, d_model] and w_down [E, d_model, d_ff] must agree")
+        self.k = k
+        self.routing = dict(score=score, groups=groups, group_keep=group_keep, group_best=group_best,
+                            renorm=renorm, scale=scale)
+        self.balance_bias = (None if balance_bias is None else
+                             torch.as_tensor(balance_bias, dtype=torch.float32).to(device))
+        self.rms_input = rms_input
+        self.hidden_dtype = hidden_dtype
+
+    def forward(self, x: torch.Tensor, logits: torch.Tensor, out_dtype=None, valid_rows=None) -> dict:
+        """x [rows, d_model], router logits [rows, E] -> {"out" [rows, d_model], the routing's
+        tensors, "h" the experts' hidden rows and "o" their output rows in slot order}.
+        valid_rows: the 0/1 padding mask; padding rows take no slots and come out as zeros."""
+        if logits.shape != (x.shape[0], self.experts):
+            raise ValueError(f"Int8MoEFFN: logits must be [{x.shape[0]}, {self.experts}], got "
+                             f"{tuple(logits.shape)}")
+        r = ops.moe_route_scored(logits, self.k, bias=self.balance_bias, valid_rows=valid_rows,
+                                 **self.routing)
+        q, s = ops.quantize_activations_bitnet(x, rms_input=self.rms_input)
+        h = ops.grouped_int8_gemm(q, s, self.up, self.up_scale, r["offsets"], perm=r["perm"],
+                                  squared_relu=True, out_dtype=self.hidden_dtype)
+        # (hidden rows past offsets[E], a padded batch's, are whatever was there: their codes are
+        # made and no expert reads them)
+        q, s = ops.quantize_activations_bitnet(h, rms_input=self.rms_input)
+        o = ops.grouped_int8_gemm(q, s, self.down, self.down_scale, r["offsets"],
+                                  out_dtype=torch.float32)
+        out = ops.moe_combine_topk(o, r["slot_of"], r["weights"], out_dtype=out_dtype or x.dtype)
+        return {"out": out, **r, "h": h, "o": o}
+
+    def router_backward(self, logits: torch.Tensor, fwd: dict, dout: torch.Tensor) -> dict:
+        """Gradients of what forward() combined, from that of its "out": dlogits (the router's; the
+        balance bias has none), dweights [rows, k] and do, of the experts' output rows "o"."""
+        do, dw = ops.moe_combine_topk_backward(dout, fwd["o"], fwd["slot_of"], fwd["weights"],
+                                               perm=fwd["perm"])
+        r = self.routing
+        dlogits = ops.moe_route_scored_backward(logits, fwd["selected"], dw, score=r["score"],
+                                                renorm=r["renorm"], scale=r["scale"])
+        return {"dlogits": dlogits, "dweights": dw, "do": do}
+
+
 class HybridBlock:
     """JambaBlock::forward with a Mamba core and an MoE feed-forward (src/jamba.cpp:3158-3375):
 
@@ -336,15 +429,16 @@ class HybridBlock:
     sensitive unless NSOS_MOE_FP_ROUTER=0 (src/jamba.cpp:8086-8098), so by default it is
     BitLinear's float path: rmsnorm(f, 1e-6) @ gate_w^T * gate_magnitude (+ gate_bias);
     ternary_gate=True builds the ternary BitLinear instead (the NSOS_MOE_FP_ROUTER=0
-    behaviour).
+    behaviour).  moe: a feed-forward to use in place of MoEFFN(w_up, w_down, k=k), an
+    Int8MoEFFN for one; w_up and w_down may then be None.
     """
 
     def __init__(self, mamba_params: dict, w_up: list, w_down: list, device="cuda", k: int = 2,
                  core_gamma=None, ff_gamma=None, gate_w=None, core_eps: float = 1e-6,
                  ff_eps: float = 1e-6, gate_magnitude=None, gate_bias=None,
-                 ternary_gate: bool = False):
+                 ternary_gate: bool = False, moe=None):
         self.mamba = HybridMambaLayer(mamba_params, device)
-        self.moe = MoEFFN(w_up, w_down, device, k=k)
+        self.moe = MoEFFN(w_up, w_down, device, k=k) if moe is None else moe
         f32 = dict(dtype=torch.float32, device=device)
         self.core_gamma = None if core_gamma is None else torch.as_tensor(core_gamma, **f32)
         self.ff_gamma = None if ff_gamma is None else torch.as_tensor(ff_gamma, **f32)
