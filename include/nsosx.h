@@ -574,8 +574,8 @@ int nsosx_moe_sparse_decode(const nsosx_linear_view* up_views,
  *   the k largest c of the groups that stay are chosen (selected, in that order);
  *   weights[r, i] = s of choice i, divided by the sum over the row's choices where renorm != 0,
  *   times scale.  The bias takes part in the choice only.
- * Choices are those of the values in 64 bits, ties to the lower index (groups too); with
- * neither a bias nor two values a group the order of c is that of x.  An expert whose logit
+ * Choices are those of the values in 64 bits, ties to the lower index (groups too); without a
+ * bias the order of c is that of x.  An expert whose logit
  * (or c) is -inf is not available: a row with fewer than k available experts gets -1 and weight
  * 0 for the rest.  A row with a NaN score gets the first k experts and NaN weights.
  *   valid_rows uint8 [rows] or NULL: a row whose byte is 0 is padding (as nsosx_moe_route's):

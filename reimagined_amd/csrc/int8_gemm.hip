@@ -114,16 +114,20 @@ static void launch_grouped_t(const I8Group& gp, void* y, hipStream_t st) {
                        st, gp, y);
 }
 
-// Which tile takes a shape: the estimated time of each in us, fitted to a sweep of K 512 .. 8192,
-// N 768 .. 8192 and 1 .. 4096 rows with the weights from HBM (within 9 % of the measured times on
-// average, and the choice within 1 % of the best one's time, 15 % at most): a fixed part and one
-// per round of 256 tiles, both linear in K.  A round is a whole one where a compute unit holds one
-// workgroup.  Measured, us (16 x 16 / 16 x 64 / 32 x 64 / 64 x 64 / 128 x 128 / 256 x 256):
+// Which tile takes a shape: the estimated time of each in us, fitted to sweeps of K 64 .. 8192,
+// N 96 .. 8192 and 1 .. 8192 rows with the weights from HBM (within 9 % of the measured times on
+// average, and the choice within 1 % of the best one's time, 15 % at most, for K of 512 and more): a
+// fixed part and one per round of 256 tiles, linear in K but no less than the tile's outputs and its
+// start take.  A round is a whole one where a compute unit holds one workgroup.  Measured, us (16 x
+// 16 / 16 x 64 / 32 x 64 / 64 x 64 / 128 x 128 / 256 x 256):
 //   K 4096, N 4096:    1 row   5.1 /  5.9 /  6.8 / 10.0 / 21   / 47
 //                     64 rows 10.7 / 11.1 /  9.6 / 12.5 / 23   / 49
 //                    200 rows    - / 29   / 16.8 / 14.1 / 23   / 51
-//                   1024 rows    - /  -   / 52   / 48   / 27   / 52
-//                   4096 rows    - /  -   /  -   /  -   / 75   / 69
+//                   1024 rows    - /  -   / 52   / 48   / 26   / 52
+//                   4096 rows    - /  -   /  -   /  -   / 72   / 66
+//   K 64, N 4096:     16 rows  3.1 /  3.4 /  3.7 /  5.0 /  5.1 /  6.0
+//                    449 rows 26   / 18   /  7.4 /  9.4 /  6.4 /  8.7
+//                   8000 rows    - /  -   /  -   /  -   / 23   / 20
 // Rows that do not start on 16 bytes go through registers on the way to LDS, which costs every
 // tile about a quarter, and have no 256 x 256 one (2048 x 2009 -> 5125 on 128 x 128: 55 us).
 constexpr int64_t kI8MaxTiles = 1 << 24;  // of 128 x 128: 256 threads each, less than 2^32
@@ -136,12 +140,12 @@ static I8Tile choose_tile(int K, bool aligned, Tiles tiles) {
     auto part = [](double t) { return std::max(1.0, t / 256); };
     auto whole = [](double t) { return std::max(1.0, std::ceil(t / 256)); };
     const double cost[] = {
-        2.8 - 0.2 * k + part(tiles(16, 16)) * 0.63 * k,
-        1.7 - 0.65 * k + part(tiles(16, 64)) * (1.26 + 1.52 * k),
-        2.6 - 0.4 * k + whole(tiles(32, 64)) * (0.6 + 1.66 * k),
-        1.0 - 0.5 * k + whole(tiles(64, 64)) * (3.25 + 2.43 * k),
-        2.7 + 0.8 * k + part(tiles(128, 128)) * (1.2 + 4.2 * k),
-        whole(tiles(256, 256)) * (6.8 + 14.7 * k),
+        2.8 - 0.2 * k + part(tiles(16, 16)) * std::max(0.8, 0.63 * k),
+        1.7 - 0.65 * k + part(tiles(16, 64)) * std::max(2.0, 1.26 + 1.52 * k),
+        2.6 - 0.4 * k + whole(tiles(32, 64)) * std::max(1.4, 0.6 + 1.66 * k),
+        1.0 - 0.5 * k + whole(tiles(64, 64)) * std::max(4.0, 3.25 + 2.43 * k),
+        2.7 + 0.8 * k + part(tiles(128, 128)) * std::max(2.6, 1.2 + 4.2 * k),
+        whole(tiles(256, 256)) * std::max(10.0, 6.8 + 14.7 * k),
     };
     // a launch holds less than 2^32 threads (tiles of 16 rows: 512 each): the larger ones always do
     const bool fits[] = {tiles(16, 16) < 4e6, tiles(16, 64) < 4e6, tiles(32, 64) < 8e6,

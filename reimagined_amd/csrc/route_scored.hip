@@ -23,11 +23,16 @@ struct RouteScored {
     int32_t* slot_of;        // [rows, k]
     int32_t* block_counts;   // workspace [E, blocks], or [blocks, E] where by_block
     int by_block;
+    int size, lanes, run;    // experts of a group, lanes that share them (a power of two), of a lane
+    int pitch;               // of a row in LDS, floats
 };
 
 // ---- sixteen lanes per row -----------------------------------------------------
-// A row's experts lie on the 16 lanes of a DPP row, expert 16 v + l in value v of lane l, so
-// that four rows share a wave and every reduction over a row is four rotations.
+// A row's experts lie on the 16 lanes of a DPP row, so that four rows share a wave and every
+// reduction over a row is four rotations: expert 16 v + l in value v of lane l or, where the
+// choice is limited to groups, each group on `lanes` neighbouring lanes of its own, a run of its
+// experts each, so that a group's score is a reduction over those lanes.  The row then goes through
+// LDS: loaded in runs, 64 lanes meet 64 cache lines a time (16384 rows of 256: 7 us more).
 
 template <int N>
 __device__ __forceinline__ uint32_t ror16(uint32_t v) {
@@ -60,17 +65,9 @@ __device__ __forceinline__ bool row_any(bool p) {
     return ((__ballot(p) >> (threadIdx.x & 48)) & 0xFFFF) != 0;
 }
 
-// The two largest of a row from each lane's two largest (a >= b).
-template <int N>
-__device__ __forceinline__ void merge2(float& a, float& b) {
-    const float oa = ror16<N>(a), ob = ror16<N>(b);
-    b = larger(fminf(a, oa), larger(b, ob));
-    a = larger(a, oa);
-}
-
-// This lane's values of a row of E floats: expert 16 v + l, -inf past E or where the row is not
-// live.  (Every load is made, from the last expert where there is none: a branch around each
-// would wait for each.)
+// This lane's values of a row of E floats, expert 16 v + l in value v, -inf past E or where the row
+// is not live.  (Every load is made, from the last expert where there is none: a branch around
+// each would wait for each.)
 template <int V, int DT>
 __device__ __forceinline__ void row_values(const void* x, int64_t base, int E, bool live, float (&c)[V]) {
     const int l = threadIdx.x & 15;
@@ -80,127 +77,65 @@ __device__ __forceinline__ void row_values(const void* x, int64_t base, int E, b
     for (int v = 0; v < V; ++v) c[v] = live && 16 * v + l < E ? c[v] : -INFINITY;
 }
 
-// Score of group `q` (its best one or two values in c; unavailable experts, -inf, add nothing),
-// the same in every lane of the row; -inf where no expert of it is available.
+// Floats first .. first + n - 1 of a row in LDS, -inf behind them; in 16-byte pieces where every
+// lane's run allows it.
 template <int V>
-__device__ __forceinline__ float group_score(const float (&c)[V], int q, int size, int best) {
-    const float none = -INFINITY;
-    const int l = threadIdx.x & 15;
-    float a = none, b = none;
+__device__ __forceinline__ void run_values(const float* row, int first, int n, bool pieces, float (&c)[V]) {
+    if (pieces && V >= 4) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        if (16 * v + 15 < q * size || 16 * v >= (q + 1) * size) continue;
-        const int e = 16 * v + l;
-        const float x = e >= q * size && e < (q + 1) * size ? c[v] : none;
-        b = larger(b, fminf(a, x));
-        a = larger(a, x);
-    }
-    merge2<8>(a, b);
-    merge2<4>(a, b);
-    merge2<2>(a, b);
-    merge2<1>(a, b);
-    return best == 2 && b > none ? a + b : a;
-}
-
-template <int N>
-__device__ __forceinline__ void outranked(float s, int l, int& rank) {
-    const float o = ror16<N>(s);
-    const int ol = ror16<N>(l);
-    rank += o > s || (o == s && ol < l) ? 1 : 0;
-}
-
-// Rank of lane l's value among the row's 16 (ties to the lower index).
-__device__ __forceinline__ int row_rank(float s, int index) {
-    int rank = 0;
-    outranked<1>(s, index, rank); outranked<2>(s, index, rank); outranked<3>(s, index, rank);
-    outranked<4>(s, index, rank); outranked<5>(s, index, rank); outranked<6>(s, index, rank);
-    outranked<7>(s, index, rank); outranked<8>(s, index, rank); outranked<9>(s, index, rank);
-    outranked<10>(s, index, rank); outranked<11>(s, index, rank); outranked<12>(s, index, rank);
-    outranked<13>(s, index, rank); outranked<14>(s, index, rank); outranked<15>(s, index, rank);
-    return rank;
-}
-
-// Up to 8 groups of 16 VS experts each (VS values of every lane): the score of group l / 2 in lane
-// l.  Each step exchanges halves (lanes 8 apart take groups 0 .. 3 or 4 .. 7, and so on), so that 8
-// groups cost 8 merges where a reduction each costs 32 (16384 rows of 256 experts in 8 groups:
-// 18.9 -> @@ us with the rest of the choice).
-template <int CTRL>
-__device__ __forceinline__ float lane_move(float v) {
-    return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(v), CTRL, 0xF, 0xF, true));
-}
-__device__ __forceinline__ void join2(float& a, float& b, float oa, float ob) {
-    b = larger(fminf(a, oa), larger(b, ob));
-    a = larger(a, oa);
-}
-template <int CTRL, int N>
-__device__ __forceinline__ void exchange_halves(float (&a)[8], float (&b)[8], bool upper) {
-#pragma unroll
-    for (int q = 0; q < N / 2; ++q) {
-        const float a0 = a[q], a1 = a[q + N / 2], b0 = b[q], b1 = b[q + N / 2];
-        const float oa = lane_move<CTRL>(upper ? a0 : a1), ob = lane_move<CTRL>(upper ? b0 : b1);
-        a[q] = upper ? a1 : a0;
-        b[q] = upper ? b1 : b0;
-        join2(a[q], b[q], oa, ob);
-    }
-}
-template <int VS, int V>
-__device__ __forceinline__ float group_scores(const float (&c)[V], int best) {
-    const float none = -INFINITY;
-    const int l = threadIdx.x & 15;
-    float a[8], b[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-        a[q] = b[q] = none;
-#pragma unroll
-        for (int v = q * VS; v < (q + 1) * VS && v < V; ++v) {
-            b[q] = larger(b[q], fminf(a[q], c[v]));
-            a[q] = larger(a[q], c[v]);
+        for (int v = 0; v + 3 < V; v += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(row + first + (v < n ? v : 0));
+            c[v] = f.x; c[v + 1] = f.y; c[v + 2] = f.z; c[v + 3] = f.w;
         }
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) c[v] = row[first + (v < n ? v : 0)];
     }
-    exchange_halves<0x128, 8>(a, b, l & 8);  // lane l ^ 8
-    exchange_halves<0x141, 4>(a, b, l & 4);  // lane l ^ 7
-    exchange_halves<0x1B, 2>(a, b, l & 2);   // lane l ^ 3
-    join2(a[0], b[0], lane_move<0xB1>(a[0]), lane_move<0xB1>(b[0]));  // lane l ^ 1
-    return best == 2 && b[0] > none ? a[0] + b[0] : a[0];
+#pragma unroll
+    for (int v = 0; v < V; ++v) c[v] = v < n ? c[v] : -INFINITY;
 }
 
+template <int CTRL>
+__device__ __forceinline__ void join2(float& a, float& b) {
+    const float oa = __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(a), CTRL, 0xF, 0xF, true));
+    const float ob = __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(b), CTRL, 0xF, 0xF, true));
+    b = fmaxf(fminf(a, oa), fmaxf(b, ob));
+    a = fmaxf(a, oa);
+}
+template <int N>
+__device__ __forceinline__ void outranked(float s, int q, int& lanes) {
+    const float o = ror16<N>(s);
+    const int oq = ror16<N>(q);
+    lanes += o > s || (o == s && oq < q) ? 1 : 0;
+}
 __device__ __forceinline__ float row_min(float v) { return -row_max(-v); }
 
-// Bit q of the result: group q is one of the `keep` best (ties to the lower group).  gap: what
-// the worst group that stays has over the best one that goes.
+// Whether this lane's group is one of the `keep` best (ties to the lower group), from the values of
+// its experts; -inf, an unavailable expert, adds nothing.  gap: what the worst group that stays has
+// over the best one that goes.
 template <int V>
-__device__ __forceinline__ uint32_t kept_groups(const float (&c)[V], const RouteScored& p, float& gap) {
+__device__ __forceinline__ bool group_stays(const RouteScored& p, const float (&c)[V], int q, float& gap) {
     const float none = -INFINITY;
-    const int l = threadIdx.x & 15;
-    const int size = p.E / p.groups;
-    float s = none;
-    int group = l;  // whose score s is
-    const int values = size % 16 == 0 && p.groups <= 8 ? size / 16 : 0;
-    if (values == 1 || values == 2 || values == 4 || values == 8) {
-        s = values == 1 ? group_scores<1>(c, p.best) : values == 2 ? group_scores<2>(c, p.best)
-            : values == 4 ? group_scores<4>(c, p.best) : group_scores<8>(c, p.best);
-        group = l >> 1;
-        if (l & 1) s = none;  // (each score once)
-    } else {
-        for (int q = 0; q < p.groups; ++q) {
-            const float v = group_score<V>(c, q, size, p.best);
-            if (l == q) s = v;
-        }
-    }
-    // (an odd lane, which has no group, ranks behind the group of its neighbour)
-    const int rank = row_rank(s, values ? l : group);
-    bool in = group < p.groups && rank < p.keep;
-    uint32_t kept = 0;
-    if (values == 1 || values == 2 || values == 4 || values == 8) {
-        in = in && !(l & 1);
-        const uint32_t bits = (uint32_t)(__ballot(in) >> (threadIdx.x & 48)) & 0xFFFFu;
+    float a = none, b = none;  // the group's two largest
 #pragma unroll
-        for (int q = 0; q < 8; ++q) kept |= ((bits >> (2 * q)) & 1u) << q;
-    } else {
-        kept = (uint32_t)(__ballot(in) >> (threadIdx.x & 48)) & 0xFFFFu;
+    for (int v = 0; v < V; ++v) {
+        b = fmaxf(b, fminf(a, c[v]));
+        a = fmaxf(a, c[v]);
     }
+    if (p.lanes >= 2) join2<0xB1>(a, b);   // lane l ^ 1
+    if (p.lanes >= 4) join2<0x4E>(a, b);   // lane l ^ 2
+    if (p.lanes >= 8) join2<0x141>(a, b);  // lane l ^ 7: the other four of eight
+    float s = p.best == 2 && b > none ? a + b : a;
+    if (q >= p.groups) s = none;
+    int better = 0;  // lanes of better groups
+    outranked<1>(s, q, better); outranked<2>(s, q, better); outranked<3>(s, q, better);
+    outranked<4>(s, q, better); outranked<5>(s, q, better); outranked<6>(s, q, better);
+    outranked<7>(s, q, better); outranked<8>(s, q, better); outranked<9>(s, q, better);
+    outranked<10>(s, q, better); outranked<11>(s, q, better); outranked<12>(s, q, better);
+    outranked<13>(s, q, better); outranked<14>(s, q, better); outranked<15>(s, q, better);
+    const bool in = q < p.groups && better < p.keep * p.lanes;
     gap = row_min(in ? s : INFINITY) - row_max(in ? none : s);
-    return kept;
+    return in;
 }
 
 // exp(x) to a unit in 64 bits: x = n ln 2 + r with |r| <= ln 2 / 2, the Taylor sum of exp(r) to
@@ -240,35 +175,23 @@ __device__ __forceinline__ void softmax_stats(const float (&x)[V], float& mx, fl
     sum = row_sum(sum);
 }
 
-// -inf for the experts of the groups that go (bit q of kept: group q stays).
-template <int V>
-__device__ __forceinline__ void close_groups(const RouteScored& p, uint32_t kept, float (&c)[V]) {
-    const int size = p.E / p.groups;
-    const int l = threadIdx.x & 15;
-    int group = l / size, left = l % size;  // of expert 16 v + l, without a division each
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        if (!((kept >> group) & 1)) c[v] = -INFINITY;
-        left += 16;
-        while (left >= size) {
-            left -= size;
-            ++group;
-        }
-    }
-}
-
 // The choice by 32-bit scores, with a proof that it is the one of 64 bits: every value becomes a
-// 32-bit key, its distance from a point below the row's largest in fixed point (2 for scores, 32
-// for logits that are compared as they are) above the complement of its index, each lane sorts its
-// keys, and k + 1 rounds take the largest of the row's 16 first ones.  The choice stands where the
-// fixed-point values of neighbours in that order differ by more than the scores' error.  Where
-// they do not (about 2 of 10^4 rows of 256 sigmoid scores with a bias), where groups lie too close
-// together, values outside the window or a NaN in the row, the whole wave chooses for the row in 64
-// bits (select_wave).  bfloat16 logits compared as they are make exact keys.
+// 32-bit key, its distance from a point below the row's largest in fixed point (2 for scores with a
+// bias, 32 for logits, whose order is that of scores without one) above the complement of its
+// index, each lane sorts its keys, and k + 1 rounds take the largest of the row's 16 first ones.
+// The choice stands where the fixed-point values of neighbours in that order differ by more than
+// the scores' error.  Where they do not (about 2 of 10^4 rows of 256 sigmoid scores with a bias),
+// where groups lie too close together, values outside the window or a NaN in the row, the whole
+// wave chooses for the row in 64 bits (select_wave).  bfloat16 logits make exact keys.
 //
-// Errors: a sigmoid by exp2 and reciprocal of one unit each is off by s (1 - s) (|x| 2^-24 + 2^-23)
-// + s 1.5 2^-23 at most, below 1.7 2^-23; a softmax score by p (|x - max| 2^-23 + (V + 8) 2^-24),
-// below 2^-18 (p |x - max| <= 0.37); the sum with the bias by 2^-24 of the value.
+// What it takes is instructions: 16384 rows of 256 experts in 8 groups, sigmoid scores and a bias,
+// are 17 MB (3.3 us) and @@ us, where k rounds of a 64-bit maximum over the row took 41.
+//
+// Errors, in units u = 2^-23: a sigmoid by exp2 and reciprocal of one unit each is off by s (1 - s)
+// (|x| / 2 + 1) + 1.5 s, below 1.7 u.  A softmax score p = e / sum: e by |x - max| + 1 of itself,
+// the sum by (V + 4) / 2 + 1 and the weighted mean of |x - max|, at most ln 512, reciprocal and
+// product 1.5, and p |x - max| <= 0.37 of the largest p: below (13 + V / 2) u of that.  The sum with
+// the bias by half a unit of the value.
 // Batcher's odd-even merge sort, descending, of N keys from LO.
 template <int A, int B, int V>
 __device__ __forceinline__ void order_pair(uint32_t (&key)[V]) {
@@ -302,39 +225,61 @@ __device__ __forceinline__ void sort_keys(uint32_t (&key)[V]) {
     }
 }
 
-// Expert index of choice l in lane l (-1: none), where `sure`.
-template <int V, int DT>
-__device__ __forceinline__ int select_fast(const RouteScored& p, int64_t row, bool live, bool& sure) {
+// Expert index of choice l in lane l (-1: none), where `sure`.  G: limited to groups.
+// s_row, s_bias (G): this row's place in LDS, the biases there.
+template <int V, int DT, bool G>
+__device__ __forceinline__ int select_fast(const RouteScored& p, int64_t row, bool live, float* s_row,
+                                           const float* s_bias, bool& sure) {
     constexpr int IB = V == 2 ? 5 : V == 4 ? 6 : V == 8 ? 7 : V == 16 ? 8 : 9;  // bits of an index
     constexpr int NB = 32 - IB;
     constexpr uint32_t kIndex = (1u << IB) - 1;
     const float none = -INFINITY;
     const int l = threadIdx.x & 15;
-    const bool scored = p.bias || (p.groups > 1 && p.best == 2);
-    float c[V], b[V];
+    const int lanes = G ? max(p.lanes, 1) : 16;
+    const int q = G ? min(l / lanes, p.groups - 1) : 0, at = G ? l % lanes * p.run : l;
+    const bool real = !G || (p.lanes > 0 && l / lanes < p.groups);  // a lane with experts
+    // this lane's experts: first + v step
+    const int first = G ? q * p.size + (at < p.size ? at : 0) : l, step = G ? 1 : 16;
+    const bool scored = p.bias || (G && p.best == 2);
+    float x[V], c[V], b[V];
     bool odd = false;  // a NaN, or an infinite logit of a softmax
-    row_values<V, DT>(p.logits, row * p.stride, p.E, live, c);
-    if (p.bias) row_values<V, NSOSX_F32>(p.bias, 0, p.E, true, b);
+    row_values<V, DT>(p.logits, row * p.stride, p.E, live, x);
+    if (G) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (16 * v + l < p.E) s_row[16 * v + l] = x[v];
+        // the wave reads what its own lanes wrote
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        const int n = real ? min(p.run, p.size - at) : 0;
+        const bool pieces = p.size % 4 == 0 && p.run % 4 == 0;
+        run_values<V>(s_row, first, n, pieces, x);
+        if (p.bias) run_values<V>(s_bias, first, n, pieces, b);
+    } else if (p.bias) {
+        row_values<V, NSOSX_F32>(p.bias, 0, p.E, true, b);
+    }
     float err = 0.0f;
     if (!p.sigmoid) {
-        float mx = c[0];
+        float mx = x[0];
 #pragma unroll
-        for (int v = 1; v < V; ++v) mx = fmaxf(mx, c[v]);
+        for (int v = 1; v < V; ++v) mx = fmaxf(mx, x[v]);
         mx = row_max(mx);
         odd |= mx == INFINITY;
         if (scored) {
             float sum = 0.0f;
 #pragma unroll
-            for (int v = 0; v < V; ++v) sum += c[v] == none ? 0.0f : __expf(c[v] - mx);
+            for (int v = 0; v < V; ++v) {
+                c[v] = x[v] == none ? 0.0f : __expf(x[v] - mx);
+                sum += c[v];
+            }
             const float inv = __builtin_amdgcn_rcpf(row_sum(sum));
 #pragma unroll
-            for (int v = 0; v < V; ++v) c[v] = c[v] == none ? none : __expf(c[v] - mx) * inv;
-            err = 0x1p-18f;
+            for (int v = 0; v < V; ++v) c[v] = x[v] == none ? none : c[v] * inv;
+            err = inv * (0x1p-23f * (13.0f + V / 2));
         }
     } else if (scored) {
 #pragma unroll
         for (int v = 0; v < V; ++v)
-            c[v] = c[v] == none ? none : __builtin_amdgcn_rcpf(1.0f + __expf(-c[v]));
+            c[v] = x[v] == none ? none : __builtin_amdgcn_rcpf(1.0f + __expf(-x[v]));
         err = 0x1p-22f;
     }
     if (p.bias) {
@@ -344,42 +289,52 @@ __device__ __forceinline__ int select_fast(const RouteScored& p, int64_t row, bo
     float mx = none;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
+        if (!scored) c[v] = x[v];
         odd |= c[v] != c[v];
         mx = fmaxf(mx, c[v]);
     }
     mx = row_max(mx);
     odd |= mx == INFINITY;
     if (scored) err += 0x1p-23f * fabsf(mx);
-    bool ok = true;
-    if (p.groups > 1) {
+    bool ok = true, open = true;
+    if (G) {
         float gap;
-        const uint32_t kept = kept_groups<V>(c, p, gap);
+        open = group_stays<V>(p, c, l / lanes, gap);
         ok = err == 0.0f || gap > 6.0f * err;  // two errors a group, the sums' rounding one more
-        close_groups<V>(p, kept, c);
     }
+    if (!p.bias) {  // the experts by their logits
+        mx = none;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            c[v] = x[v];
+            mx = fmaxf(mx, open ? c[v] : none);
+        }
+        mx = row_max(mx);
+    }
+    const bool keyed = p.bias != nullptr;
     uint32_t key[V];
     uint32_t apart = 1;  // by how much fixed-point neighbours have to differ
     constexpr bool kExact = DT == NSOSX_BF16;
-    const bool exact = kExact && !scored;
+    const bool exact = kExact && !keyed;
     if (exact) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             // (adding +0 turns -0 into +0: equal values make equal keys)
             const uint32_t u = __float_as_uint(c[v] + 0.0f) >> 16;
             const uint32_t o = u & 0x8000u ? ~u & 0xFFFFu : u | 0x8000u;
-            key[v] = c[v] == none ? 0u : (o << 16) | (0xFFFFu - (16 * v + l));
+            key[v] = open && c[v] != none ? (o << 16) | (0xFFFFu - (first + v * step)) : 0u;
         }
     } else {
-        const float scale = scored ? (float)(1u << (NB - 1)) : (float)(1u << (NB - 5));
-        const float base = mx - (scored ? 2.0f : 32.0f);
+        const float scale = keyed ? (float)(1u << (NB - 1)) : (float)(1u << (NB - 5));
+        const float base = mx - (keyed ? 2.0f : 32.0f);
         const float top = (float)(1u << NB) - (NB > 24 ? (float)(1u << (NB - 24)) : 1.0f);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const float t = fminf(fmaxf((c[v] - base) * scale, 0.0f), top);
-            key[v] = c[v] == none ? 0u : ((uint32_t)t << IB) | (kIndex - (16 * v + l));
+            key[v] = open && c[v] != none ? ((uint32_t)t << IB) | (kIndex - (first + v * step)) : 0u;
         }
         // both values' errors, the difference's and the product's rounding, the truncation
-        if (scored) apart = (uint32_t)fminf(2.0f * err * scale, 1e9f) + (1u << (NB > 24 ? NB - 23 : 1)) + 2;
+        if (keyed) apart = (uint32_t)fminf(2.0f * err * scale, 1e9f) + (1u << (NB > 24 ? NB - 23 : 1)) + 2;
     }
     sort_keys<0, V>(key);
     auto take = [&] {  // the row's largest key, out of its lane's list
@@ -459,14 +414,16 @@ __device__ __forceinline__ int select_wave(const RouteScored& p, int64_t row, bo
     const double none = -(double)INFINITY;
     const int lane = threadIdx.x & 63;
     const bool scored = p.bias || (p.groups > 1 && p.best == 2);
+    float x[W];
     double c[W];
     bool nan = false;
 #pragma unroll
     for (int v = 0; v < W; ++v) {
         const int e = 64 * v + lane;
-        const float x = load_act<DT>(p.logits, row * p.stride + min(e, p.E - 1));
-        nan |= x != x;
-        c[v] = e < p.E ? (double)x : none;
+        x[v] = load_act<DT>(p.logits, row * p.stride + min(e, p.E - 1));
+        x[v] = e < p.E ? x[v] : -INFINITY;
+        nan |= x[v] != x[v];
+        c[v] = (double)x[v];
     }
     if (p.sigmoid) {
         if (scored) {
@@ -509,9 +466,9 @@ __device__ __forceinline__ int select_wave(const RouteScored& p, int64_t row, bo
 #pragma unroll
             for (int v = 0; v < W; ++v) {
                 const int e = 64 * v + lane;
-                const double x = e >= q * size && e < (q + 1) * size ? c[v] : none;
-                b = fmax(b, fmin(a, x));
-                a = fmax(a, x);
+                const double u = e >= q * size && e < (q + 1) * size ? c[v] : none;
+                b = fmax(b, fmin(a, u));
+                a = fmax(a, u);
             }
             wave_max2(a, b);
             if (lane == q) s = p.best == 2 && b > none ? a + b : a;
@@ -525,6 +482,7 @@ __device__ __forceinline__ int select_wave(const RouteScored& p, int64_t row, bo
 #pragma unroll
         for (int v = 0; v < W; ++v) {
             const int e = 64 * v + lane;
+            if (!p.bias) c[v] = (double)x[v];  // the experts by their logits
             if (e < p.E && !((kept >> (e / size)) & 1)) c[v] = none;
         }
     }
@@ -612,21 +570,25 @@ __device__ __forceinline__ void scan_counts(const int32_t* counts, int E, int32_
 
 // A workgroup of 16 RB threads routes RB rows, ranks them per expert through 64-bit row masks
 // and leaves its counts per expert, or, where it is the only one, the whole dispatch.
-template <int V, int DT>
+template <int V, int DT, bool G>
 __global__ __launch_bounds__(V > 16 ? 512 : 1024) void route_scored_kernel(RouteScored p) {
     __shared__ uint64_t s_mask[kScoredMaxExperts];
     __shared__ int32_t s_cnt[kScoredMaxExperts], s_off[kScoredMaxExperts + 1];
     const int l = threadIdx.x & 15, rl = threadIdx.x >> 4;
     const int row = blockIdx.x * (blockDim.x >> 4) + rl;
+    extern __shared__ __align__(16) float s_rows[];  // G: a row each, and the biases
+    float* s_bias = s_rows + (blockDim.x >> 4) * p.pitch;
     const bool dispatch = p.counts != nullptr;
-    if (dispatch) {
-        for (int e = threadIdx.x; e < p.E; e += blockDim.x) s_mask[e] = 0;
-        __syncthreads();
+    for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
+        if (dispatch) s_mask[e] = 0;
+        if (G && p.bias) s_bias[e] = p.bias[e];
     }
+    __syncthreads();
     const int in = min(row, p.rows - 1);  // a row to read, past the last one too
     const bool live = row < p.rows && (!p.valid || p.valid[in] != 0);
     bool bad = false, sure;
-    int mine = select_fast<V, DT>(p, in, live, sure);
+    int mine = select_fast<V, DT, G>(p, in, live, s_rows + rl * p.pitch, s_bias, sure);
+    if (G && p.lanes == 0) sure = !live;  // groups that the lanes cannot hold
     for (uint64_t left = __ballot(!sure && l == 0); left; left &= left - 1) {
         const int first = __builtin_ctzll(left);
         bool wrong;
@@ -870,10 +832,21 @@ __global__ __launch_bounds__(256) void route_scored_bwd_kernel(RouteScoredBwd p)
         store_act<DT>(p.dlogits, first + i, s_g[i]);
 }
 
-static int scored_block_rows(int rows, int E) {
+// Lanes of each group and values of a lane where G groups of `size` experts share 16 lanes.
+struct ScoredLayout {
+    int lanes, values;
+};
+static ScoredLayout scored_layout(int E, int groups) {
+    int lanes = 16;
+    while (lanes * groups > 16) lanes /= 2;
+    return {lanes, (E / groups + lanes - 1) / lanes};
+}
+
+// wide: lanes of 32 values, whose kernel has the registers of half as many threads.
+static int scored_block_rows(int rows, bool wide) {
     if (rows <= 16) return 16;
     if (rows <= 32) return 32;
-    const int most = E > 256 ? 32 : 64;
+    const int most = wide ? 32 : 64;
     if (rows <= 64) return most;
     return rows <= 4096 ? 16 : rows <= 8192 ? 32 : most;
 }
@@ -884,7 +857,7 @@ using namespace nsosx;
 
 extern "C" int64_t nsosx_moe_route_scored_workspace(int rows, int experts) {
     if (rows <= 0 || experts <= 0 || experts > kScoredMaxExperts) return 0;
-    const int rb = scored_block_rows(rows, experts);
+    const int rb = scored_block_rows(rows, experts > 128);  // (128 or less are never wide)
     return (int64_t)((rows - 1) / rb + 1) * experts;
 }
 
@@ -924,23 +897,34 @@ extern "C" int nsosx_moe_route_scored(const void* logits, int logits_dtype, int6
         return fail(NSOSX_ERR_INVALID, "moe_route_scored: k exceeds the experts of the kept groups");
     if ((int64_t)rows * k > 2147483647LL)
         return fail(NSOSX_ERR_OVERFLOW, "moe_route_scored: rows*k too large");
-    const int rb = scored_block_rows(rows, experts);
+    const int limited = group_keep == groups ? 1 : groups;
+    ScoredLayout at = scored_layout(experts, limited);
+    // more experts of a group than its lanes hold (more than 288 in 9 .. 15 groups, say): every row is
+    // chosen by a wave
+    const bool spread = at.values <= 32;
+    if (!spread) at = {0, 32};
+    const int rb = scored_block_rows(rows, at.values > 16);
     const int blocks = (rows - 1) / rb + 1;
-    RouteScored p{logits, logits_stride, valid_rows, bias, rows, experts, k, sigmoid != 0,
-                  group_keep == groups ? 1 : groups, group_keep, group_best, renorm != 0, scale,
-                  weights, selected, counts, offsets, perm, slot_of, workspace,
-                  (int64_t)blocks * experts <= kScoredPlaceCounts};
+    const RouteScored p{logits, logits_stride, valid_rows, bias, rows, experts, k, sigmoid != 0, limited,
+                        group_keep, group_best, renorm != 0, scale, weights, selected, counts, offsets,
+                        perm, slot_of, workspace, (int64_t)blocks * experts <= kScoredPlaceCounts,
+                        experts / limited, at.lanes, at.values,
+                        (experts + 63) / 64 * 64 + 16};  // (four rows' lanes on different banks)
+    const int smem = limited > 1 ? (rb * p.pitch + (experts + 3) / 4 * 4) * 4 : 0;
     hipStream_t st = static_cast<hipStream_t>(stream);
-#define NSOSX_RS(V)                                                                             \
-    do {                                                                                        \
-        if (logits_dtype == NSOSX_F32)                                                          \
-            hipLaunchKernelGGL((route_scored_kernel<V, NSOSX_F32>), dim3(blocks), dim3(16 * rb), \
-                               0, st, p);                                                       \
-        else                                                                                    \
-            hipLaunchKernelGGL((route_scored_kernel<V, NSOSX_BF16>), dim3(blocks), dim3(16 * rb), \
-                               0, st, p);                                                       \
+#define NSOSX_RS_DT(V, G)                                                                       \
+    if (logits_dtype == NSOSX_F32)                                                              \
+        hipLaunchKernelGGL((route_scored_kernel<V, NSOSX_F32, G>), dim3(blocks), dim3(16 * rb), \
+                           smem, st, p);                                                        \
+    else                                                                                        \
+        hipLaunchKernelGGL((route_scored_kernel<V, NSOSX_BF16, G>), dim3(blocks), dim3(16 * rb), \
+                           smem, st, p);
+#define NSOSX_RS(V)                                                    \
+    do {                                                               \
+        if (p.groups > 1) { NSOSX_RS_DT(V, true) } else { NSOSX_RS_DT(V, false) } \
     } while (0)
-    NSOSX_SCORED_V(experts, NSOSX_RS);
+    NSOSX_SCORED_V(16 * at.values, NSOSX_RS);
+#undef NSOSX_RS_DT
 #undef NSOSX_RS
     if (!select_only && blocks > 1 && p.by_block) {
         hipLaunchKernelGGL(route_scored_scan_place_kernel, dim3(blocks), dim3(256), 0, st, p, blocks, rb);

@@ -333,3 +333,19 @@ def test_gradient_ignores_unavailable_experts(dev):
             g = ops.moe_route_scored_backward(x, r["selected"], torch.ones(3, 3, device=dev),
                                               score=score, renorm=renorm)
             assert torch.isfinite(g).all() and (g[1, 2:] == 0).all() and (g[2] == 0).all()
+
+
+@pytest.mark.parametrize("e,groups,keep", [(504, 9, 4), (495, 15, 2), (330, 3, 2), (320, 5, 4), (252, 12, 5),
+                                           (9, 3, 2), (64, 2, 1), (512, 2, 1), (40, 8, 3), (144, 16, 7), (56, 2, 1), (112, 4, 3),
+                                           (24, 2, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_group_layouts(dev, e, groups, keep, dtype):
+    """Groups over every number of lanes, and more experts of a group than its lanes hold."""
+    rng = np.random.default_rng([e, groups])
+    for rows in (3, 70, 333):
+        x = rng.normal(0, 1.5, (rows, e))
+        bias = rng.normal(0, 0.1, e).astype(np.float32)
+        for best in (1, 2):
+            for b in (None, bias):
+                check(dev, x, min(4, keep * (e // groups)), dtype=dtype, score="softmax" if best == 1 else "sigmoid",
+                      bias=b, groups=groups, group_keep=keep, group_best=best)
