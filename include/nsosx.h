@@ -575,8 +575,7 @@ int nsosx_moe_sparse_decode(const nsosx_linear_view* up_views,
  *   weights[r, i] = s of choice i, divided by the sum over the row's choices where renorm != 0,
  *   times scale.  The bias takes part in the choice only.
  * Choices are those of the values in 64 bits, ties to the lower index (groups too); without a
- * bias the order of c is that of x.  An expert whose logit
- * (or c) is -inf is not available: a row with fewer than k available experts gets -1 and weight
+ * bias the order of c is that of x.  An expert whose logit (or c) is -inf is not available: a row with fewer than k available experts gets -1 and weight
  * 0 for the rest.  A row with a NaN score gets the first k experts and NaN weights.
  *   valid_rows uint8 [rows] or NULL: a row whose byte is 0 is padding (as nsosx_moe_route's):
  *   weights 0, selected and slot_of -1, no slots.
@@ -585,7 +584,8 @@ int nsosx_moe_sparse_decode(const nsosx_linear_view* up_views,
  *   rows ascending; -1 past offsets[E]); slot_of int32 [rows, k].
  *   workspace: int32, nsosx_moe_route_scored_workspace(rows, E) elements.
  * counts, offsets, perm, slot_of and workspace all NULL: weights and selected only.
- * E <= 512, k <= 16, k <= group_keep * E / groups, groups <= 16 dividing E, rows * k < 2^31. */
+ * E <= 512, k <= 16, k <= group_keep * E / groups, groups <= 16 dividing E, rows * k < 2^31,
+ * rows <= 2^28 - 64. */
 int64_t nsosx_moe_route_scored_workspace(int rows, int experts);
 int nsosx_moe_route_scored(const void* logits, int logits_dtype, int64_t logits_stride,
                            const uint8_t* valid_rows, const float* bias, int rows, int experts,
@@ -597,7 +597,8 @@ int nsosx_moe_route_scored(const void* logits, int logits_dtype, int64_t logits_
 /* Gradient of the logits from that of nsosx_moe_route_scored's weights (the choice itself and
  * the bias have none): selected int32 [rows, k] as the forward left it (-1 or an index past E
  * adds nothing, an expert named twice gets both), dweights f32 [rows, k]; dlogits [rows, E]
- * contiguous in logits_dtype, every element written (a padding row's with zeros). */
+ * contiguous in logits_dtype, every element written (a padding row's with zeros), which must
+ * not overlap the inputs. */
 int nsosx_moe_route_scored_backward(const void* logits, int logits_dtype, int64_t logits_stride,
                                     const int32_t* selected, const float* dweights, int rows,
                                     int experts, int k, int sigmoid, int renorm, float scale,
@@ -605,7 +606,7 @@ int nsosx_moe_route_scored_backward(const void* logits, int logits_dtype, int64_
 
 /* out[r] = sum_i expert_out[slot_of[r, i]] * weights[r, i], i ascending, f32 sums; a slot
  * outside [0, slots) adds nothing.  expert_out [slots, dim] (in_dtype), out [rows, dim]
- * (out_dtype), which must not overlap; any number of experts, k <= 16. */
+ * (out_dtype), which must not overlap; any number of experts, k <= 16, dim <= 2^30. */
 int nsosx_moe_combine_topk(const void* expert_out, int in_dtype, const int32_t* slot_of,
                            const float* weights, int rows, int slots, int k, int dim, void* out,
                            int out_dtype, void* stream);
@@ -626,7 +627,8 @@ int nsosx_moe_combine_topk_backward(const void* dout, int dout_dtype, const void
  * (exact int32 sums, then each step rounded to f32, no fma).  q int8 [M, K] and act_scale f32
  * [M] as nsosx_quantize_act_i8 leaves them (w and w_scale too: it quantizes a weight
  * matrix's rows); w int8 [N, K]; w_scale, bias (or NULL) f32 [N]; y [M, N] f32 or bf16.
- * Any M, N and K <= 131071, any alignment (16-byte aligned rows are the fast ones). */
+ * Any M and N <= 2^30 (fewer than 2^24 tiles of 128 x 128), K <= 131071, any alignment
+ * (16-byte aligned rows are the fast ones); y must not overlap q or w. */
 int nsosx_int8_gemm(const int8_t* q, const float* act_scale, const int8_t* w,
                     const float* w_scale, const float* bias, int M, int K, int N, void* y,
                     int y_dtype, void* stream);
@@ -635,7 +637,8 @@ int nsosx_int8_gemm(const int8_t* q, const float* act_scale, const int8_t* w,
  * < offsets[e+1], device int32 [experts + 1]) multiplies row perm[s] of q (row s with perm
  * NULL) with w[e]; then, where squared_relu != 0, max(v, 0)^2.  w int8 [experts, N, K];
  * w_scale, bias (or NULL) f32 [experts, N]; q int8 [q_rows, K], act_scale f32 [q_rows]; y
- * [slots, N], whose rows past offsets[experts] are left as they were.  experts <= 1024. */
+ * [slots, N], whose rows past offsets[experts] are left as they were and which must not overlap
+ * q or w.  experts <= 1024. */
 int nsosx_grouped_int8_gemm(const int8_t* q, const float* act_scale, int q_rows, const int8_t* w,
                             const float* w_scale, const float* bias, const int32_t* offsets,
                             const int32_t* perm, int slots, int experts, int K, int N,

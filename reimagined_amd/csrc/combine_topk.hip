@@ -5,6 +5,7 @@
 namespace nsosx {
 
 constexpr int kTopkMax = 16;
+constexpr int kTopkMaxDim = 1 << 30;  // a lane's element, and the step behind the last, in int
 constexpr int kZeroSlots = 4;  // of a wave that clears unused rows
 
 template <int V, int DT>
@@ -194,8 +195,8 @@ extern "C" int nsosx_moe_combine_topk(const void* expert_out, int in_dtype, cons
     const bool v8 = vector_rows(dim, expert_out, out, nullptr);
     const int pieces = (dim - 1) / (v8 ? 512 : 64) + 1;
     const int64_t grid = ((int64_t)rows * pieces + 3) / 4;
-    if (grid > 0x7fffffffLL / 256)  // a launch holds less than 2^32 threads
-        return fail(NSOSX_ERR_OVERFLOW, "moe_combine_topk: rows * dim too large");
+    if (dim > kTopkMaxDim || grid > 0x7fffffffLL / 256)  // a launch holds less than 2^32 threads
+        return fail(NSOSX_ERR_OVERFLOW, "moe_combine_topk: dim or rows * dim too large");
     hipStream_t st = static_cast<hipStream_t>(stream);
 #define NSOSX_CT_K(I, O, V)                                                                        \
     do {                                                                                           \
@@ -245,7 +246,8 @@ extern "C" int nsosx_moe_combine_topk_backward(const void* dout, int dout_dtype,
     const int per = v8 ? 512 : 64;
     const int waves = dim > 2 * per ? 4 : dim > per ? 2 : 1;
     const int64_t grid = rows + (perm ? ((int64_t)slots - 1) / (kZeroSlots * waves) + 1 : 0);
-    if (grid > 0x7fffffffLL / 256) return fail(NSOSX_ERR_OVERFLOW, "moe_combine_topk_backward: too many rows");
+    if (dim > kTopkMaxDim || grid > 0x7fffffffLL / 256)
+        return fail(NSOSX_ERR_OVERFLOW, "moe_combine_topk_backward: rows, slots or dim too large");
     const dim3 block(64 * waves);
     hipStream_t st = static_cast<hipStream_t>(stream);
 #define NSOSX_CB_L(D, E, V, KT)                                                                     \

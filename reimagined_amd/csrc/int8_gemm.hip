@@ -74,9 +74,10 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesPerSimd) void i8_gemm_kernel(
 // One row tile of one segment a workgroup.  Outputs are fastest, so that where their tiles divide
 // by the 8 XCDs, each XCD reads an eighth of every expert's weights.  Where they do not, and an
 // expert has more than one row tile to share its weights, the large tiles are dealt to the XCDs in
-// contiguous runs, as those of one matrix, so that they are read by one or two (8192 rows to 8 of 128 experts of 2048 -> 768, 128 x 128 tiles: 169
-// us, and 200 with outputs fastest; to 2 of 8 experts of 1024 -> 4096: 112 and 105).  The launch
-// holds as many workgroups as there can be tiles; those past the real ones end here.
+// contiguous runs, as those of one matrix, so that they are read by one or two (128 x 128 tiles,
+// 8192 rows to 8 of 128 experts of 2048 -> 768: 169 us, and 200 with outputs fastest; to 2 of 8
+// experts of 1024 -> 4096, whose tiles do divide: 112 and 105).  The launch holds as many
+// workgroups as there can be tiles; those past the real ones end here.
 template <class T, int YDT>
 __global__ __launch_bounds__(T::kThreads, T::kWavesPerSimd) void i8_grouped_kernel(I8Group gp,
                                                                                  void* __restrict__ y) {
@@ -131,6 +132,7 @@ static void launch_grouped_t(const I8Group& gp, void* y, hipStream_t st) {
 // Rows that do not start on 16 bytes go through registers on the way to LDS, which costs every
 // tile about a quarter, and have no 256 x 256 one (2048 x 2009 -> 5125 on 128 x 128: 55 us).
 constexpr int64_t kI8MaxTiles = 1 << 24;  // of 128 x 128: 256 threads each, less than 2^32
+constexpr int kI8MaxSide = 1 << 30;       // a tile's first row or output, and what it adds, in int
 
 enum class I8Tile { k16x16, k16x64, k32x64, k64x64, k128x128, k256x256 };
 
@@ -223,8 +225,12 @@ extern "C" int nsosx_int8_gemm(const int8_t* q, const float* act_scale, const in
         return fail(NSOSX_ERR_INVALID, "int8_gemm: M, K and N must be positive");
     if (!valid_dtype(y_dtype)) return fail(NSOSX_ERR_INVALID, "int8_gemm: bad dtype");
     if (K > kI8MaxK) return fail(NSOSX_ERR_OVERFLOW, "int8_gemm: K past the int32 sums (131071)");
-    if (((int64_t)N + 127) / 128 * (((int64_t)M + 127) / 128) >= kI8MaxTiles)
-        return fail(NSOSX_ERR_OVERFLOW, "int8_gemm: M * N too large");
+    if (M > kI8MaxSide || N > kI8MaxSide ||
+        ((int64_t)N + 127) / 128 * (((int64_t)M + 127) / 128) >= kI8MaxTiles)
+        return fail(NSOSX_ERR_OVERFLOW, "int8_gemm: M, N or M * N too large");
+    const int64_t yb = (int64_t)M * N * (y_dtype == NSOSX_F32 ? 4 : 2);
+    if (overlaps(y, yb, q, (int64_t)M * K) || overlaps(y, yb, w, (int64_t)N * K))
+        return fail(NSOSX_ERR_INVALID, "int8_gemm: y overlaps an input");
     const I8Problem pb{w, w_scale, bias, N, K, 0};
     const I8Rows rows{q, act_scale, nullptr, 0, M, M};
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -248,8 +254,12 @@ extern "C" int nsosx_grouped_int8_gemm(const int8_t* q, const float* act_scale, 
     if (!valid_dtype(y_dtype)) return fail(NSOSX_ERR_INVALID, "grouped_int8_gemm: bad dtype");
     if (K > kI8MaxK)
         return fail(NSOSX_ERR_OVERFLOW, "grouped_int8_gemm: K past the int32 sums (131071)");
-    if (((int64_t)N + 127) / 128 * ((int64_t)slots / 128 + experts) >= kI8MaxTiles)
-        return fail(NSOSX_ERR_OVERFLOW, "grouped_int8_gemm: slots * N too large");
+    if (slots > kI8MaxSide || N > kI8MaxSide ||
+        ((int64_t)N + 127) / 128 * ((int64_t)slots / 128 + experts) >= kI8MaxTiles)
+        return fail(NSOSX_ERR_OVERFLOW, "grouped_int8_gemm: slots, N or slots * N too large");
+    const int64_t yb = (int64_t)slots * N * (y_dtype == NSOSX_F32 ? 4 : 2);
+    if (overlaps(y, yb, q, (int64_t)q_rows * K) || overlaps(y, yb, w, (int64_t)experts * N * K))
+        return fail(NSOSX_ERR_INVALID, "grouped_int8_gemm: y overlaps an input");
     const I8Group gp{w, w_scale, bias, q, act_scale, offsets, perm, q_rows, slots, experts, N, K,
                      squared_relu != 0};
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -1,5 +1,5 @@
-// Tiles of the int8 x int8 products (int8_gemm.hip): the few-row tile, whose waves split K,
-// and the LDS-staged block tile.
+// Tiles of the int8 x int8 products (int8_gemm.hip): the one for few tiles, whose waves split K,
+// and the block tiles, through registers (any alignment) or straight into LDS.
 #pragma once
 #include "common.hpp"
 
@@ -389,8 +389,7 @@ __device__ __forceinline__ void i8_epilogue_as(const I8Problem& pb, const I8Rows
     const int nw = n0 + 64 * wn;
     const bool whole = nw + 64 <= pb.N && pb.N % (16 / kSize) == 0 &&
                        (reinterpret_cast<uintptr_t>(y) & 15) == 0;
-    // the scales and biases of this lane's outputs, once for all TM tiles (a ds_read_b128 takes 16
-    // clocks however many lanes share an address; read for each tile they were most of the epilogue)
+    // the scales and biases of this lane's outputs, once for all TM tiles
     float4 sc[8], bs[8];
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
@@ -547,12 +546,12 @@ __device__ __forceinline__ void i8_tile(const I8Problem& pb, const I8Rows& rows,
 // The same tile with its stages brought straight into LDS (global_load_lds, 16 bytes a lane: the
 // rows have to start on 16 bytes), and the last quarter of a stage multiplied after the barrier
 // that frees its buffer, so that the barrier's wait and the first reads of the next stage lie
-// under matrix instructions.  256 x 256 blocks of eight waves, 4096 x 4096 x 8192: 127 .. 137 us,
-// 2.0 .. 2.16 POP/s (128 x 128 blocks 147 .. 154, through registers 186 .. 194); matrix instructions
-// alone reach 3.1 POP/s on such data.  LDS bounds it: 192 KB read and 64 KB written a stage at 64
+// under matrix instructions.  256 x 256 blocks of eight waves, 4096 x 4096 x 8192: 129 us,
+// 2.1 POP/s (128 x 128 blocks 145, through registers 170 .. 178); matrix instructions alone reach
+// 3.1 POP/s on such data.  LDS bounds it: 192 KB read and 64 KB written a stage at 64
 // bytes a clock.  64-deep stages in rings of three or four, and 256 x 128 blocks of four waves, two
 // a compute unit, were no faster at any size (138 -> 142 .. 159 us).  At K 1024 the stores show, which
-// all compute units make at once (8192 x 1024 x 4096: 46 us, 13 of them 67 MB of outputs).
+// all compute units make at once (8192 x 1024 x 4096: 43.5 us, about 13 of them 67 MB of outputs).
 template <int YDT, int NWN, int NWM, int TM>
 __device__ __forceinline__ void i8_wide_tile(const I8Problem& pb, const I8Rows& rows, int n0, int m0,
                                              void* __restrict__ y, char* smem) {

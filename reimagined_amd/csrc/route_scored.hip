@@ -6,6 +6,7 @@
 namespace nsosx {
 
 constexpr int kScoredMaxExperts = 512, kScoredMaxK = 16, kScoredMaxGroups = 16;
+constexpr int kScoredMaxRows = (1 << 28) - 64;  // 16 threads each: a launch holds fewer than 2^32
 
 struct RouteScored {
     const void* logits;
@@ -175,23 +176,6 @@ __device__ __forceinline__ void softmax_stats(const float (&x)[V], float& mx, fl
     sum = row_sum(sum);
 }
 
-// The choice by 32-bit scores, with a proof that it is the one of 64 bits: every value becomes a
-// 32-bit key, its distance from a point below the row's largest in fixed point (2 for scores with a
-// bias, 32 for logits, whose order is that of scores without one) above the complement of its
-// index, each lane sorts its keys, and k + 1 rounds take the largest of the row's 16 first ones.
-// The choice stands where the fixed-point values of neighbours in that order differ by more than
-// the scores' error.  Where they do not (about 2 of 10^4 rows of 256 sigmoid scores with a bias),
-// where groups lie too close together, values outside the window or a NaN in the row, the whole
-// wave chooses for the row in 64 bits (select_wave).  bfloat16 logits make exact keys.
-//
-// What it takes is instructions: 16384 rows of 256 experts in 8 groups, sigmoid scores and a bias,
-// are 17 MB (3.3 us) and @@ us, where k rounds of a 64-bit maximum over the row took 41.
-//
-// Errors, in units u = 2^-23: a sigmoid by exp2 and reciprocal of one unit each is off by s (1 - s)
-// (|x| / 2 + 1) + 1.5 s, below 1.7 u.  A softmax score p = e / sum: e by |x - max| + 1 of itself,
-// the sum by (V + 4) / 2 + 1 and the weighted mean of |x - max|, at most ln 512, reciprocal and
-// product 1.5, and p |x - max| <= 0.37 of the largest p: below (13 + V / 2) u of that.  The sum with
-// the bias by half a unit of the value.
 // Batcher's odd-even merge sort, descending, of N keys from LO.
 template <int A, int B, int V>
 __device__ __forceinline__ void order_pair(uint32_t (&key)[V]) {
@@ -225,6 +209,26 @@ __device__ __forceinline__ void sort_keys(uint32_t (&key)[V]) {
     }
 }
 
+// The choice by 32-bit scores, with a proof that it is the one of 64 bits: every value becomes a
+// 32-bit key, its distance from a point below the row's largest in fixed point (2 for scores with a
+// bias, 32 for logits, whose order is that of scores without one) above the complement of its
+// index, each lane sorts its keys, and k + 1 rounds take the largest of the row's 16 first ones.
+// The choice stands where the fixed-point values of neighbours in that order differ by more than
+// the scores' error.  Where they do not (about 2 of 10^4 rows of 256 sigmoid scores with a bias),
+// where groups lie too close together, values outside the window or a NaN in the row, the whole
+// wave chooses for the row in 64 bits (select_wave).  bfloat16 logits make exact keys.
+//
+// What it takes is instructions: 16384 rows of 256 experts in 8 groups, sigmoid scores and a bias,
+// are 17 MB (3.3 us) and 20 us, where k rounds of a 64-bit maximum over the row took 41.  Without
+// the rows left to select_wave, three or four of those 16384, it is 12: a wave that meets one takes 8
+// us longer, and the launch ends with it.
+//
+// Errors, in units u = 2^-23: a sigmoid by exp2 and reciprocal of one unit each is off by s (1 - s)
+// (|x| / 2 + 1) + 1.5 s, below 1.7 u.  A softmax score p = e / sum: e by |x - max| + 1 of itself,
+// the sum by (V + 4) / 2 + 1 and the weighted mean of |x - max|, at most ln 512, reciprocal and
+// product 1.5, and p |x - max| <= 0.37 of the largest p: below (13 + V / 2) u of that.  The sum with
+// the bias by half a unit of the value.
+//
 // Expert index of choice l in lane l (-1: none), where `sure`.  G: limited to groups.
 // s_row, s_bias (G): this row's place in LDS, the biases there.
 template <int V, int DT, bool G>
@@ -337,15 +341,6 @@ __device__ __forceinline__ int select_fast(const RouteScored& p, int64_t row, bo
         if (keyed) apart = (uint32_t)fminf(2.0f * err * scale, 1e9f) + (1u << (NB > 24 ? NB - 23 : 1)) + 2;
     }
     sort_keys<0, V>(key);
-    auto take = [&] {  // the row's largest key, out of its lane's list
-        const uint32_t m = row_max(key[0]);
-        if (key[0] == m) {  // (as selects, the compiler made this a search through the array)
-#pragma unroll
-            for (int v = 0; v + 1 < V; ++v) key[v] = key[v + 1];
-            key[V - 1] = 0;
-        }
-        return m;
-    };
     uint32_t mine = 0, before = 0;  // choice l's key, in lane l
     for (int i = 0; i <= p.k; ++i) {
         const uint32_t m = row_max(key[0]);
@@ -687,8 +682,8 @@ __global__ __launch_bounds__(256) void route_scored_place_kernel(RouteScored p, 
 }
 
 // The same with the scans over the blocks, for few counts (kScoredPlaceCounts): a workgroup for each
-// block of rows, which sums every expert's counts, and those before its own block, by itself (4096
-// rows of 60 experts: @@ us less than the two launches).
+// block of rows, which sums every expert's counts, and those before its own block, by itself (4099
+// rows of 60 experts: 4.9 us, the two launches 2.8 + 3.6).
 constexpr int kScoredPlaceCounts = 16384;
 
 __global__ __launch_bounds__(256) void route_scored_scan_place_kernel(RouteScored p, int blocks,
@@ -895,8 +890,8 @@ extern "C" int nsosx_moe_route_scored(const void* logits, int logits_dtype, int6
                     "group_best 1 or 2");
     if (k > group_keep * (experts / groups))
         return fail(NSOSX_ERR_INVALID, "moe_route_scored: k exceeds the experts of the kept groups");
-    if ((int64_t)rows * k > 2147483647LL)
-        return fail(NSOSX_ERR_OVERFLOW, "moe_route_scored: rows*k too large");
+    if ((int64_t)rows * k > 2147483647LL || rows > kScoredMaxRows)
+        return fail(NSOSX_ERR_OVERFLOW, "moe_route_scored: rows*k or rows too large");
     const int limited = group_keep == groups ? 1 : groups;
     ScoredLayout at = scored_layout(experts, limited);
     // more experts of a group than its lanes hold (more than 288 in 9 .. 15 groups, say): every row is
@@ -953,8 +948,13 @@ extern "C" int nsosx_moe_route_scored_backward(const void* logits, int logits_dt
                     "moe_route_scored_backward: need rows > 0, 0 < k <= 16, k <= E <= 512");
     if (logits_stride < experts)
         return fail(NSOSX_ERR_INVALID, "moe_route_scored_backward: logits_stride below E");
-    if ((int64_t)rows * k > 2147483647LL)
-        return fail(NSOSX_ERR_OVERFLOW, "moe_route_scored_backward: rows*k too large");
+    if ((int64_t)rows * k > 2147483647LL || rows > kScoredMaxRows)
+        return fail(NSOSX_ERR_OVERFLOW, "moe_route_scored_backward: rows*k or rows too large");
+    const int64_t size = logits_dtype == NSOSX_F32 ? 4 : 2, db = (int64_t)rows * experts * size;
+    if (overlaps(dlogits, db, logits, ((int64_t)(rows - 1) * logits_stride + experts) * size) ||
+        overlaps(dlogits, db, selected, (int64_t)rows * k * 4) ||
+        overlaps(dlogits, db, dweights, (int64_t)rows * k * 4))
+        return fail(NSOSX_ERR_INVALID, "moe_route_scored_backward: dlogits overlaps an input");
     const RouteScoredBwd p{logits, logits_stride, selected, dweights, rows, experts, k, sigmoid != 0,
                            renorm != 0, scale, dlogits};
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -38,6 +38,44 @@ def test_route_overflow():
     assert "too large" in refused("nsosx_moe_route_scored", *route(rows=2**31 - 1, k=2), status=2)
 
 
+def test_route_rows_of_a_launch():
+    """16 threads a row and fewer than 2^32 a launch."""
+    assert "too large" in refused("nsosx_moe_route_scored",
+                                  *route(rows=2**28, e=1, stride=1, k=1), status=2)
+    assert "too large" in refused("nsosx_moe_route_scored_backward", P, 0, 1, P, P, 2**28, 1, 1, 0, 1, 1.0,
+                                  P, None, status=2)
+
+
+@pytest.mark.parametrize("logits,selected,dweights", [(4, 0, 1024), (1024, 4, 2048), (1024, 2048, 124)])
+def test_route_backward_overlaps(logits, selected, dweights):
+    """dlogits: 4 rows of 8 floats at 4 P; the input named by the small distance meets it."""
+    at = 4 * P
+    assert "overlaps" in refused("nsosx_moe_route_scored_backward", at + logits, 0, 8, at - 8 + selected if selected
+                                 else at + 4096, at + dweights, 4, 8, 2, 0, 1, 1.0, at, None)
+
+
+def test_dims_past_an_int():
+    assert "too large" in refused("nsosx_moe_combine_topk", P, 0, P, P, 1, 1, 1, 2**30 + 8, 2**40, 0, None,
+                                  status=2)
+    assert "too large" in refused("nsosx_moe_combine_topk_backward", P, 0, 2**41, 0, P, P, None, 1, 1, 1,
+                                  2**30 + 8, 2**40, P, None, status=2)
+    assert "too large" in refused("nsosx_int8_gemm", P, P, P, P, None, 1, 16, 2**31 - 130, P, 0, None, status=2)
+    assert "too large" in refused("nsosx_int8_gemm", P, P, P, P, None, 2**31 - 130, 16, 1, P, 0, None, status=2)
+    assert "too large" in refused("nsosx_grouped_int8_gemm", P, P, 4, P, P, None, P, P, 2**30 + 1, 1, 16, 16, 0,
+                                  P, 0, None, status=2)
+
+
+def test_int8_overlaps():
+    """y [4, 16] f32 over the codes' or the weights' last bytes, and right behind them."""
+    far = 64 * P
+    assert "overlaps" in refused("nsosx_int8_gemm", P, P, far, P, None, 4, 32, 16, P + 127, 0, None)
+    assert "overlaps" in refused("nsosx_int8_gemm", P, P, far, P, None, 4, 32, 16, far - 255, 0, None)
+    assert "overlaps" in refused("nsosx_grouped_int8_gemm", P, P, 4, far, P, None, P, None, 4, 2, 32, 16, 0,
+                                 far + 1023, 0, None)
+    assert "overlaps" in refused("nsosx_grouped_int8_gemm", P, P, 4, far, P, None, P, None, 4, 2, 32, 16, 0,
+                                 P + 127, 0, None)
+
+
 def test_route_workspace():
     lib = _lib.lib()
     assert lib.nsosx_moe_route_scored_workspace(0, 8) == 0
