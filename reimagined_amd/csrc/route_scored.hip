@@ -22,7 +22,7 @@ struct RouteScored {
     int32_t* offsets;        // [E + 1]
     int32_t* perm;           // [rows * k]
     int32_t* slot_of;        // [rows, k]
-    int32_t* block_counts;   // workspace [E, blocks], or [blocks, E] where by_block
+    int32_t* block_counts;   // workspace [E, blocks]; where by_block, bytes [blocks, words of 4]
     int by_block;
     int size, lanes, run;    // experts of a group, lanes that share them (a power of two), of a lane
     int pitch;               // of a row in LDS, floats
@@ -163,6 +163,22 @@ __device__ __forceinline__ double exp_of(double x) {
     return ldexp(p, (int)n);
 }
 
+// Whether lane l - N of the row has a larger value (or the same one and a lower index).
+template <int N>
+__device__ __forceinline__ void outranked64(double v, int e, int& rank) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint64_t lo = ror16<N>((uint32_t)u), hi = ror16<N>((uint32_t)(u >> 32));
+    const double o = __builtin_bit_cast(double, lo | (hi << 32));
+    const int oe = ror16<N>(e);
+    rank += o > v || (o == v && oe < e) ? 1 : 0;
+}
+// Of rank << 16 | index in each lane, the one whose rank is this lane's number.
+template <int N>
+__device__ __forceinline__ void ranked_here(uint32_t at, int l, uint32_t& got) {
+    const uint32_t o = ror16<N>(at);
+    got = (int)(o >> 16) == l ? o : got;
+}
+
 // The maximum and the scores' sum of a softmax row (unavailable experts are -inf).
 template <int V>
 __device__ __forceinline__ void softmax_stats(const float (&x)[V], float& mx, float& sum) {
@@ -214,14 +230,16 @@ __device__ __forceinline__ void sort_keys(uint32_t (&key)[V]) {
 // bias, 32 for logits, whose order is that of scores without one) above the complement of its
 // index, each lane sorts its keys, and k + 1 rounds take the largest of the row's 16 first ones.
 // The choice stands where the fixed-point values of neighbours in that order differ by more than
-// the scores' error.  Where they do not (about 2 of 10^4 rows of 256 sigmoid scores with a bias),
-// where groups lie too close together, values outside the window or a NaN in the row, the whole
-// wave chooses for the row in 64 bits (select_wave).  bfloat16 logits make exact keys.
+// the scores' error.  Where they do not (about 7 of 10^4 rows of 256 sigmoid scores with a bias), but
+// the k + 1 largest are apart from all others, those are put in order in 64 bits, one a lane.
+// What is left (groups too close together, more values than that, values outside the window, a NaN in
+// the row) the whole wave chooses in 64 bits, a row at a time (select_wave).  bfloat16 logits make
+// exact keys.
 //
 // What it takes is instructions: 16384 rows of 256 experts in 8 groups, sigmoid scores and a bias,
-// are 17 MB (3.3 us) and 20 us, where k rounds of a 64-bit maximum over the row took 41.  Without
-// the rows left to select_wave, three or four of those 16384, it is 12: a wave that meets one takes 8
-// us longer, and the launch ends with it.
+// are 17 MB (3.3 us) and 14 us, 12 without the rows that 32 bits cannot decide.  (k rounds of a
+// 64-bit maximum over every row took 41; select_wave alone for those rows, 4 us of one wave while the
+// launch waits for it, 18.)
 //
 // Errors, in units u = 2^-23: a sigmoid by exp2 and reciprocal of one unit each is off by s (1 - s)
 // (|x| / 2 + 1) + 1.5 s, below 1.7 u.  A softmax score p = e / sum: e by |x - max| + 1 of itself,
@@ -341,23 +359,58 @@ __device__ __forceinline__ int select_fast(const RouteScored& p, int64_t row, bo
         if (keyed) apart = (uint32_t)fminf(2.0f * err * scale, 1e9f) + (1u << (NB > 24 ? NB - 23 : 1)) + 2;
     }
     sort_keys<0, V>(key);
-    uint32_t mine = 0, before = 0;  // choice l's key, in lane l
-    for (int i = 0; i <= p.k; ++i) {
+    uint32_t mine = 0, before = 0;  // lane l's: the key of choice l, and of the one behind the last
+    bool inside = true, clear = true;
+    auto next = [&](int i) {  // the row's largest key, out of its lane's list
         const uint32_t m = row_max(key[0]);
-        // (the key behind the last choice only has to be apart from it)
-        ok = ok && (exact || ((i == 0 || (before >> IB) >= (m >> IB) + apart) &&
-                              (i == p.k || (m >> IB) != 0)));
+        clear = clear && (exact || i == 0 || (before >> IB) >= (m >> IB) + apart);
         before = m;
-        if (l == i && i < p.k) mine = m;
+        if (l == i) mine = m;
         if (key[0] == m) {  // (as selects, the compiler made this a search through the array)
 #pragma unroll
             for (int v = 0; v + 1 < V; ++v) key[v] = key[v + 1];
             key[V - 1] = 0;
         }
+        return m;
+    };
+    for (int i = 0; i < p.k; ++i) {
+        const uint32_t m = next(i);
+        inside = inside && (exact || (m >> IB) != 0);
     }
-    sure = !live || (ok && !row_any(odd));
-    if (!live || mine == 0) return -1;
-    return exact ? (int)(0xFFFFu - (mine & 0xFFFFu)) : (int)(kIndex - (mine & kIndex));
+    next(p.k);  // (it only has to be apart from the last choice)
+    odd = row_any(odd);
+    sure = !live || (ok && inside && clear && !odd);
+    int choice = l >= p.k || mine == 0 ? -1
+                                       : exact ? (int)(0xFFFFu - (mine & 0xFFFFu)) : (int)(kIndex - (mine & kIndex));
+    // Only choices too close to each other: where the k + 1 largest are apart from all others, they are
+    // put in order in 64 bits, one a lane.
+    const bool close = live && ok && inside && !clear && !odd && !exact && p.k < 16 && (!p.bias || p.sigmoid);
+    if (__any(close)) {
+        const uint32_t m = row_max(key[0]);
+        const bool settled = close && (before >> IB) >= (m >> IB) + apart;
+        const int e = min((int)(kIndex - (mine & kIndex)), p.E - 1);
+        double val = (double)load_act<DT>(p.logits, row * p.stride + e);
+        if (p.bias) val = 1.0 / (1.0 + exp_of(-val)) + (double)p.bias[e];
+        if (l > p.k || mine == 0) val = -(double)INFINITY;
+        int rank = 0;
+        outranked64<1>(val, e, rank); outranked64<2>(val, e, rank); outranked64<3>(val, e, rank);
+        outranked64<4>(val, e, rank); outranked64<5>(val, e, rank); outranked64<6>(val, e, rank);
+        outranked64<7>(val, e, rank); outranked64<8>(val, e, rank); outranked64<9>(val, e, rank);
+        outranked64<10>(val, e, rank); outranked64<11>(val, e, rank); outranked64<12>(val, e, rank);
+        outranked64<13>(val, e, rank); outranked64<14>(val, e, rank); outranked64<15>(val, e, rank);
+        const uint32_t at = (uint32_t)(l > p.k ? 16 : rank) << 16 | (uint32_t)e;
+        uint32_t got = at;
+        ranked_here<1>(at, l, got); ranked_here<2>(at, l, got); ranked_here<3>(at, l, got);
+        ranked_here<4>(at, l, got); ranked_here<5>(at, l, got); ranked_here<6>(at, l, got);
+        ranked_here<7>(at, l, got); ranked_here<8>(at, l, got); ranked_here<9>(at, l, got);
+        ranked_here<10>(at, l, got); ranked_here<11>(at, l, got); ranked_here<12>(at, l, got);
+        ranked_here<13>(at, l, got); ranked_here<14>(at, l, got); ranked_here<15>(at, l, got);
+        if (settled) {
+            sure = true;
+            choice = l < p.k ? (int)(got & 0xFFFFu) : -1;
+        }
+    }
+    return live ? choice : -1;
 }
 
 // Step O of a reduction over a wave: a rotation within the 16-lane rows for 1 .. 8, the rows
@@ -399,24 +452,51 @@ __device__ __forceinline__ void wave_max2(double& a, double& b) {
     a = fmax(a, oa);
     if constexpr (O > 1) wave_max2<O / 2>(a, b);
 }
+template <int CTRL>
+__device__ __forceinline__ double dpp_move(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint64_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xF, 0xF, true);
+    const uint64_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(u >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, lo | (hi << 32));
+}
+// The two largest of a and b here and in another lane.
+__device__ __forceinline__ void join_two(double& a, double& b, double oa, double ob) {
+    b = fmax(fmin(a, oa), fmax(b, ob));
+    a = fmax(a, oa);
+}
+__device__ __forceinline__ double lane_value(double v, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+    const uint64_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), lane);
+    return __builtin_bit_cast(double, lo | (hi << 32));
+}
 
-// One row (the same in every lane) chosen by a whole wave in 64 bits, expert 64 v + lane in value v:
-// choice i in every lane whose number mod 16 is i (-1 where no expert is left).  bad: the row
-// holds a NaN, or an infinite logit that its softmax cannot take.
-template <int V, int DT>
+// One row (the same in every lane) chosen by a whole wave in 64 bits: choice i in every lane whose
+// number mod 16 is i (-1 where no expert is left).  bad: the row holds a NaN, or an infinite logit
+// that its softmax cannot take.  A lane has a run of experts, sorted, so that a round looks at one
+// value a lane, and ties go to the lowest lane; groups (G) lie on lanes of their own.  One wave does
+// this while the rest of its launch has ended, so every instruction shows (256 experts of 8 groups: 4
+// us, and 8 with the experts strewn over the lanes and a wave's reduction for each group).
+template <int V, int DT, bool G>
 __device__ __forceinline__ int select_wave(const RouteScored& p, int64_t row, bool& bad) {
     constexpr int W = V > 4 ? V / 4 : 1;
     const double none = -(double)INFINITY;
     const int lane = threadIdx.x & 63;
-    const bool scored = p.bias || (p.groups > 1 && p.best == 2);
+    const bool scored = p.bias || (G && p.best == 2);
+    const bool apart = G && (V < 32 || p.lanes > 0);  // groups on lanes of their own
+    const int lanes = apart ? 4 * p.lanes : 64;  // (a power of two)
+    const int q = lane / lanes, all = apart ? p.size : p.E;
+    const int run = (all + lanes - 1) / lanes, at = (lane & (lanes - 1)) * run;
+    const int first = q * all + at, n = q * all < p.E ? min(run, all - at) : 0;
     float x[W];
     double c[W];
+    int expert[W];
     bool nan = false;
 #pragma unroll
     for (int v = 0; v < W; ++v) {
-        const int e = 64 * v + lane;
-        x[v] = load_act<DT>(p.logits, row * p.stride + min(e, p.E - 1));
-        x[v] = e < p.E ? x[v] : -INFINITY;
+        expert[v] = min(first + v, p.E - 1);
+        x[v] = load_act<DT>(p.logits, row * p.stride + expert[v]);
+        x[v] = v < n ? x[v] : -INFINITY;
         nan |= x[v] != x[v];
         c[v] = (double)x[v];
     }
@@ -424,7 +504,7 @@ __device__ __forceinline__ int select_wave(const RouteScored& p, int64_t row, bo
         if (scored) {
 #pragma unroll
             for (int v = 0; v < W; ++v)
-                if (c[v] > none) c[v] = 1.0 / (1.0 + exp_of(-c[v]));
+                c[v] = c[v] > none ? 1.0 / (1.0 + exp_of(-c[v])) : c[v];
         }
     } else {
         double mx = c[0], sum = 0.0;
@@ -435,68 +515,100 @@ __device__ __forceinline__ int select_wave(const RouteScored& p, int64_t row, bo
         if (scored) {
 #pragma unroll
             for (int v = 0; v < W; ++v) {
-                if (c[v] > none) c[v] = exp_of(c[v] - mx);
+                c[v] = c[v] > none ? exp_of(c[v] - mx) : c[v];
                 sum += c[v] > none ? c[v] : 0.0;
             }
             sum = wave_sum(sum);
 #pragma unroll
-            for (int v = 0; v < W; ++v)
-                if (c[v] > none) c[v] = c[v] / sum;
+            for (int v = 0; v < W; ++v) c[v] = c[v] > none ? c[v] / sum : c[v];
         }
     }
     if (p.bias) {
 #pragma unroll
         for (int v = 0; v < W; ++v) {
-            const float b = p.bias[min(64 * v + lane, p.E - 1)];
-            if (c[v] > none) c[v] += (double)b;
+            const double b = (double)p.bias[expert[v]];
+            c[v] = c[v] > none ? c[v] + b : c[v];
             nan |= c[v] != c[v];
         }
     }
     bad = __any(nan);
-    if (p.groups > 1) {
-        const int size = p.E / p.groups;
-        double s = none;  // lane q's: the score of group q
-        for (int q = 0; q < p.groups; ++q) {
+    if (apart) {
+        double a = none, b = none;  // the group's two largest
+#pragma unroll
+        for (int v = 0; v < W; ++v) {
+            b = fmax(b, fmin(a, c[v]));
+            a = fmax(a, c[v]);
+        }
+        join_two(a, b, dpp_move<0xB1>(a), dpp_move<0xB1>(b));  // lane l ^ 1
+        join_two(a, b, dpp_move<0x4E>(a), dpp_move<0x4E>(b));  // lane l ^ 2
+        if (lanes >= 8) join_two(a, b, dpp_move<0x141>(a), dpp_move<0x141>(b));  // l ^ 7: the other four
+        if (lanes >= 16) join_two(a, b, dpp_move<0x140>(a), dpp_move<0x140>(b));  // l ^ 15: the other eight
+        if (lanes >= 32) join_two(a, b, wave_move<16>(a), wave_move<16>(b));
+        const double s = p.best == 2 && b > none ? a + b : a;
+        int rank = 0;
+        for (int g = 0; g < p.groups; ++g) {
+            const double o = lane_value(s, g * lanes);
+            rank += o > s || (o == s && g < q) ? 1 : 0;
+        }
+        const bool open = rank < p.keep;
+#pragma unroll
+        for (int v = 0; v < W; ++v) {
+            if (!p.bias) c[v] = (double)x[v];  // the experts by their logits
+            c[v] = open && v < n ? c[v] : none;
+        }
+    } else if constexpr (G && V == 32) {
+        double s = none;  // lane g's: the score of group g
+        for (int g = 0; g < p.groups; ++g) {
             double a = none, b = none;
 #pragma unroll
             for (int v = 0; v < W; ++v) {
-                const int e = 64 * v + lane;
-                const double u = e >= q * size && e < (q + 1) * size ? c[v] : none;
+                const int e = first + v;
+                const double u = e >= g * p.size && e < (g + 1) * p.size ? c[v] : none;
                 b = fmax(b, fmin(a, u));
                 a = fmax(a, u);
             }
             wave_max2(a, b);
-            if (lane == q) s = p.best == 2 && b > none ? a + b : a;
+            if (lane == g) s = p.best == 2 && b > none ? a + b : a;
         }
         int rank = 0;
-        for (int q = 0; q < p.groups; ++q) {
-            const double o = __shfl(s, q, kWave);
-            rank += o > s || (o == s && q < lane) ? 1 : 0;
+        for (int g = 0; g < p.groups; ++g) {
+            const double o = lane_value(s, g);
+            rank += o > s || (o == s && g < lane) ? 1 : 0;
         }
         const uint64_t kept = __ballot(lane < p.groups && rank < p.keep);
 #pragma unroll
         for (int v = 0; v < W; ++v) {
-            const int e = 64 * v + lane;
-            if (!p.bias) c[v] = (double)x[v];  // the experts by their logits
-            if (e < p.E && !((kept >> (e / size)) & 1)) c[v] = none;
+            if (!p.bias) c[v] = (double)x[v];
+            if (!((kept >> (expert[v] / p.size)) & 1)) c[v] = none;
         }
     }
+    // (neighbours change places only where the first is smaller: equal values stay in order)
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+        for (int v = i & 1; v + 1 < W; v += 2) {
+            const bool swap = c[v] < c[v + 1];
+            const double hi = swap ? c[v + 1] : c[v], lo = swap ? c[v] : c[v + 1];
+            const int eh = swap ? expert[v + 1] : expert[v], el = swap ? expert[v] : expert[v + 1];
+            c[v] = hi;
+            c[v + 1] = lo;
+            expert[v] = eh;
+            expert[v + 1] = el;
+        }
     int mine = -1;
     for (int i = 0; i < p.k; ++i) {
-        double top = c[0];
+        const double top = wave_max(c[0]);
+        const uint64_t holders = __ballot(c[0] == top);
+        const int holder = holders ? __builtin_ctzll(holders) : 0;
+        const int e = top > none ? __builtin_amdgcn_readlane(expert[0], holder) : -1;
+        if (lane == holder) {
 #pragma unroll
-        for (int v = 1; v < W; ++v) top = fmax(top, c[v]);
-        top = wave_max(top);
-        int e = -1;  // the lowest index of that value
-#pragma unroll
-        for (int v = W - 1; v >= 0; --v) {
-            const uint64_t at = __ballot(c[v] == top);
-            e = at ? 64 * v + __builtin_ctzll(at) : e;
+            for (int v = 0; v + 1 < W; ++v) {
+                c[v] = c[v + 1];
+                expert[v] = expert[v + 1];
+            }
+            c[W - 1] = none;
         }
-        if (!(top > none)) e = -1;
-#pragma unroll
-        for (int v = 0; v < W; ++v)
-            if (e == 64 * v + lane) c[v] = none;
         if ((lane & 15) == i) mine = e;
     }
     return mine;
@@ -587,7 +699,7 @@ __global__ __launch_bounds__(V > 16 ? 512 : 1024) void route_scored_kernel(Route
     for (uint64_t left = __ballot(!sure && l == 0); left; left &= left - 1) {
         const int first = __builtin_ctzll(left);
         bool wrong;
-        const int c = select_wave<V, DT>(p, __builtin_amdgcn_readlane(in, first), wrong);
+        const int c = select_wave<V, DT, G>(p, __builtin_amdgcn_readlane(in, first), wrong);
         if ((int)(threadIdx.x & 48) == first) {
             mine = c;
             bad = wrong;
@@ -609,9 +721,19 @@ __global__ __launch_bounds__(V > 16 ? 512 : 1024) void route_scored_kernel(Route
     const int rank = slot ? __popcll(s_mask[mine] & ((1ull << rl) - 1)) : -1;
     if (gridDim.x > 1) {
         if (entry) p.slot_of[at] = rank;  // the rank within the block, until the placement
-        for (int e = threadIdx.x; e < p.E; e += blockDim.x)
-            p.block_counts[p.by_block ? (int64_t)blockIdx.x * p.E + e : (int64_t)e * gridDim.x + blockIdx.x] =
-                __popcll(s_mask[e]);
+        if (p.by_block) {
+            const int words = (p.E + 3) / 4;
+            for (int i = threadIdx.x; i < words; i += blockDim.x) {
+                uint32_t w = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (4 * i + j < p.E) w |= (uint32_t)__popcll(s_mask[4 * i + j]) << (8 * j);
+                p.block_counts[blockIdx.x * words + i] = (int32_t)w;
+            }
+        } else {
+            for (int e = threadIdx.x; e < p.E; e += blockDim.x)
+                p.block_counts[(int64_t)e * gridDim.x + blockIdx.x] = __popcll(s_mask[e]);
+        }
         return;
     }
     for (int e = threadIdx.x; e < p.E; e += blockDim.x) p.counts[e] = s_cnt[e] = __popcll(s_mask[e]);
@@ -681,46 +803,59 @@ __global__ __launch_bounds__(256) void route_scored_place_kernel(RouteScored p, 
     if (entry) place_entry(p, s_off, i, row, e, rank);
 }
 
-// The same with the scans over the blocks, for few counts (kScoredPlaceCounts): a workgroup for each
-// block of rows, which sums every expert's counts, and those before its own block, by itself (4099
-// rows of 60 experts: 4.9 us, the two launches 2.8 + 3.6).
-constexpr int kScoredPlaceCounts = 16384;
+// The same with the scans over the blocks, for few counts (kScoredPlaceWords): a workgroup for each
+// block of rows, which sums every expert's counts, and those before its own block, by itself.  A
+// block has at most 64 rows, so its counts are bytes, four experts a word, summed in pairs of 16
+// bits (an expert's count is at most the rows, below 65536); a thread loads 16 words at most, all
+// at once, and places one entry.  4096 rows of 60 experts: 4.8 us behind the selection, 16384 of 256
+// 6.9, where the two launches took 5.7 and 9.5.
+constexpr int kScoredPlaceThreads = 1024, kScoredPlaceWords = 16 * kScoredPlaceThreads;
 
-__global__ __launch_bounds__(256) void route_scored_scan_place_kernel(RouteScored p, int blocks,
-                                                                      int block_rows) {
-    __shared__ int32_t s_off[kScoredMaxExperts + 1], s_all[kScoredMaxExperts], s_before[kScoredMaxExperts];
+__global__ __launch_bounds__(kScoredPlaceThreads) void route_scored_scan_place_kernel(RouteScored p,
+                                                                                      int blocks,
+                                                                                      int block_rows) {
+    static_assert(kScoredMaxK * 64 <= kScoredPlaceThreads, "a thread an entry");
+    __shared__ uint32_t s_sum[4][kScoredMaxExperts / 4];  // even and odd bytes: all, before this block
+    __shared__ int32_t s_all[kScoredMaxExperts], s_before[kScoredMaxExperts], s_off[kScoredMaxExperts + 1];
     const int tid = threadIdx.x;
-    // as many threads an expert as there are, a run of the blocks each
-    const int parts = max(256 / p.E, 1);
-    for (int e = tid; e < p.E; e += 256) s_all[e] = s_before[e] = 0;
+    const int64_t i = (int64_t)blockIdx.x * block_rows * p.k + tid;
+    const bool entry = tid < block_rows * p.k && i < (int64_t)p.rows * p.k;
+    const int e = entry ? p.selected[i] : -1, rank = entry ? p.slot_of[i] : 0;
+    const int words = (p.E + 3) / 4, parts = min(kScoredPlaceThreads / words, (blocks + 15) / 16);
+    if (tid < kScoredMaxExperts) (&s_sum[0][0])[tid] = 0;
     __syncthreads();
-    for (int t = tid; t < p.E * parts; t += 256) {
-        const int part = t / p.E, e = t - part * p.E;
-        const int32_t* column = p.block_counts + e;
+    const int part = tid / words, w = tid - part * words;
+    if (part < parts) {
+        const uint32_t* column = reinterpret_cast<const uint32_t*>(p.block_counts) + w;
         const int b0 = blocks * part / parts, b1 = blocks * (part + 1) / parts;
-        int before = 0, all = 0;
+        uint32_t even = 0, odd = 0, even_before = 0, odd_before = 0;
 #pragma unroll 16
         for (int b = b0; b < b1; ++b) {
-            const int v = column[b * p.E];
-            all += v;
-            before += b < (int)blockIdx.x ? v : 0;
+            const uint32_t c = column[b * words], lo = c & 0x00FF00FFu, hi = (c >> 8) & 0x00FF00FFu;
+            even += lo;
+            odd += hi;
+            even_before += b < (int)blockIdx.x ? lo : 0;
+            odd_before += b < (int)blockIdx.x ? hi : 0;
         }
-        atomicAdd(&s_all[e], all);  // (whole numbers: in any order)
-        atomicAdd(&s_before[e], before);
+        atomicAdd(&s_sum[0][w], even);  // (whole numbers: in any order)
+        atomicAdd(&s_sum[1][w], odd);
+        atomicAdd(&s_sum[2][w], even_before);
+        atomicAdd(&s_sum[3][w], odd_before);
+    }
+    __syncthreads();
+    if (tid < p.E) {
+        const int shift = tid & 2 ? 16 : 0;
+        s_all[tid] = (s_sum[tid & 1][tid >> 2] >> shift) & 0xFFFF;
+        s_before[tid] = (s_sum[2 + (tid & 1)][tid >> 2] >> shift) & 0xFFFF;
     }
     __syncthreads();
     scan_counts(s_all, p.E, s_off);
     __syncthreads();
     if (blockIdx.x == 0) {
-        for (int j = tid; j <= p.E; j += 256) p.offsets[j] = s_off[j];
-        for (int j = tid; j < p.E; j += 256) p.counts[j] = s_all[j];
+        if (tid <= p.E) p.offsets[tid] = s_off[tid];
+        if (tid < p.E) p.counts[tid] = s_all[tid];
     }
-    const int64_t first = (int64_t)blockIdx.x * block_rows * p.k;
-    const int64_t end = min(first + (int64_t)block_rows * p.k, (int64_t)p.rows * p.k);
-    for (int64_t i = first + tid; i < end; i += 256) {
-        const int e = p.selected[i];
-        place_entry(p, s_off, i, (int)(i / p.k), e, e >= 0 ? s_before[e] + p.slot_of[i] : -1);
-    }
+    if (entry) place_entry(p, s_off, i, (int)(i / p.k), e, e >= 0 ? s_before[e] + rank : -1);
 }
 
 // ---- gradient ---------------------------------------------------------------------
@@ -902,7 +1037,8 @@ extern "C" int nsosx_moe_route_scored(const void* logits, int logits_dtype, int6
     const int blocks = (rows - 1) / rb + 1;
     const RouteScored p{logits, logits_stride, valid_rows, bias, rows, experts, k, sigmoid != 0, limited,
                         group_keep, group_best, renorm != 0, scale, weights, selected, counts, offsets,
-                        perm, slot_of, workspace, (int64_t)blocks * experts <= kScoredPlaceCounts,
+                        perm, slot_of, workspace,
+                        rows <= 65535 && (int64_t)blocks * ((experts + 3) / 4) <= kScoredPlaceWords,
                         experts / limited, at.lanes, at.values,
                         (experts + 63) / 64 * 64 + 16};  // (four rows' lanes on different banks)
     const int smem = limited > 1 ? (rb * p.pitch + (experts + 3) / 4 * 4) * 4 : 0;
@@ -922,7 +1058,8 @@ extern "C" int nsosx_moe_route_scored(const void* logits, int logits_dtype, int6
 #undef NSOSX_RS_DT
 #undef NSOSX_RS
     if (!select_only && blocks > 1 && p.by_block) {
-        hipLaunchKernelGGL(route_scored_scan_place_kernel, dim3(blocks), dim3(256), 0, st, p, blocks, rb);
+        hipLaunchKernelGGL(route_scored_scan_place_kernel, dim3(blocks), dim3(kScoredPlaceThreads), 0, st, p,
+                           blocks, rb);
     } else if (!select_only && blocks > 1) {
         hipLaunchKernelGGL(route_scored_scan_kernel, dim3((experts + 3) / 4), dim3(256), 0, st,
                            workspace, blocks, experts, counts);

@@ -349,3 +349,53 @@ def test_group_layouts(dev, e, groups, keep, dtype):
             for b in (None, bias):
                 check(dev, x, min(4, keep * (e // groups)), dtype=dtype, score="softmax" if best == 1 else "sigmoid",
                       bias=b, groups=groups, group_keep=keep, group_best=best)
+
+
+@pytest.mark.parametrize("e,k,groups", [(64, 8, 1), (256, 8, 8), (256, 15, 1), (256, 16, 1), (512, 5, 4),
+                                        (40, 1, 1), (24, 11, 2)])
+@pytest.mark.parametrize("near", ["choices", "one more", "two more"])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_only_the_choices_lie_together(dev, e, k, groups, near, score):
+    """The k largest values (and one, or two, behind them) within 2^-24 of each other in an order that
+    32 bits do not show, all others far below: of logits, and of scores with a bias."""
+    rng = np.random.default_rng([e, k, groups])
+    rows, half = 131, e // 2 if groups > 1 else e  # (the near ones in the groups that stay)
+    count = min(k + {"choices": 0, "one more": 1, "two more": 2}[near], half)
+    kw = dict(score=score, groups=groups, group_keep=max(groups // 2, 1))
+    x = rng.uniform(-3, -2, (rows, e))
+    for r in range(rows):
+        at = rng.permutation(half)[:count]
+        x[r, at] = 1.0 + rng.permutation(count) % 5 * 2.0**-23
+        if groups > 1:  # and a value in each of those groups that keeps them clear of the others
+            size = e // groups
+            for g in range(groups // 2):
+                x[r, g * size:g * size + 2] = np.maximum(x[r, g * size:g * size + 2], 0.5 + 0.01 * g)
+    x = x.astype(np.float32)
+    check(dev, x, k, **kw)
+    # sums with a bias: each row's near experts get the same place by their own logits
+    y = x[:1].repeat(rows, 0)
+    s = scores64(y[:1].astype(np.float64), score)[0]
+    bias = np.where(x[0] >= 1.0, 0.9 - s, -0.05).astype(np.float32)
+    check(dev, y, k, bias=bias, **kw)
+
+
+@pytest.mark.parametrize("rows,e,k", [(16384, 256, 8), (16500, 256, 3), (65535, 4, 1), (65536, 4, 1),
+                                      (65535, 5, 3), (8192, 509, 2), (3000, 6, 6)])
+def test_counts_of_blocks(dev, rows, e, k):
+    """Around what the counts' bytes and pairs hold, an expert that every row takes among them."""
+    rng = np.random.default_rng([rows, e])
+    x = rng.normal(0, 1, (rows, e))
+    x[:, e // 2] = 9.0
+    r = ops.moe_route_scored(torch.from_numpy(x.astype(np.float32)).to(dev), k)
+    got = {n: v.cpu().numpy() for n, v in r.items()}
+    want = np.argsort(-x.astype(np.float32), axis=1, kind="stable")[:, :k]
+    np.testing.assert_array_equal(got["selected"], want)
+    counts = np.bincount(want.ravel(), minlength=e)
+    offsets = np.concatenate([[0], np.cumsum(counts)])
+    # slots: expert-major, rows ascending
+    perm = np.argsort(want.ravel(), kind="stable")
+    slot_of = np.empty(rows * k, np.int64)
+    slot_of[perm] = np.arange(rows * k)
+    for n, v in (("counts", counts), ("offsets", offsets), ("perm", perm // k),
+                 ("slot_of", slot_of.reshape(rows, k))):
+        np.testing.assert_array_equal(got[n], v, err_msg=n)
