@@ -116,9 +116,9 @@ static void launch_grouped_t(const I8Group& gp, void* y, hipStream_t st) {
 }
 
 // Which tile takes a shape: the estimated time of each in us, fitted to sweeps of K 64 .. 8192,
-// N 96 .. 8192 and 1 .. 8192 rows with the weights from HBM (within 9 % of the measured times on
-// average, and the choice within 1 % of the best one's time, 15 % at most, for K of 512 and more): a
-// fixed part and one per round of 256 tiles, linear in K but no less than the tile's outputs and its
+// N 16 .. 8192 and 1 .. 16384 rows with the weights from HBM (within 10 % of the measured times on
+// average, and the choice within 1 % of the best one's time on average, 27 % at most): a fixed part
+// and one per round of 256 tiles, linear in K but no less than the tile's outputs and its
 // start take.  A round is a whole one where a compute unit holds one workgroup.  Measured, us (16 x
 // 16 / 16 x 64 / 32 x 64 / 64 x 64 / 128 x 128 / 256 x 256):
 //   K 4096, N 4096:    1 row   5.1 /  5.9 /  6.8 / 10.0 / 21   / 47
@@ -142,8 +142,8 @@ static I8Tile choose_tile(int K, bool aligned, Tiles tiles) {
     auto part = [](double t) { return std::max(1.0, t / 256); };
     auto whole = [](double t) { return std::max(1.0, std::ceil(t / 256)); };
     const double cost[] = {
-        2.8 - 0.2 * k + part(tiles(16, 16)) * std::max(0.8, 0.63 * k),
-        1.7 - 0.65 * k + part(tiles(16, 64)) * std::max(2.0, 1.26 + 1.52 * k),
+        2.2 - 0.15 * k + part(tiles(16, 16)) * std::max(0.9, 0.7 + 0.45 * k),
+        1.6 - k + whole(tiles(16, 64)) * std::max(2.3, 1.64 + 1.75 * k),
         2.6 - 0.4 * k + whole(tiles(32, 64)) * std::max(1.4, 0.6 + 1.66 * k),
         1.0 - 0.5 * k + whole(tiles(64, 64)) * std::max(4.0, 3.25 + 2.43 * k),
         2.7 + 0.8 * k + part(tiles(128, 128)) * std::max(2.6, 1.2 + 4.2 * k),
