@@ -806,8 +806,8 @@ __global__ __launch_bounds__(256) void route_scored_place_kernel(RouteScored p, 
 // The same with the scans over the blocks, for few counts (kScoredPlaceWords): a workgroup for each
 // block of rows, which sums every expert's counts, and those before its own block, by itself.  A
 // block has at most 64 rows, so its counts are bytes, four experts a word, summed in pairs of 16
-// bits (an expert's count is at most the rows, below 65536); a thread loads 16 words at most, all
-// at once, and places one entry.  4096 rows of 60 experts: 4.8 us behind the selection, 16384 of 256
+// bits (an expert's count is at most the rows, below 65536); a thread loads its words (16, a few
+// more at some widths) 16 at once, without a branch, and places one entry.  4096 rows of 60 experts: 4.8 us behind the selection, 16384 of 256
 // 6.8, where the two launches took 5.7 (their counts summed in one) and 7.7.
 constexpr int kScoredPlaceThreads = 1024, kScoredPlaceWords = 16 * kScoredPlaceThreads;
 
@@ -829,13 +829,19 @@ __global__ __launch_bounds__(kScoredPlaceThreads) void route_scored_scan_place_k
         const uint32_t* column = reinterpret_cast<const uint32_t*>(p.block_counts) + w;
         const int b0 = blocks * part / parts, b1 = blocks * (part + 1) / parts;
         uint32_t even = 0, odd = 0, even_before = 0, odd_before = 0;
-#pragma unroll 16
-        for (int b = b0; b < b1; ++b) {
-            const uint32_t c = column[b * words], lo = c & 0x00FF00FFu, hi = (c >> 8) & 0x00FF00FFu;
-            even += lo;
-            odd += hi;
-            even_before += b < (int)blockIdx.x ? lo : 0;
-            odd_before += b < (int)blockIdx.x ? hi : 0;
+        for (int first = b0; first < b1; first += 16) {  // (once or twice; loads past the end are clamped)
+            uint32_t c[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) c[j] = column[min(first + j, b1 - 1) * words];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int b = first + j;
+                const uint32_t lo = b < b1 ? c[j] & 0x00FF00FFu : 0, hi = b < b1 ? (c[j] >> 8) & 0x00FF00FFu : 0;
+                even += lo;
+                odd += hi;
+                even_before += b < (int)blockIdx.x ? lo : 0;
+                odd_before += b < (int)blockIdx.x ? hi : 0;
+            }
         }
         atomicAdd(&s_sum[0][w], even);  // (whole numbers: in any order)
         atomicAdd(&s_sum[1][w], odd);
@@ -1033,7 +1039,9 @@ extern "C" int nsosx_moe_route_scored(const void* logits, int logits_dtype, int6
     // chosen by a wave
     const bool spread = at.values <= 32;
     if (!spread) at = {0, 32};
-    const int rb = scored_block_rows(rows, at.values > 16);
+    // without the dispatch a row needs no other: the smallest blocks (64 rows of 256 experts on one CU
+    // 12 us, on four 7)
+    const int rb = select_only ? 16 : scored_block_rows(rows, at.values > 16);
     const int blocks = (rows - 1) / rb + 1;
     const RouteScored p{logits, logits_stride, valid_rows, bias, rows, experts, k, sigmoid != 0, limited,
                         group_keep, group_best, renorm != 0, scale, weights, selected, counts, offsets,
