@@ -78,9 +78,9 @@ __device__ __forceinline__ void row_values(const void* x, int64_t base, int E, b
     for (int v = 0; v < V; ++v) c[v] = live && 16 * v + l < E ? c[v] : -INFINITY;
 }
 
-// Floats first .. first + n - 1 of a row in LDS, -inf behind them; in 16-byte pieces where every
-// lane's run allows it.
-template <int V>
+// Floats first .. first + n - 1 of a row in LDS, behind them -inf (or, where FILL is not, any value of
+// the run); in 16-byte pieces where every lane's run allows it.
+template <int V, bool FILL = true>
 __device__ __forceinline__ void run_values(const float* row, int first, int n, bool pieces, float (&c)[V]) {
     if (pieces && V >= 4) {
 #pragma unroll
@@ -92,8 +92,10 @@ __device__ __forceinline__ void run_values(const float* row, int first, int n, b
 #pragma unroll
         for (int v = 0; v < V; ++v) c[v] = row[first + (v < n ? v : 0)];
     }
+    if constexpr (FILL) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) c[v] = v < n ? c[v] : -INFINITY;
+        for (int v = 0; v < V; ++v) c[v] = v < n ? c[v] : -INFINITY;
+    }
 }
 
 template <int CTRL>
@@ -275,11 +277,13 @@ __device__ __forceinline__ int select_fast(const RouteScored& p, int64_t row, bo
         const int n = real ? min(p.run, p.size - at) : 0;
         const bool pieces = p.size % 4 == 0 && p.run % 4 == 0;
         run_values<V>(s_row, first, n, pieces, x);
-        if (p.bias) run_values<V>(s_bias, first, n, pieces, b);
+        if (p.bias) run_values<V, false>(s_bias, first, n, pieces, b);
     } else if (p.bias) {
         row_values<V, NSOSX_F32>(p.bias, 0, p.E, true, b);
     }
     float err = 0.0f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) c[v] = x[v];
     if (!p.sigmoid) {
         float mx = x[0];
 #pragma unroll
@@ -304,14 +308,13 @@ __device__ __forceinline__ int select_fast(const RouteScored& p, int64_t row, bo
             c[v] = x[v] == none ? none : __builtin_amdgcn_rcpf(1.0f + __expf(-x[v]));
         err = 0x1p-22f;
     }
-    if (p.bias) {
+    if (p.bias) {  // (-inf stays, unless the bias is infinite or a NaN: then the row is odd)
 #pragma unroll
-        for (int v = 0; v < V; ++v) c[v] = c[v] == none ? none : c[v] + b[v];
+        for (int v = 0; v < V; ++v) c[v] += b[v];
     }
     float mx = none;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        if (!scored) c[v] = x[v];
         odd |= c[v] != c[v];
         mx = fmaxf(mx, c[v]);
     }
@@ -352,8 +355,10 @@ __device__ __forceinline__ int select_fast(const RouteScored& p, int64_t row, bo
         const float top = (float)(1u << NB) - (NB > 24 ? (float)(1u << (NB - 24)) : 1.0f);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const float t = fminf(fmaxf((c[v] - base) * scale, 0.0f), top);
-            key[v] = open && c[v] != none ? ((uint32_t)t << IB) | (kIndex - (first + v * step)) : 0u;
+            // (nothing available, -inf, lies below the window, whose keys are never trusted; an index
+            // past the last expert's is one of those)
+            const float t = fminf(fmaxf(((open ? c[v] : none) - base) * scale, 0.0f), top);
+            key[v] = ((uint32_t)t << IB) | ((kIndex - (first + v * step)) & kIndex);
         }
         // both values' errors, the difference's and the product's rounding, the truncation
         if (keyed) apart = (uint32_t)fminf(2.0f * err * scale, 1e9f) + (1u << (NB > 24 ? NB - 23 : 1)) + 2;
