@@ -385,8 +385,8 @@ __device__ __forceinline__ int select_fast(const RouteScored& p, int64_t row, bo
     next(p.k);  // (it only has to be apart from the last choice)
     odd = row_any(odd);
     sure = !live || (ok && inside && clear && !odd);
-    int choice = l >= p.k || mine == 0 ? -1
-                                       : exact ? (int)(0xFFFFu - (mine & 0xFFFFu)) : (int)(kIndex - (mine & kIndex));
+    int choice = exact ? (int)(0xFFFFu - (mine & 0xFFFFu)) : (int)(kIndex - (mine & kIndex));
+    if (l >= p.k || mine == 0) choice = -1;
     // Only choices too close to each other: where the k + 1 largest are apart from all others, they are
     // put in order in 64 bits, one a lane.
     const bool close = live && ok && inside && !clear && !odd && !exact && p.k < 16 && (!p.bias || p.sigmoid);

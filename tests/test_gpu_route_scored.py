@@ -399,3 +399,18 @@ def test_counts_of_blocks(dev, rows, e, k):
     for n, v in (("counts", counts), ("offsets", offsets), ("perm", perm // k),
                  ("slot_of", slot_of.reshape(rows, k))):
         np.testing.assert_array_equal(got[n], v, err_msg=n)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e,groups", [(24, 1), (24, 4), (256, 8), (300, 1)])
+def test_infinite_biases(dev, score, e, groups):
+    """-inf takes an expert out for every row, +inf puts one first, also where a logit is -inf."""
+    rng = np.random.default_rng([e, groups])
+    x = rng.normal(0, 1, (70, e)).astype(np.float32)
+    x[::3, 5] = x[1::4, 7] = -np.inf
+    bias = rng.normal(0, 0.1, e).astype(np.float32)
+    bias[2] = bias[7] = -np.inf
+    kw = dict(score=score, groups=groups, group_keep=max(groups // 2, 1))
+    check(dev, x, 4, bias=bias, **kw)
+    bias[5] = np.inf
+    check(dev, x, 4, bias=bias, **kw)
