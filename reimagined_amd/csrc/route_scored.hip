@@ -114,10 +114,15 @@ __device__ __forceinline__ void outranked(float s, int q, int& lanes) {
 __device__ __forceinline__ float row_min(float v) { return -row_max(-v); }
 
 // Whether this lane's group is one of the `keep` best (ties to the lower group), from the values of
-// its experts; -inf, an unavailable expert, adds nothing.  gap: what the worst group that stays has
-// over the best one that goes.
+// its experts; -inf, an unavailable expert, adds nothing.  err: the scores' error.  clear: whether
+// every group that stays is above every one that goes by more than both groups' errors.  Those are each
+// group's own: its two scores', and, in units u = 2^-23, half a unit of each value (the sum with the
+// bias), of the group's sum, and of that less or plus `room`, together below 1.5 u (|a| + |b|).  Where a
+// group's second value holds a mask that is large and finite (-1e4, say), that is far more than
+// the row's largest value would give.
 template <int V>
-__device__ __forceinline__ bool group_stays(const RouteScored& p, const float (&c)[V], int q, float& gap) {
+__device__ __forceinline__ bool group_stays(const RouteScored& p, const float (&c)[V], int q, float err,
+                                            bool& clear) {
     const float none = -INFINITY;
     float a = none, b = none;  // the group's two largest
 #pragma unroll
@@ -128,7 +133,8 @@ __device__ __forceinline__ bool group_stays(const RouteScored& p, const float (&
     if (p.lanes >= 2) join2<0xB1>(a, b);   // lane l ^ 1
     if (p.lanes >= 4) join2<0x4E>(a, b);   // lane l ^ 2
     if (p.lanes >= 8) join2<0x141>(a, b);  // lane l ^ 7: the other four of eight
-    float s = p.best == 2 && b > none ? a + b : a;
+    const bool two = p.best == 2 && b > none;
+    float s = two ? a + b : a;
     if (q >= p.groups) s = none;
     int better = 0;  // lanes of better groups
     outranked<1>(s, q, better); outranked<2>(s, q, better); outranked<3>(s, q, better);
@@ -137,7 +143,11 @@ __device__ __forceinline__ bool group_stays(const RouteScored& p, const float (&
     outranked<10>(s, q, better); outranked<11>(s, q, better); outranked<12>(s, q, better);
     outranked<13>(s, q, better); outranked<14>(s, q, better); outranked<15>(s, q, better);
     const bool in = q < p.groups && better < p.keep * p.lanes;
-    gap = row_min(in ? s : INFINITY) - row_max(in ? none : s);
+    // (each term by itself: |a| + |b| may pass the largest float)
+    const float room = 2.0f * err + 0x1p-22f * fabsf(a) + (two ? 0x1p-22f * fabsf(b) : 0.0f);
+    const float low = row_min(in ? s - room : INFINITY);
+    // (a group without an available expert, which ranks last, has s and room infinite)
+    clear = low > row_max(in || s == none ? none : s + room);
     return in;
 }
 
@@ -320,13 +330,12 @@ __device__ __forceinline__ int select_fast(const RouteScored& p, int64_t row, bo
     }
     mx = row_max(mx);
     odd |= mx == INFINITY;
-    if (scored) err += 0x1p-23f * fabsf(mx);
     bool ok = true, open = true;
     if (G) {
-        float gap;
-        open = group_stays<V>(p, c, l / lanes, gap);
-        ok = err == 0.0f || gap > 6.0f * err;  // two errors a group, the sums' rounding one more
+        open = group_stays<V>(p, c, l / lanes, err, ok);
+        ok = ok || !scored;  // (the largest logits themselves: equal ones go by the index)
     }
+    if (scored) err += 0x1p-23f * fabsf(mx);
     if (!p.bias) {  // the experts by their logits
         mx = none;
 #pragma unroll

@@ -414,3 +414,41 @@ def test_infinite_biases(dev, score, e, groups):
     check(dev, x, 4, bias=bias, **kw)
     bias[5] = np.inf
     check(dev, x, 4, bias=bias, **kw)
+
+
+@pytest.mark.parametrize("mask", [-20.0, -100.0, -1e3, -1e4, -1e5, 1e4])
+@pytest.mark.parametrize("usable", [1, 2])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [True, False])
+def test_groups_behind_large_finite_biases(dev, mask, usable, score, renorm):
+    """A mask that stays finite on all but `usable` experts of a group: with one, a group's score holds
+    the mask, and its step in 32 bits is far above that of the scores.  The groups' sums lie
+    within a few such steps of each other, in an order that only 64 bits show."""
+    rng = np.random.default_rng([int(abs(mask)), usable, score == "softmax"])
+    rows, groups, size = 400, 4, 4
+    step = float(np.spacing(np.float32(abs(mask))))
+    s = rng.uniform(0.02, 0.03, (rows, groups, size))
+    s[:, :, 0] = rng.uniform(0.3, 0.6, (rows, groups))
+    s[:, :, 1] = np.clip(0.9 - s[:, :, 0] + rng.uniform(-2, 2, (rows, groups)) * step, 1e-3, 0.95)
+    s = s.reshape(rows, -1)
+    x = (np.log(s) if score == "softmax" else np.log(s / (1 - s))).astype(np.float32)
+    bias = np.zeros((groups, size), np.float32)
+    bias[:, usable:] = mask
+    check(dev, x, 2, score=score, bias=bias.ravel(), groups=groups, group_keep=2, renorm=renorm, scale=2.5)
+
+
+def test_groups_of_two_masks(dev):
+    """Sums of -9999.173378 and -9999.173233, which rounding to 32 bits puts in the other order."""
+    x = np.array([[-0.50692, -0.19781, 0.52821, -1.40072]], np.float32)
+    check(dev, x, 1, score="sigmoid", bias=np.array([0, -1e4, 0, -1e4], np.float32), groups=2, group_keep=1)
+
+
+@pytest.mark.parametrize("mask", [-1e3, -1e5, float(np.finfo(np.float32).min)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_groups_masked_whole(dev, mask, score):
+    """Groups without a usable expert beside groups with one, two and all of them."""
+    rng = np.random.default_rng(13)
+    x = rng.normal(0, 1.5, (300, 48)).astype(np.float32)
+    bias = rng.normal(0, 0.1, (6, 8)).astype(np.float32)
+    bias[0] = bias[1, 1:] = bias[3, 2:] = mask
+    check(dev, x, 3, score=score, bias=bias.ravel(), groups=6, group_keep=3)
