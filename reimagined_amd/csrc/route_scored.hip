@@ -921,6 +921,7 @@ __global__ __launch_bounds__(256) void route_scored_bwd_kernel(RouteScoredBwd p)
     const bool dense = !p.renorm && !p.sigmoid;
     float mx = none, sum = 1.0f, dot = 0.0f;
     float all[V];
+    const bool chosen = row_any(e >= 0);  // a row without a choice, padding's, may hold anything
     if (dense) {
         row_values<V, DT>(p.logits, base, p.E, live, all);
         softmax_stats<V>(all, mx, sum);
@@ -957,7 +958,8 @@ __global__ __launch_bounds__(256) void route_scored_bwd_kernel(RouteScoredBwd p)
             const int j = 16 * v + l;
             if (j < p.E) {
                 const float d = s_g[rl * p.E + j];
-                s_g[rl * p.E + j] = all[v] == none ? 0.0f : (expf(all[v] - mx) / sum) * (d - dot);
+                s_g[rl * p.E + j] =
+                    !chosen || all[v] == none ? 0.0f : (expf(all[v] - mx) / sum) * (d - dot);
             }
         }
     }

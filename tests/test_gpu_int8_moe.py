@@ -257,3 +257,25 @@ def test_same_bits_every_time(dev):
         if first is None:
             first = [v.clone() for v in now]
         assert all(torch.equal(a, b) for a, b in zip(now, first))
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [True, False])
+def test_router_gradient_of_padding_rows(dev, score, renorm):
+    """Padding rows whose logits and output gradients are NaN or infinite leave the gate's gradient,
+    dlogits^T x, what it is without them."""
+    rng = np.random.default_rng(8)
+    up, down = experts(rng, 6, 96, 64)
+    moe = Int8MoEFFN(up, down, dev, k=2, score=score, renorm=renorm)
+    x, logits, dout = (torch.randn(20, c, device=dev) for c in (64, 6, 64))
+    pad, rest = [0, 5, 19], [i for i in range(20) if i not in (0, 5, 19)]
+    logits[0, 2], logits[5], logits[19, 0] = torch.nan, torch.inf, -torch.inf
+    logits[19, 1] = torch.inf
+    dout[pad] = torch.nan
+    valid = np.ones(20, np.uint8)
+    valid[pad] = 0
+    g = moe.router_backward(logits, moe.forward(x, logits, valid_rows=valid), dout)
+    part = [v[rest].contiguous() for v in (x, logits, dout)]
+    want = moe.router_backward(part[1], moe.forward(part[0], part[1]), part[2])
+    assert (g["dlogits"][pad] == 0).all() and (g["dweights"][pad] == 0).all()
+    assert torch.isfinite(want["dlogits"]).all() and torch.equal(g["dlogits"][rest], want["dlogits"])

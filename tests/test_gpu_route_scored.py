@@ -452,3 +452,29 @@ def test_groups_masked_whole(dev, mask, score):
     bias = rng.normal(0, 0.1, (6, 8)).astype(np.float32)
     bias[0] = bias[1, 1:] = bias[3, 2:] = mask
     check(dev, x, 3, score=score, bias=bias.ravel(), groups=6, group_keep=3)
+
+
+@pytest.mark.parametrize("e,k", [(12, 4), (256, 8)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradient_of_padding_rows_that_hold_anything(dev, e, k, score, renorm, dtype):
+    """NaN and infinite logits, and gradients, of a padding row: its gradient is zero, the other rows'
+    are what they are without it."""
+    rng = np.random.default_rng([e, k])
+    x = torch.from_numpy(rng.normal(0, 1.5, (40, e)).astype(np.float32)).to(dtype)
+    x[1, 3], x[2, :], x[7, 0], x[8, 1] = torch.nan, torch.nan, torch.inf, -torch.inf
+    x[9, :], x[39, e - 1] = torch.inf, torch.nan
+    pad = [1, 2, 7, 8, 9, 39]
+    valid = np.ones(40, np.uint8)
+    valid[pad] = 0
+    x = x.to(dev)
+    r = ops.moe_route_scored(x, k, score=score, renorm=renorm, valid_rows=valid)
+    g = torch.from_numpy(rng.normal(0, 1, (40, k)).astype(np.float32))
+    g[pad] = torch.nan
+    got = ops.moe_route_scored_backward(x, r["selected"], g.to(dev), score=score, renorm=renorm)
+    assert (got[pad] == 0).all()
+    rest = [i for i in range(40) if i not in pad]
+    alone = ops.moe_route_scored_backward(x[rest].contiguous(), r["selected"][rest].contiguous(),
+                                          g[rest].to(dev), score=score, renorm=renorm)
+    assert torch.isfinite(alone).all() and torch.equal(got[rest], alone)
