@@ -615,7 +615,7 @@ int nsosx_moe_combine_topk(const void* expert_out, int in_dtype, const int32_t* 
  * dweights[r, i] = <dout[r], expert_out[slot_of[r, i]]> (f32; 0 for a slot outside
  * [0, slots)).  perm (int32 [slots], the routing's) or NULL: rows of dexpert whose perm is -1
  * are written as zeros; with NULL the rows that no slot_of names are left as they were.  No
- * slot may be named twice; dexpert must not overlap an input. */
+ * slot may be named twice; dexpert must not overlap an input or dweights. */
 int nsosx_moe_combine_topk_backward(const void* dout, int dout_dtype, const void* expert_out,
                                     int expert_dtype, const int32_t* slot_of,
                                     const float* weights, const int32_t* perm, int rows,

@@ -240,8 +240,13 @@ extern "C" int nsosx_moe_combine_topk_backward(const void* dout, int dout_dtype,
         return fail(NSOSX_ERR_INVALID, "moe_combine_topk_backward: bad dtype");
     const int64_t db = (int64_t)rows * dim * (dout_dtype == NSOSX_F32 ? 4 : 2);
     const int64_t eb = (int64_t)slots * dim * (expert_dtype == NSOSX_F32 ? 4 : 2);
-    if (overlaps(dexpert, eb, expert_out, eb) || overlaps(dexpert, eb, dout, db))
+    const int64_t kb = (int64_t)rows * k * 4;
+    if (overlaps(dexpert, eb, expert_out, eb) || overlaps(dexpert, eb, dout, db) ||
+        overlaps(dexpert, eb, slot_of, kb) || overlaps(dexpert, eb, weights, kb) ||
+        (perm && overlaps(dexpert, eb, perm, (int64_t)slots * 4)))
         return fail(NSOSX_ERR_INVALID, "moe_combine_topk_backward: dexpert overlaps an input");
+    if (overlaps(dexpert, eb, dweights, kb))
+        return fail(NSOSX_ERR_INVALID, "moe_combine_topk_backward: dexpert overlaps dweights");
     const bool v8 = vector_rows(dim, dout, expert_out, dexpert);
     const int per = v8 ? 512 : 64;
     const int waves = dim > 2 * per ? 4 : dim > per ? 2 : 1;

@@ -170,3 +170,15 @@ I8, F, I32 = torch.int8, torch.float32, torch.int32
 def test_wrapper_refusals_on_cpu_tensors(fn, text):
     with pytest.raises(ValueError, match=text):
         fn()
+
+
+@pytest.mark.parametrize("meets", ["slot_of", "weights", "perm", "dweights"])
+@pytest.mark.parametrize("end", ["first", "last"])
+def test_combine_backward_overlaps(meets, end):
+    """dexpert: 8 slots of 16 floats at 4 P, over the first or the last bytes of the small arrays (4 rows
+    of k 2, 32 bytes, and 8 slots' perm, 32 too)."""
+    at, far = 4 * P, {n: (8 + i) * P for i, n in enumerate(("slot_of", "weights", "perm", "dweights"))}
+    far[meets] = at + 8 * 16 * 4 - 4 if end == "first" else at - 28
+    text = refused("nsosx_moe_combine_topk_backward", P, 0, 2 * P, 0, far["slot_of"], far["weights"], far["perm"], 4,
+                   8, 2, 16, at, far["dweights"], None)
+    assert "overlaps dweights" in text if meets == "dweights" else "overlaps an input" in text
