@@ -201,7 +201,7 @@ __device__ __forceinline__ void i8_store4(const I8Problem& pb, const I8Rows& row
 // ===========================================================================
 template <int NT, int MT, int W, int D>
 constexpr int i8_split_smem() {
-    const int ring = W * D * (NT + MT) * 1024, sums = W > 1 ? W * NT * MT * 1024 : 0;
+    const int ring = W * D * (NT + MT) * 1024, sums = W * NT * MT * 1024;
     return ring > sums ? ring : sums;
 }
 
@@ -296,27 +296,19 @@ __device__ __forceinline__ void i8_split_tile(const I8Problem& pb, const I8Rows&
         mul();
     }
     // accumulator c of lane l: output n0 + 16 n + 4 (l / 16) + c, token m0 + 16 t + l % 16
-    if constexpr (W > 1) {
-        __syncthreads();  // every wave is done with its ring
-        char* part = smem + wave * (NT * MT * 1024) + lane * 16;
+    __syncthreads();  // every wave is done with its ring
+    char* part = smem + wave * (NT * MT * 1024) + lane * 16;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int t = 0; t < MT; ++t) *reinterpret_cast<i8x16*>(part + (n * MT + t) * 1024) = acc[n][t];
-        __syncthreads();
-        for (int i = wave; i < NT * MT; i += W) {  // the waves share the 16 x 16 tiles out
-            i8x16 sum = {0, 0, 0, 0};
+        for (int t = 0; t < MT; ++t) *reinterpret_cast<i8x16*>(part + (n * MT + t) * 1024) = acc[n][t];
+    __syncthreads();
+    for (int i = wave; i < NT * MT; i += W) {  // the waves share the 16 x 16 tiles out
+        i8x16 sum = {0, 0, 0, 0};
 #pragma unroll
-            for (int p = 0; p < W; ++p)
-                sum += *reinterpret_cast<const i8x16*>(smem + (p * NT * MT + i) * 1024 + lane * 16);
-            i8_store4<YDT>(pb, rows, n0 + 16 * (i / MT) + 4 * g, m0 + 16 * (i % MT) + r, sum, y);
-        }
-    } else {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-                i8_store4<YDT>(pb, rows, n0 + 16 * n + 4 * g, m0 + 16 * t + r, acc[n][t], y);
+        for (int p = 0; p < W; ++p)
+            sum += *reinterpret_cast<const i8x16*>(smem + (p * NT * MT + i) * 1024 + lane * 16);
+        i8_store4<YDT>(pb, rows, n0 + 16 * (i / MT) + 4 * g, m0 + 16 * (i % MT) + r, sum, y);
     }
 }
 
