@@ -644,6 +644,13 @@ int nsosx_grouped_int8_gemm(const int8_t* q, const float* act_scale, int q_rows,
                             const int32_t* perm, int slots, int experts, int K, int N,
                             int squared_relu, void* y, int y_dtype, void* stream);
 
+/* Which tile (outputs x tokens) a product of `rows` rows (or slots) takes: 0 for 16 x 16, 1 for
+ * 16 x 64, 2 for 32 x 64, 3 for 64 x 64, 4 for 128 x 128, 5 for 256 x 256; -1 for sizes that are refused.
+ * experts 0: nsosx_int8_gemm, else nsosx_grouped_int8_gemm.  aligned: q and w start on 16 bytes (a
+ * K that is no multiple of 16 makes unaligned rows by itself).  Every tile gives the same bits;
+ * this is for tests and timings that have to know which one ran. */
+int nsosx_int8_gemm_tile(int rows, int K, int N, int experts, int aligned);
+
 /* ---------------------------------------------------------------------------
  * Row norms of the hybrid block and the decode conv ring.
  * ------------------------------------------------------------------------- */

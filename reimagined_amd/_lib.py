@@ -92,6 +92,7 @@ SIGNATURES = {
     "nsosx_moe_combine_topk": (_i, [_vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _i, _vp]),
     "nsosx_moe_combine_topk_backward": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _vp,
                                              _vp, _vp]),
+    "nsosx_int8_gemm_tile": (_i, [_i, _i, _i, _i, _i]),
     "nsosx_int8_gemm": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _vp]),
     "nsosx_grouped_int8_gemm": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i,
                                      _vp, _i, _vp]),

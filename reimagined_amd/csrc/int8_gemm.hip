@@ -134,6 +134,12 @@ static void launch_grouped_t(const I8Group& gp, void* y, hipStream_t st) {
 constexpr int64_t kI8MaxTiles = 1 << 24;  // of 128 x 128: 256 threads each, less than 2^32
 constexpr int kI8MaxSide = 1 << 30;       // a tile's first row or output, and what it adds, in int
 
+// (experts 0: one matrix)
+static bool too_large(int rows, int N, int experts) {
+    const int64_t mtiles = experts ? (int64_t)rows / 128 + experts : ((int64_t)rows + 127) / 128;
+    return rows > kI8MaxSide || N > kI8MaxSide || ((int64_t)N + 127) / 128 * mtiles >= kI8MaxTiles;
+}
+
 enum class I8Tile { k16x16, k16x64, k32x64, k64x64, k128x128, k256x256 };
 
 template <class Tiles>
@@ -158,12 +164,25 @@ static I8Tile choose_tile(int K, bool aligned, Tiles tiles) {
     return static_cast<I8Tile>(best);
 }
 
+// The tile of M rows and one weight matrix.
+static I8Tile matrix_tile(int M, int K, int N, bool aligned) {
+    return choose_tile(K, aligned, [&](int n, int m) {
+        return (double)((N - 1) / n + 1) * ((M - 1) / m + 1);
+    });
+}
+
+// The tile of the experts' slots, whose counts are on the device: each expert's last tile is taken
+// as three quarters of a tile more than its share.
+static I8Tile experts_tile(int slots, int K, int N, int experts, bool aligned) {
+    return choose_tile(K, aligned, [&](int n, int m) {
+        return (double)((N - 1) / n + 1) *
+               std::min<double>(slots, std::ceil((double)slots / m + 0.75 * experts));
+    });
+}
+
 template <int YDT, bool A>
 static void launch_int8_t(const I8Problem& pb, const I8Rows& rows, void* y, hipStream_t st) {
-    auto tiles = [&](int n, int m) {
-        return (double)((pb.N - 1) / n + 1) * ((rows.count - 1) / m + 1);
-    };
-    switch (choose_tile(pb.K, A, tiles)) {
+    switch (matrix_tile(rows.count, pb.K, pb.N, A)) {
         case I8Tile::k16x16: return launch_gemm_t<Split16x16<A>, YDT>(pb, rows, y, st);
         case I8Tile::k16x64: return launch_gemm_t<Split16x64<A>, YDT>(pb, rows, y, st);
         case I8Tile::k32x64: return launch_gemm_t<Split32x64<A>, YDT>(pb, rows, y, st);
@@ -177,13 +196,7 @@ static void launch_int8_t(const I8Problem& pb, const I8Rows& rows, void* y, hipS
 
 template <int YDT, bool A>
 static void launch_grouped_a(const I8Group& gp, void* y, hipStream_t st) {
-    // the experts' row counts are on the device: each expert's last tile is taken as three quarters
-    // of a tile more than its share
-    auto tiles = [&](int n, int m) {
-        return (double)((gp.N - 1) / n + 1) *
-               std::min<double>(gp.slots, std::ceil((double)gp.slots / m + 0.75 * gp.experts));
-    };
-    switch (choose_tile(gp.K, A, tiles)) {
+    switch (experts_tile(gp.slots, gp.K, gp.N, gp.experts, A)) {
         case I8Tile::k16x16: return launch_grouped_t<Split16x16<A>, YDT>(gp, y, st);
         case I8Tile::k16x64: return launch_grouped_t<Split16x64<A>, YDT>(gp, y, st);
         case I8Tile::k32x64: return launch_grouped_t<Split32x64<A>, YDT>(gp, y, st);
@@ -216,6 +229,14 @@ static void launch_grouped(const I8Group& gp, void* y, hipStream_t st) {
 
 using namespace nsosx;
 
+extern "C" int nsosx_int8_gemm_tile(int rows, int K, int N, int experts, int aligned) {
+    if (rows <= 0 || K <= 0 || K > kI8MaxK || N <= 0 || experts < 0 || experts > kI8MaxExperts ||
+        too_large(rows, N, experts))
+        return -1;
+    const bool a = aligned && K % 16 == 0;
+    return static_cast<int>(experts ? experts_tile(rows, K, N, experts, a) : matrix_tile(rows, K, N, a));
+}
+
 extern "C" int nsosx_int8_gemm(const int8_t* q, const float* act_scale, const int8_t* w,
                                const float* w_scale, const float* bias, int M, int K, int N,
                                void* y, int y_dtype, void* stream) {
@@ -225,8 +246,7 @@ extern "C" int nsosx_int8_gemm(const int8_t* q, const float* act_scale, const in
         return fail(NSOSX_ERR_INVALID, "int8_gemm: M, K and N must be positive");
     if (!valid_dtype(y_dtype)) return fail(NSOSX_ERR_INVALID, "int8_gemm: bad dtype");
     if (K > kI8MaxK) return fail(NSOSX_ERR_OVERFLOW, "int8_gemm: K past the int32 sums (131071)");
-    if (M > kI8MaxSide || N > kI8MaxSide ||
-        ((int64_t)N + 127) / 128 * (((int64_t)M + 127) / 128) >= kI8MaxTiles)
+    if (too_large(M, N, 0))
         return fail(NSOSX_ERR_OVERFLOW, "int8_gemm: M, N or M * N too large");
     const int64_t yb = (int64_t)M * N * (y_dtype == NSOSX_F32 ? 4 : 2);
     if (overlaps(y, yb, q, (int64_t)M * K) || overlaps(y, yb, w, (int64_t)N * K))
@@ -254,8 +274,7 @@ extern "C" int nsosx_grouped_int8_gemm(const int8_t* q, const float* act_scale, 
     if (!valid_dtype(y_dtype)) return fail(NSOSX_ERR_INVALID, "grouped_int8_gemm: bad dtype");
     if (K > kI8MaxK)
         return fail(NSOSX_ERR_OVERFLOW, "grouped_int8_gemm: K past the int32 sums (131071)");
-    if (slots > kI8MaxSide || N > kI8MaxSide ||
-        ((int64_t)N + 127) / 128 * ((int64_t)slots / 128 + experts) >= kI8MaxTiles)
+    if (too_large(slots, N, experts))
         return fail(NSOSX_ERR_OVERFLOW, "grouped_int8_gemm: slots, N or slots * N too large");
     const int64_t yb = (int64_t)slots * N * (y_dtype == NSOSX_F32 ? 4 : 2);
     if (overlaps(y, yb, q, (int64_t)q_rows * K) || overlaps(y, yb, w, (int64_t)experts * N * K))
