@@ -575,8 +575,10 @@ int nsosx_moe_sparse_decode(const nsosx_linear_view* up_views,
  *   weights[r, i] = s of choice i, divided by the sum over the row's choices where renorm != 0,
  *   times scale.  The bias takes part in the choice only.
  * Choices are those of the values in 64 bits, ties to the lower index (groups too); without a
- * bias the order of c is that of x.  An expert whose logit (or c) is -inf is not available: a row with fewer than k available experts gets -1 and weight
- * 0 for the rest.  A row with a NaN score gets the first k experts and NaN weights.
+ * bias the order of c is that of x.  The weights are formed in f32 (exponentials, sum, quotient and
+ * product each rounded).  An expert whose logit (or c) is -inf is not available: a row with
+ * fewer than k available experts gets -1 and weight 0 for the rest.  A row with a NaN score gets
+ * the first k experts and NaN weights.
  *   valid_rows uint8 [rows] or NULL: a row whose byte is 0 is padding (as nsosx_moe_route's):
  *   weights 0, selected and slot_of -1, no slots.
  *   weights f32 [rows, k]; selected int32 [rows, k].
@@ -597,8 +599,8 @@ int nsosx_moe_route_scored(const void* logits, int logits_dtype, int64_t logits_
 /* Gradient of the logits from that of nsosx_moe_route_scored's weights (the choice itself and
  * the bias have none): selected int32 [rows, k] as the forward left it (-1 or an index past E
  * adds nothing, an expert named twice gets both), dweights f32 [rows, k]; dlogits [rows, E]
- * contiguous in logits_dtype, every element written (a padding row's with zeros), which must
- * not overlap the inputs. */
+ * contiguous in logits_dtype, every element written (with zeros in a row without a choice, as a
+ * padding row's, whatever its logits hold), which must not overlap the inputs. */
 int nsosx_moe_route_scored_backward(const void* logits, int logits_dtype, int64_t logits_stride,
                                     const int32_t* selected, const float* dweights, int rows,
                                     int experts, int k, int sigmoid, int renorm, float scale,

@@ -116,8 +116,9 @@ static void launch_grouped_t(const I8Group& gp, void* y, hipStream_t st) {
 }
 
 // Which tile takes a shape: the estimated time of each in us, fitted to sweeps of K 64 .. 8192,
-// N 16 .. 8192 and 1 .. 16384 rows with the weights from HBM (within 10 % of the measured times on
-// average, and the choice within 1 % of the best one's time on average, 27 % at most): a fixed part
+// N 16 .. 8192 and 1 .. 16384 rows with the weights from HBM (330 shapes, of one matrix: within 10 % of
+// the measured times on average, and the choice within 1 % of the best one's time on average, 27 % at
+// most; experts whose rows are very uneven were not among them): a fixed part
 // and one per round of 256 tiles, linear in K but no less than the tile's outputs and its
 // start take.  A round is a whole one where a compute unit holds one workgroup.  Measured, us (16 x
 // 16 / 16 x 64 / 32 x 64 / 64 x 64 / 128 x 128 / 256 x 256):

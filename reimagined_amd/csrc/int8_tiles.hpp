@@ -196,8 +196,9 @@ __device__ __forceinline__ void i8_store4(const I8Problem& pb, const I8Rows& row
 // The way through LDS is there for the loads: four neighbouring lanes fetch the 64 bytes of one
 // row, which the vector cache serves at 60 bytes a clock, where lanes in the operand's order
 // (neighbours on different rows) get 16.  A fragment's row r has its 16-byte chunk c in place
-// c ^ (r / 4), so that the 16 lanes that read one chunk of 16 rows meet 64 different banks.  LDS
-// moves 64 bytes a clock, written and read, and that bounds a tile: 32 (NT + MT) bytes a step of K.
+// c ^ (r / 4), so that the 16 lanes that read one chunk of 16 rows meet 64 different banks.  What
+// bounds a tile is the wait for its loads: of 77 x 2009 -> 5125 the waves wait for 62 % of their time,
+// LDS is busy for 18 % and the matrix units for 8 (on the compute units that have a tile).
 // ===========================================================================
 template <int NT, int MT, int W, int D>
 constexpr int i8_split_smem() {
@@ -316,8 +317,8 @@ __device__ __forceinline__ void i8_split_tile(const I8Problem& pb, const I8Rows&
 // Block tile: 64 NWN outputs x 32 TM NWM tokens, NWN x NWM waves of 64 x 32 TM = 2 x TM tiles
 // of v_mfma_i32_32x32x32_i8, over 128-deep stages double-buffered in LDS.  A stage is fetched
 // into registers while the one before it is multiplied.  16-byte chunk c of row r sits in slot
-// c ^ ((r / 2) % 8), so that the 16 rows that one clock of a ds_read_b128 serves lie in
-// different banks.
+// c ^ ((r / 2) % 8), so that 16 neighbouring lanes of a ds_read_b128, 16 rows, lie in different
+// banks.
 // ===========================================================================
 constexpr int kI8BK = 128;
 
@@ -540,10 +541,12 @@ __device__ __forceinline__ void i8_tile(const I8Problem& pb, const I8Rows& rows,
 // that frees its buffer, so that the barrier's wait and the first reads of the next stage lie
 // under matrix instructions.  256 x 256 blocks of eight waves, 4096 x 4096 x 8192: 129 us,
 // 2.1 POP/s (128 x 128 blocks 145, through registers 170 .. 178); matrix instructions alone reach
-// 3.1 POP/s on such data.  LDS bounds it: 192 KB read and 64 KB written a stage at 64
-// bytes a clock.  64-deep stages in rings of three or four, and 256 x 128 blocks of four waves, two
-// a compute unit, were no faster at any size (138 -> 142 .. 159 us).  At K 1024 the stores show, which
-// all compute units make at once (8192 x 1024 x 4096: 43.5 us, about 13 of them 67 MB of outputs).
+// 3.1 .. 3.5 POP/s on such data.  No unit bounds it by its rate: the matrix units are busy for 53 % of
+// the clocks and LDS for 22 (4 clocks a ds_read_b128 of a wave); the two waves of a SIMD wait for 34 %
+// of their time, at the stage's barrier and for its first reads.  64-deep stages in rings of three or
+// four, and 256 x 128 blocks of four waves, two a compute unit, were no faster at any size (138 -> 142 ..
+// 159 us).  At K 1024 the stores show, which all compute units make at once (8192 x 1024 x 4096: 43.5
+// us, about 13 of them 67 MB of outputs).
 template <int YDT, int NWN, int NWM, int TM>
 __device__ __forceinline__ void i8_wide_tile(const I8Problem& pb, const I8Rows& rows, int n0, int m0,
                                              void* __restrict__ y, char* smem) {

@@ -249,9 +249,11 @@ __device__ __forceinline__ void sort_keys(uint32_t (&key)[V]) {
 // exact keys.
 //
 // What it takes is instructions: 16384 rows of 256 experts in 8 groups, sigmoid scores and a bias,
-// are 17 MB (3.3 us) and 14 us, 12 without the rows that 32 bits cannot decide.  (k rounds of a
-// 64-bit maximum over every row took 41; select_wave alone for those rows, 4 us of one wave while the
-// launch waits for it, 18.)
+// are 17 MB (3.3 us) and 14 .. 15 us, 12 without the rows that 32 bits cannot decide; vector
+// instructions are issued in 77 % of the clocks.  (k rounds of a 64-bit maximum over every row took 41;
+// select_wave alone for those rows, 4 us of one wave while the launch waits for it, 18.)  Where
+// select_wave has every row, a call of 20 us takes 42 .. 48: all values equal, scores of 2e-9 that
+// only their sums in a group part, a mask of -1e4 on all experts of each group but one.
 //
 // Errors, in units u = 2^-23: a sigmoid by exp2 and reciprocal of one unit each is off by s (1 - s)
 // (|x| / 2 + 1) + 1.5 s, below 1.7 u.  A softmax score p = e / sum: e by |x - max| + 1 of itself,

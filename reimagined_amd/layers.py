@@ -406,7 +406,9 @@ class Int8MoEFFN:
 
     def router_backward(self, logits: torch.Tensor, fwd: dict, dout: torch.Tensor) -> dict:
         """Gradients of what forward() combined, from that of its "out": dlogits (the router's; the
-        balance bias has none), dweights [rows, k] and do, of the experts' output rows "o"."""
+        balance bias has none), dweights [rows, k] and do, of the experts' output rows "o".  The
+        experts' int8 products have no gradient: do goes to a caller who has one, and a router below
+        this layer gets nothing through it."""
         do, dw = ops.moe_combine_topk_backward(dout, fwd["o"], fwd["slot_of"], fwd["weights"],
                                                perm=fwd["perm"])
         r = self.routing

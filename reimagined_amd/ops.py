@@ -781,7 +781,8 @@ def moe_route_scored(logits: torch.Tensor, k: int, score: str = "softmax", bias=
 
     logits f32 or bf16 [rows, E].  -> weights f32 [rows, k], selected int32 [rows, k], and,
     unless select_only, counts [E], offsets [E+1], perm [rows*k] (-1 past offsets[E]) and
-    slot_of [rows, k] for grouped_int8_gemm and moe_combine_topk.  valid_rows as moe_route."""
+    slot_of [rows, k] for grouped_int8_gemm and moe_combine_topk.  valid_rows as moe_route.
+    No autograd: the results are detached, moe_route_scored_backward gives the logits' gradient."""
     fn = "moe_route_scored"
     stride = _logit_rows(fn, logits)
     rows, e = logits.shape
@@ -845,7 +846,8 @@ def _combine_shapes(fn, expert_out, slot_of, weights):
 def moe_combine_topk(expert_out: torch.Tensor, slot_of: torch.Tensor, weights: torch.Tensor,
                      out_dtype=torch.float32) -> torch.Tensor:
     """out[r] = sum_i weights[r, i] * expert_out[slot_of[r, i]] (nsosx_moe_combine_topk): the
-    combine of moe_route_scored's weights [rows, k]; slot -1 adds nothing."""
+    combine of moe_route_scored's weights [rows, k]; slot -1 adds nothing.  No autograd: the result
+    is detached, moe_combine_topk_backward gives both gradients."""
     fn = "moe_combine_topk"
     rows, k, slots, dim = _combine_shapes(fn, expert_out, slot_of, weights)
     if out_dtype not in _DT:
@@ -876,7 +878,7 @@ def int8_gemm(q: torch.Tensor, act_scale: torch.Tensor, w: torch.Tensor, w_scale
               bias=None, out_dtype=torch.float32) -> torch.Tensor:
     """y = (q @ w^T) * act_scale[:, None] * w_scale (+ bias) (nsosx_int8_gemm): int8 codes q
     [M, K] and weights w [N, K], a scale per token and per output, both as
-    quantize_activations_bitnet gives them; y [M, N] f32 or bf16."""
+    quantize_activations_bitnet gives them; y [M, N] f32 or bf16.  It has no gradient."""
     fn = "int8_gemm"
     if q.dim() != 2 or w.dim() != 2 or q.shape[1] != w.shape[1] or not (q.numel() and w.numel()):
         raise ValueError(f"{fn}: q [M, K] and w [N, K] must agree in K, got {tuple(q.shape)} and "
@@ -900,7 +902,8 @@ def grouped_int8_gemm(q: torch.Tensor, act_scale: torch.Tensor, w: torch.Tensor,
                       squared_relu: bool = False, out_dtype=torch.float32) -> torch.Tensor:
     """int8_gemm of every expert's rows (nsosx_grouped_int8_gemm): w [E, N, K], w_scale and bias
     [E, N], the segments offsets [E+1] and, where q holds the unrouted rows, the slots' rows
-    perm (else q is in slot order).  -> y [slots, N]; rows past offsets[E] are not written."""
+    perm (else q is in slot order).  -> y [slots, N]; rows past offsets[E] are not written.  It has
+    no gradient."""
     fn = "grouped_int8_gemm"
     if q.dim() != 2 or w.dim() != 3 or q.shape[1] != w.shape[2] or not (q.numel() and w.numel()):
         raise ValueError(f"{fn}: q [rows, K] and w [E, N, K] must agree in K, got "
