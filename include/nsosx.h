@@ -606,6 +606,35 @@ int nsosx_moe_route_scored_backward(const void* logits, int logits_dtype, int64_
                                     int experts, int k, int sigmoid, int renorm, float scale,
                                     void* dlogits, void* stream);
 
+/* Balance loss of the router over a packed batch, per-expert counts and mean probabilities.  With p
+ * the normalised scores of a row (softmax, or for sigmoid != 0 the sigmoids over their sum), N_s
+ * the valid rows of sequence s, M the sequences that have any and count_se the choices of e in s:
+ *   loss = 1/M sum_s E sum_e count_se / (k N_s) * mean_prob_se,  mean_prob_se = sum_r p_re / N_s
+ * logits [rows, E] (logits_dtype) with row stride logits_stride; selected int32 [rows, k] as the
+ * routing left it (an entry outside [0, E) counts for nothing); valid_rows uint8 [rows] or NULL,
+ * 0 for padding; cu_seqlens int32 [S + 1], not decreasing, or NULL with S = 1 for the whole batch
+ * as one; rows of no sequence count as padding.  loss f32 [1] (0 without a valid row); counts int32
+ * and mean_prob f32 [S, E], tokens int32 [S] (N_s), zeros for a sequence without valid rows.
+ * E <= 512, k <= 16.  The same inputs give the same bits. */
+int64_t nsosx_moe_balance_loss_workspace(int rows, int experts, int S);
+int nsosx_moe_balance_loss(const void* logits, int logits_dtype, int64_t logits_stride,
+                           const int32_t* selected, const uint8_t* valid_rows, int rows,
+                           int experts, int k, int sigmoid, const int32_t* cu_seqlens, int S,
+                           float* loss, int32_t* counts, int32_t* tokens, float* mean_prob,
+                           void* workspace, void* stream);
+
+/* Gradient of that loss in the logits (counts are constants): dlogits [rows, E] contiguous in
+ * logits_dtype = scale * (dloss ? *dloss : 1) * dloss/dlogits (+ add).  counts, tokens as the
+ * forward left them; dloss a device f32 or NULL; add [rows, E] contiguous in logits_dtype (the
+ * routing's gradient, say; may be dlogits itself) or NULL.  Padding rows get zeros (+ add)
+ * whatever their logits hold. */
+int nsosx_moe_balance_loss_backward(const void* logits, int logits_dtype, int64_t logits_stride,
+                                    const int32_t* counts, const int32_t* tokens,
+                                    const uint8_t* valid_rows, int rows, int experts, int k,
+                                    int sigmoid, const int32_t* cu_seqlens, int S, float scale,
+                                    const float* dloss, const void* add, void* dlogits,
+                                    void* stream);
+
 /* out[r] = sum_i expert_out[slot_of[r, i]] * weights[r, i], i ascending, f32 sums; a slot
  * outside [0, slots) adds nothing.  expert_out [slots, dim] (in_dtype), out [rows, dim]
  * (out_dtype), which must not overlap; any number of experts, k <= 16, dim <= 2^30. */
@@ -683,6 +712,27 @@ int nsosx_rmsnorm_gated_quant(const void* y, const void* z, const float* gamma, 
 int nsosx_add_rmsnorm(const void* x, const void* delta, const float* gamma, int rows, int dim,
                       float eps, int act_dtype, void* residual_out, void* norm_out, void* stream);
 
+/* Layer norm y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias over rows [rows, dim]; with
+ * delta the residual add comes first: s = x + delta as stored in act_dtype, kept in sum_out (which
+ * may be x or delta).  delta and sum_out both or neither; weight, bias f32 [dim] or NULL; x, delta,
+ * sum_out in act_dtype, y in out_dtype; mean, rstd f32 [rows] (what the gradients need) or both
+ * NULL.  Contiguous rows at any alignment; f32 sums, the variance from the centred row. */
+int nsosx_layernorm(const void* x, const void* delta, const float* weight, const float* bias,
+                    int rows, int dim, float eps, int act_dtype, void* sum_out, void* y,
+                    int out_dtype, float* mean, float* rstd, void* stream);
+
+/* Its gradients from dy [rows, dim] (dy_dtype), the normed rows x (the sum, where there was one)
+ * and their mean and rstd: with n = (x - mean) rstd and g = dy weight,
+ *   dx = rstd (g - mean(g) - n mean(g n)) (+ dresidual), dweight = sum_rows dy n, dbias = sum_rows dy
+ * dx and dresidual (the gradient that reached the sum by another way, or NULL; may be dx) in
+ * act_dtype; dweight, dbias f32 [dim], each or NULL, the same bits for the same inputs.
+ * workspace: nsosx_layernorm_backward_workspace bytes (unused where both are NULL). */
+int64_t nsosx_layernorm_backward_workspace(int rows, int dim);
+int nsosx_layernorm_backward(const void* dy, int dy_dtype, const void* x, const float* mean,
+                             const float* rstd, const float* weight, const void* dresidual,
+                             int rows, int dim, int act_dtype, void* dx, float* dweight,
+                             float* dbias, void* workspace, void* stream);
+
 /* Decode conv ring step, the role of launch_mamba2_faithful_conv_step
  * (src/cuda/mamba_kernels.cu:3332-3374; CPU src/mamba2.cpp:4072-4090):
  *   v = bias[c] + sum_{j<W} w[c,j] * (j < W-1 ? ring[r][j][c] : x[r,c])
@@ -692,6 +742,53 @@ int nsosx_add_rmsnorm(const void* x, const void* delta, const float* gamma, int 
 int nsosx_conv_step(const void* x, int x_dtype, int64_t x_stride, int rows, int channels,
                     const float* weight, const float* bias, int width, float* ring,
                     int apply_silu, void* out, int out_dtype, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Gated linear recurrence over packed ragged batches.
+ * ------------------------------------------------------------------------- */
+
+/* Per channel, with a = exp(-rate softplus(lam) sigmoid(rg)):
+ *   h_t = a_t h_(t-1) + sqrt(1 - a_t^2) sigmoid(ig_t) x_t,  y = h
+ * x, rg, ig, y: [T, D] in act_dtype with row strides in elements (columns of a wider buffer are
+ * fine); lam f32 [D]; cu_seqlens int32 [S + 1], not decreasing, empty sequences allowed.
+ * initial_state f32 [S, D] or NULL (zeros); final_state f32 [S, D] or NULL (an empty sequence's
+ * is its initial state).  Rows of no sequence (past cu_seqlens[S]) are left as they were, or
+ * with zero_rest != 0 written as zeros.  carry f32 [ceil(T / tile), D] or NULL: the states between
+ * tiles of nsosx_gated_recurrence_tile() tokens, which the gradients start from.  The state is f32
+ * throughout; the same inputs give the same bits.  workspace: device,
+ * nsosx_gated_recurrence_workspace bytes. */
+int nsosx_gated_recurrence_tile(void);
+int64_t nsosx_gated_recurrence_workspace(int T, int D);
+int nsosx_gated_recurrence(const void* x, int64_t x_stride, const void* rg, int64_t rg_stride,
+                           const void* ig, int64_t ig_stride, const float* lam, float rate,
+                           const int32_t* cu_seqlens, int S, int T, int D, int act_dtype,
+                           const float* initial_state, int zero_rest, void* y, int64_t y_stride,
+                           float* final_state, float* carry, void* workspace, void* stream);
+
+/* Its gradients from dy [T, D] and, where not NULL, dfinal f32 [S, D] (of the final states):
+ * dx, drg, dig [T, D] in act_dtype with row strides, dlam f32 [D], dinitial f32 [S, D] or NULL.
+ * x, rg, ig, lam, rate, cu_seqlens, initial_state and carry as the forward had and left them; h is
+ * formed again, y is not needed.  Rows of no sequence as in the forward.  The gradients must
+ * not overlap each other or an input (side by side in one buffer's rows is fine). */
+int64_t nsosx_gated_recurrence_backward_workspace(int T, int D);
+int nsosx_gated_recurrence_backward(const void* dy, int64_t dy_stride, const void* x,
+                                    int64_t x_stride, const void* rg, int64_t rg_stride,
+                                    const void* ig, int64_t ig_stride, const float* lam,
+                                    float rate, const int32_t* cu_seqlens, int S, int T, int D,
+                                    int act_dtype, const float* initial_state, const float* carry,
+                                    const float* dfinal, int zero_rest, void* dx,
+                                    int64_t dx_stride, void* drg, int64_t drg_stride, void* dig,
+                                    int64_t dig_stride, float* dlam, float* dinitial,
+                                    void* workspace, void* stream);
+
+/* One token per row: state_out = a state + sqrt(1 - a^2) sigmoid(ig) x, y = state_out rounded to
+ * act_dtype.  state, state_out f32 [rows, D] (the same buffer for an update in place); the rest as
+ * above with rows in place of T. */
+int nsosx_gated_recurrence_step(const void* x, int64_t x_stride, const void* rg,
+                                int64_t rg_stride, const void* ig, int64_t ig_stride,
+                                const float* lam, float rate, int rows, int D, int act_dtype,
+                                const float* state, float* state_out, void* y, int64_t y_stride,
+                                void* stream);
 
 /* ---------------------------------------------------------------------------
  * Quantization-aware training: fake-quant forward and the STE weight-gradient

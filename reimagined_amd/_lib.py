@@ -96,6 +96,25 @@ SIGNATURES = {
     "nsosx_int8_gemm": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _vp]),
     "nsosx_grouped_int8_gemm": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i,
                                      _vp, _i, _vp]),
+    "nsosx_moe_balance_loss_workspace": (_i64, [_i, _i, _i]),
+    "nsosx_moe_balance_loss": (_i, [_vp, _i, _i64, _vp, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp,
+                                    _vp, _vp, _vp]),
+    "nsosx_moe_balance_loss_backward": (_i, [_vp, _i, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _i,
+                                             _f, _vp, _vp, _vp, _vp]),
+    "nsosx_layernorm": (_i, [_vp, _vp, _vp, _vp, _i, _i, _f, _i, _vp, _vp, _i, _vp, _vp, _vp]),
+    "nsosx_layernorm_backward_workspace": (_i64, [_i, _i]),
+    "nsosx_layernorm_backward": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp,
+                                      _vp, _vp]),
+    "nsosx_gated_recurrence_tile": (_i, []),
+    "nsosx_gated_recurrence_workspace": (_i64, [_i, _i]),
+    "nsosx_gated_recurrence": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _f, _vp, _i, _i, _i, _i,
+                                    _vp, _i, _vp, _i64, _vp, _vp, _vp, _vp]),
+    "nsosx_gated_recurrence_backward_workspace": (_i64, [_i, _i]),
+    "nsosx_gated_recurrence_backward": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _f,
+                                             _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _i64, _vp,
+                                             _i64, _vp, _i64, _vp, _vp, _vp, _vp]),
+    "nsosx_gated_recurrence_step": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _f, _i, _i, _i, _vp,
+                                         _vp, _vp, _i64, _vp]),
     "nsosx_sha256_hex": (_i, [_vp, ctypes.c_uint64, _vp]),
 }
 

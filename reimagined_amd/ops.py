@@ -835,6 +835,74 @@ def moe_route_scored_backward(logits: torch.Tensor, selected: torch.Tensor, dwei
     return out
 
 
+def _segments(fn: str, cu_seqlens, dev: int) -> int:
+    """Sequences of a packed batch's bounds int32 [S + 1] (None: the batch is one)."""
+    if cu_seqlens is None:
+        return 1
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+        raise ValueError(f"{fn}: cu_seqlens must be [sequences + 1], got {tuple(cu_seqlens.shape)}")
+    _on(fn, dev, ("cu_seqlens", cu_seqlens, torch.int32, None))
+    return cu_seqlens.numel() - 1
+
+
+def moe_balance_loss(logits: torch.Tensor, selected: torch.Tensor, score: str = "softmax",
+                     cu_seqlens=None, valid_rows=None) -> dict:
+    """The router's balance loss E sum_e f_e P_e (nsosx_moe_balance_loss): f_e the share of the
+    choices that fell on expert e, P_e its mean probability (softmax, or sigmoids over their sum);
+    over the whole batch, or with cu_seqlens int32 [S + 1] per sequence and averaged over the
+    sequences that have a valid row.
+
+    logits f32 or bf16 [rows, E], selected int32 [rows, k] as moe_route_scored gives it.
+    -> loss f32 [1], counts int32 [S, E], tokens int32 [S] (valid rows), mean_prob f32 [S, E], with
+    S = 1 for the whole batch.  valid_rows as moe_route.  No autograd:
+    moe_balance_loss_backward gives the logits' gradient."""
+    fn = "moe_balance_loss"
+    stride = _logit_rows(fn, logits)
+    rows, e = logits.shape
+    if selected.dim() != 2 or selected.shape[0] != rows or selected.shape[1] < 1:
+        raise ValueError(f"{fn}: selected must be [rows, k], got {tuple(selected.shape)}")
+    k = selected.shape[1]
+    sig = _score_mode(fn, score)
+    dev = logits.get_device()
+    mask = valid_rows_mask(valid_rows, rows, logits.device)
+    _on(fn, dev, ("selected", selected, torch.int32, None), ("valid_rows", mask, torch.uint8, None))
+    s = _segments(fn, cu_seqlens, dev)
+    ws = int(lib().nsosx_moe_balance_loss_workspace(rows, e, s)) // 4
+    buf = torch.empty(1 + 2 * s * e + s + ws, dtype=torch.float32, device=logits.device)
+    loss, mean, counts, tokens, ws = buf.split((1, s * e, s * e, s, ws))
+    counts, tokens = counts.view(torch.int32).view(s, e), tokens.view(torch.int32)
+    call("nsosx_moe_balance_loss", _p(logits), _dt(logits), stride, _p(selected), _p(mask), rows, e, k,
+         sig, _p(cu_seqlens), s, _p(loss), _p(counts), _p(tokens), _p(mean), _p(ws), _stream_on(dev))
+    return {"loss": loss, "counts": counts, "tokens": tokens, "mean_prob": mean.view(s, e)}
+
+
+def moe_balance_loss_backward(logits: torch.Tensor, counts: torch.Tensor, tokens: torch.Tensor, k: int,
+                              score: str = "softmax", cu_seqlens=None, valid_rows=None, dloss=1.0,
+                              add=None) -> torch.Tensor:
+    """Gradient of moe_balance_loss's logits [rows, E] (their dtype) times dloss, a number or a
+    device f32 tensor of one element (nsosx_moe_balance_loss_backward); counts and tokens are the
+    forward's, k its choices a row.  add: a gradient of the same shape and dtype
+    (moe_route_scored_backward's) that is added to it."""
+    fn = "moe_balance_loss_backward"
+    stride = _logit_rows(fn, logits)
+    rows, e = logits.shape
+    sig = _score_mode(fn, score)
+    dev = logits.get_device()
+    mask = valid_rows_mask(valid_rows, rows, logits.device)
+    s = _segments(fn, cu_seqlens, dev)
+    scalar = dloss if isinstance(dloss, torch.Tensor) else None
+    if scalar is not None and scalar.numel() != 1:
+        raise ValueError(f"{fn}: dloss must hold one element, got {tuple(scalar.shape)}")
+    _on(fn, dev, ("counts", counts, torch.int32, (s, e)), ("tokens", tokens, torch.int32, (s,)),
+        ("valid_rows", mask, torch.uint8, None), ("dloss", scalar, torch.float32, None),
+        ("add", add, logits.dtype, (rows, e)))
+    out = logits.new_empty((rows, e))
+    call("nsosx_moe_balance_loss_backward", _p(logits), _dt(logits), stride, _p(counts), _p(tokens),
+         _p(mask), rows, e, k, sig, _p(cu_seqlens), s, 1.0 if scalar is not None else float(dloss),
+         _p(scalar), _p(add), _p(out), _stream_on(dev))
+    return out
+
+
 def _combine_shapes(fn, expert_out, slot_of, weights):
     if expert_out.dim() != 2 or slot_of.dim() != 2 or 0 in expert_out.shape or 0 in slot_of.shape:
         raise ValueError(f"{fn}: expert_out must be [slots, dim] and slot_of [rows, k]")
@@ -927,7 +995,7 @@ def grouped_int8_gemm(q: torch.Tensor, act_scale: torch.Tensor, w: torch.Tensor,
     return y
 
 
-# ---- row norms of the hybrid block and the decode conv ring -----------------
+# ---- row norms of the hybrid block --------------------------------------------
 
 def rmsnorm_gated(y: torch.Tensor, z=None, gamma=None, eps: float = 1e-5,
                   out_dtype=None) -> torch.Tensor:
@@ -991,6 +1059,188 @@ def add_rmsnorm(x: torch.Tensor, delta: torch.Tensor, gamma=None, eps: float = 1
          _p(res), _p(norm), _stream())
     return res, norm
 
+
+# ---- layer norm and its gradients -------------------------------------------------
+
+def _norm_rows(fn: str, x: torch.Tensor, name: str = "x") -> tuple:
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"{fn}: {name} must be [rows, dim], got {tuple(x.shape)}")
+    _dt(x)
+    return x.shape
+
+
+def layernorm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out_dtype=None,
+              want_stats: bool = False):
+    """y = (x - mean) * rstd * weight + bias over the last dimension (nsosx_layernorm): x f32 or
+    bf16 [rows, dim], weight and bias f32 [dim] or None.  -> y, or with want_stats (y, mean, rstd),
+    f32 [rows] each, which layernorm_backward takes.  No autograd."""
+    fn = "layernorm"
+    rows, dim = _norm_rows(fn, x)
+    odt = out_dtype or x.dtype
+    if odt not in _DT:
+        raise ValueError(f"{fn}: out_dtype must be float32 or bfloat16")
+    dev = x.get_device()
+    _on(fn, dev, ("x", x, None, None), ("weight", weight, torch.float32, (dim,)),
+        ("bias", bias, torch.float32, (dim,)))
+    y = x.new_empty((rows, dim), dtype=odt)
+    mean = rstd = None
+    if want_stats:
+        mean, rstd = x.new_empty((2, rows), dtype=torch.float32).unbind(0)
+    call("nsosx_layernorm", _p(x), None, _p(weight), _p(bias), rows, dim, eps, _dt(x), None, _p(y),
+         _DT[odt], _p(mean), _p(rstd), _stream_on(dev))
+    return (y, mean, rstd) if want_stats else y
+
+
+def add_layernorm(x: torch.Tensor, delta: torch.Tensor, weight=None, bias=None, eps: float = 1e-5,
+                  want_stats: bool = False) -> tuple:
+    """residual = x + delta, y = layernorm(residual as stored), in one pass (nsosx_layernorm).
+    -> (residual, y), or with want_stats (residual, y, mean, rstd)."""
+    fn = "add_layernorm"
+    rows, dim = _norm_rows(fn, x)
+    dev = x.get_device()
+    _on(fn, dev, ("x", x, None, None), ("delta", delta, x.dtype, (rows, dim)),
+        ("weight", weight, torch.float32, (dim,)), ("bias", bias, torch.float32, (dim,)))
+    res, y = torch.empty_like(x), torch.empty_like(x)
+    mean = rstd = None
+    if want_stats:
+        mean, rstd = x.new_empty((2, rows), dtype=torch.float32).unbind(0)
+    call("nsosx_layernorm", _p(x), _p(delta), _p(weight), _p(bias), rows, dim, eps, _dt(x), _p(res),
+         _p(y), _dt(x), _p(mean), _p(rstd), _stream_on(dev))
+    return (res, y, mean, rstd) if want_stats else (res, y)
+
+
+def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                       weight=None, dresidual=None, want_params: bool = True) -> dict:
+    """Gradients of layernorm / add_layernorm (nsosx_layernorm_backward): x the normed rows (the
+    residual, where there was an add), mean and rstd as the forward gave them.  -> dx (x's dtype;
+    of both x and delta of an add) and, with want_params, dweight and dbias f32 [dim].  dresidual:
+    the gradient that reached the residual by another way, added to dx."""
+    fn = "layernorm_backward"
+    rows, dim = _norm_rows(fn, x)
+    _dt(dy)
+    dev = x.get_device()
+    _on(fn, dev, ("x", x, None, None), ("dy", dy, None, (rows, dim)),
+        ("mean", mean, torch.float32, (rows,)), ("rstd", rstd, torch.float32, (rows,)),
+        ("weight", weight, torch.float32, (dim,)), ("dresidual", dresidual, x.dtype, (rows, dim)))
+    dx = torch.empty_like(x)
+    dw = db = ws = None
+    if want_params:
+        n = int(lib().nsosx_layernorm_backward_workspace(rows, dim)) // 4
+        dw, db, ws = x.new_empty(2 * dim + n, dtype=torch.float32).split((dim, dim, n))
+    call("nsosx_layernorm_backward", _p(dy), _dt(dy), _p(x), _p(mean), _p(rstd), _p(weight),
+         _p(dresidual), rows, dim, _dt(x), _p(dx), _p(dw), _p(db), _p(ws), _stream_on(dev))
+    return {"dx": dx, "dweight": dw, "dbias": db} if want_params else {"dx": dx}
+
+
+# ---- gated linear recurrence --------------------------------------------------------
+
+def _rec_view(fn: str, dev: int, name: str, t: torch.Tensor, dtype, shape) -> int:
+    """Checks a [T, D] view with unit column stride (a column slice is fine); its row stride."""
+    if t.get_device() != dev or dev < 0:
+        raise ValueError(f"{fn}: {name} must be a device tensor on x's device")
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{fn}: {name} must be {tuple(shape)} {dtype}, got {tuple(t.shape)} {t.dtype}")
+    rows, d = shape
+    if (d > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < d):
+        raise ValueError(f"{fn}: {name} needs unit column stride and rows that do not overlap")
+    return t.stride(0) if rows > 1 else d
+
+
+def _rec_inputs(fn: str, x, rg, ig, lam) -> tuple:
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"{fn}: x must be [tokens, dim], got {tuple(x.shape)}")
+    dt = _dt(x)
+    if not x.is_cuda:
+        raise ValueError("x must be a device tensor")
+    dev = x.get_device()
+    strides = [_rec_view(fn, dev, n, t, x.dtype, x.shape) for n, t in (("x", x), ("rg", rg), ("ig", ig))]
+    _on(fn, dev, ("lam", lam, torch.float32, (x.shape[1],)))
+    return dev, dt, *strides
+
+
+def gated_recurrence(x: torch.Tensor, rg: torch.Tensor, ig: torch.Tensor, lam: torch.Tensor,
+                     cu_seqlens: torch.Tensor, rate: float = 8.0, initial_state=None,
+                     want_final: bool = True, want_carry: bool = False, out=None) -> tuple:
+    """Gated linear recurrence over a packed ragged batch (nsosx_gated_recurrence):
+
+        a = exp(-rate softplus(lam) sigmoid(rg)),  h_t = a_t h_(t-1) + sqrt(1 - a_t^2) sigmoid(ig_t) x_t
+
+    x, the decay gate's logits rg and the input gate's ig f32 or bf16 [T, D] (column slices are
+    fine), lam f32 [D], cu_seqlens int32 [S + 1], initial_state f32 [S, D] or None.  -> (y [T, D] in
+    x's dtype, final_state f32 [S, D] or None), and with want_carry a third tensor that
+    gated_recurrence_backward takes.  out: a [T, D] view to write y into, whose rows past the
+    last sequence are left as they were (a fresh y has zeros there).  No autograd."""
+    fn = "gated_recurrence"
+    dev, dt, xs, rs, igs = _rec_inputs(fn, x, rg, ig, lam)
+    t, d = x.shape
+    s = _segments(fn, cu_seqlens, dev)
+    _on(fn, dev, ("initial_state", initial_state, torch.float32, (s, d)))
+    y = x.new_empty((t, d)) if out is None else out
+    ys = d if out is None else _rec_view(fn, dev, "out", out, x.dtype, (t, d))
+    final = x.new_empty((s, d), dtype=torch.float32) if want_final else None
+    tiles = -(-t // lib().nsosx_gated_recurrence_tile())
+    carry = x.new_empty((tiles, d), dtype=torch.float32) if want_carry else None
+    ws = x.new_empty(int(lib().nsosx_gated_recurrence_workspace(t, d)), dtype=torch.uint8)
+    call("nsosx_gated_recurrence", _p(x), xs, _p(rg), rs, _p(ig), igs, _p(lam), rate, _p(cu_seqlens), s,
+         t, d, dt, _p(initial_state), int(out is None), _p(y), ys, _p(final), _p(carry), _p(ws),
+         _stream_on(dev))
+    return (y, final, carry) if want_carry else (y, final)
+
+
+def gated_recurrence_backward(dy: torch.Tensor, x: torch.Tensor, rg: torch.Tensor, ig: torch.Tensor,
+                              lam: torch.Tensor, cu_seqlens: torch.Tensor, carry: torch.Tensor,
+                              rate: float = 8.0, initial_state=None, dfinal=None, out=None) -> dict:
+    """Gradients of gated_recurrence (nsosx_gated_recurrence_backward) from dy [T, D] (x's dtype) and,
+    where the final states went on, dfinal f32 [S, D]; carry is the forward's, the rest its
+    arguments.  -> dx, drg, dig [T, D], dlam f32 [D] and, with an initial_state or dfinal, dinitial f32
+    [S, D].  out: three [T, D] views (dx, drg, dig) to write into, side by side in one buffer for
+    one; their rows past the last sequence are left as they were (fresh ones have zeros there)."""
+    fn = "gated_recurrence_backward"
+    dev, dt, xs, rs, igs = _rec_inputs(fn, x, rg, ig, lam)
+    t, d = x.shape
+    s = _segments(fn, cu_seqlens, dev)
+    dys = _rec_view(fn, dev, "dy", dy, x.dtype, (t, d))
+    tiles = -(-t // lib().nsosx_gated_recurrence_tile())
+    _on(fn, dev, ("carry", carry, torch.float32, (tiles, d)),
+        ("initial_state", initial_state, torch.float32, (s, d)), ("dfinal", dfinal, torch.float32, (s, d)))
+    if out is None:
+        grads, gs = x.new_empty((3, t, d)).unbind(0), (d, d, d)
+    else:
+        if len(out) != 3:
+            raise ValueError(f"{fn}: out must hold dx, drg and dig")
+        grads = out
+        gs = [_rec_view(fn, dev, "out", g, x.dtype, (t, d)) for g in out]
+    dlam = lam.new_empty(d)
+    want0 = initial_state is not None or dfinal is not None
+    dinit = lam.new_empty((s, d)) if want0 else None
+    ws = x.new_empty(int(lib().nsosx_gated_recurrence_backward_workspace(t, d)), dtype=torch.uint8)
+    call("nsosx_gated_recurrence_backward", _p(dy), dys, _p(x), xs, _p(rg), rs, _p(ig), igs, _p(lam),
+         rate, _p(cu_seqlens), s, t, d, dt, _p(initial_state), _p(carry), _p(dfinal), int(out is None),
+         _p(grads[0]), gs[0], _p(grads[1]), gs[1], _p(grads[2]), gs[2], _p(dlam), _p(dinit), _p(ws),
+         _stream_on(dev))
+    r = {"dx": grads[0], "drg": grads[1], "dig": grads[2], "dlam": dlam}
+    if want0:
+        r["dinitial"] = dinit
+    return r
+
+
+def gated_recurrence_step(x: torch.Tensor, rg: torch.Tensor, ig: torch.Tensor, lam: torch.Tensor,
+                          state: torch.Tensor, rate: float = 8.0, state_out=None) -> torch.Tensor:
+    """One token per row through gated_recurrence (nsosx_gated_recurrence_step): x, rg, ig [R, D],
+    state f32 [R, D], updated in place or written to state_out.  -> y [R, D] in x's dtype."""
+    fn = "gated_recurrence_step"
+    dev, dt, xs, rs, igs = _rec_inputs(fn, x, rg, ig, lam)
+    r, d = x.shape
+    if state_out is None:
+        state_out = state
+    _on(fn, dev, ("state", state, torch.float32, (r, d)), ("state_out", state_out, torch.float32, (r, d)))
+    y = x.new_empty((r, d))
+    call("nsosx_gated_recurrence_step", _p(x), xs, _p(rg), rs, _p(ig), igs, _p(lam), rate, r, d, dt,
+         _p(state), _p(state_out), _p(y), d, _stream_on(dev))
+    return y
+
+
+# ---- the decode conv ring -----------------------------------------------------
 
 def conv_step(x: torch.Tensor, weight: torch.Tensor, bias, ring, apply_silu: bool = True,
               out_dtype=None) -> torch.Tensor:
