@@ -43,6 +43,7 @@ template <> struct Pair<NSOSX_BF16, 2> {
     __device__ __forceinline__ void load(const Rows& v, uint32_t lane, int row) {
         w = __builtin_amdgcn_raw_buffer_load_b32(v.r, lane, row * v.row, 0);
     }
+    __device__ __forceinline__ void forget() { asm volatile("" : "+v"(w)); }
     __device__ __forceinline__ float get(int k) const {
         return __uint_as_float(k ? w & 0xffff0000u : w << 16);
     }
@@ -56,6 +57,7 @@ template <> struct Pair<NSOSX_F32, 2> {
     __device__ __forceinline__ void load(const Rows& v, uint32_t lane, int row) {
         w = __builtin_amdgcn_raw_buffer_load_b64(v.r, lane, row * v.row, 0);
     }
+    __device__ __forceinline__ void forget() { asm volatile("" : "+v"(w)); }
     __device__ __forceinline__ float get(int k) const { return __uint_as_float(k ? w.y : w.x); }
     static __device__ __forceinline__ void store(const Rows& v, uint32_t lane, int row, const float (&f)[2]) {
         const u32x2 w = {__float_as_uint(f[0]), __float_as_uint(f[1])};
@@ -67,6 +69,7 @@ template <int DT> struct Pair<DT, 1> {
     __device__ __forceinline__ void load(const Rows& p, uint32_t lane, int row) {
         v = raw_to_f32<DT>(buf_load_raw<DT>(p.r, lane + row * p.row));
     }
+    __device__ __forceinline__ void forget() { asm volatile("" : "+v"(v)); }
     __device__ __forceinline__ float get(int) const { return v; }
     static __device__ __forceinline__ void store(const Rows& p, uint32_t lane, int row, const float (&f)[1]) {
         buf_store_act<DT>(p.r, lane + row * p.row, f[0]);
@@ -89,6 +92,14 @@ __device__ __forceinline__ float decay_rate(float lam, float rate) {
     return rate * (fmaxf(lam, 0.0f) + log1pf(expf(-fabsf(lam)))) * kLog2e;
 }
 
+// From here on the words are loaded ones to the compiler.  Where it would form what two branches (or two
+// phases) both need ahead of them, in registers that are not there, one of them forgets.
+template <typename P, int R>
+__device__ __forceinline__ void forget(P (&p)[R]) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) p[j].forget();
+}
+
 // p = 1 - a^2 for a = 2^-q.  Where a is near 1 the difference would cancel: below t = -log(a^2) = 0.25
 // (q = kSmall) it is q times a fit of (1 - e^-t) / t in q (own least-squares fit, relative error 1e-7 with
 // its roundings); above, 1 - a^2 is exact to 7e-7.
@@ -108,35 +119,34 @@ __device__ __forceinline__ float one_less_square(float q, float a) {
     return SMALL || q < kSmall ? p : __fmaf_rn(-a, a, 1.0f);
 }
 
-// Where the tile's sequences start and end: s_start[i] / s_end[i] hold the sequence whose first /
-// last token is token i of the tile, else -1.  Every workgroup reads all of cu_seqlens, a few loads
-// that do not depend on each other, rather than search it in log2(S) that do.
-template <int NT, int L>
-__device__ __forceinline__ void tile_borders(const int32_t* __restrict__ cu, int S, int64_t t0,
-                                             int32_t* s_start, int32_t* s_end) {
-    for (int i = threadIdx.x; i < L; i += NT) s_start[i] = s_end[i] = -1;
-    __syncthreads();
-    for (int s = threadIdx.x; s < S; s += NT) {
-        const int64_t lo = cu[s], hi = cu[s + 1];
-        if (hi <= lo) continue;
-        if (lo >= t0 && lo < t0 + L) s_start[lo - t0] = s;
-        if (hi > t0 && hi <= t0 + L) s_end[hi - 1 - t0] = s;
+// What a wave's R tokens are, a bit per token; their sequences are left in LDS.
+struct Tokens {
+    uint32_t starts, ends, inside;
+    template <int R> __device__ __forceinline__ bool plain() const {
+        return !starts && !ends && inside == (1u << R) - 1;
     }
-    __syncthreads();
-}
+};
 
-// A bit per token of this wave's R: starts, ends, and tokens of some sequence.
+// cu holds S + 1 bounds: a search per lane, in LDS but for thousands of sequences.  seqs: the wave's R.
 template <int R>
-__device__ __forceinline__ void wave_masks(const int32_t* s_start, const int32_t* s_end, int wave,
-                                           int64_t t0, int64_t lo, int64_t hi, uint32_t& starts,
-                                           uint32_t& ends, uint32_t& inside) {
-    const int lane = threadIdx.x & 63;
-    const int i = wave * R + min(lane, R - 1);
-    const int64_t t = t0 + i;
-    const bool mine = lane < R;
-    starts = (uint32_t)__ballot(mine & (s_start[i] >= 0));
-    ends = (uint32_t)__ballot(mine & (s_end[i] >= 0));
-    inside = (uint32_t)__ballot(mine & (t >= lo) & (t < hi));
+__device__ __forceinline__ Tokens find_tokens(const int32_t* cu, int S, int lane, int64_t first, int64_t T,
+                                              int32_t* seqs) {
+    const int i = min(lane, R - 1);
+    const int64_t t = first + i;
+    int lo = 0, hi = S + 1;  // the first bound past t: the last of several empty sequences is not t's
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (cu[mid] <= t) lo = mid + 1;
+        else hi = mid;
+    }
+    const int s = min(max(lo - 1, 0), max(S - 1, 0));
+    const bool in = (lo > 0) & (lo <= S) & (t < T) & (lane < R);
+    seqs[i] = s;
+    Tokens r;
+    r.inside = (uint32_t)__ballot(in);
+    r.starts = (uint32_t)__ballot(in & (cu[s] == t));
+    r.ends = (uint32_t)__ballot(in & (cu[min(s + 1, S)] == t + 1));
+    return r;
 }
 
 // What an empty sequence leaves: its initial state (or zeros), both ways.
@@ -157,88 +167,158 @@ __device__ __forceinline__ void empty_states(const int32_t* __restrict__ cu, int
     }
 }
 
+// h -> A h + H; A = 0 passes nothing on, whatever h holds (it may be another sequence's infinity)
+__device__ __forceinline__ float through(float A, float H, float h) {
+    return A == 0.0f ? H : __fmaf_rn(A, h, H);
+}
+
 // ---- the state that enters a tile ---------------------------------------------------
 //
-// A word per (tile, channel) in the order of the scan: 0 until the tile has something to say, then its
-// pair (A's bits with the sign set, H), then the state behind it (kWhole, P).  Words are 64 bits, written
-// and read whole at device scope, so nothing else needs to be ordered with them.
-// P_k = fma(A_k, P_(k-1), H_k) always, however far back a tile finds a P: the same bits every run.
-// Every wait ends: workgroups take their tiles by a ticket, in the order of the scan, so whoever waits
-// waits for workgroups that have started, and those leave their pair before they wait themselves.
+// Tiles meet through words in memory, one per (tile, channel) with the tile's pair, and one per
+// (group of kGroup tiles, channel) with the group's pair and later the state P behind it.  A word is 64
+// bits, written and read whole at device scope, so nothing else has to be ordered with it: 0 until
+// there is something to say, (A's bits with the sign set, H) for a pair, (kWhole, P) for a state.
+//   P_g = A_g P_(g-1) + H_g,  a tile's state is P_(g-1) through the pairs of its group's tiles before it
+// in that order however far back a group finds a P, so the bits are the same every run.
+// A tile waits on flags (per 64 channels; 1: a pair is there, 2: a state), a few bytes a look, and reads
+// words only when the flags say that they are there: words polled by themselves took as much time as
+// everything else.  The flags are hints, the words' own tags decide.
+// Every wait ends: workgroups take their tiles by a ticket, in the order of the scan, and leave a tile's
+// pair before they wait for another's, so whoever waits waits for tiles that a started workgroup has
+// left or will leave without waiting for a later one.
 constexpr uint32_t kWhole = 1;
-constexpr int kWindow = 4;          // tiles looked back at a time
+constexpr int kGroup = 4;           // tiles
 constexpr int kMaxPolls = 1 << 22;  // seconds; then the state is NaN and the kernel ends
+
+struct RecShared {
+    uint32_t* ticket;           // NULL where there is one tile in time: no tile waits for another
+    uint64_t *words, *groups;   // [tiles, D], [groups, D]
+    uint32_t *flags, *gflags;   // [D / 64 up, tiles], [D / 64 up, groups]
+    float* k2;                  // [D]: the channels' decay rates, formed once
+};
 
 __device__ __forceinline__ void leave(uint64_t* word, uint32_t tag, float v) {
     __hip_atomic_store(word, ((uint64_t)tag << 32) | __float_as_uint(v), __ATOMIC_RELAXED,
                        __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// One wave, V channels a lane: tile k of the scan has the pair (A, H); c becomes the state before it.
-template <int V>
-__device__ __forceinline__ void state_before(uint64_t* words, int64_t k, int64_t D, uint32_t ch,
-                                             const float (&A)[V], const float (&H)[V], float (&c)[V]) {
-    uint64_t* mine = words + k * D + ch;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        // nothing enters the first tile, and nothing passes a sequence's border
-        const bool whole = k == 0 || A[v] == 0.0f;
-        leave(mine + v, whole ? kWhole : __float_as_uint(A[v]) | 0x80000000u, H[v]);
-        c[v] = 0.0f;
-    }
-    if (k == 0) return;
-    bool done = false;
-    for (int polls = 0; !__all(done); ++polls) {
-        if (polls > 0) __builtin_amdgcn_s_sleep(1);
-        uint64_t w[kWindow][V];
-#pragma unroll
-        for (int i = 0; i < kWindow; ++i)
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                w[i][v] = __hip_atomic_load(words + max(k - 1 - i, (int64_t)0) * D + (ch + v), __ATOMIC_RELAXED,
-                                            __HIP_MEMORY_SCOPE_AGENT);
-        done = true;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            int found = kWindow;  // the nearest tile whose P is known, behind nothing but pairs
-#pragma unroll
-            for (int i = kWindow - 1; i >= 0; --i) {
-                const uint32_t tag = (uint32_t)(w[i][v] >> 32);
-                found = tag == kWhole ? i : tag == 0 ? kWindow : found;
-            }
-            float s = 0.0f;
-#pragma unroll
-            for (int i = kWindow - 1; i >= 0; --i) {
-                const float a = __uint_as_float((uint32_t)(w[i][v] >> 32) & 0x7fffffffu);
-                const float h = __uint_as_float((uint32_t)w[i][v]);
-                s = i == found ? h : i < found ? __fmaf_rn(a, s, h) : s;
-            }
-            c[v] = s;
-            done = done && found < kWindow;
-        }
-        if (polls >= kMaxPolls) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) c[v] = __builtin_nanf("");
-            break;
-        }
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-        if (A[v] != 0.0f) leave(mine + v, kWhole, __fmaf_rn(A[v], c[v], H[v]));
+__device__ __forceinline__ uint64_t look(const uint64_t* row, uint32_t bytes) {
+    return __hip_atomic_load(reinterpret_cast<const uint64_t*>(reinterpret_cast<const char*>(row) + bytes),
+                             __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// The workgroup's place in the scan: ticket, or its index where there is one tile in time.
-__device__ __forceinline__ int take_ticket(uint32_t* ticket) {
-    if (!ticket) return blockIdx.x;
-    __shared__ uint32_t s_ticket;
-    if (threadIdx.x == 0) s_ticket = atomicAdd(ticket, 1u);
-    __syncthreads();
-    return __builtin_amdgcn_readfirstlane(s_ticket);
+__device__ __forceinline__ void raise_flag(uint32_t* flag, uint32_t v) {
+    if ((threadIdx.x & 63) == 0) __hip_atomic_store(flag, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-__global__ __launch_bounds__(256) void recurrence_clear_kernel(uint4* __restrict__ p, int64_t n) {
+__device__ __forceinline__ uint32_t see_flag(const uint32_t* flag) {
+    return __hip_atomic_load(flag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ uint32_t tag_of(uint64_t w) { return (uint32_t)(w >> 32); }
+__device__ __forceinline__ float pair_a(uint64_t w) { return __uint_as_float(tag_of(w) & 0x7fffffffu); }
+__device__ __forceinline__ float pair_h(uint64_t w) { return __uint_as_float((uint32_t)w); }
+
+// One wave, a channel a lane: tile k of the scan has the pair (A, H); the return value is the state
+// before it.  part: the wave's 64 channels among all; s_w [kGroup - 1] words of LDS a lane, `step` apart
+// (registers are the tile's).
+template <typename Shared>
+__device__ __forceinline__ float state_before(const Shared& sh, int k, int tiles, int64_t D, int part, uint32_t ch,
+                                              float A, float H, uint64_t* s_w, int step) {
+    const int g = k / kGroup, pos = k % kGroup, lane = threadIdx.x & 63;
+    const int ngroups = (tiles - 1) / kGroup + 1;
+    uint32_t* flags = sh.flags + (int64_t)part * tiles;
+    uint32_t* gflags = sh.gflags + (int64_t)part * ngroups;
+    uint64_t* behind = sh.groups + g * D + ch;
+    leave(sh.words + k * D + ch, __float_as_uint(A) | 0x80000000u, H);
+    raise_flag(flags + k, 1);
+    int polls = 0;
+    if (pos > 0) {  // the pairs of the tiles before this one in its group
+        const uint64_t* row = sh.words + (int64_t)g * kGroup * D;
+        bool all = false;
+#pragma unroll 1
+        while (!all && polls <= kMaxPolls) {
+            while (!__all(see_flag(flags + g * kGroup + min(lane, pos - 1)) != 0) && ++polls <= kMaxPolls)
+                __builtin_amdgcn_s_sleep(4);
+            uint64_t w[kGroup - 1];
+            uint32_t at = ch * 8;
+            asm volatile("" : "+v"(at));  // (or every word's address would be kept in registers)
+#pragma unroll
+            for (int i = 0; i < kGroup - 1; ++i)
+                if (i < pos) w[i] = look(row + i * D, at);
+            all = true;
+#pragma unroll
+            for (int i = 0; i < kGroup - 1; ++i)
+                if (i < pos) {
+                    all = all & (tag_of(w[i]) != 0);
+                    s_w[i * step] = w[i];
+                }
+            all = __all(all);
+            ++polls;
+        }
+    }
+    float Ag = 1.0f, Hg = 0.0f, c = 0.0f;
+    if (pos == kGroup - 1) {
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+            const float a = i < kGroup - 1 ? pair_a(s_w[i * step]) : A;
+            Hg = through(a, i < kGroup - 1 ? pair_h(s_w[i * step]) : H, Hg);
+            Ag = a == 0.0f ? 0.0f : Ag * a;
+        }
+        // nothing enters the first group, and nothing passes a sequence's border
+        const bool whole = g == 0 || Ag == 0.0f;
+        leave(behind, whole ? kWhole : __float_as_uint(Ag) | 0x80000000u, Hg);
+        raise_flag(gflags + g, __all(whole) ? 2 : 1);
+    }
+    if (g > 0) {
+        bool all = false;
+#pragma unroll 1
+        while (!all && polls <= kMaxPolls) {
+            int far;  // the nearest group whose state is known, with pairs of all groups between
+            for (;; __builtin_amdgcn_s_sleep(4)) {
+                const uint32_t f = lane < g ? see_flag(gflags + g - 1 - lane) : 0;
+                const uint64_t whole = __ballot(f == 2), some = __ballot(f != 0);
+                far = whole ? __builtin_ctzll(whole) : 64;
+                const uint64_t between = far < 64 ? (1ull << far) - 1 : ~0ull;
+                if ((far < 64 && (some & between) == between) || ++polls > kMaxPolls) break;
+            }
+            // (a word may say less than its flag, for a moment, or more: any P on the way is as good)
+            all = far < 64;
+            bool known = false;
+#pragma unroll 1
+            for (int i0 = min(far, 63) & ~3; i0 >= 0; i0 -= 4) {
+                uint64_t p[4];
+                uint32_t at = ch * 8;
+                asm volatile("" : "+v"(at));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[i] = look(sh.groups + max(g - 1 - i0 - i, 0) * D, at);
+#pragma unroll
+                for (int i = 3; i >= 0; --i)
+                    if (i0 + i <= far) {
+                        const uint32_t tag = tag_of(p[i]);
+                        c = tag == kWhole ? pair_h(p[i]) : __fmaf_rn(pair_a(p[i]), c, pair_h(p[i]));
+                        known = tag == kWhole || (known && tag != 0);
+                    }
+            }
+            all = __all(known) && all;
+            ++polls;
+        }
+        if (pos == kGroup - 1) {
+            if (Ag != 0.0f) leave(behind, kWhole, __fmaf_rn(Ag, c, Hg));
+            raise_flag(gflags + g, 2);
+        }
+    }
+    for (int i = 0; i < pos; ++i) c = through(pair_a(s_w[i * step]), pair_h(s_w[i * step]), c);
+    return polls > kMaxPolls ? __builtin_nanf("") : c;
+}
+
+// Words and flags to 0, the decay rates.
+__global__ __launch_bounds__(256) void recurrence_clear_kernel(RecShared s, int64_t n16, int D,
+                                                               const float* __restrict__ lam, float rate) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < n) p[i] = make_uint4(0, 0, 0, 0);
+    for (int64_t j = i; j < n16; j += (int64_t)gridDim.x * 256)
+        reinterpret_cast<uint4*>(s.ticket)[j] = make_uint4(0, 0, 0, 0);
+    for (int64_t j = i; j < D; j += (int64_t)gridDim.x * 256) s.k2[j] = decay_rate(lam[j], rate);
 }
 
 // A state row a sequence brings in, or zeros.
@@ -254,33 +334,31 @@ __device__ __forceinline__ void put_state(float* to, int s, int D, int ch, const
     for (int k = 0; k < V; ++k) to[(int64_t)s * D + ch + k] = h[k];
 }
 
-// h -> A h + H; A = 0 passes nothing on, whatever h holds (it may be another sequence's infinity)
-__device__ __forceinline__ float through(float A, float H, float h) {
-    return A == 0.0f ? H : __fmaf_rn(A, h, H);
-}
-
-// What a workgroup and a wave of it work on.
+// A tile of 64 V channels: the at-th of the scan.
+template <int V>
 struct Place {
-    int64_t t0, order;              // first token; the tile's number in the scan
-    int ch, cb, lane, wave, real;   // the lane's first channel, the block's; tokens the tile really has
-    bool act;                       // false: a lane past the last channel, which computes the last ones again
-    uint32_t starts, ends, inside;  // a bit per token of the wave
+    int64_t t0;    // first token
+    int order;     // its number in the scan
+    int c0, ch;    // the first channel; the lane's first
+    int real;      // tokens the tile really has
+    bool act;      // false: a lane past the last channel, which computes the last ones again
+    __device__ __forceinline__ Place(int at, int tile, int block, int64_t T, int D, int lane, bool reverse) {
+        order = at;
+        c0 = block * 64 * V;
+        t0 = (reverse ? (T - 1) / tile - order : order) * tile;
+        ch = min(c0 + lane * V, D - V);
+        act = c0 + lane * V < D;
+        real = (int)min((int64_t)tile, T - t0);
+    }
 };
 
-template <int V, int L, int R>
-__device__ __forceinline__ Place find_place(uint32_t* ticket, int T, int D, bool reverse) {
-    Place p;
-    p.lane = threadIdx.x & 63;
-    p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int blocks = (D - 1) / (64 * V) + 1, at = take_ticket(ticket), order = at / blocks;
-    const int c0 = (at - order * blocks) * 64 * V;
-    p.order = order;
-    p.t0 = (int64_t)(reverse ? (T - 1) / L - order : order) * L;
-    p.ch = min(c0 + p.lane * V, D - V);
-    p.cb = min(c0, D - V);
-    p.act = c0 + p.lane * V < D;
-    p.real = (int)min((int64_t)L, T - p.t0);
-    return p;
+// The bounds, in LDS where they fit.
+constexpr int kCuLds = 2048;
+
+template <int NT>
+__device__ __forceinline__ void stage_bounds(const int32_t* __restrict__ cu, int S, int32_t* lds) {
+    if (S >= kCuLds) return;
+    for (int i = threadIdx.x; i <= S; i += NT) lds[i] = cu[i];
 }
 
 struct RecFwd {
@@ -294,46 +372,106 @@ struct RecFwd {
     void* y;
     int64_t ys;
     float *final, *carry;  // carry [T / kKept up, D]: the state before every kKept-th token
-    uint32_t* ticket;      // NULL where there is one tile in time
-    uint64_t* words;       // [tiles, D]
+    RecShared sh;
 };
 
-// A workgroup takes a tile of 128 channels, two a lane; each wave takes R of the tile's tokens.
+// The kernel's argument, read again where it is asked for: what a loop over tiles keeps of it (and of
+// addresses formed from it) from one tile to the next would take the registers of the tile.
+template <typename T>
+__device__ __forceinline__ const __attribute__((address_space(4))) T& argument() {
+    auto p = (const __attribute__((address_space(4))) T*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *p;
+}
+
+// The workgroup's block of channels.  Tiles of a block end in the order of the scan, so its workgroups move
+// in step; each XCD and each CU holds workgroups of different blocks, whose steps differ, so that some
+// compute while others load (65536 x 1024: 215 us with a block on one XCD, 165 so).
+__device__ __forceinline__ int my_block(int blocks) {
+    // (up to 32 blocks are all named by the first 256 workgroups)
+    return (blocks <= 32 && gridDim.x >= 256 ? blockIdx.x / 8 + blockIdx.x / 256 : blockIdx.x) % blocks;
+}
+
+// The lane's decay rates; whether they all stay below kSmall, as most do: those take fewer steps.
+template <int V, typename Args>
+__device__ __forceinline__ bool decay_rates(const Args& arg, int block, float (&k2)[V]) {
+    bool small = true;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int ch = min(block * 64 * V + (int)(threadIdx.x & 63) * V, arg.D - V) + k;
+        k2[k] = arg.sh.k2 ? arg.sh.k2[ch] : decay_rate(arg.lam[ch], arg.rate);
+        small = small && k2[k] < kSmall;
+    }
+    return __all(small);
+}
+
+// The look back over the workgroup's 64 V slots (a lane's V channels side by side), a slot a lane of the
+// first V waves: the waves' pairs (s_a, s_h) in the scan's order make the tile's, and s_c gets the state
+// before it.
+template <int V, int WAVES, typename Shared>
+__device__ __forceinline__ void look_back(const Shared& sh, int order, int tiles, int c0, int D, bool reverse, int slot,
+                                          const float (&s_a)[WAVES][64 * V], const float (&s_h)[WAVES][64 * V],
+                                          float (&s_c)[64 * V], uint64_t* s_w) {
+    const int ch = min(c0 + slot / V * V, D - V) + slot % V;
+    float A = 1.0f, H = 0.0f;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+        const int w = reverse ? WAVES - 1 - i : i;
+        const float aw = s_a[w][slot];
+        H = through(aw, s_h[w][slot], H);
+        A = aw == 0.0f ? 0.0f : A * aw;
+    }
+    const int part = __builtin_amdgcn_readfirstlane((c0 + slot) / 64);
+    s_c[slot] = sh.ticket ? state_before(sh, order, tiles, D, part, ch, A, H, s_w + slot, 64 * V)
+                          : 0.0f;
+}
+
+// Workgroups take tiles of kTile tokens and 64 V channels, V a lane, in the order of the scan; each wave
+// takes R of the tile's tokens.
 template <int DT, int V, int R>
-__global__ __launch_bounds__(64 * (kTile / R), 4) void recurrence_kernel(RecFwd P) {
-    constexpr int L = kTile, WAVES = L / R, NT = 64 * WAVES;
-    constexpr uint32_t ALL = (1u << R) - 1;
-    __shared__ int32_t s_start[L], s_end[L];
-    __shared__ float s_k2[64 * V], s_c[V][64], s_a[WAVES][V][64], s_h[WAVES][V][64];
-    Place p = find_place<V, L, R>(P.ticket, P.T, P.D, false);
-    const int lane = p.lane, wave = p.wave, ch = p.ch;
-    const uint32_t off = ch * (DT == NSOSX_F32 ? 4 : 2);
-    float a[R][V], u[R][V];
-    {
+__global__ __launch_bounds__(64 * (kTile / R), 4) void recurrence_kernel(RecFwd arg) {
+    constexpr int WAVES = kTile / R, NT = 64 * WAVES;
+    __shared__ int32_t s_cu[kCuLds];
+    __shared__ uint64_t s_w[(kGroup - 1) * 64 * V];
+    __shared__ int32_t s_seq[kTile];
+    __shared__ int s_next;
+    __shared__ float s_c[64 * V], s_a[2][WAVES][64 * V], s_h[2][WAVES][64 * V];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tiles = (int)((arg.T - 1) / kTile + 1), block = my_block((arg.D - 1) / (64 * V) + 1);
+    stage_bounds<NT>(arg.cu, arg.S, s_cu);
+    if (threadIdx.x == 0) s_next = arg.sh.ticket ? (int)atomicAdd(arg.sh.ticket + block * 16, 1u) : 0;
+    __syncthreads();
+    int at = __builtin_amdgcn_readfirstlane(s_next);
+    float k2[V];
+    const bool small = decay_rates<V>(arg, block, k2);
+    for (int turn = 0; at < tiles; turn ^= 1) {
+        const auto& P = argument<RecFwd>();
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const Place<V> p(at, kTile, block, P.T, P.D, lane, false);
+        const int ch = p.ch;
+        const uint32_t off = ch * (DT == NSOSX_F32 ? 4 : 2);
         Pair<DT, V> x[R], r[R], g[R];
-        const Rows vx = tile_rows<DT>(P.x, P.xs, p.t0), vr = tile_rows<DT>(P.rg, P.rs, p.t0),
-                   vg = tile_rows<DT>(P.ig, P.is, p.t0);
+        {
+            const Rows vx = tile_rows<DT>(P.x, P.xs, p.t0), vr = tile_rows<DT>(P.rg, P.rs, p.t0),
+                       vg = tile_rows<DT>(P.ig, P.is, p.t0);
 #pragma unroll
-        for (int j = 0; j < R; ++j) {
-            const int t = min(wave * R + j, p.real - 1);
-            r[j].load(vr, off, t);
-            g[j].load(vg, off, t);
-            x[j].load(vx, off, t);
+            for (int j = 0; j < R; ++j) {
+                const int t = min(wave * R + j, p.real - 1);
+                r[j].load(vr, off, t);
+                g[j].load(vg, off, t);
+                x[j].load(vx, off, t);
+            }
         }
-        for (int i = threadIdx.x; i < 64 * V; i += NT)
-            s_k2[i] = decay_rate(P.lam[min(p.cb + i, P.D - 1)], P.rate);
-        tile_borders<NT, L>(P.cu, P.S, p.t0, s_start, s_end);
-        wave_masks<R>(s_start, s_end, wave, p.t0, P.cu[0], min(P.cu[P.S], P.T), p.starts, p.ends, p.inside);
-        float k2[V];
-        bool small = true;
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            k2[k] = s_k2[ch - p.cb + k];
-            small = small && k2[k] < kSmall;
-        }
+        const Tokens tok = find_tokens<R>(P.S < kCuLds ? s_cu : P.cu, P.S, lane, p.t0 + wave * R, P.T, s_seq + wave * R);
+        const bool plain = tok.template plain<R>();
+        float a[R][V], u[R][V];
         auto gates = [&](auto fits) {
 #pragma unroll
-            for (int j = 0; j < R; ++j)
+            for (int j = 0; j < R; ++j) {
+                r[j].forget();
+                g[j].forget();
+                x[j].forget();
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     const float q = k2[k] * sigmoid_of(exp_neg(r[j].get(k)));
@@ -341,78 +479,73 @@ __global__ __launch_bounds__(64 * (kTile / R), 4) void recurrence_kernel(RecFwd 
                     u[j][k] = __builtin_amdgcn_sqrtf(one_less_square<decltype(fits)::value>(q, a[j][k])) *
                               (sigmoid_of(exp_neg(g[j].get(k))) * x[j].get(k));
                 }
+                __builtin_amdgcn_sched_barrier(0);  // token after token, or all of them are half done at once
+            }
         };
-        // (decays that stay above 0.88 even at open gates, as most do, take a third fewer steps)
-        if (__all(small)) gates(std::true_type{});
+        // (decays that stay above 0.88 even at open gates, as most do, take fewer steps)
+        if (small) gates(std::true_type{});
         else gates(std::false_type{});
-    }
-    const bool plain = !p.starts && !p.ends && p.inside == ALL;  // no border, no row of no sequence
-    float A[V], H[V];
+        float A[V], H[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) A[k] = 1.0f, H[k] = 0.0f;
-    auto local = [&](auto borders) {
+        for (int k = 0; k < V; ++k) A[k] = 1.0f, H[k] = 0.0f;
+        auto local = [&](auto borders) {
 #pragma unroll
-        for (int j = 0; j < R; ++j) {
-            const bool start = decltype(borders)::value && (p.starts >> j & 1);
-            if (start) take_state<V>(P.initial, s_start[wave * R + j], P.D, ch, H);
+            for (int j = 0; j < R; ++j) {
+                const bool start = decltype(borders)::value && (tok.starts >> j & 1);
+                if (start) take_state<V>(P.initial, s_seq[wave * R + j], P.D, ch, H);
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                H[k] = __fmaf_rn(a[j][k], H[k], u[j][k]);
-                A[k] = start ? 0.0f : A[k] * a[j][k];
+                for (int k = 0; k < V; ++k) {
+                    H[k] = __fmaf_rn(a[j][k], H[k], u[j][k]);
+                    A[k] = start ? 0.0f : A[k] * a[j][k];
+                }
             }
-        }
-    };
-    if (plain) local(std::false_type{});
-    else local(std::true_type{});
+        };
+        if (plain) local(std::false_type{});
+        else local(std::true_type{});
 #pragma unroll
-    for (int k = 0; k < V; ++k) s_a[wave][k][lane] = A[k], s_h[wave][k][lane] = H[k];
-    __syncthreads();
-    if (wave == 0) {
-        float c[V];
+        for (int k = 0; k < V; ++k) s_a[turn][wave][lane * V + k] = A[k], s_h[turn][wave][lane * V + k] = H[k];
+        __syncthreads();
+        if (wave < V) look_back<V, WAVES>(P.sh, p.order, tiles, p.c0, P.D, false, wave * 64 + lane, s_a[turn], s_h[turn], s_c, s_w);
+        __syncthreads();
+        int next = tiles;  // (taken no earlier: a ticket that lies with a waiting workgroup holds all later ones up)
+        if (threadIdx.x == 0 && P.sh.ticket) next = (int)atomicAdd(P.sh.ticket + block * 16, 1u);
+        float h[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            c[k] = 0.0f;
+        for (int k = 0; k < V; ++k) h[k] = s_c[lane * V + k];
 #pragma unroll
-            for (int w = 1; w < WAVES; ++w) {
-                const float aw = s_a[w][k][lane];
-                H[k] = through(aw, s_h[w][k][lane], H[k]);
-                A[k] = aw == 0.0f ? 0.0f : A[k] * aw;
+        for (int k = 0; k < V; ++k)
+            for (int w = 0; w < wave; ++w)
+                h[k] = through(s_a[turn][w][lane * V + k], s_h[turn][w][lane * V + k], h[k]);
+        if (wave * R % kKept == 0 && P.carry && wave * R < p.real && p.act)
+            put_state<V>(P.carry, (int)((p.t0 + wave * R) / kKept), P.D, ch, h);
+        const Rows vy = tile_rows<DT>(P.y, P.ys, p.t0);
+        auto apply = [&](auto borders) {
+            constexpr bool B = decltype(borders)::value;
+            const float zero[V] = {};
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                const int t = wave * R + j;
+                if (B && !(tok.inside >> j & 1)) {
+                    if (P.rest && t < p.real && p.act) Pair<DT, V>::store(vy, off, t, zero);
+                    continue;
+                }
+                if (B && (tok.starts >> j & 1)) take_state<V>(P.initial, s_seq[wave * R + j], P.D, ch, h);
+#pragma unroll
+                for (int k = 0; k < V; ++k) h[k] = __fmaf_rn(a[j][k], h[k], u[j][k]);
+                if (p.act) Pair<DT, V>::store(vy, off, t, h);
+                if (B && (tok.ends >> j & 1) && P.final) {
+                    const int seq = s_seq[wave * R + j];
+                    if (p.act) put_state<V>(P.final, seq, P.D, ch, h);
+                }
             }
-        }
-        if (P.ticket) state_before<V>(P.words, p.order, P.D, ch, A, H, c);
-#pragma unroll
-        for (int k = 0; k < V; ++k) s_c[k][lane] = c[k];
+        };
+        if (plain) apply(std::false_type{});
+        else apply(std::true_type{});
+        if (threadIdx.x == 0) s_next = next;
+        __syncthreads();
+        at = __builtin_amdgcn_readfirstlane(s_next);
+        if (p.order == 0 && P.final) empty_states<V, NT>(P.cu, P.S, P.D, ch, p.act, P.initial, P.final);
     }
-    __syncthreads();
-    float h[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-        h[k] = s_c[k][lane];
-        for (int w = 0; w < wave; ++w) h[k] = through(s_a[w][k][lane], s_h[w][k][lane], h[k]);
-    }
-    if (wave * R % kKept == 0 && P.carry && wave * R < p.real && p.act)
-        put_state<V>(P.carry, (int)((p.t0 + wave * R) / kKept), P.D, ch, h);
-    const Rows vy = tile_rows<DT>(P.y, P.ys, p.t0);
-    auto apply = [&](auto borders) {
-        constexpr bool B = decltype(borders)::value;
-        const float zero[V] = {};
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            const int t = wave * R + j;
-            if (B && !(p.inside >> j & 1)) {
-                if (P.rest && t < p.real && p.act) Pair<DT, V>::store(vy, off, t, zero);
-                continue;
-            }
-            if (B && (p.starts >> j & 1)) take_state<V>(P.initial, s_start[t], P.D, ch, h);
-#pragma unroll
-            for (int k = 0; k < V; ++k) h[k] = __fmaf_rn(a[j][k], h[k], u[j][k]);
-            if (p.act) Pair<DT, V>::store(vy, off, t, h);
-            if (B && (p.ends >> j & 1) && P.final && p.act) put_state<V>(P.final, s_end[t], P.D, ch, h);
-        }
-    };
-    if (plain) apply(std::false_type{});
-    else apply(std::true_type{});
-    if (p.order == 0 && P.final) empty_states<V, NT>(P.cu, P.S, P.D, ch, p.act, P.initial, P.final);
 }
 
 struct RecBwd {
@@ -426,211 +559,203 @@ struct RecBwd {
     void *dx, *drg, *dig;
     int64_t dxs, drs, dis;
     float *dinitial, *dlam_part;  // dlam_part [tiles, D]
-    uint32_t* ticket;
-    uint64_t* words;  // [tiles, D], of the reversed stream
+    RecShared sh;
 };
 
-// The same from the last tile to the first.  With q = g / log 2, w = a q and b2 = p = 1 - a^2:
+// The same from the last tile to the first.  With q = g / log 2, w = a q and b2 = 1 - a^2:
 //   e = dh (s x a w / beta - w h_before), in units of log 2;  what 1 / beta multiplies goes to 0 with it
 template <int DT, int V, int R>
-__global__ __launch_bounds__(64 * (kKept / R), 4) void recurrence_bwd_kernel(RecBwd P) {
-    constexpr int L = kKept, WAVES = L / R, NT = 64 * WAVES;
-    constexpr uint32_t ALL = (1u << R) - 1;
-    __shared__ int32_t s_start[L], s_end[L];
-    __shared__ float s_k2[64 * V], s_c[V][64], s_a[WAVES][V][64], s_h[WAVES][V][64], s_b[WAVES][V][64],
-        s_m[WAVES][V][64];
-    Place p = find_place<V, L, R>(P.ticket, P.T, P.D, true);
-    const int lane = p.lane, wave = p.wave, ch = p.ch;
-    const uint32_t off = ch * (DT == NSOSX_F32 ? 4 : 2);
-    // kept over the wait: a, u (then the state before each token), e^-rg, e^-ig, x and dy as loaded
-    float a[R][V], u[R][V], er[R][V], eg[R][V], k2[V];
-    Pair<DT, V> x[R], d[R];
-    float h0[V];
-    {
-        Pair<DT, V> r[R], g[R];
-        const Rows vx = tile_rows<DT>(P.x, P.xs, p.t0), vr = tile_rows<DT>(P.rg, P.rs, p.t0),
-                   vg = tile_rows<DT>(P.ig, P.is, p.t0), vd = tile_rows<DT>(P.dy, P.dys, p.t0);
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            const int t = min(wave * R + j, p.real - 1);
-            r[j].load(vr, off, t);
-            g[j].load(vg, off, t);
-            x[j].load(vx, off, t);
-            d[j].load(vd, off, t);
-        }
-        take_state<V>(P.carry, (int)(p.t0 / kKept), P.D, ch, h0);
-        for (int i = threadIdx.x; i < 64 * V; i += NT)
-            s_k2[i] = decay_rate(P.lam[min(p.cb + i, P.D - 1)], P.rate);
-        tile_borders<NT, L>(P.cu, P.S, p.t0, s_start, s_end);
-        wave_masks<R>(s_start, s_end, wave, p.t0, P.cu[0], min(P.cu[P.S], P.T), p.starts, p.ends, p.inside);
-#pragma unroll
-        for (int j = 0; j < R; ++j)
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                er[j][k] = exp_neg(r[j].get(k));
-                eg[j][k] = exp_neg(g[j].get(k));
-            }
-    }
-    bool small = true;
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-        k2[k] = s_k2[ch - p.cb + k];
-        small = small && k2[k] < kSmall;
-    }
-    small = __all(small);
-    auto gates = [&](auto fits) {
-#pragma unroll
-        for (int j = 0; j < R; ++j)
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float q = k2[k] * sigmoid_of(er[j][k]);
-                a[j][k] = __builtin_amdgcn_exp2f(-q);
-                u[j][k] = __builtin_amdgcn_sqrtf(one_less_square<decltype(fits)::value>(q, a[j][k])) *
-                          (sigmoid_of(eg[j][k]) * x[j].get(k));
-            }
-    };
-    if (small) gates(std::true_type{});
-    else gates(std::false_type{});
-    const bool plain = !p.starts && !p.ends && p.inside == ALL;
-    float A[V], H[V], B[V], M[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) A[k] = B[k] = 1.0f, H[k] = M[k] = 0.0f;
-    auto local = [&](auto borders) {
-        constexpr bool BORDERS = decltype(borders)::value;
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            const bool start = BORDERS && (p.starts >> j & 1);
-            if (start) take_state<V>(P.initial, s_start[wave * R + j], P.D, ch, H);
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                H[k] = __fmaf_rn(a[j][k], H[k], u[j][k]);
-                A[k] = start ? 0.0f : A[k] * a[j][k];
-            }
-        }
-#pragma unroll
-        for (int j = R - 1; j >= 0; --j) {
-            const bool end = BORDERS && (p.ends >> j & 1), out = BORDERS && !(p.inside >> j & 1);
-            if (end) take_state<V>(P.dfinal, s_end[wave * R + j], P.D, ch, M);
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                M[k] = out ? 0.0f : a[j][k] * (d[j].get(k) + M[k]);
-                B[k] = end || out ? 0.0f : B[k] * a[j][k];
-            }
-        }
-    };
-    if (plain) local(std::false_type{});
-    else local(std::true_type{});
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-        s_a[wave][k][lane] = A[k], s_h[wave][k][lane] = H[k];
-        s_b[wave][k][lane] = B[k], s_m[wave][k][lane] = M[k];
-    }
+__global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_bwd_kernel(RecBwd arg) {
+    constexpr int WAVES = kKept / R, NT = 64 * WAVES;
+    __shared__ int32_t s_cu[kCuLds];
+    __shared__ uint64_t s_w[(kGroup - 1) * 64 * V];
+    __shared__ int32_t s_seq[kKept];
+    __shared__ int s_next;
+    __shared__ float s_c[64 * V], s_a[WAVES][64 * V], s_h[WAVES][64 * V], s_b[WAVES][64 * V],
+        s_m[WAVES][64 * V];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tiles = (int)((arg.T - 1) / kKept + 1), block = my_block((arg.D - 1) / (64 * V) + 1);
+    stage_bounds<NT>(arg.cu, arg.S, s_cu);
+    if (threadIdx.x == 0) s_next = arg.sh.ticket ? (int)atomicAdd(arg.sh.ticket + block * 16, 1u) : 0;
     __syncthreads();
-    if (wave == WAVES - 1) {
-        float c[V];
+    int at = __builtin_amdgcn_readfirstlane(s_next);
+    float k2[V];
+    const bool small = decay_rates<V>(arg, block, k2);
+    while (at < tiles) {
+        const auto& P = argument<RecBwd>();
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const Place<V> p(at, kKept, block, P.T, P.D, lane, true);
+        const int ch = p.ch;
+        const uint32_t off = ch * (DT == NSOSX_F32 ? 4 : 2);
+        // kept over the wait: a, u (then the state before each token), e^-rg, e^-ig, x and dy as loaded
+        float a[R][V], u[R][V], er[R][V], eg[R][V], h[V];
+        Pair<DT, V> x[R], d[R];
+        {
+            Pair<DT, V> r[R], g[R];
+            const Rows vx = tile_rows<DT>(P.x, P.xs, p.t0), vr = tile_rows<DT>(P.rg, P.rs, p.t0),
+                       vg = tile_rows<DT>(P.ig, P.is, p.t0), vd = tile_rows<DT>(P.dy, P.dys, p.t0);
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                const int t = min(wave * R + j, p.real - 1);
+                r[j].load(vr, off, t);
+                g[j].load(vg, off, t);
+                x[j].load(vx, off, t);
+                d[j].load(vd, off, t);
+            }
+            take_state<V>(P.carry, (int)(p.t0 / kKept), P.D, ch, h);
+#pragma unroll
+            for (int j = 0; j < R; ++j)
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    er[j][k] = exp_neg(r[j].get(k));
+                    eg[j][k] = exp_neg(g[j].get(k));
+                }
+        }
+        const Tokens tok = find_tokens<R>(P.S < kCuLds ? s_cu : P.cu, P.S, lane, p.t0 + wave * R, P.T, s_seq + wave * R);
+        const bool plain = tok.template plain<R>();
+        auto gates = [&](auto fits) {
+#pragma unroll
+            for (int j = 0; j < R; ++j)
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const float q = k2[k] * sigmoid_of(er[j][k]);
+                    a[j][k] = __builtin_amdgcn_exp2f(-q);
+                    u[j][k] = __builtin_amdgcn_sqrtf(one_less_square<decltype(fits)::value>(q, a[j][k])) *
+                              (sigmoid_of(eg[j][k]) * x[j].get(k));
+                }
+        };
+        if (small) gates(std::true_type{});
+        else gates(std::false_type{});
+        float A[V], H[V], B[V], M[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) A[k] = B[k] = 1.0f, H[k] = M[k] = 0.0f;
+        auto local = [&](auto borders) {
+            constexpr bool BORDERS = decltype(borders)::value;
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                const bool start = BORDERS && (tok.starts >> j & 1);
+                if (start) take_state<V>(P.initial, s_seq[wave * R + j], P.D, ch, H);
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    H[k] = __fmaf_rn(a[j][k], H[k], u[j][k]);
+                    A[k] = start ? 0.0f : A[k] * a[j][k];
+                }
+            }
+#pragma unroll
+            for (int j = R - 1; j >= 0; --j) {
+                const bool end = BORDERS && (tok.ends >> j & 1), out = BORDERS && !(tok.inside >> j & 1);
+                if (end) take_state<V>(P.dfinal, s_seq[wave * R + j], P.D, ch, M);
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    M[k] = out ? 0.0f : a[j][k] * (d[j].get(k) + M[k]);
+                    B[k] = end || out ? 0.0f : B[k] * a[j][k];
+                }
+            }
+        };
+        if (plain) local(std::false_type{});
+        else local(std::true_type{});
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            c[k] = 0.0f;
-#pragma unroll
-            for (int w = WAVES - 2; w >= 0; --w) {
-                const float bw = s_b[w][k][lane];
-                M[k] = through(bw, s_m[w][k][lane], M[k]);
-                B[k] = bw == 0.0f ? 0.0f : B[k] * bw;
-            }
+            s_a[wave][lane * V + k] = A[k], s_h[wave][lane * V + k] = H[k];
+            s_b[wave][lane * V + k] = B[k], s_m[wave][lane * V + k] = M[k];
         }
-        if (P.ticket) state_before<V>(P.words, p.order, P.D, ch, B, M, c);
-#pragma unroll
-        for (int k = 0; k < V; ++k) s_c[k][lane] = c[k];
-    }
-    float h[V], m[V], e[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-        h[k] = h0[k];
-        for (int w = 0; w < wave; ++w) h[k] = through(s_a[w][k][lane], s_h[w][k][lane], h[k]);
-    }
-    // u becomes the state before each token
-    auto states = [&](auto borders) {
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            if (decltype(borders)::value && (p.starts >> j & 1))
-                take_state<V>(P.initial, s_start[wave * R + j], P.D, ch, h);
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float before = h[k];
-                h[k] = __fmaf_rn(a[j][k], h[k], u[j][k]);
-                u[j][k] = before;
-            }
-        }
-    };
-    if (plain) states(std::false_type{});
-    else states(std::true_type{});
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-        m[k] = s_c[k][lane];
-        for (int w = WAVES - 1; w > wave; --w) m[k] = through(s_b[w][k][lane], s_m[w][k][lane], m[k]);
-        e[k] = 0.0f;
-    }
-    // (the compiler would keep the gates since their first use, in registers that are not there)
-#pragma unroll
-    for (int j = 0; j < R; ++j)
-#pragma unroll
-        for (int k = 0; k < V; ++k) asm volatile("" : "+v"(er[j][k]), "+v"(eg[j][k]));
-    const Rows vx = tile_rows<DT>(P.dx, P.dxs, p.t0), vr = tile_rows<DT>(P.drg, P.drs, p.t0),
-               vg = tile_rows<DT>(P.dig, P.dis, p.t0);
-    auto apply = [&](auto borders, auto fits) {
-        constexpr bool BORDERS = decltype(borders)::value;
-        const float zero[V] = {};
-#pragma unroll
-        for (int j = R - 1; j >= 0; --j) {
-            const int t = wave * R + j;
-            if (BORDERS && !(p.inside >> j & 1)) {
-                if (P.rest && t < p.real && p.act) {
-                    Pair<DT, V>::store(vx, off, t, zero);
-                    Pair<DT, V>::store(vr, off, t, zero);
-                    Pair<DT, V>::store(vg, off, t, zero);
-                }
-                continue;
-            }
-            if (BORDERS && (p.ends >> j & 1)) take_state<V>(P.dfinal, s_end[t], P.D, ch, m);
-            float ox[V], orr[V], oi[V];
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float sr = sigmoid_of(er[j][k]), si = sigmoid_of(eg[j][k]);
-                const float q = k2[k] * sr, xv = x[j].get(k), av = a[j][k];
-                const float b2 = one_less_square<decltype(fits)::value>(q, av);
-                const float rb = __builtin_amdgcn_rsqf(fmaxf(b2, 1e-37f));  // 1 / beta
-                const float w = av * q, dh = d[j].get(k) + m[k];
-                const float ev = dh * __fmaf_rn(si * xv, av * w * rb, -(w * u[j][k]));
-                ox[k] = dh * (b2 * rb) * si;
-                oi[k] = ox[k] * xv * rest_of(eg[j][k], si);
-                orr[k] = ev * rest_of(er[j][k], sr) * kLn2;
-                e[k] += ev;
-                m[k] = av * dh;
-            }
-            if (p.act) {
-                Pair<DT, V>::store(vx, off, t, ox);
-                Pair<DT, V>::store(vr, off, t, orr);
-                Pair<DT, V>::store(vg, off, t, oi);
-            }
-            if (BORDERS && (p.starts >> j & 1) && P.dinitial && p.act)
-                put_state<V>(P.dinitial, s_start[t], P.D, ch, m);
-        }
-    };
-    if (!plain) apply(std::true_type{}, std::false_type{});
-    else if (small) apply(std::false_type{}, std::true_type{});
-    else apply(std::false_type{}, std::false_type{});
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < V; ++k) s_a[wave][k][lane] = e[k];
-    __syncthreads();
-    if (wave == 0 && p.act) {
+        __syncthreads();
+        if (wave < V) look_back<V, WAVES>(P.sh, p.order, tiles, p.c0, P.D, true, wave * 64 + lane, s_b, s_m, s_c, s_w);
 #pragma unroll
         for (int k = 0; k < V; ++k)
-            for (int w = 1; w < WAVES; ++w) e[k] += s_a[w][k][lane];
-        put_state<V>(P.dlam_part, (int)(p.t0 / L), P.D, ch, e);
+            for (int w = 0; w < wave; ++w) h[k] = through(s_a[w][lane * V + k], s_h[w][lane * V + k], h[k]);
+        // u becomes the state before each token
+        auto states = [&](auto borders) {
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                if (decltype(borders)::value && (tok.starts >> j & 1))
+                    take_state<V>(P.initial, s_seq[wave * R + j], P.D, ch, h);
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const float before = h[k];
+                    h[k] = __fmaf_rn(a[j][k], h[k], u[j][k]);
+                    u[j][k] = before;
+                }
+            }
+        };
+        if (plain) states(std::false_type{});
+        else states(std::true_type{});
+        __syncthreads();
+        int next = tiles;  // (taken no earlier: a ticket that lies with a waiting workgroup holds all later ones up)
+        if (threadIdx.x == 0 && P.sh.ticket) next = (int)atomicAdd(P.sh.ticket + block * 16, 1u);
+        float m[V], e[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            m[k] = s_c[lane * V + k];
+            for (int w = WAVES - 1; w > wave; --w) m[k] = through(s_b[w][lane * V + k], s_m[w][lane * V + k], m[k]);
+            e[k] = 0.0f;
+        }
+        // (the compiler would keep the gates since their first use, in registers that are not there)
+#pragma unroll
+        for (int j = 0; j < R; ++j)
+#pragma unroll
+            for (int k = 0; k < V; ++k) asm volatile("" : "+v"(er[j][k]), "+v"(eg[j][k]));
+        const Rows vx = tile_rows<DT>(P.dx, P.dxs, p.t0), vr = tile_rows<DT>(P.drg, P.drs, p.t0),
+                   vg = tile_rows<DT>(P.dig, P.dis, p.t0);
+        auto apply = [&](auto borders, auto fits) {
+            constexpr bool BORDERS = decltype(borders)::value;
+            const float zero[V] = {};
+#pragma unroll
+            for (int j = R - 1; j >= 0; --j) {
+                const int t = wave * R + j;
+                if (BORDERS && !(tok.inside >> j & 1)) {
+                    if (P.rest && t < p.real && p.act) {
+                        Pair<DT, V>::store(vx, off, t, zero);
+                        Pair<DT, V>::store(vr, off, t, zero);
+                        Pair<DT, V>::store(vg, off, t, zero);
+                    }
+                    continue;
+                }
+                if (BORDERS && (tok.ends >> j & 1)) take_state<V>(P.dfinal, s_seq[wave * R + j], P.D, ch, m);
+                float ox[V], orr[V], oi[V];
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const float sr = sigmoid_of(er[j][k]), si = sigmoid_of(eg[j][k]);
+                    const float q = k2[k] * sr, xv = x[j].get(k), av = a[j][k];
+                    const float b2 = one_less_square<decltype(fits)::value>(q, av);
+                    const float rb = __builtin_amdgcn_rsqf(fmaxf(b2, 1e-37f));  // 1 / beta
+                    const float w = av * q, dh = d[j].get(k) + m[k];
+                    const float ev = dh * __fmaf_rn(si * xv, av * w * rb, -(w * u[j][k]));
+                    ox[k] = dh * (b2 * rb) * si;
+                    oi[k] = ox[k] * xv * rest_of(eg[j][k], si);
+                    orr[k] = ev * rest_of(er[j][k], sr) * kLn2;
+                    e[k] += ev;
+                    m[k] = av * dh;
+                }
+                if (p.act) {
+                    Pair<DT, V>::store(vx, off, t, ox);
+                    Pair<DT, V>::store(vr, off, t, orr);
+                    Pair<DT, V>::store(vg, off, t, oi);
+                }
+                if (BORDERS && (tok.starts >> j & 1) && P.dinitial) {
+                    const int seq = s_seq[wave * R + j];
+                    if (p.act) put_state<V>(P.dinitial, seq, P.D, ch, m);
+                }
+            }
+        };
+        if (!plain) apply(std::true_type{}, std::false_type{});
+        else if (small) apply(std::false_type{}, std::true_type{});
+        else apply(std::false_type{}, std::false_type{});
+        __syncthreads();  // (s_a is read by now)
+#pragma unroll
+        for (int k = 0; k < V; ++k) s_a[wave][lane * V + k] = e[k];
+        if (threadIdx.x == 0) s_next = next;
+        __syncthreads();
+        at = __builtin_amdgcn_readfirstlane(s_next);
+        if (wave == 0 && p.act) {
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                for (int w = 1; w < WAVES; ++w) e[k] += s_a[w][lane * V + k];
+            put_state<V>(P.dlam_part, (int)(p.t0 / kKept), P.D, ch, e);
+        }
+        if (p.order == 0 && P.dinitial) empty_states<V, NT>(P.cu, P.S, P.D, ch, p.act, P.dfinal, P.dinitial);
     }
-    if (p.order == 0 && P.dinitial) empty_states<V, NT>(P.cu, P.S, P.D, ch, p.act, P.dfinal, P.dinitial);
 }
 
 // dlam = sigmoid(lam) / softplus(lam) * sum_t e, e in units of log 2: the tiles' sums in a fixed order (64 channels a
@@ -701,31 +826,65 @@ static const char* rec_check(int S, int64_t T, int D, int dtype, float rate) {
     return nullptr;
 }
 
-// ticket (16 bytes), then the words
-static int64_t rec_words_bytes(int64_t tiles, int D) { return tiles > 1 ? 16 + (tiles * D * 8 + 15) / 16 * 16 : 0; }
-
-template <typename P>
-static void clear_words(P& p, int64_t tiles, void* workspace, hipStream_t st) {
-    p.ticket = nullptr;
-    p.words = nullptr;
-    if (tiles == 1) return;
-    const int64_t n = rec_words_bytes(tiles, p.D) / 16;
-    p.ticket = static_cast<uint32_t*>(workspace);
-    p.words = reinterpret_cast<uint64_t*>(p.ticket + 4);
-    hipLaunchKernelGGL(recurrence_clear_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st,
-                       static_cast<uint4*>(workspace), n);
+// What the tiles share, in the workspace: ticket (16 bytes), words, flags, decay rates; nothing for one
+// tile in time.
+static RecShared rec_shared(int64_t tiles, int D, void* workspace, int64_t* clear, int64_t* bytes) {
+    RecShared s{};
+    const int64_t groups = (tiles - 1) / kGroup + 1, parts = ((int64_t)D + 63) / 64 + 1;
+    *clear = *bytes = 0;
+    if (tiles <= 1) return s;
+    char* at = static_cast<char*>(workspace);
+    int64_t n = 64 * parts;
+    s.ticket = reinterpret_cast<uint32_t*>(at);
+    s.words = reinterpret_cast<uint64_t*>(at + n);
+    n += tiles * D * 8;
+    s.groups = reinterpret_cast<uint64_t*>(at + n);
+    n += groups * D * 8;
+    s.flags = reinterpret_cast<uint32_t*>(at + n);
+    n += parts * tiles * 4;
+    s.gflags = reinterpret_cast<uint32_t*>(at + n);
+    n = (n + parts * groups * 4 + 15) / 16 * 16;
+    *clear = n / 16;
+    s.k2 = reinterpret_cast<float*>(at + n);
+    *bytes = n + ((int64_t)D * 4 + 15) / 16 * 16;
+    return s;
 }
 
+static int64_t rec_shared_bytes(int64_t tiles, int D) {
+    int64_t clear, bytes;
+    rec_shared(tiles, D, nullptr, &clear, &bytes);
+    return bytes;
+}
+
+static RecShared start_shared(int64_t tiles, int D, const float* lam, float rate, void* workspace, hipStream_t st) {
+    int64_t clear, bytes;
+    const RecShared s = rec_shared(tiles, D, workspace, &clear, &bytes);
+    if (!bytes) return s;
+    const int64_t blocks = (clear + 1023) / 1024;
+    hipLaunchKernelGGL(recurrence_clear_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st,
+                       s, clear, D, lam, rate);
+    return s;
+}
+
+// Workgroups: as many as the card holds at once, the same number for every block of channels.
+static unsigned rec_grid(int64_t tiles, int D, int V, int resident) {
+    const int64_t blocks = (D - 1) / (64 * V) + 1, each = resident / blocks;
+    return (unsigned)(blocks * (each < 1 ? 1 : each < tiles ? each : tiles));
+}
+
+// bf16: two channels a lane, f32 one (64 channels are a full line there, and the registers carry more
+// workgroups: 16384 x 2048 f32 121 us and 208 back, with two 167 and 273).
 template <int DT, int V>
 static void launch_recurrence(const RecFwd& p, hipStream_t st) {
-    const dim3 grid((unsigned)(rec_tiles(p.T, kTile) * ((p.D - 1) / (64 * V) + 1)));
-    hipLaunchKernelGGL((recurrence_kernel<DT, V, 16>), grid, dim3(64 * (kTile / 16)), 0, st, p);
+    hipLaunchKernelGGL((recurrence_kernel<DT, V, 16>), dim3(rec_grid(rec_tiles(p.T, kTile), p.D, V, 512)),
+                       dim3(64 * (kTile / 16)), 0, st, p);
 }
 
 template <int DT, int V>
 static void launch_recurrence_bwd(const RecBwd& p, hipStream_t st) {
-    const dim3 grid((unsigned)(rec_tiles(p.T, kKept) * ((p.D - 1) / (64 * V) + 1)));
-    hipLaunchKernelGGL((recurrence_bwd_kernel<DT, V, 8>), grid, dim3(64 * (kKept / 8)), 0, st, p);
+    hipLaunchKernelGGL((recurrence_bwd_kernel<DT, V, 8>),
+                       dim3(rec_grid(rec_tiles(p.T, kKept), p.D, V, V == 1 ? 768 : 512)), dim3(64 * (kKept / 8)),
+                       0, st, p);
 }
 
 // No token: every sequence is empty, its final state is its initial one.
@@ -749,7 +908,7 @@ extern "C" int nsosx_gated_recurrence_tile(void) { return kKept; }
 
 extern "C" int64_t nsosx_gated_recurrence_workspace(int T, int D) {
     if (T <= 0 || D <= 0) return 0;
-    return rec_words_bytes(rec_tiles(T, kTile), D);
+    return rec_shared_bytes(rec_tiles(T, kTile), D);
 }
 
 extern "C" int nsosx_gated_recurrence(const void* x, int64_t x_stride, const void* rg, int64_t rg_stride,
@@ -786,11 +945,10 @@ extern "C" int nsosx_gated_recurrence(const void* x, int64_t x_stride, const voi
     if (final_state && initial_state && overlaps(final_state, sd * 4, initial_state, sd * 4))
         return fail(NSOSX_ERR_INVALID, "gated_recurrence: final_state overlaps initial_state");
     RecFwd p{x, rg, ig, x_stride, rg_stride, ig_stride, lam, rate, cu_seqlens, S, T, D, zero_rest,
-             initial_state, y, y_stride, final_state, carry, nullptr, nullptr};
-    clear_words(p, rec_tiles(T, kTile), workspace, st);
+             initial_state, y, y_stride, final_state, carry,
+             start_shared(rec_tiles(T, kTile), D, lam, rate, workspace, st)};
     if (act_dtype == NSOSX_F32) {
-        if (D > 1) launch_recurrence<NSOSX_F32, 2>(p, st);
-        else launch_recurrence<NSOSX_F32, 1>(p, st);
+        launch_recurrence<NSOSX_F32, 1>(p, st);
     } else {
         if (D > 1) launch_recurrence<NSOSX_BF16, 2>(p, st);
         else launch_recurrence<NSOSX_BF16, 1>(p, st);
@@ -800,7 +958,7 @@ extern "C" int nsosx_gated_recurrence(const void* x, int64_t x_stride, const voi
 
 extern "C" int64_t nsosx_gated_recurrence_backward_workspace(int T, int D) {
     if (T <= 0 || D <= 0) return 0;
-    return rec_words_bytes(rec_tiles(T, kKept), D) + rec_tiles(T, kKept) * D * 4;
+    return rec_shared_bytes(rec_tiles(T, kKept), D) + rec_tiles(T, kKept) * D * 4;
 }
 
 extern "C" int nsosx_gated_recurrence_backward(
@@ -851,12 +1009,10 @@ extern "C" int nsosx_gated_recurrence_backward(
         return fail(NSOSX_ERR_INVALID, "gated_recurrence_backward: dinitial overlaps an input");
     RecBwd p{dy, x, rg, ig, dy_stride, x_stride, rg_stride, ig_stride, lam, rate, cu_seqlens, S, T, D,
              zero_rest, initial_state, carry, dfinal, dx, drg, dig, dx_stride, drg_stride, dig_stride,
-             dinitial, reinterpret_cast<float*>(static_cast<char*>(workspace) + rec_words_bytes(rec_tiles(T, kKept), D)),
-             nullptr, nullptr};
-    clear_words(p, rec_tiles(T, kKept), workspace, st);
+             dinitial, reinterpret_cast<float*>(static_cast<char*>(workspace) + rec_shared_bytes(rec_tiles(T, kKept), D)),
+             start_shared(rec_tiles(T, kKept), D, lam, rate, workspace, st)};
     if (act_dtype == NSOSX_F32) {
-        if (D > 1) launch_recurrence_bwd<NSOSX_F32, 2>(p, st);
-        else launch_recurrence_bwd<NSOSX_F32, 1>(p, st);
+        launch_recurrence_bwd<NSOSX_F32, 1>(p, st);
     } else {
         if (D > 1) launch_recurrence_bwd<NSOSX_BF16, 2>(p, st);
         else launch_recurrence_bwd<NSOSX_BF16, 1>(p, st);

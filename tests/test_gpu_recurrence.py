@@ -84,6 +84,23 @@ def test_against_float64(dev, lens, d, dtype, initial):
     assert none is None and torch.equal(y, y3)
 
 
+@pytest.mark.parametrize("d", [2050, 4200, 8200])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_wide(dev, d, dtype):
+    """Many blocks of channels (the last one narrow), several tiles of each, against the same channels in
+    a narrow call of their own."""
+    c, _ = make(dev, [300, 500], d, dtype, True)
+    y, final, carry = forward(c)
+    got = backward(c, carry)
+    for lo, hi in ((0, 64), (2000, 2050), (d - 70, d), (d - 1, d)):
+        p = {k: v if k == "cu" else v[..., lo:hi].contiguous() for k, v in c.items()}
+        py, pfinal, pcarry = forward(p)
+        want = backward(p, pcarry)
+        assert torch.equal(y[:, lo:hi], py) and torch.equal(final[:, lo:hi], pfinal)
+        for k in want:
+            assert torch.equal(got[k][..., lo:hi], want[k]), k
+
+
 def test_long_sequence(dev):
     """Many tiles behind one another (a state that crosses hundreds of them)."""
     c, n = make(dev, [40000, 7], 6, "f32", True)
