@@ -13,8 +13,9 @@ constexpr int kLnMaxDim = 1 << 30;
 constexpr int kLnRegDim = 16384;  // longest row that is held in registers
 
 // The sum over the TPR threads of a row, the same bits in each of them.  Rows of more than a wave add
-// the waves' sums in wave order; `turn` alternates the LDS slots, so that one barrier is enough.
-template <int TPR, int N>
+// the waves' sums in wave order; `turn` alternates the LDS slots, so that one barrier is enough.  NT: of
+// the workgroup.
+template <int TPR, int N, int NT>
 __device__ __forceinline__ void row_sums(float (&v)[N], float* lds, int turn) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -27,7 +28,7 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* lds, int turn) {
     }
     if constexpr (TPR > 64) {
         constexpr int W = TPR / 64;
-        const int waves = blockDim.x >> 6;
+        constexpr int waves = NT / 64;
         const int wave = threadIdx.x >> 6;
         float* at = lds + (turn & 1) * waves * N;
         if ((threadIdx.x & 63) == 0) {
@@ -46,6 +47,29 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* lds, int turn) {
     }
 }
 
+// Which of the workgroup's rows a thread works on: known to be one for a wave where a row takes whole waves,
+// so that its addresses are a scalar and a lane's offset.
+template <int TPR>
+__device__ __forceinline__ int row_group() {
+    const int g = threadIdx.x / TPR;
+    return TPR >= 64 ? __builtin_amdgcn_readfirstlane(g) : g;
+}
+
+// A thread's eight elements of piece c of a row of dim >= 8.  Those that would pass the row's end are the
+// last eight of it instead, `skip` of which are another thread's: they stay out of the sums and are
+// computed and stored twice, the same.  So no row needs a path for its tail, whatever its length.
+template <int TPR, int CH>
+struct Elements {
+    int at[CH], skip;  // skip: of the last piece; the others are whole
+    __device__ __forceinline__ Elements(int l, int dim) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) at[c] = min((c * TPR + l) * 8, dim - 8);
+        skip = min(((CH - 1) * TPR + l) * 8 - at[CH - 1], 8);
+    }
+    __device__ __forceinline__ bool mine(int c, int j) const { return c < CH - 1 || j >= skip; }
+    __device__ __forceinline__ bool any(int c) const { return c < CH - 1 || skip < 8; }
+};
+
 // y (and, with delta, the stored sum) of one row per TPR threads.
 template <int DT, int ODT, int TPR, int CH>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layernorm_kernel(
@@ -55,54 +79,59 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layernorm_kernel(
     constexpr int NT = TPR > 256 ? TPR : 256;
     __shared__ float lds[2 * (NT / 64)];
     const int l = threadIdx.x % TPR;
-    const int64_t row = (int64_t)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
+    const int64_t row = (int64_t)blockIdx.x * (NT / TPR) + row_group<TPR>();
     const bool real = row < rows;
-    const int64_t base = row * dim;
+    const int64_t base = (real ? row : rows - 1) * dim;
+    const Elements<TPR, CH> el(l, dim);
     float v[CH][8];
-    int n[CH];
+    {
+        Raw8<DT> r[CH], d[CH];
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        n[c] = real ? max(0, min(8, dim - (c * TPR + l) * 8)) : 0;
-        load8_part<DT>(x, base + (c * TPR + l) * 8, n[c], v[c]);
-    }
-    if (delta) {
-        float d[CH][8];
+        for (int c = 0; c < CH; ++c) r[c].load(x, base + el.at[c]);
+        if (delta) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) load8_part<DT>(delta, base + (c * TPR + l) * 8, n[c], d[c]);
+            for (int c = 0; c < CH; ++c) d[c].load(delta, base + el.at[c]);
+        }
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[c][j] = round_act<DT>(v[c][j] + d[c][j]);
-            store8_part<DT>(sum, base + (c * TPR + l) * 8, n[c], v[c]);
+            for (int j = 0; j < 8; ++j) v[c][j] = delta ? round_act<DT>(r[c].get(j) + d[c].get(j)) : r[c].get(j);
         }
     }
     float s[1] = {0.0f};
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[0] += v[c][j];
-    row_sums<TPR, 1>(s, lds, 0);
+        for (int j = 0; j < 8; ++j) s[0] += el.mine(c, j) ? v[c][j] : 0.0f;
+    row_sums<TPR, 1, NT>(s, lds, 0);
+    // (behind the sums: a sum over x or delta is read twice at a row's tail before it is written)
+    if (delta && real) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+            if (el.any(c)) store8_any<DT>(sum, base + el.at[c], v[c]);
+    }
     const float mean = s[0] / static_cast<float>(dim);
     s[0] = 0.0f;
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            v[c][j] = c < CH - 1 || j < n[c] ? v[c][j] - mean : 0.0f;
-            s[0] = __fmaf_rn(v[c][j], v[c][j], s[0]);
+            v[c][j] -= mean;
+            const float d = el.mine(c, j) ? v[c][j] : 0.0f;
+            s[0] = __fmaf_rn(d, d, s[0]);
         }
-    row_sums<TPR, 1>(s, lds, 1);
+    row_sums<TPR, 1, NT>(s, lds, 1);
     const float rstd = 1.0f / sqrtf(s[0] / static_cast<float>(dim) + eps);
-    if (real && l == 0 && mean_out) {
+    if (!real) return;
+    if (l == 0 && mean_out) {
         mean_out[row] = mean;
         rstd_out[row] = rstd;
     }
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        const int e = (c * TPR + l) * 8;
         float w[8], b[8];
-        if (weight) load8_part<NSOSX_F32>(weight, e, n[c], w);
-        if (bias) load8_part<NSOSX_F32>(bias, e, n[c], b);
+        if (weight) load8_any<NSOSX_F32>(weight, el.at[c], w);
+        if (bias) load8_any<NSOSX_F32>(bias, el.at[c], b);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             v[c][j] *= rstd;
@@ -110,22 +139,22 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layernorm_kernel(
             else if (weight) v[c][j] *= w[j];
             else if (bias) v[c][j] += b[j];
         }
-        store8_part<ODT>(y, base + e, n[c], v[c]);
+        if (el.any(c)) store8_any<ODT>(y, base + el.at[c], v[c]);
     }
 }
 
-// Rows past kLnRegDim: a workgroup of 1024 threads per row, which it reads again from the caches for
-// the variance and for y.
-template <int DT, int ODT>
-__global__ __launch_bounds__(1024) void layernorm_long_kernel(
+// Rows past kLnRegDim (and below 8): a workgroup per row, which it reads again from the caches for the
+// variance and for y.
+template <int DT, int ODT, int NT>
+__global__ __launch_bounds__(NT) void layernorm_long_kernel(
     const void* x, const void* delta, const float* __restrict__ weight,
     const float* __restrict__ bias, int dim, float eps, void* sum, void* __restrict__ y,
     float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-    __shared__ float lds[2 * 16];
+    __shared__ float lds[2 * (NT / 64)];
     const int64_t base = (int64_t)blockIdx.x * dim;
     const void* src = delta ? sum : x;
     float s[1] = {0.0f};
-    for (int e = threadIdx.x; e < dim; e += 1024) {
+    for (int e = threadIdx.x; e < dim; e += NT) {
         float v = load_act<DT>(x, base + e);
         if (delta) {  // each thread reads again only what it stored itself
             v = round_act<DT>(v + load_act<DT>(delta, base + e));
@@ -133,20 +162,20 @@ __global__ __launch_bounds__(1024) void layernorm_long_kernel(
         }
         s[0] += v;
     }
-    row_sums<1024, 1>(s, lds, 0);
+    row_sums<NT, 1, NT>(s, lds, 0);
     const float mean = s[0] / static_cast<float>(dim);
     s[0] = 0.0f;
-    for (int e = threadIdx.x; e < dim; e += 1024) {
+    for (int e = threadIdx.x; e < dim; e += NT) {
         const float d = load_act<DT>(src, base + e) - mean;
         s[0] = __fmaf_rn(d, d, s[0]);
     }
-    row_sums<1024, 1>(s, lds, 1);
+    row_sums<NT, 1, NT>(s, lds, 1);
     const float rstd = 1.0f / sqrtf(s[0] / static_cast<float>(dim) + eps);
     if (threadIdx.x == 0 && mean_out) {
         mean_out[blockIdx.x] = mean;
         rstd_out[blockIdx.x] = rstd;
     }
-    for (int e = threadIdx.x; e < dim; e += 1024) {
+    for (int e = threadIdx.x; e < dim; e += NT) {
         float v = (load_act<DT>(src, base + e) - mean) * rstd;
         if (weight) v = __fmaf_rn(v, weight[e], bias ? bias[e] : 0.0f);
         else if (bias) v += bias[e];
@@ -154,71 +183,90 @@ __global__ __launch_bounds__(1024) void layernorm_long_kernel(
     }
 }
 
+// Threads of a workgroup of the gradients (a longer row takes 1024): eight waves share one row of partial
+// sums.  16384 x 2048 bf16 with a residual: 8 elements a thread in 128 registers 49 us, 16 elements 54 - 58
+// (they spill), workgroups of 256 51.
+constexpr int kLnBwdThreads = 512;
+
+template <int TPR> constexpr int ln_bwd_threads() { return TPR > kLnBwdThreads ? TPR : kLnBwdThreads; }
+
 // dx of a row per TPR threads, the rows in turn over the grid; each thread keeps its columns' sums of
 // dy n and dy, which the workgroup adds in group order and leaves in part[0 / 1][workgroup][dim].
 template <int DT, int GDT, int TPR, int CH>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layernorm_bwd_kernel(
+__global__ __launch_bounds__((ln_bwd_threads<TPR>()), 4) void layernorm_bwd_kernel(
     const void* __restrict__ dy, const void* __restrict__ x, const float* __restrict__ mean,
     const float* __restrict__ rstd, const float* __restrict__ weight, const void* dres, int rows,
     int dim, void* dx, float* __restrict__ part) {
-    constexpr int NT = TPR > 256 ? TPR : 256, GROUPS = NT / TPR;
+    constexpr int NT = ln_bwd_threads<TPR>(), GROUPS = NT / TPR;
     constexpr bool SHARE = GROUPS > 1;  // several rows a workgroup: their sums meet in LDS
     __shared__ float lds[2 * 2 * (NT / 64)];
     __shared__ float s_cols[SHARE ? 2 * TPR * 8 * CH : 1];
-    const int l = threadIdx.x % TPR, group = threadIdx.x / TPR;
-    float w[CH][8], aw[CH][8], ab[CH][8];
-    int n[CH];
+    const int l = threadIdx.x % TPR, group = row_group<TPR>();
+    const Elements<TPR, CH> el(l, dim);
+    float aw[CH][8], ab[CH][8];
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) aw[c][j] = ab[c][j] = 0.0f;
+    const float inv_dim = 1.0f / static_cast<float>(dim);
+    float w[CH][8];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        n[c] = max(0, min(8, dim - (c * TPR + l) * 8));
-        if (weight) load8_part<NSOSX_F32>(weight, (c * TPR + l) * 8, n[c], w[c]);
+        if (weight) load8_any<NSOSX_F32>(weight, el.at[c], w[c]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (!weight) w[c][j] = 1.0f;
-            aw[c][j] = ab[c][j] = 0.0f;
-        }
+        for (int j = 0; j < 8; ++j) w[c][j] = weight ? w[c][j] : 1.0f;
     }
-    const float inv_dim = 1.0f / static_cast<float>(dim);
     int turn = 0;
-    for (int64_t r0 = (int64_t)blockIdx.x * GROUPS; r0 < rows; r0 += (int64_t)gridDim.x * GROUPS) {
-        const int64_t row = r0 + group;
-        const bool real = row < rows;
+    auto pass = [&](int64_t row, bool real) {
         const int64_t base = row * dim;
-        float v[CH][8], g[CH][8];
+        Raw8<DT> xr[CH], dr[CH];
+        Raw8<GDT> gr[CH];
+        float mu = mean[row], q = rstd[row];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            load8_part<DT>(x, base + (c * TPR + l) * 8, real ? n[c] : 0, v[c]);
-            load8_part<GDT>(dy, base + (c * TPR + l) * 8, real ? n[c] : 0, g[c]);
+            xr[c].load(x, base + el.at[c]);
+            gr[c].load(dy, base + el.at[c]);
         }
-        const float mu = real ? mean[row] : 0.0f, q = real ? rstd[row] : 0.0f;
+        if (dres) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) dr[c].load(dres, base + el.at[c]);
+        }
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                v[c][j] = c < CH - 1 || j < n[c] ? (v[c][j] - mu) * q : 0.0f;
-                aw[c][j] = __fmaf_rn(g[c][j], v[c][j], aw[c][j]);
-                ab[c][j] += g[c][j];
-                g[c][j] *= w[c][j];
-                s[0] += g[c][j];
-                s[1] = __fmaf_rn(g[c][j], v[c][j], s[1]);
+                const float v = (xr[c].get(j) - mu) * q, d = real ? gr[c].get(j) : 0.0f;
+                aw[c][j] = __fmaf_rn(d, v, aw[c][j]);
+                ab[c][j] += d;
+                const float m = el.mine(c, j) ? d * w[c][j] : 0.0f;
+                s[0] += m;
+                s[1] = __fmaf_rn(m, v, s[1]);
             }
-        row_sums<TPR, 2>(s, lds, turn++);
+        if (dres && TPR > 64) {
+            // dx may be dres, and a row's last two threads share elements across waves: read before any is
+            // written
+#pragma unroll
+            for (int c = 0; c < CH; ++c) dr[c].wait();
+        }
+        row_sums<TPR, 2, NT>(s, lds, turn++);
+        if (!real) return;
         const float m1 = s[0] * inv_dim, m2 = s[1] * inv_dim;
-        if (!real) continue;
+        asm volatile("" : "+v"(mu), "+v"(q));  // (both are formed again, not kept in registers)
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
+            float o[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) g[c][j] = q * (g[c][j] - m1 - v[c][j] * m2);
-            if (dres) {
-                float d[8];
-                load8_part<DT>(dres, base + (c * TPR + l) * 8, n[c], d);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) g[c][j] += d[j];
+            for (int j = 0; j < 8; ++j) {
+                o[j] = q * (gr[c].get(j) * w[c][j] - m1 - (xr[c].get(j) - mu) * q * m2);
+                if (dres) o[j] += dr[c].get(j);
             }
-            store8_part<DT>(dx, base + (c * TPR + l) * 8, n[c], g[c]);
+            if (el.any(c)) store8_any<DT>(dx, base + el.at[c], o);
         }
-    }
+    };
+    int64_t r0 = (int64_t)blockIdx.x * GROUPS;
+    for (; r0 + GROUPS <= rows; r0 += (int64_t)gridDim.x * GROUPS) pass(r0 + group, true);
+    if (r0 < rows) pass(min(r0 + group, (int64_t)rows - 1), r0 + group < rows);
     if (!part) return;
     float* pw = part + (int64_t)blockIdx.x * dim;
     float* pb = pw + (int64_t)gridDim.x * dim;
@@ -231,7 +279,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layernorm_bwd_kernel(
                 for (int c = 0; c < CH; ++c)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const int e = (c * TPR + l) * 8 + j;
+                        // (element j of lane l at j * TPR + l: a wave's lanes on banks of their own; what
+                        // the tail's threads hold twice is the same sums)
+                        const int e = (c * 8 + j) * TPR + l;
                         sw[e] = k ? sw[e] + aw[c][j] : aw[c][j];
                         sb[e] = k ? sb[e] + ab[c][j] : ab[c][j];
                     }
@@ -239,38 +289,43 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layernorm_bwd_kernel(
             __syncthreads();
         }
         for (int e = threadIdx.x; e < dim; e += NT) {
-            pw[e] = sw[e];
-            pb[e] = sb[e];
+            // the last piece's tail lies with the thread whose elements end the row
+            int p = e / 8, j = e % 8;
+            if (p * 8 > dim - 8) j = e - (dim - 8);
+            const int at = (p / TPR * 8 + j) * TPR + p % TPR;
+            pw[e] = sw[at];
+            pb[e] = sb[at];
         }
     } else {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            store8_part<NSOSX_F32>(pw, (c * TPR + l) * 8, n[c], aw[c]);
-            store8_part<NSOSX_F32>(pb, (c * TPR + l) * 8, n[c], ab[c]);
-        }
+        for (int c = 0; c < CH; ++c)
+            if (el.any(c)) {
+                store8_any<NSOSX_F32>(pw, el.at[c], aw[c]);
+                store8_any<NSOSX_F32>(pb, el.at[c], ab[c]);
+            }
     }
 }
 
-// Rows past kLnRegDim: dx with a workgroup per row, in two readings of it.
-template <int DT, int GDT>
-__global__ __launch_bounds__(1024) void layernorm_bwd_long_kernel(
+// Rows past kLnRegDim (and below 8): dx with a workgroup per row, in two readings of it.
+template <int DT, int GDT, int NT>
+__global__ __launch_bounds__(NT) void layernorm_bwd_long_kernel(
     const void* __restrict__ dy, const void* __restrict__ x, const float* __restrict__ mean,
     const float* __restrict__ rstd, const float* __restrict__ weight, const void* dres, int dim,
     void* dx) {
-    __shared__ float lds[2 * 2 * 16];
+    __shared__ float lds[2 * 2 * (NT / 64)];
     const int64_t base = (int64_t)blockIdx.x * dim;
     const float mu = mean[blockIdx.x], q = rstd[blockIdx.x];
     float s[2] = {0.0f, 0.0f};
-    for (int e = threadIdx.x; e < dim; e += 1024) {
+    for (int e = threadIdx.x; e < dim; e += NT) {
         const float n = (load_act<DT>(x, base + e) - mu) * q;
         const float g = load_act<GDT>(dy, base + e) * (weight ? weight[e] : 1.0f);
         s[0] += g;
         s[1] = __fmaf_rn(g, n, s[1]);
     }
-    row_sums<1024, 2>(s, lds, 0);
+    row_sums<NT, 2, NT>(s, lds, 0);
     const float inv_dim = 1.0f / static_cast<float>(dim);
     const float m1 = s[0] * inv_dim, m2 = s[1] * inv_dim;
-    for (int e = threadIdx.x; e < dim; e += 1024) {
+    for (int e = threadIdx.x; e < dim; e += NT) {
         const float n = (load_act<DT>(x, base + e) - mu) * q;
         const float g = load_act<GDT>(dy, base + e) * (weight ? weight[e] : 1.0f);
         float d = q * (g - m1 - n * m2);
@@ -296,21 +351,24 @@ __global__ __launch_bounds__(256) void layernorm_cols_kernel(
     part[((int64_t)gridDim.y + blockIdx.y) * dim + e] = ab;
 }
 
-// 64 columns a workgroup; its 16 waves take every 16th partial row each, and meet in wave order.
+// 16 columns a workgroup (64 B of a row), a row of partial sums per 16 lanes: enough workgroups for
+// every load to be on its way at once.  Each thread adds its rows in order, the threads as a tree.
 __global__ __launch_bounds__(1024) void column_sums_kernel(const float* __restrict__ part, int n,
                                                            int cols, float* out0, float* out1) {
     float* out = blockIdx.y ? out1 : out0;
     if (!out) return;
-    __shared__ float s[16][64];
+    __shared__ float s[16][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
-    const float* p = part + (int64_t)blockIdx.y * n * cols;
+    const int64_t c = (int64_t)blockIdx.x * 16 + (lane & 15);
+    const float* p = part + (int64_t)blockIdx.y * n * cols + min(c, (int64_t)cols - 1);
     float sum = 0.0f;
-    if (c < cols)
-        for (int r = wave; r < n; r += 16) sum += p[(int64_t)r * cols + c];
-    s[wave][lane] = sum;
+#pragma unroll 8
+    for (int r = threadIdx.x >> 4; r < n; r += 64) sum += p[(int64_t)r * cols];
+    sum += lane_xor<16>(sum);
+    sum += lane_xor<32>(sum);
+    if (lane < 16) s[wave][lane] = sum;
     __syncthreads();
-    if (wave == 0 && c < cols) {
+    if (threadIdx.x < 16 && c < cols) {
         for (int w = 1; w < 16; ++w) sum += s[w][lane];
         out[c] = sum;
     }
@@ -318,7 +376,7 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const float* __restri
 
 void launch_column_sums(const float* part, int arrays, int n, int cols, float* out0, float* out1,
                         hipStream_t st) {
-    hipLaunchKernelGGL(column_sums_kernel, dim3((cols + 63) / 64, arrays), dim3(1024), 0, st, part,
+    hipLaunchKernelGGL(column_sums_kernel, dim3((cols + 15) / 16, arrays), dim3(1024), 0, st, part,
                        n, cols, out0, out1);
 }
 
@@ -333,6 +391,27 @@ static LnShape ln_shape(int dim) {
     if (dim <= 8192) return {256, (dim + 2047) / 2048};
     return {1024, 2};
 }
+
+// ... of the gradients, whose threads hold three rows' pieces and two sums of them: 8 elements each
+// (16 past 8192, where a workgroup takes a row)
+static LnShape ln_bwd_shape(int dim) {
+    int tpr = 8;
+    while (tpr < 1024 && tpr * 8 < dim) tpr *= 2;
+    return {tpr, tpr * 8 < dim ? 2 : 1};
+}
+
+#define NSOSX_LN_BWD_SHAPES(GO)                                                                 \
+    switch (sh.tpr * sh.ch) {                                                                   \
+        case 8: GO(8, 1); break;                                                                \
+        case 16: GO(16, 1); break;                                                              \
+        case 32: GO(32, 1); break;                                                              \
+        case 64: GO(64, 1); break;                                                              \
+        case 128: GO(128, 1); break;                                                            \
+        case 256: GO(256, 1); break;                                                            \
+        case 512: GO(512, 1); break;                                                            \
+        case 1024: GO(1024, 1); break;                                                          \
+        default: GO(1024, 2); break;                                                            \
+    }
 
 #define NSOSX_LN_SHAPES(GO)                                                                     \
     switch (sh.tpr * 8 + sh.ch) {                                                               \
@@ -351,25 +430,30 @@ static LnShape ln_shape(int dim) {
 
 // threads of the pass that gives a row to TPR threads (all but the gradients' short rows)
 static int64_t ln_threads(int rows, int dim) {
-    return (int64_t)rows * (dim > kLnRegDim ? 1024 : ln_shape(dim).tpr) + 1024;
+    return (int64_t)rows * (dim > kLnRegDim ? 1024 : dim < 8 ? 64 : ln_shape(dim).tpr) + 1024;
 }
 
-constexpr int kLnWorkgroups = 512;  // of the backward pass at most: each leaves a row of partial sums
+constexpr int kLnWorkgroups = 512;  // of the gradients at most: each leaves a row of partial sums
 
 static int ln_bwd_workgroups(int rows, int dim) {
-    if (dim > kLnRegDim) return rows < 64 ? rows : 64;
-    const int tpr = ln_shape(dim).tpr, groups = tpr > 256 ? 1 : 256 / tpr;
+    if (dim > kLnRegDim || dim < 8) return rows < 64 ? rows : 64;
+    const int tpr = ln_bwd_shape(dim).tpr, groups = tpr > kLnBwdThreads ? 1 : kLnBwdThreads / tpr;
     const int need = (rows + groups - 1) / groups;
-    return need < kLnWorkgroups ? need : kLnWorkgroups;
+    const int most = tpr > kLnBwdThreads ? kLnWorkgroups / 2 : kLnWorkgroups;  // (one a CU, else two)
+    return need < most ? need : most;
 }
 
 template <int DT, int ODT>
 static void launch_layernorm(const void* x, const void* delta, const float* weight,
                              const float* bias, int rows, int dim, float eps, void* sum, void* y,
                              float* mean, float* rstd, hipStream_t st) {
-    if (dim > kLnRegDim) {
-        hipLaunchKernelGGL((layernorm_long_kernel<DT, ODT>), dim3(rows), dim3(1024), 0, st, x, delta,
-                           weight, bias, dim, eps, sum, y, mean, rstd);
+    if (dim > kLnRegDim || dim < 8) {
+#define NSOSX_LN(NT)                                                                                      \
+    hipLaunchKernelGGL((layernorm_long_kernel<DT, ODT, NT>), dim3(rows), dim3(NT), 0, st, x, delta, weight, \
+                       bias, dim, eps, sum, y, mean, rstd)
+        if (dim < 8) NSOSX_LN(64);
+        else NSOSX_LN(1024);
+#undef NSOSX_LN
         return;
     }
     const LnShape sh = ln_shape(dim);
@@ -387,20 +471,24 @@ static void launch_layernorm_bwd(const void* dy, const void* x, const float* mea
                                  const float* weight, const void* dres, int rows, int dim, void* dx,
                                  float* part, hipStream_t st) {
     const int wgs = ln_bwd_workgroups(rows, dim);
-    if (dim > kLnRegDim) {
-        hipLaunchKernelGGL((layernorm_bwd_long_kernel<DT, GDT>), dim3(rows), dim3(1024), 0, st, dy, x,
-                           mean, rstd, weight, dres, dim, dx);
+    if (dim > kLnRegDim || dim < 8) {
+#define NSOSX_LN(NT)                                                                                       \
+    hipLaunchKernelGGL((layernorm_bwd_long_kernel<DT, GDT, NT>), dim3(rows), dim3(NT), 0, st, dy, x, mean, \
+                       rstd, weight, dres, dim, dx)
+        if (dim < 8) NSOSX_LN(64);
+        else NSOSX_LN(1024);
+#undef NSOSX_LN
         if (part)
             hipLaunchKernelGGL((layernorm_cols_kernel<DT, GDT>), dim3((dim - 1) / 256 + 1, wgs),
                                dim3(256), 0, st, dy, x, mean, rstd, rows, dim, part);
         return;
     }
-    const LnShape sh = ln_shape(dim);
-    const dim3 grid(wgs), block(sh.tpr > 256 ? sh.tpr : 256);
+    const LnShape sh = ln_bwd_shape(dim);
+    const dim3 grid(wgs), block(sh.tpr > kLnBwdThreads ? sh.tpr : kLnBwdThreads);
 #define NSOSX_LN(T, C)                                                                             \
     hipLaunchKernelGGL((layernorm_bwd_kernel<DT, GDT, T, C>), grid, block, 0, st, dy, x, mean, rstd, \
                        weight, dres, rows, dim, dx, part)
-    NSOSX_LN_SHAPES(NSOSX_LN)
+    NSOSX_LN_BWD_SHAPES(NSOSX_LN)
 #undef NSOSX_LN
 }
 

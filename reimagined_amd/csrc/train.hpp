@@ -44,30 +44,34 @@ __device__ __forceinline__ void store8_any(void* p, int64_t i, const float (&v)[
     }
 }
 
-// The first n (0 .. 8) of eight elements; the rest read as zeros and are not written.
-template <int DT>
-__device__ __forceinline__ void load8_part(const void* p, int64_t i, int n, float (&v)[8]) {
-    if (n >= 8) {
-        load8_any<DT>(p, i, v);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < n ? load_act<DT>(p, i + j) : 0.0f;
+// Eight elements as loaded: what is asked for early is kept in this form, half the registers for bf16,
+// and costs no wait before it is used.
+template <int DT> struct Raw8;
+template <> struct Raw8<NSOSX_BF16> {
+    bf16x8_any w;
+    __device__ __forceinline__ void load(const void* p, int64_t i) {
+        w = *reinterpret_cast<const bf16x8_any*>(static_cast<const uint16_t*>(p) + i);
     }
-}
-
-template <int DT>
-__device__ __forceinline__ void store8_part(void* p, int64_t i, int n, const float (&v)[8]) {
-    if (n >= 8) {
-        store8_any<DT>(p, i, v);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < n) store_act<DT>(p, i + j, v[j]);
+    __device__ __forceinline__ float get(int j) const {
+        return __uint_as_float(j & 1 ? w.w[j / 2] & 0xffff0000u : w.w[j / 2] << 16);
     }
-}
+    __device__ __forceinline__ void wait() {  // (a use: the load is back behind it)
+        asm volatile("" : "+v"(w.w[0]), "+v"(w.w[1]), "+v"(w.w[2]), "+v"(w.w[3])::"memory");
+    }
+};
+template <> struct Raw8<NSOSX_F32> {
+    f32x8_any v;
+    __device__ __forceinline__ void load(const void* p, int64_t i) {
+        v = *reinterpret_cast<const f32x8_any*>(static_cast<const float*>(p) + i);
+    }
+    __device__ __forceinline__ float get(int j) const { return v.v[j]; }
+    __device__ __forceinline__ void wait() {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(v.v[j])::"memory");
+    }
+};
 
-// out[a][c] = scale[c] * sum_n part[a][n][c] for a < arrays (out NULL entries are skipped), in a
-// fixed order; scale NULL: 1.
+// out_a[c] = sum_n part[a][n][c] for a < arrays (1 or 2; a NULL out is skipped), in a fixed order.
 void launch_column_sums(const float* part, int arrays, int n, int cols, float* out0, float* out1,
                         hipStream_t st);
 
