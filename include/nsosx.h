@@ -615,7 +615,8 @@ int nsosx_moe_route_scored_backward(const void* logits, int logits_dtype, int64_
  * 0 for padding; cu_seqlens int32 [S + 1], not decreasing, or NULL with S = 1 for the whole batch
  * as one; rows of no sequence count as padding.  loss f32 [1] (0 without a valid row); counts int32
  * and mean_prob f32 [S, E], tokens int32 [S] (N_s), zeros for a sequence without valid rows.
- * E <= 512, k <= 16.  The same inputs give the same bits. */
+ * E <= 512, k <= 16, S <= 65535.  The same inputs give the same bits.  workspace: device, 8-byte
+ * aligned, nsosx_moe_balance_loss_workspace bytes. */
 int64_t nsosx_moe_balance_loss_workspace(int rows, int experts, int S);
 int nsosx_moe_balance_loss(const void* logits, int logits_dtype, int64_t logits_stride,
                            const int32_t* selected, const uint8_t* valid_rows, int rows,

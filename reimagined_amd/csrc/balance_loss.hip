@@ -3,14 +3,19 @@
 // s, M the sequences that have any, and count_se the choices of expert e in s:
 //   loss = 1/M sum_s E sum_e (count_se / (k N_s)) (sum_r p_re / N_s)
 //   dloss/dx_rj = E / (M k N_s^2) p_rj (count_sj - sum_e count_se p_re)  [(1 - sigmoid) for sigmoids]
-// Sixteen lanes per row, as in the scored routing: the row's sums are four lane exchanges, the
-// columns' sums stay in registers over a block of rows.
+// Sixteen lanes per row, as in the scored routing, four neighbouring columns a load: the row's sums are
+// four lane exchanges, and one read of the logits is all either pass does.  Both are bound by latency up
+// to some ten thousand rows: 16384 x 256 f32 sigmoids, k 8, take 7 us for the blocks' sums, 8 to add
+// them up (a chain of loads, barriers and one atomic) and 9 back (17 MB read and written: 3.8 TB/s).
+// With a scalar load a column they took 13, 14 and 15, with one workgroup a sequence to add them up 14.
 #include "train.hpp"
 
 namespace nsosx {
 
-constexpr int kBalRows = 128;   // of a block of the forward pass
+constexpr int kBalRows = 64;  // of a block of the forward pass: all of them in flight at once
 constexpr int kBalMaxE = 512, kBalMaxK = 16;
+constexpr int kBalCols = 16;  // columns of a workgroup that adds the blocks' sums
+constexpr float kLog2e = 1.44269504088896340736f;
 
 struct Balance {
     const void* logits;
@@ -36,47 +41,119 @@ __device__ __forceinline__ float max16(float v) {
     return fmaxf(v, lane_xor<1>(v));
 }
 
-// The row's normalised scores, columns i * 16 + l; `rest`, for sigmoids, their 1 - sigmoid.
-template <int DT, int NC, bool SIG, bool REST>
-__device__ __forceinline__ void row_probs(const void* logits, int64_t base, int E, int l, float (&p)[NC],
-                                          float (&rest)[NC]) {
-    float mx = -INFINITY, sum = 0.0f;
+// V neighbouring columns, at any alignment.
+template <int DT, int V> struct Cols;
+template <> struct Cols<NSOSX_F32, 4> { struct __attribute__((packed, aligned(4))) T { float v[4]; }; };
+template <> struct Cols<NSOSX_BF16, 4> { struct __attribute__((packed, aligned(2))) T { uint32_t v[2]; }; };
+
+template <int DT, int V>
+__device__ __forceinline__ void load_cols(const void* p, int64_t i, float (&f)[V]) {
+    if constexpr (V == 1) {
+        f[0] = load_act<DT>(p, i);
+    } else if constexpr (DT == NSOSX_F32) {
+        const auto t = *reinterpret_cast<const typename Cols<DT, V>::T*>(static_cast<const float*>(p) + i);
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        const int c = i * 16 + l;
-        p[i] = c < E ? load_act<DT>(logits, base + c) : -INFINITY;
+        for (int v = 0; v < V; ++v) f[v] = t.v[v];
+    } else {
+        const auto t = *reinterpret_cast<const typename Cols<DT, V>::T*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            f[v] = __uint_as_float(v & 1 ? t.v[v / 2] & 0xffff0000u : t.v[v / 2] << 16);
     }
+}
+
+template <int DT, int V>
+__device__ __forceinline__ void store_cols(void* p, int64_t i, const float (&f)[V]) {
+    if constexpr (V == 1) {
+        store_act<DT>(p, i, f[0]);
+    } else {
+        typename Cols<DT, V>::T t;
+        if constexpr (DT == NSOSX_F32) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) t.v[v] = f[v];
+            *reinterpret_cast<typename Cols<DT, V>::T*>(static_cast<float*>(p) + i) = t;
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; v += 2) t.v[v / 2] = pack_bf16x2(f[v], f[v + 1]);
+            *reinterpret_cast<typename Cols<DT, V>::T*>(static_cast<uint16_t*>(p) + i) = t;
+        }
+    }
+}
+
+// A lane's columns: NV times V of them, at[i] the first.  Those that would pass the row's end are its last
+// V instead; the first skip[i] of them are another lane's and stay out of the row's sums.  (V is 1 below
+// four experts.)
+template <int NV, int V>
+struct Lane {
+    int at[NV], skip[NV];
+    __device__ __forceinline__ Lane(int l, int E) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * 16 + l) * V;
+            at[i] = min(c, E - V);
+            skip[i] = min(c - at[i], V);
+        }
+    }
+};
+
+template <int DT, int NV, int V>
+__device__ __forceinline__ void load_row(const void* logits, int64_t base, const Lane<NV, V>& ln, float (&x)[NV][V]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load_cols<DT, V>(logits, base + ln.at[i], x[i]);
+}
+
+// The row's normalised scores in place of its logits, and for sigmoids with REST their 1 - sigmoid; the
+// exponential and reciprocal units, whose results are off by a few half steps.
+template <int NV, int V, bool SIG, bool REST>
+__device__ __forceinline__ void row_probs(const Lane<NV, V>& ln, float (&p)[NV][V], float (&rest)[NV][V]) {
+    float mx = -INFINITY, sum = 0.0f;
     if constexpr (!SIG) {
 #pragma unroll
-        for (int i = 0; i < NC; ++i) mx = fmaxf(mx, p[i]);
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int v = 0; v < V; ++v) mx = fmaxf(mx, p[i][v]);
         mx = max16(mx);
     }
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        if constexpr (SIG) {
-            const float e = expf(-fabsf(p[i])), big = 1.0f / (1.0f + e), small = e * big;
-            if constexpr (REST) rest[i] = p[i] < 0.0f ? big : small;
-            p[i] = p[i] < 0.0f ? small : big;
-        } else {
-            p[i] = i * 16 + l < E ? expf(p[i] - mx) : 0.0f;
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if constexpr (SIG) {
+                const float e = __builtin_amdgcn_exp2f(fabsf(p[i][v]) * -kLog2e);
+                const float big = __builtin_amdgcn_rcpf(1.0f + e), small = e * big;
+                if constexpr (REST) rest[i][v] = p[i][v] < 0.0f ? big : small;
+                p[i][v] = p[i][v] < 0.0f ? small : big;
+            } else {
+                p[i][v] = __builtin_amdgcn_exp2f((p[i][v] - mx) * kLog2e);
+            }
+            sum += v >= ln.skip[i] ? p[i][v] : 0.0f;
         }
-        sum += p[i];
-    }
     const float inv = 1.0f / sum16(sum);
 #pragma unroll
-    for (int i = 0; i < NC; ++i) p[i] *= inv;
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int v = 0; v < V; ++v) p[i][v] *= inv;
 }
 
-// One block of rows: for each sequence in it, the sums of p and the counts, left in slot block +
-// sequence (no two pairs share one: along the rows each step raises one of them or both).
-template <int DT, int NC, bool SIG>
+// One block of rows, a row per sixteen lanes: for each sequence in it, the sums of p and the counts, left
+// in slot block + sequence (no two pairs share one: along the rows each step raises one of them or both).
+template <int DT, int NV, int V, bool SIG>
 __global__ __launch_bounds__(1024) void balance_sums_kernel(Balance P, float* __restrict__ part,
                                                             int32_t* __restrict__ counts,
-                                                            int32_t* __restrict__ tokens) {
-    __shared__ float s_sum[16][NC * 16];
-    __shared__ int32_t s_count[NC * 16], s_tokens, s_first, s_last;
+                                                            int32_t* __restrict__ tokens,
+                                                            uint32_t* __restrict__ arrived) {
+    __shared__ float s_sum[16][NV * 16 * V];
+    __shared__ int32_t s_count[NV * 16 * V], s_tokens, s_first, s_last;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = threadIdx.x & 15;
     const int64_t r0 = (int64_t)blockIdx.x * kBalRows, r1 = min(r0 + kBalRows, (int64_t)P.rows);
+    const Lane<NV, V> ln(l, P.E);
+    const int64_t r = r0 + (threadIdx.x >> 4), rr = min(r, r1 - 1);
+    const bool valid = r < r1 && (!P.valid || P.valid[rr]);
+    float p[NV][V], rest[NV][V];
+    load_row<DT, NV, V>(P.logits, rr * P.stride, ln, p);
+    const int chosen = valid && l < P.k ? P.selected[rr * P.k + l] : -1;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;  // of the next launch
+    row_probs<NV, V, SIG, false>(ln, p, rest);
     int first = 0, last = 0;
     if (P.cu) {
         if (threadIdx.x == 0) s_first = P.S, s_last = -1;
@@ -95,33 +172,23 @@ __global__ __launch_bounds__(1024) void balance_sums_kernel(Balance P, float* __
         for (int e = threadIdx.x; e < P.E; e += 1024) s_count[e] = 0;
         if (threadIdx.x == 0) s_tokens = 0;
         __syncthreads();
-        float acc[NC];
-        int mine = 0;
+        const bool in = valid && r >= lo && r < hi;
+        if (in && chosen >= 0 && chosen < P.E) atomicAdd(&s_count[chosen], 1);
+        if (in && l == 0) atomicAdd(&s_tokens, 1);
 #pragma unroll
-        for (int i = 0; i < NC; ++i) acc[i] = 0.0f;
-        for (int64_t r = lo + (threadIdx.x >> 4); r < hi; r += 64) {
-            if (P.valid && !P.valid[r]) continue;
-            float p[NC], rest[NC];
-            row_probs<DT, NC, SIG, false>(P.logits, r * P.stride, P.E, l, p, rest);
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int i = 0; i < NC; ++i) acc[i] += p[i];
-            if (l < P.k) {
-                const int e = P.selected[r * P.k + l];
-                if (e >= 0 && e < P.E) atomicAdd(&s_count[e], 1);
+            for (int v = 0; v < V; ++v) {
+                float sum = in ? p[i][v] : 0.0f;
+                sum += lane_xor<16>(sum);
+                sum += lane_xor<32>(sum);
+                if (lane < 16) s_sum[wave][ln.at[i] + v] = sum;  // (what two lanes hold is the same)
             }
-            ++mine;
-        }
-        if (l == 0 && mine) atomicAdd(&s_tokens, mine);
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            acc[i] += lane_xor<16>(acc[i]);
-            acc[i] += lane_xor<32>(acc[i]);
-            if (lane < 16) s_sum[wave][i * 16 + l] = acc[i];
-        }
         __syncthreads();
         const int64_t slot = (int64_t)blockIdx.x + s;
         for (int e = threadIdx.x; e < P.E; e += 1024) {
             float sum = s_sum[0][e];
+#pragma unroll
             for (int w = 1; w < 16; ++w) sum += s_sum[w][e];
             part[slot * P.E + e] = sum;
             counts[slot * P.E + e] = s_count[e];
@@ -131,91 +198,107 @@ __global__ __launch_bounds__(1024) void balance_sums_kernel(Balance P, float* __
     }
 }
 
-// A sequence: its blocks' sums in order.  512 threads a column pair of four runs of blocks.
-__global__ __launch_bounds__(1024) void balance_finish_kernel(Balance P, const float* __restrict__ part,
-                                                              const int32_t* __restrict__ pcounts,
-                                                              const int32_t* __restrict__ ptokens,
-                                                              int32_t* __restrict__ counts,
-                                                              int32_t* __restrict__ tokens,
-                                                              float* __restrict__ mean,
-                                                              float* __restrict__ seq_loss) {
-    __shared__ float s_sum[1024];
-    __shared__ int32_t s_count[1024], s_tokens;
-    __shared__ double s_loss[16];
-    const int s = blockIdx.x;
+// kBalCols columns of a sequence: its blocks' sums, sixteen runs of them side by side.  The workgroup that
+// arrives last adds the loss's parts in their order.
+__global__ __launch_bounds__(256) void balance_finish_kernel(Balance P, const float* __restrict__ part,
+                                                             const int32_t* __restrict__ pcounts,
+                                                             const int32_t* __restrict__ ptokens,
+                                                             int32_t* __restrict__ counts, int32_t* tokens,
+                                                             float* __restrict__ mean, double* loss_part,
+                                                             uint32_t* arrived, float* __restrict__ loss) {
+    __shared__ float s_sum[16][kBalCols];
+    __shared__ int32_t s_count[16][kBalCols], s_tokens, s_last;
+    __shared__ double s_loss[256];
+    __shared__ int32_t s_some[256];
+    const int s = blockIdx.y;
     const int64_t lo = P.cu ? max(0, P.cu[s]) : 0, hi = P.cu ? min(P.rows, P.cu[s + 1]) : P.rows;
     const int64_t b0 = lo / kBalRows, b1 = hi > lo ? (hi - 1) / kBalRows + 1 : b0;
-    const int cols = P.E <= 64 ? 64 : P.E <= 256 ? 256 : 512, runs = 1024 / cols;
-    const int e = threadIdx.x % cols, run = threadIdx.x / cols;
+    const int l = threadIdx.x % kBalCols, run = threadIdx.x / kBalCols, e = blockIdx.x * kBalCols + l;
     float sum = 0.0f;
-    int32_t count = 0;
+    int32_t count = 0, n = 0;
     if (threadIdx.x == 0) s_tokens = 0;
     __syncthreads();
-    if (e < P.E)
-        for (int64_t b = b0 + run; b < b1; b += runs) {
+    for (int64_t b = b0 + threadIdx.x; b < b1; b += 256) n += ptokens[b + s];
+    if (e < P.E) {
+#pragma unroll 4
+        for (int64_t b = b0 + run; b < b1; b += 16) {
             sum += part[(b + s) * P.E + e];
             count += pcounts[(b + s) * P.E + e];
         }
-    int32_t n = 0;
-    for (int64_t b = b0 + threadIdx.x; b < b1; b += 1024) n += ptokens[b + s];
+    }
     if (n) atomicAdd(&s_tokens, n);
-    s_sum[threadIdx.x] = sum;
-    s_count[threadIdx.x] = count;
+    s_sum[run][l] = sum;
+    s_count[run][l] = count;
     __syncthreads();
     const int32_t total = s_tokens;
-    double loss = 0.0;
-    if (run == 0 && e < P.E) {
-        for (int q = 1; q < runs; ++q) {
-            sum += s_sum[q * cols + e];
-            count += s_count[q * cols + e];
+    if (threadIdx.x < kBalCols) {
+        for (int q = 1; q < 16; ++q) {
+            sum += s_sum[q][l];
+            count += s_count[q][l];
         }
         const float avg = total ? sum / static_cast<float>(total) : 0.0f;
-        counts[(int64_t)s * P.E + e] = count;
-        mean[(int64_t)s * P.E + e] = avg;
-        loss = total ? (double)count * avg : 0.0;
+        double f = 0.0;
+        if (e < P.E) {
+            counts[(int64_t)s * P.E + e] = count;
+            mean[(int64_t)s * P.E + e] = avg;
+            f = total ? (double)count * avg * P.E / ((double)P.k * total) : 0.0;
+        }
+        for (int o = kBalCols / 2; o > 0; o >>= 1) f += __shfl_xor(f, o, kBalCols);
+        if (l == 0) {
+            const int64_t at = (int64_t)s * gridDim.x + blockIdx.x;
+            __hip_atomic_store(loss_part + at, f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (blockIdx.x == 0) __hip_atomic_store(tokens + s, total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const uint32_t before =
+                __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+            s_last = before == gridDim.x * gridDim.y - 1;
+        }
     }
-    for (int o = 32; o > 0; o >>= 1) loss += __shfl_xor(loss, o, 64);
-    if ((threadIdx.x & 63) == 0) s_loss[threadIdx.x >> 6] = loss;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) loss += s_loss[w];
-        tokens[s] = total;
-        seq_loss[s] = total ? (float)(loss * P.E / ((double)P.k * total)) : 0.0f;
-    }
-}
-
-// The mean over the sequences with a valid row.
-__global__ __launch_bounds__(256) void balance_mean_kernel(const float* __restrict__ seq_loss,
-                                                           const int32_t* __restrict__ tokens, int S,
-                                                           float* __restrict__ loss) {
-    __shared__ double s_sum[256];
-    __shared__ int32_t s_some[256];
-    double sum = 0.0;
+    if (!s_last) return;
+    double f = 0.0;
     int32_t some = 0;
-    for (int s = threadIdx.x; s < S; s += 256) {
-        sum += seq_loss[s];
-        some += tokens[s] > 0;
-    }
-    s_sum[threadIdx.x] = sum;
+    const int64_t parts = (int64_t)gridDim.x * gridDim.y;
+    for (int64_t i = threadIdx.x; i < parts; i += 256)
+        f += __hip_atomic_load(loss_part + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int i = threadIdx.x; i < P.S; i += 256)
+        some += __hip_atomic_load(tokens + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) > 0;
+    s_loss[threadIdx.x] = f;
     s_some[threadIdx.x] = some;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < 256; ++i) {
-            sum += s_sum[i];
-            some += s_some[i];
+    for (int o = 128; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) {
+            s_loss[threadIdx.x] += s_loss[threadIdx.x + o];
+            s_some[threadIdx.x] += s_some[threadIdx.x + o];
         }
-        *loss = some ? (float)(sum / some) : 0.0f;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *loss = s_some[0] ? (float)(s_loss[0] / s_some[0]) : 0.0f;
+}
+
+// Nothing to add up: no row, or no sequence.
+__global__ __launch_bounds__(256) void balance_none_kernel(int S, int E, float* loss, int32_t* counts,
+                                                           int32_t* tokens, float* mean) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i == 0) *loss = 0.0f;
+    if (i < S) tokens[i] = 0;
+    if (i < (int64_t)S * E) {
+        counts[i] = 0;
+        mean[i] = 0.0f;
     }
 }
 
-template <int DT, int NC, bool SIG>
+template <int DT, int NV, int V, bool SIG>
 __global__ __launch_bounds__(256) void balance_bwd_kernel(Balance P, const int32_t* __restrict__ counts,
                                                           const int32_t* __restrict__ tokens, float scale,
                                                           const float* __restrict__ dloss, const void* add,
                                                           void* dlogits) {
     __shared__ int32_t s_seq[16], s_some;
     const int l = threadIdx.x & 15, group = threadIdx.x >> 4;
-    const int64_t r0 = (int64_t)blockIdx.x * 16;
+    const int64_t r0 = (int64_t)blockIdx.x * 16, r = r0 + group, rr = min(r, (int64_t)P.rows - 1);
+    const Lane<NV, V> ln(l, P.E);
+    float p[NV][V], rest[NV][V], a[NV][V];
+    load_row<DT, NV, V>(P.logits, rr * P.stride, ln, p);
+    if (add) load_row<DT, NV, V>(add, rr * P.E, ln, a);
     if (threadIdx.x < 16) s_seq[threadIdx.x] = P.cu ? -1 : 0;
     if (threadIdx.x == 0) s_some = 0;
     __syncthreads();
@@ -224,64 +307,71 @@ __global__ __launch_bounds__(256) void balance_bwd_kernel(Balance P, const int32
         some += tokens[s] > 0;
         if (P.cu) {
             const int64_t lo = max((int64_t)P.cu[s], r0), hi = min((int64_t)P.cu[s + 1], r0 + 16);
-            for (int64_t r = lo; r < hi; ++r) s_seq[r - r0] = s;
+            for (int64_t q = lo; q < hi; ++q) s_seq[q - r0] = s;
         }
     }
     if (some) atomicAdd(&s_some, some);
     __syncthreads();
-    const int64_t r = r0 + group;
     if (r >= P.rows) return;
     const int s = s_seq[group];
     const int n = s >= 0 ? tokens[s] : 0;
-    float g[NC];
-#pragma unroll
-    for (int i = 0; i < NC; ++i) g[i] = 0.0f;
+    float g[NV][V];
     if (n > 0 && !(P.valid && !P.valid[r])) {
-        float p[NC], rest[NC], dot = 0.0f;
-        row_probs<DT, NC, SIG, true>(P.logits, r * P.stride, P.E, l, p, rest);
+        float dot = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            g[i] = i * 16 + l < P.E ? static_cast<float>(counts[(int64_t)s * P.E + i * 16 + l]) : 0.0f;
-            dot = __fmaf_rn(g[i], p[i], dot);
-        }
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int v = 0; v < V; ++v) g[i][v] = static_cast<float>(counts[(int64_t)s * P.E + ln.at[i] + v]);
+        row_probs<NV, V, SIG, true>(ln, p, rest);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int v = 0; v < V; ++v) dot += v >= ln.skip[i] ? g[i][v] * p[i][v] : 0.0f;
         dot = sum16(dot);
         const float nf = static_cast<float>(n);
         const float f = scale * (dloss ? *dloss : 1.0f) * static_cast<float>(P.E) /
                         (static_cast<float>(P.k) * static_cast<float>(s_some) * nf) / nf;
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            g[i] = p[i] * (g[i] - dot) * f;
-            if constexpr (SIG) g[i] *= rest[i];
-        }
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                g[i][v] = p[i][v] * (g[i][v] - dot) * f;
+                if constexpr (SIG) g[i][v] *= rest[i][v];
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int v = 0; v < V; ++v) g[i][v] = 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        const int c = i * 16 + l;
-        if (c >= P.E) continue;
-        if (add) g[i] += load_act<DT>(add, r * P.E + c);
-        store_act<DT>(dlogits, r * P.E + c, g[i]);
+    for (int i = 0; i < NV; ++i) {
+        if (add) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) g[i][v] += a[i][v];
+        }
+        if (ln.skip[i] < V) store_cols<DT, V>(dlogits, r * P.E + ln.at[i], g[i]);
     }
 }
 
 static int64_t bal_blocks(int rows) { return ((int64_t)rows + kBalRows - 1) / kBalRows; }
 
-#define NSOSX_BAL_NC(GO, DT, SIG)                 \
+#define NSOSX_BAL_NV(GO, DT, SIG)                 \
     do {                                          \
-        if (p.E <= 16) GO(DT, 1, SIG);            \
-        else if (p.E <= 32) GO(DT, 2, SIG);       \
-        else if (p.E <= 64) GO(DT, 4, SIG);       \
-        else if (p.E <= 128) GO(DT, 8, SIG);      \
-        else if (p.E <= 256) GO(DT, 16, SIG);     \
-        else GO(DT, 32, SIG);                     \
+        if (p.E < 4) GO(DT, 1, 1, SIG);           \
+        else if (p.E <= 64) GO(DT, 1, 4, SIG);    \
+        else if (p.E <= 128) GO(DT, 2, 4, SIG);   \
+        else if (p.E <= 256) GO(DT, 4, 4, SIG);   \
+        else GO(DT, 8, 4, SIG);                   \
     } while (0)
 #define NSOSX_BAL(GO, dtype, sig)                                                    \
     do {                                                                             \
         if ((dtype) == NSOSX_F32) {                                                  \
-            if (sig) NSOSX_BAL_NC(GO, NSOSX_F32, true);                              \
-            else NSOSX_BAL_NC(GO, NSOSX_F32, false);                                 \
+            if (sig) NSOSX_BAL_NV(GO, NSOSX_F32, true);                              \
+            else NSOSX_BAL_NV(GO, NSOSX_F32, false);                                 \
         } else {                                                                     \
-            if (sig) NSOSX_BAL_NC(GO, NSOSX_BF16, true);                             \
-            else NSOSX_BAL_NC(GO, NSOSX_BF16, false);                                \
+            if (sig) NSOSX_BAL_NV(GO, NSOSX_BF16, true);                             \
+            else NSOSX_BAL_NV(GO, NSOSX_BF16, false);                                \
         }                                                                            \
     } while (0)
 
@@ -294,7 +384,7 @@ static int bal_check(const char* fn, const Balance& p, int dtype) {
         return fail(NSOSX_ERR_INVALID, name + ": need sequences >= 0, 1 without cu_seqlens");
     if (p.rows > 1 && p.stride < p.E)
         return fail(NSOSX_ERR_INVALID, name + ": the logits' row stride is less than E");
-    if ((int64_t)p.rows * 16 + 256 > 0xffffffffLL || p.S > 0xffffffffLL / 1024 - 1)
+    if ((int64_t)p.rows * 16 + 256 > 0xffffffffLL || p.S > 65535)
         return fail(NSOSX_ERR_OVERFLOW, name + ": rows or sequences too large");
     return NSOSX_OK;
 }
@@ -303,10 +393,12 @@ static int bal_check(const char* fn, const Balance& p, int dtype) {
 
 using namespace nsosx;
 
-// workspace: per slot (block + sequence) E sums, E counts and the rows, then the sequences' losses
+// workspace: the loss's parts (f64), the arrivals (16 bytes), per slot (block + sequence) E sums, E counts
+// and the rows
 extern "C" int64_t nsosx_moe_balance_loss_workspace(int rows, int experts, int S) {
     if (rows < 0 || experts <= 0 || S < 0) return 0;
-    return ((bal_blocks(rows) + S) * (2 * (int64_t)experts + 1) + S) * 4;
+    const int64_t parts = (int64_t)S * ((experts + kBalCols - 1) / kBalCols);
+    return parts * 8 + 16 + (bal_blocks(rows) + S) * (2 * (int64_t)experts + 1) * 4;
 }
 
 extern "C" int nsosx_moe_balance_loss(const void* logits, int logits_dtype, int64_t logits_stride,
@@ -319,22 +411,28 @@ extern "C" int nsosx_moe_balance_loss(const void* logits, int logits_dtype, int6
     if (!loss || (S > 0 && (!counts || !tokens || !mean_prob || !workspace)) ||
         (rows > 0 && (!logits || !selected)))
         return fail(NSOSX_ERR_INVALID, "moe_balance_loss: null pointer");
+    if (reinterpret_cast<uintptr_t>(workspace) & 7)
+        return fail(NSOSX_ERR_INVALID, "moe_balance_loss: workspace must be 8-byte aligned");
     hipStream_t st = static_cast<hipStream_t>(stream);
+    if (rows == 0 || S == 0) {
+        hipLaunchKernelGGL(balance_none_kernel, dim3((unsigned)(((int64_t)S * experts + 255) / 256 + 1)), dim3(256),
+                           0, st, S, experts, loss, counts, tokens, mean_prob);
+        return check_launch("moe_balance_loss");
+    }
     const int64_t blocks = bal_blocks(rows), slots = blocks + S;
-    float* part = static_cast<float*>(workspace);
+    const dim3 grid((experts + kBalCols - 1) / kBalCols, S);
+    double* loss_part = static_cast<double*>(workspace);
+    uint32_t* arrived = reinterpret_cast<uint32_t*>(loss_part + (int64_t)grid.x * S);
+    float* part = reinterpret_cast<float*>(arrived + 4);
     int32_t* pcounts = reinterpret_cast<int32_t*>(part + slots * experts);
     int32_t* ptokens = pcounts + slots * experts;
-    float* seq_loss = reinterpret_cast<float*>(ptokens + slots);
-#define NSOSX_BAL_GO(DT, NC, SIG)                                                                     \
-    hipLaunchKernelGGL((balance_sums_kernel<DT, NC, SIG>), dim3((unsigned)blocks), dim3(1024), 0, st, p, \
-                       part, pcounts, ptokens)
-    if (rows > 0 && S > 0) NSOSX_BAL(NSOSX_BAL_GO, logits_dtype, sigmoid);
+#define NSOSX_BAL_GO(DT, NV, V, SIG)                                                                     \
+    hipLaunchKernelGGL((balance_sums_kernel<DT, NV, V, SIG>), dim3((unsigned)blocks), dim3(1024), 0, st, p, \
+                       part, pcounts, ptokens, arrived)
+    NSOSX_BAL(NSOSX_BAL_GO, logits_dtype, sigmoid);
 #undef NSOSX_BAL_GO
-    if (S > 0)
-        hipLaunchKernelGGL(balance_finish_kernel, dim3(S), dim3(1024), 0, st, p, part, pcounts, ptokens,
-                           counts, tokens, mean_prob, S == 1 ? loss : seq_loss);
-    if (S != 1)
-        hipLaunchKernelGGL(balance_mean_kernel, dim3(1), dim3(256), 0, st, seq_loss, tokens, S, loss);
+    hipLaunchKernelGGL(balance_finish_kernel, grid, dim3(256), 0, st, p, part, pcounts, ptokens, counts, tokens,
+                       mean_prob, loss_part, arrived, loss);
     return check_launch("moe_balance_loss");
 }
 
@@ -356,8 +454,8 @@ extern "C" int nsosx_moe_balance_loss_backward(const void* logits, int logits_dt
         return fail(NSOSX_ERR_INVALID, "moe_balance_loss_backward: dlogits overlaps an input (it may be add)");
     hipStream_t st = static_cast<hipStream_t>(stream);
     const dim3 grid((unsigned)(((int64_t)rows + 15) / 16));
-#define NSOSX_BAL_GO(DT, NC, SIG)                                                                       \
-    hipLaunchKernelGGL((balance_bwd_kernel<DT, NC, SIG>), grid, dim3(256), 0, st, p, counts, tokens, scale, \
+#define NSOSX_BAL_GO(DT, NV, V, SIG)                                                                       \
+    hipLaunchKernelGGL((balance_bwd_kernel<DT, NV, V, SIG>), grid, dim3(256), 0, st, p, counts, tokens, scale, \
                        dloss, add, dlogits)
     NSOSX_BAL(NSOSX_BAL_GO, logits_dtype, sigmoid);
 #undef NSOSX_BAL_GO

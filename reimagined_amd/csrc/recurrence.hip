@@ -92,14 +92,6 @@ __device__ __forceinline__ float decay_rate(float lam, float rate) {
     return rate * (fmaxf(lam, 0.0f) + log1pf(expf(-fabsf(lam)))) * kLog2e;
 }
 
-// From here on the words are loaded ones to the compiler.  Where it would form what two branches (or two
-// phases) both need ahead of them, in registers that are not there, one of them forgets.
-template <typename P, int R>
-__device__ __forceinline__ void forget(P (&p)[R]) {
-#pragma unroll
-    for (int j = 0; j < R; ++j) p[j].forget();
-}
-
 // p = 1 - a^2 for a = 2^-q.  Where a is near 1 the difference would cancel: below t = -log(a^2) = 0.25
 // (q = kSmall) it is q times a fit of (1 - e^-t) / t in q (own least-squares fit, relative error 1e-7 with
 // its roundings); above, 1 - a^2 is exact to 7e-7.
@@ -758,20 +750,23 @@ __global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_b
     }
 }
 
-// dlam = sigmoid(lam) / softplus(lam) * sum_t e, e in units of log 2: the tiles' sums in a fixed order (64 channels a
-// workgroup, its 16 waves take every 16th tile).
+// dlam = sigmoid(lam) / softplus(lam) * sum_t e, e in units of log 2: the tiles' sums in a fixed order (16
+// channels a workgroup, 64 runs of tiles: a short chain of loads, as the sums are few).
 __global__ __launch_bounds__(1024) void recurrence_dlam_kernel(const float* __restrict__ part, int tiles,
                                                                int D, const float* __restrict__ lam,
                                                                float* __restrict__ dlam) {
-    __shared__ float s[16][64];
+    __shared__ float s[16][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    const int64_t c = (int64_t)blockIdx.x * 16 + (lane & 15);
+    const float* p = part + min(c, (int64_t)D - 1);
     float sum = 0.0f;
-    if (c < D)
-        for (int i = wave; i < tiles; i += 16) sum += part[(int64_t)i * D + c];
-    s[wave][lane] = sum;
+#pragma unroll 8
+    for (int i = threadIdx.x >> 4; i < tiles; i += 64) sum += p[(int64_t)i * D];
+    sum += lane_xor<16>(sum);
+    sum += lane_xor<32>(sum);
+    if (lane < 16) s[wave][lane] = sum;
     __syncthreads();
-    if (wave != 0 || c >= D) return;
+    if (threadIdx.x >= 16 || c >= D) return;
     for (int w = 1; w < 16; ++w) sum += s[w][lane];
     // sigmoid / softplus goes to 1 as both go to e^lam
     const float l = lam[c], en = expf(-fabsf(l));
@@ -908,7 +903,8 @@ extern "C" int nsosx_gated_recurrence_tile(void) { return kKept; }
 
 extern "C" int64_t nsosx_gated_recurrence_workspace(int T, int D) {
     if (T <= 0 || D <= 0) return 0;
-    return rec_shared_bytes(rec_tiles(T, kTile), D);
+    const int64_t bytes = rec_shared_bytes(rec_tiles(T, kTile), D);
+    return bytes < 16 ? 16 : bytes;
 }
 
 extern "C" int nsosx_gated_recurrence(const void* x, int64_t x_stride, const void* rg, int64_t rg_stride,
@@ -929,7 +925,7 @@ extern "C" int nsosx_gated_recurrence(const void* x, int64_t x_stride, const voi
         if (final_state) launch_empty(initial_state, sd, final_state, st);
         return check_launch("gated_recurrence");
     }
-    if (!x || !rg || !ig || !y || (!workspace && rec_tiles(T, kTile) > 1))
+    if (!x || !rg || !ig || !y || !workspace)
         return fail(NSOSX_ERR_INVALID, "gated_recurrence: null pointer");
     if (reinterpret_cast<uintptr_t>(workspace) & 15)
         return fail(NSOSX_ERR_INVALID, "gated_recurrence: workspace must be 16-byte aligned");
@@ -1017,7 +1013,7 @@ extern "C" int nsosx_gated_recurrence_backward(
         if (D > 1) launch_recurrence_bwd<NSOSX_BF16, 2>(p, st);
         else launch_recurrence_bwd<NSOSX_BF16, 1>(p, st);
     }
-    hipLaunchKernelGGL(recurrence_dlam_kernel, dim3((D + 63) / 64), dim3(1024), 0, st, p.dlam_part,
+    hipLaunchKernelGGL(recurrence_dlam_kernel, dim3((D + 15) / 16), dim3(1024), 0, st, p.dlam_part,
                        (int)rec_tiles(T, kKept), D, lam, dlam);
     return check_launch("gated_recurrence_backward");
 }

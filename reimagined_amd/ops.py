@@ -867,9 +867,10 @@ def moe_balance_loss(logits: torch.Tensor, selected: torch.Tensor, score: str = 
     mask = valid_rows_mask(valid_rows, rows, logits.device)
     _on(fn, dev, ("selected", selected, torch.int32, None), ("valid_rows", mask, torch.uint8, None))
     s = _segments(fn, cu_seqlens, dev)
-    ws = int(lib().nsosx_moe_balance_loss_workspace(rows, e, s)) // 4
-    buf = torch.empty(1 + 2 * s * e + s + ws, dtype=torch.float32, device=logits.device)
-    loss, mean, counts, tokens, ws = buf.split((1, s * e, s * e, s, ws))
+    # (the workspace in front: its sums of 64 bits are aligned)
+    ws = (int(lib().nsosx_moe_balance_loss_workspace(rows, e, s)) + 7) // 8 * 2
+    buf = torch.empty(ws + 1 + 2 * s * e + s, dtype=torch.float32, device=logits.device)
+    ws, loss, mean, counts, tokens = buf.split((ws, 1, s * e, s * e, s))
     counts, tokens = counts.view(torch.int32).view(s, e), tokens.view(torch.int32)
     call("nsosx_moe_balance_loss", _p(logits), _dt(logits), stride, _p(selected), _p(mask), rows, e, k,
          sig, _p(cu_seqlens), s, _p(loss), _p(counts), _p(tokens), _p(mean), _p(ws), _stream_on(dev))
