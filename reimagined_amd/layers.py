@@ -13,6 +13,8 @@
   Int8MoEFFN         the routed feed-forward with int8 experts behind a scored router
                      (softmax or sigmoid scores, balance bias, expert groups), and the
                      gradients that train that router
+  RecurrentLayer     layer norm -> ternary in_proj -> gated linear recurrence -> ternary
+                     out_proj on a residual stream, its gradients and its decode step
   HybridBlock        JambaBlock::forward (src/jamba.cpp:3158-3375) for a Mamba
                      core and an MoE feed-forward: block norms, residual adds
 
@@ -404,17 +406,139 @@ class Int8MoEFFN:
         out = ops.moe_combine_topk(o, r["slot_of"], r["weights"], out_dtype=out_dtype or x.dtype)
         return {"out": out, **r, "h": h, "o": o}
 
-    def router_backward(self, logits: torch.Tensor, fwd: dict, dout: torch.Tensor) -> dict:
+    def balance_loss(self, logits: torch.Tensor, fwd: dict, cu_seqlens=None, valid_rows=None) -> dict:
+        """ops.moe_balance_loss of what forward() chose, on this layer's scores: "loss" [1], "counts" (the
+        experts' loads, for an update of balance_bias as well), "tokens", "mean_prob"; of the whole batch or
+        with cu_seqlens per sequence.  valid_rows: forward()'s."""
+        return ops.moe_balance_loss(logits, fwd["selected"], score=self.routing["score"],
+                                    cu_seqlens=cu_seqlens, valid_rows=valid_rows)
+
+    def router_backward(self, logits: torch.Tensor, fwd: dict, dout: torch.Tensor, balance=None,
+                        dbalance=1.0, cu_seqlens=None, valid_rows=None) -> dict:
         """Gradients of what forward() combined, from that of its "out": dlogits (the router's; the
         balance bias has none), dweights [rows, k] and do, of the experts' output rows "o".  The
         experts' int8 products have no gradient: do goes to a caller who has one, and a router below
-        this layer gets nothing through it."""
+        this layer gets nothing through it.  balance: what balance_loss() gave for the same cu_seqlens
+        and valid_rows; its gradient times dbalance (the loss's weight, or a device tensor of one
+        element) is added to dlogits."""
         do, dw = ops.moe_combine_topk_backward(dout, fwd["o"], fwd["slot_of"], fwd["weights"],
                                                perm=fwd["perm"])
         r = self.routing
         dlogits = ops.moe_route_scored_backward(logits, fwd["selected"], dw, score=r["score"],
                                                 renorm=r["renorm"], scale=r["scale"])
+        if balance is not None:
+            dlogits = ops.moe_balance_loss_backward(logits, balance["counts"], balance["tokens"], self.k,
+                                                    score=r["score"], cu_seqlens=cu_seqlens,
+                                                    valid_rows=valid_rows, dloss=dbalance, add=dlogits)
         return {"dlogits": dlogits, "dweights": dw, "do": do}
+
+
+class RecurrentLayer:
+    """A sequence mixer that can be trained and decoded, on a residual stream:
+
+        r   = x + delta                              (delta: the layer's before; none for the first)
+        f   = layernorm(r) * norm_w + norm_b
+        p   = f @ w_in^T + b_in                      ternary, int8 codes of f, no further input norm
+        y   = gated_recurrence(p[x], p[rg], p[ig])   over the packed batch cu_seqlens
+        out = y @ w_out^T                            ternary; the next layer's delta
+
+    params: w_in [3 inner, d_model] (the rows of x, then rg, then ig), w_out [d_model, inner], lam [inner];
+    optional b_in [3 inner], norm_w and norm_b [d_model], rate (8) and eps (1e-5).  d_model and inner
+    are multiples of 16 (the packed words).  The latent weights w_in and w_out stay on the device in f32: the
+    gradients are theirs (straight through the ternary and the int8 rounding), and repack() forms the
+    ternary ones again after an update.  Activations run in x's type.  Nothing is kept between calls
+    but the weights."""
+
+    def __init__(self, params: dict, device="cuda"):
+        f32 = dict(dtype=torch.float32, device=device)
+        tensor = lambda k: None if params.get(k) is None else torch.as_tensor(params[k], **f32).contiguous()
+        self.w_in, self.w_out, self.lam = tensor("w_in"), tensor("w_out"), tensor("lam")
+        self.b_in, self.norm_w, self.norm_b = tensor("b_in"), tensor("norm_w"), tensor("norm_b")
+        self.rate, self.eps = float(params.get("rate", 8.0)), float(params.get("eps", 1e-5))
+        self.inner, self.d_model = self.lam.numel(), self.w_in.shape[-1]
+        if tuple(self.w_in.shape) != (3 * self.inner, self.d_model) or \
+                tuple(self.w_out.shape) != (self.d_model, self.inner) or self.inner % 16 or self.d_model % 16:
+            raise ValueError("RecurrentLayer: w_in must be [3 inner, d_model] and w_out [d_model, inner], "
+                             "lam [inner], inner and d_model multiples of 16")
+        if self.b_in is not None and self.b_in.numel() != 3 * self.inner:
+            raise ValueError("RecurrentLayer: b_in must be [3 inner]")
+        self.device = device
+        self.repack()
+
+    def repack(self) -> None:
+        """The ternary weights of the latent ones as they are now (through the host)."""
+        linear = lambda w, b: BitLinear(w.cpu().numpy(), self.device, rms_input=False, bias=b)
+        self.in_proj, self.out_proj = linear(self.w_in, self.b_in), linear(self.w_out, None)
+
+    def _norm(self, x, delta, want_stats: bool):
+        """-> r, f and with want_stats the norm's mean and rstd."""
+        if delta is None:
+            f = ops.layernorm(x, self.norm_w, self.norm_b, eps=self.eps, want_stats=want_stats)
+            return (x, *f) if want_stats else (x, f)
+        return ops.add_layernorm(x, delta, self.norm_w, self.norm_b, eps=self.eps, want_stats=want_stats)
+
+    @staticmethod
+    def _project(linear: BitLinear, x: torch.Tensor):
+        """-> x's product, and the codes and scales that it was formed from."""
+        m = x.shape[0]
+        y = x.new_empty((m, linear.out_features))
+        q, s = ops.quantize_activations_bitnet(x, rms_input=False)
+        linear.gemm(q, s, m, y, _stream(), linear.magnitude, linear.bias)
+        return y, q, s
+
+    def _split(self, p: torch.Tensor):
+        return p[:, :self.inner], p[:, self.inner:2 * self.inner], p[:, 2 * self.inner:]
+
+    def forward(self, x: torch.Tensor, cu_seqlens: torch.Tensor, delta=None, initial_state=None,
+                train: bool = False) -> dict:
+        """x (and delta) [T, d_model] f32 or bf16 over the packed batch -> {"residual", "out",
+        "final_state" f32 [S, inner]}; with train what backward() takes as well."""
+        r, f, *stats = self._norm(x, delta, train)
+        p, fq, fs = self._project(self.in_proj, f)
+        y, final, *carry = ops.gated_recurrence(*self._split(p), self.lam, cu_seqlens, rate=self.rate,
+                                                initial_state=initial_state, want_carry=train)
+        out, yq, ys = self._project(self.out_proj, y)
+        fwd = {"residual": r, "out": out, "final_state": final}
+        if train:
+            fwd.update(f=f, mean=stats[0], rstd=stats[1], p=p, fq=fq, fs=fs, y=y, yq=yq, ys=ys, carry=carry[0],
+                       cu_seqlens=cu_seqlens, initial_state=initial_state)
+        return fwd
+
+    def backward(self, fwd: dict, dout: torch.Tensor, dresidual=None, dfinal=None) -> dict:
+        """Gradients from those of forward()'s "out" [T, d_model] (any type), "residual" (x's type) and
+        "final_state" -> dx (of x and of delta alike), dw_in, dw_out, dlam, dnorm_w, dnorm_b, db_in (with a
+        b_in) and dinitial (with an initial state or dfinal).  "dy" and "dp", of the recurrence's output
+        and inputs, come along."""
+        p, r = fwd["p"], fwd["residual"]
+        o = ops.bitlinear_ste_backward(None, fwd["yq"], fwd["ys"], self.w_out, self.out_proj.packed,
+                                       self.out_proj.weight_scale, dout.float(), rms_input=False)
+        dy = o["dx"].to(p.dtype)
+        dp = torch.empty_like(p)
+        g = ops.gated_recurrence_backward(dy, *self._split(p), self.lam, fwd["cu_seqlens"], fwd["carry"],
+                                          rate=self.rate, initial_state=fwd["initial_state"], dfinal=dfinal,
+                                          out=self._split(dp), zero_rest=True)
+        i = ops.bitlinear_ste_backward(None, fwd["fq"], fwd["fs"], self.w_in, self.in_proj.packed,
+                                       self.in_proj.weight_scale, dp.float(), rms_input=False,
+                                       want_dbias=self.b_in is not None)
+        n = ops.layernorm_backward(i["dx"], r, fwd["mean"], fwd["rstd"], self.norm_w, dresidual=dresidual)
+        grads = {"dx": n["dx"], "dw_in": i["dW"], "dw_out": o["dW"], "dlam": g["dlam"], "dnorm_w": n["dweight"],
+                 "dnorm_b": n["dbias"], "dy": dy, "dp": dp}
+        if self.b_in is not None:
+            grads["db_in"] = i["dbias"]
+        if "dinitial" in g:
+            grads["dinitial"] = g["dinitial"]
+        return grads
+
+    def new_decode_state(self, rows: int, device) -> torch.Tensor:
+        return torch.zeros((rows, self.inner), dtype=torch.float32, device=device)
+
+    def step(self, x: torch.Tensor, state: torch.Tensor, delta=None) -> tuple:
+        """One token per row, x (and delta) [R, d_model]; state f32 [R, inner] is updated in place.
+        -> (residual, out)."""
+        r, f = self._norm(x, delta, False)
+        p, _, _ = self._project(self.in_proj, f)
+        y = ops.gated_recurrence_step(*self._split(p), self.lam, state, rate=self.rate)
+        return r, self._project(self.out_proj, y)[0]
 
 
 class HybridBlock:

@@ -1161,7 +1161,8 @@ def _rec_inputs(fn: str, x, rg, ig, lam) -> tuple:
 
 def gated_recurrence(x: torch.Tensor, rg: torch.Tensor, ig: torch.Tensor, lam: torch.Tensor,
                      cu_seqlens: torch.Tensor, rate: float = 8.0, initial_state=None,
-                     want_final: bool = True, want_carry: bool = False, out=None) -> tuple:
+                     want_final: bool = True, want_carry: bool = False, out=None,
+                     zero_rest=None) -> tuple:
     """Gated linear recurrence over a packed ragged batch (nsosx_gated_recurrence):
 
         a = exp(-rate softplus(lam) sigmoid(rg)),  h_t = a_t h_(t-1) + sqrt(1 - a_t^2) sigmoid(ig_t) x_t
@@ -1169,8 +1170,8 @@ def gated_recurrence(x: torch.Tensor, rg: torch.Tensor, ig: torch.Tensor, lam: t
     x, the decay gate's logits rg and the input gate's ig f32 or bf16 [T, D] (column slices are
     fine), lam f32 [D], cu_seqlens int32 [S + 1], initial_state f32 [S, D] or None.  -> (y [T, D] in
     x's dtype, final_state f32 [S, D] or None), and with want_carry a third tensor that
-    gated_recurrence_backward takes.  out: a [T, D] view to write y into, whose rows past the
-    last sequence are left as they were (a fresh y has zeros there).  No autograd."""
+    gated_recurrence_backward takes.  out: a [T, D] view to write y into.  zero_rest: rows of no
+    sequence become zeros (a fresh y's by default) or stay as they were (out's).  No autograd."""
     fn = "gated_recurrence"
     dev, dt, xs, rs, igs = _rec_inputs(fn, x, rg, ig, lam)
     t, d = x.shape
@@ -1183,19 +1184,20 @@ def gated_recurrence(x: torch.Tensor, rg: torch.Tensor, ig: torch.Tensor, lam: t
     carry = x.new_empty((tiles, d), dtype=torch.float32) if want_carry else None
     ws = x.new_empty(int(lib().nsosx_gated_recurrence_workspace(t, d)), dtype=torch.uint8)
     call("nsosx_gated_recurrence", _p(x), xs, _p(rg), rs, _p(ig), igs, _p(lam), rate, _p(cu_seqlens), s,
-         t, d, dt, _p(initial_state), int(out is None), _p(y), ys, _p(final), _p(carry), _p(ws),
-         _stream_on(dev))
+         t, d, dt, _p(initial_state), int(out is None if zero_rest is None else zero_rest), _p(y), ys,
+         _p(final), _p(carry), _p(ws), _stream_on(dev))
     return (y, final, carry) if want_carry else (y, final)
 
 
 def gated_recurrence_backward(dy: torch.Tensor, x: torch.Tensor, rg: torch.Tensor, ig: torch.Tensor,
                               lam: torch.Tensor, cu_seqlens: torch.Tensor, carry: torch.Tensor,
-                              rate: float = 8.0, initial_state=None, dfinal=None, out=None) -> dict:
+                              rate: float = 8.0, initial_state=None, dfinal=None, out=None,
+                              zero_rest=None) -> dict:
     """Gradients of gated_recurrence (nsosx_gated_recurrence_backward) from dy [T, D] (x's dtype) and,
     where the final states went on, dfinal f32 [S, D]; carry is the forward's, the rest its
     arguments.  -> dx, drg, dig [T, D], dlam f32 [D] and, with an initial_state or dfinal, dinitial f32
     [S, D].  out: three [T, D] views (dx, drg, dig) to write into, side by side in one buffer for
-    one; their rows past the last sequence are left as they were (fresh ones have zeros there)."""
+    one.  zero_rest as in gated_recurrence."""
     fn = "gated_recurrence_backward"
     dev, dt, xs, rs, igs = _rec_inputs(fn, x, rg, ig, lam)
     t, d = x.shape
@@ -1216,7 +1218,8 @@ def gated_recurrence_backward(dy: torch.Tensor, x: torch.Tensor, rg: torch.Tenso
     dinit = lam.new_empty((s, d)) if want0 else None
     ws = x.new_empty(int(lib().nsosx_gated_recurrence_backward_workspace(t, d)), dtype=torch.uint8)
     call("nsosx_gated_recurrence_backward", _p(dy), dys, _p(x), xs, _p(rg), rs, _p(ig), igs, _p(lam),
-         rate, _p(cu_seqlens), s, t, d, dt, _p(initial_state), _p(carry), _p(dfinal), int(out is None),
+         rate, _p(cu_seqlens), s, t, d, dt, _p(initial_state), _p(carry), _p(dfinal),
+         int(out is None if zero_rest is None else zero_rest),
          _p(grads[0]), gs[0], _p(grads[1]), gs[1], _p(grads[2]), gs[2], _p(dlam), _p(dinit), _p(ws),
          _stream_on(dev))
     r = {"dx": grads[0], "drg": grads[1], "dig": grads[2], "dlam": dlam}

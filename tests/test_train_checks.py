@@ -187,3 +187,12 @@ def test_balance_wrappers():
         ops.moe_balance_loss(x, sel)
     with pytest.raises(ValueError, match="device tensor"):
         ops.moe_balance_loss_backward(x, sel, sel, 2)
+
+
+def test_layer_refusals():
+    from reimagined_amd.layers import RecurrentLayer
+    p = lambda **kw: {"w_in": torch.zeros(96, 48), "w_out": torch.zeros(48, 32), "lam": torch.zeros(32), **kw}
+    for bad in (dict(w_in=torch.zeros(95, 48)), dict(w_out=torch.zeros(32, 48)), dict(lam=torch.zeros(31)),
+                dict(w_in=torch.zeros(96, 40), w_out=torch.zeros(40, 32)), dict(b_in=torch.zeros(32))):
+        with pytest.raises(ValueError, match="RecurrentLayer"):
+            RecurrentLayer(p(**bad), "cpu")
