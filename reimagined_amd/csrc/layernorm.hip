@@ -5,6 +5,9 @@
 //   dw = sum_rows dy n,  db = sum_rows dy
 // Every pass is bound by memory: a row is read once, held in registers (up to 16384 elements) by
 // TPR threads of 8 CH elements each, and its sums are f32, the variance from the centred row.
+// 67 million bf16 places, add and norm (537 MB): 92 us at rows of 64 to 256 and of 1024 (5.8 TB/s), 94 to
+// 100 at 2048 to 16384, 110 at 777, 121 at 32; the gradients with a residual (as much): 101 to 108 at
+// 128 to 8192, 114 at 64, 179 at 16384.
 #include "train.hpp"
 
 namespace nsosx {
@@ -185,7 +188,8 @@ __global__ __launch_bounds__(NT) void layernorm_long_kernel(
 
 // Threads of a workgroup of the gradients (a longer row takes 1024): eight waves share one row of partial
 // sums.  16384 x 2048 bf16 with a residual: 8 elements a thread in 128 registers 49 us, 16 elements 54 - 58
-// (they spill), workgroups of 256 51.
+// (they spill), workgroups of 256 51.  Rows past 8192 have no more threads to give and take 16 each; with the
+// weights held too 4096 x 16384 took 215 us, without 179, reading the rows twice 308.
 constexpr int kLnBwdThreads = 512;
 
 template <int TPR> constexpr int ln_bwd_threads() { return TPR > kLnBwdThreads ? TPR : kLnBwdThreads; }
@@ -209,13 +213,15 @@ __global__ __launch_bounds__((ln_bwd_threads<TPR>()), 4) void layernorm_bwd_kern
 #pragma unroll
         for (int j = 0; j < 8; ++j) aw[c][j] = ab[c][j] = 0.0f;
     const float inv_dim = 1.0f / static_cast<float>(dim);
-    float w[CH][8];
+    // (with 16 elements a thread the weights are read again, from the caches, where they are used)
+    constexpr bool HOLD = CH == 1;
+    auto weights = [&](int c, float (&w)[8]) {
+        if (weight) load8_any<NSOSX_F32>(weight, el.at[c], w);
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        if (weight) load8_any<NSOSX_F32>(weight, el.at[c], w[c]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[c][j] = weight ? w[c][j] : 1.0f;
-    }
+        for (int j = 0; j < 8; ++j) w[j] = weight ? w[j] : 1.0f;
+    };
+    float held[8];
+    if constexpr (HOLD) weights(0, held);
     int turn = 0;
     auto pass = [&](int64_t row, bool real) {
         const int64_t base = row * dim;
@@ -233,16 +239,19 @@ __global__ __launch_bounds__((ln_bwd_threads<TPR>()), 4) void layernorm_bwd_kern
         }
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
+        for (int c = 0; c < CH; ++c) {
+            float w[8];
+            if constexpr (!HOLD) weights(c, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float v = (xr[c].get(j) - mu) * q, d = real ? gr[c].get(j) : 0.0f;
                 aw[c][j] = __fmaf_rn(d, v, aw[c][j]);
                 ab[c][j] += d;
-                const float m = el.mine(c, j) ? d * w[c][j] : 0.0f;
+                const float m = el.mine(c, j) ? d * (HOLD ? held[j] : w[j]) : 0.0f;
                 s[0] += m;
                 s[1] = __fmaf_rn(m, v, s[1]);
             }
+        }
         if (dres && TPR > 64) {
             // dx may be dres, and a row's last two threads share elements across waves: read before any is
             // written
@@ -255,10 +264,11 @@ __global__ __launch_bounds__((ln_bwd_threads<TPR>()), 4) void layernorm_bwd_kern
         asm volatile("" : "+v"(mu), "+v"(q));  // (both are formed again, not kept in registers)
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            float o[8];
+            float o[8], w[8];
+            if constexpr (!HOLD) weights(c, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                o[j] = q * (gr[c].get(j) * w[c][j] - m1 - (xr[c].get(j) - mu) * q * m2);
+                o[j] = q * (gr[c].get(j) * (HOLD ? held[j] : w[j]) - m1 - (xr[c].get(j) - mu) * q * m2);
                 if (dres) o[j] += dr[c].get(j);
             }
             if (el.any(c)) store8_any<DT>(dx, base + el.at[c], o);
@@ -380,7 +390,11 @@ void launch_column_sums(const float* part, int arrays, int n, int cols, float* o
                        n, cols, out0, out1);
 }
 
-// Threads a row and elements a thread (8 CH): as few threads as hold the row in registers.
+// Threads a row and elements a thread (8 CH): as few threads as hold the row in registers.  Add and norm
+// of 67 million bf16 places: rows of 32 to 256 in a whole wave 707, 374, 206 and 119 us, in 8 to 32 threads
+// 121, 92, 92 and 92; of 777, 1024 and 2048 in 256 threads 326, 160 and 106, in a wave 110, 92 and 97; of
+// 4096 and 8192 in 1024 threads 171 and 114, in 256 94 and 99; rows that are read again (the kernel
+// without a row in registers) 370, 340 and 305 at 4096, 8192 and 16384.
 struct LnShape { int tpr, ch; };
 
 static LnShape ln_shape(int dim) {

@@ -6,12 +6,10 @@
 
 namespace nsosx {
 
-// Eight (two) consecutive elements in one load or store at the elements' own alignment: the memory
+// Eight consecutive elements in one load or store at the elements' own alignment: the memory
 // unit takes a 16-byte access at any address, so rows of an odd length need no path of their own.
 struct __attribute__((packed, aligned(2))) bf16x8_any { uint32_t w[4]; };
 struct __attribute__((packed, aligned(4))) f32x8_any { float v[8]; };
-struct __attribute__((packed, aligned(2))) bf16x2_any { uint32_t w; };
-struct __attribute__((packed, aligned(4))) f32x2_any { float v[2]; };
 
 template <int DT>
 __device__ __forceinline__ void load8_any(const void* p, int64_t i, float (&v)[8]) {
