@@ -107,24 +107,27 @@ __device__ __forceinline__ void load_row(const void* logits, int64_t base, const
 template <int NV, int V, bool SIG, bool REST>
 __device__ __forceinline__ void row_probs(const Lane<NV, V>& ln, float (&p)[NV][V], float (&rest)[NV][V]) {
     float mx = -INFINITY, sum = 0.0f;
-    if constexpr (!SIG) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int v = 0; v < V; ++v) mx = fmaxf(mx, p[i][v]);
-        mx = max16(mx);
-    }
+        for (int v = 0; v < V; ++v) mx = fmaxf(mx, p[i][v]);
+    mx = max16(mx);
+    // Sigmoids of a row whose logits are all far below 0 would sum to 0: they are taken times e^-mx.
+    const float shift = SIG && mx > -60.0f ? 0.0f : mx;
+    const bool far = SIG && __any(shift != 0.0f);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             if constexpr (SIG) {
                 const float e = __builtin_amdgcn_exp2f(fabsf(p[i][v]) * -kLog2e);
-                const float big = __builtin_amdgcn_rcpf(1.0f + e), small = e * big;
+                const float big = __builtin_amdgcn_rcpf(1.0f + e);
+                float small = e * big;
                 if constexpr (REST) rest[i][v] = p[i][v] < 0.0f ? big : small;
+                if (far && p[i][v] < 0.0f) small = __builtin_amdgcn_exp2f((p[i][v] - shift) * kLog2e) * big;
                 p[i][v] = p[i][v] < 0.0f ? small : big;
             } else {
-                p[i][v] = __builtin_amdgcn_exp2f((p[i][v] - mx) * kLog2e);
+                p[i][v] = __builtin_amdgcn_exp2f((p[i][v] - shift) * kLog2e);
             }
             sum += v >= ln.skip[i] ? p[i][v] : 0.0f;
         }

@@ -174,3 +174,27 @@ def test_streams_and_graphs(dev):
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e", [3, 24, 200])
+def test_far_logits(dev, dtype, score, e):
+    """Rows far below 0, whose sigmoids a float cannot hold, and experts masked by the type's lowest value."""
+    rng = np.random.default_rng(e)
+    rows, k = 150, 2
+    x = 2.0 * rng.standard_normal((rows, e)) + np.array([0.0, -55.0, -62.0, -88.0, -300.0, 80.0])[np.arange(rows) % 6, None]
+    t = torch.from_numpy(x.astype(np.float32)).to(DT[dtype])
+    t[::7, 1] = torch.finfo(DT[dtype]).min
+    x = t.double().numpy()
+    sel = np.argsort(-x, axis=1, kind="stable")[:, :k].astype(np.int32)
+    t, sel_t = t.to(dev), torch.from_numpy(sel).to(dev)
+    f = ops.moe_balance_loss(t, sel_t, score=score)
+    loss, counts, _, mean, dx, lim = ref.balance(x, sel, score, None, None, 1.0)
+    assert np.array_equal(f["counts"].cpu().numpy(), counts)
+    # (as above; what is masked adds nothing, and of a row only the largest matter: 320 at most)
+    rel = (2 * 321 + 80 + 64 + 1) * ref.U
+    near(f["mean_prob"], mean, rel * mean, "mean_prob")
+    near(f["loss"], np.array([loss]), np.array([(rel + 4 * ref.U) * loss]), "loss")
+    d = ops.moe_balance_loss_backward(t, f["counts"], f["tokens"], k, score=score)
+    near(d, dx, lim + ref.HALF_STEP[dtype] * np.abs(dx) * (1 + 2.0**-7), "dlogits")
