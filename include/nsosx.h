@@ -727,7 +727,7 @@ int nsosx_layernorm(const void* x, const void* delta, const float* weight, const
  *   dx = rstd (g - mean(g) - n mean(g n)) (+ dresidual), dweight = sum_rows dy n, dbias = sum_rows dy
  * dx and dresidual (the gradient that reached the sum by another way, or NULL; may be dx) in
  * act_dtype; dweight, dbias f32 [dim], each or NULL, the same bits for the same inputs.
- * workspace: nsosx_layernorm_backward_workspace bytes (unused where both are NULL). */
+ * workspace: device, nsosx_layernorm_backward_workspace bytes (unused where both are NULL). */
 int64_t nsosx_layernorm_backward_workspace(int rows, int dim);
 int nsosx_layernorm_backward(const void* dy, int dy_dtype, const void* x, const float* mean,
                              const float* rstd, const float* weight, const void* dresidual,
@@ -751,13 +751,14 @@ int nsosx_conv_step(const void* x, int x_dtype, int64_t x_stride, int rows, int 
 /* Per channel, with a = exp(-rate softplus(lam) sigmoid(rg)):
  *   h_t = a_t h_(t-1) + sqrt(1 - a_t^2) sigmoid(ig_t) x_t,  y = h
  * x, rg, ig, y: [T, D] in act_dtype with row strides in elements (columns of a wider buffer are
- * fine); lam f32 [D]; cu_seqlens int32 [S + 1], not decreasing, empty sequences allowed.
+ * fine) of at most 2^22; lam f32 [D]; cu_seqlens int32 [S + 1], not decreasing, within [0, T], empty
+ * sequences allowed.
  * initial_state f32 [S, D] or NULL (zeros); final_state f32 [S, D] or NULL (an empty sequence's
- * is its initial state).  Rows of no sequence (past cu_seqlens[S]) are left as they were, or
- * with zero_rest != 0 written as zeros.  carry f32 [ceil(T / tile), D] or NULL: the states between
+ * is its initial state).  Rows of no sequence (before cu_seqlens[0], past cu_seqlens[S]) are left as
+ * they were, or with zero_rest != 0 written as zeros.  carry f32 [ceil(T / tile), D] or NULL: the states between
  * tiles of nsosx_gated_recurrence_tile() tokens, which the gradients start from.  The state is f32
- * throughout; the same inputs give the same bits.  workspace: device,
- * nsosx_gated_recurrence_workspace bytes. */
+ * throughout; the same inputs give the same bits.  workspace: device, 16-byte aligned,
+ * nsosx_gated_recurrence_workspace bytes, one for each call that may run at the same time. */
 int nsosx_gated_recurrence_tile(void);
 int64_t nsosx_gated_recurrence_workspace(int T, int D);
 int nsosx_gated_recurrence(const void* x, int64_t x_stride, const void* rg, int64_t rg_stride,
@@ -770,7 +771,8 @@ int nsosx_gated_recurrence(const void* x, int64_t x_stride, const void* rg, int6
  * dx, drg, dig [T, D] in act_dtype with row strides, dlam f32 [D], dinitial f32 [S, D] or NULL.
  * x, rg, ig, lam, rate, cu_seqlens, initial_state and carry as the forward had and left them; h is
  * formed again, y is not needed.  Rows of no sequence as in the forward.  The gradients must
- * not overlap each other or an input (side by side in one buffer's rows is fine). */
+ * not overlap each other or an input (side by side in one buffer's rows is fine).  workspace as in
+ * the forward, nsosx_gated_recurrence_backward_workspace bytes. */
 int64_t nsosx_gated_recurrence_backward_workspace(int T, int D);
 int nsosx_gated_recurrence_backward(const void* dy, int64_t dy_stride, const void* x,
                                     int64_t x_stride, const void* rg, int64_t rg_stride,
@@ -784,7 +786,7 @@ int nsosx_gated_recurrence_backward(const void* dy, int64_t dy_stride, const voi
 
 /* One token per row: state_out = a state + sqrt(1 - a^2) sigmoid(ig) x, y = state_out rounded to
  * act_dtype.  state, state_out f32 [rows, D] (the same buffer for an update in place); the rest as
- * above with rows in place of T. */
+ * above with rows in place of T, at most 262140. */
 int nsosx_gated_recurrence_step(const void* x, int64_t x_stride, const void* rg,
                                 int64_t rg_stride, const void* ig, int64_t ig_stride,
                                 const float* lam, float rate, int rows, int D, int act_dtype,

@@ -509,6 +509,8 @@ class RecurrentLayer:
         "final_state" -> dx (of x and of delta alike), dw_in, dw_out, dlam, dnorm_w, dnorm_b, db_in (with a
         b_in) and dinitial (with an initial state or dfinal).  "dy" and "dp", of the recurrence's output
         and inputs, come along."""
+        if "carry" not in fwd:
+            raise ValueError("RecurrentLayer: backward() needs what forward(train=True) gave")
         p, r = fwd["p"], fwd["residual"]
         o = ops.bitlinear_ste_backward(None, fwd["yq"], fwd["ys"], self.w_out, self.out_proj.packed,
                                        self.out_proj.weight_scale, dout.float(), rms_input=False)

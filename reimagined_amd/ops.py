@@ -1137,11 +1137,17 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rs
 
 def _rec_view(fn: str, dev: int, name: str, t: torch.Tensor, dtype, shape) -> int:
     """Checks a [T, D] view with unit column stride (a column slice is fine); its row stride."""
+    # (one line where all is well, as in _on)
+    if t.get_device() == dev >= 0 and t.dtype == dtype and t.shape == shape:
+        rs, cs = t.stride()
+        if cs == 1 and rs >= shape[1]:
+            return rs
     if t.get_device() != dev or dev < 0:
         raise ValueError(f"{fn}: {name} must be a device tensor on x's device")
     if t.dtype != dtype or tuple(t.shape) != tuple(shape):
         raise ValueError(f"{fn}: {name} must be {tuple(shape)} {dtype}, got {tuple(t.shape)} {t.dtype}")
     rows, d = shape
+    # (a stride over one element says nothing)
     if (d > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < d):
         raise ValueError(f"{fn}: {name} needs unit column stride and rows that do not overlap")
     return t.stride(0) if rows > 1 else d

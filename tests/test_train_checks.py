@@ -196,3 +196,5 @@ def test_layer_refusals():
                 dict(w_in=torch.zeros(96, 40), w_out=torch.zeros(40, 32)), dict(b_in=torch.zeros(32))):
         with pytest.raises(ValueError, match="RecurrentLayer"):
             RecurrentLayer(p(**bad), "cpu")
+    with pytest.raises(ValueError, match="train=True"):
+        RecurrentLayer.backward(None, {"residual": None, "out": None, "final_state": None}, None)
