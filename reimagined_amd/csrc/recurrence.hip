@@ -304,7 +304,7 @@ __device__ __forceinline__ float state_before(const Shared& sh, int k, int tiles
     return polls > kMaxPolls ? __builtin_nanf("") : c;
 }
 
-// Words and flags to 0, the decay rates.
+// Words and flags to 0, the decay rates: 2.5 us, most of it the launch.
 __global__ __launch_bounds__(256) void recurrence_clear_kernel(RecShared s, int64_t n16, int D,
                                                                const float* __restrict__ lam, float rate) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -384,16 +384,22 @@ __device__ __forceinline__ int my_block(int blocks) {
     return (blocks <= 32 && gridDim.x >= 256 ? blockIdx.x / 8 + blockIdx.x / 256 : blockIdx.x) % blocks;
 }
 
-// The lane's decay rates; whether they all stay below kSmall, as most do: those take fewer steps.
+// The lane's decay rates.
 template <int V, typename Args>
-__device__ __forceinline__ bool decay_rates(const Args& arg, int block, float (&k2)[V]) {
-    bool small = true;
+__device__ __forceinline__ void decay_rates(const Args& arg, int block, float (&k2)[V]) {
 #pragma unroll
     for (int k = 0; k < V; ++k) {
         const int ch = min(block * 64 * V + (int)(threadIdx.x & 63) * V, arg.D - V) + k;
         k2[k] = arg.sh.k2 ? arg.sh.k2[ch] : decay_rate(arg.lam[ch], arg.rate);
-        small = small && k2[k] < kSmall;
     }
+}
+
+// Whether they all stay below kSmall, as most do: those take fewer steps.
+template <int V>
+__device__ __forceinline__ bool all_small(const float (&k2)[V]) {
+    bool small = true;
+#pragma unroll
+    for (int k = 0; k < V; ++k) small = small && k2[k] < kSmall;
     return __all(small);
 }
 
@@ -419,7 +425,11 @@ __device__ __forceinline__ void look_back(const Shared& sh, int order, int tiles
 }
 
 // Workgroups take tiles of kTile tokens and 64 V channels, V a lane, in the order of the scan; each wave
-// takes R of the tile's tokens.
+// takes R of the tile's tokens.  Bound by waiting for the tiles before: 65536 x 1024 bf16 (537 MB) 146 us,
+// 115 in a copy that does not wait, 106 at a copy's rate; vector units busy for 36 % of the clocks (29
+// instructions a place, 6 of them exponentials, roots or reciprocals).  As fast: 16 tokens a wave and two
+// workgroups a CU, 8 tokens and three.  Slower: the next tiles' inputs on their way and their pair left before
+// a tile's state is looked up (that takes 256 registers, two waves a SIMD: 220 us).
 template <int DT, int V, int R>
 __global__ __launch_bounds__(64 * (kTile / R), 4) void recurrence_kernel(RecFwd arg) {
     constexpr int WAVES = kTile / R, NT = 64 * WAVES;
@@ -430,12 +440,16 @@ __global__ __launch_bounds__(64 * (kTile / R), 4) void recurrence_kernel(RecFwd 
     __shared__ float s_c[64 * V], s_a[2][WAVES][64 * V], s_h[2][WAVES][64 * V];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles = (int)((arg.T - 1) / kTile + 1), block = my_block((arg.D - 1) / (64 * V) + 1);
+    // (ticket, rates and bounds on their way at once)
+    int first = 0;
+    if (threadIdx.x == 0 && arg.sh.ticket) first = (int)atomicAdd(arg.sh.ticket + block * 16, 1u);
+    float k2[V];
+    decay_rates<V>(arg, block, k2);
     stage_bounds<NT>(arg.cu, arg.S, s_cu);
-    if (threadIdx.x == 0) s_next = arg.sh.ticket ? (int)atomicAdd(arg.sh.ticket + block * 16, 1u) : 0;
+    if (threadIdx.x == 0) s_next = first;
     __syncthreads();
     int at = __builtin_amdgcn_readfirstlane(s_next);
-    float k2[V];
-    const bool small = decay_rates<V>(arg, block, k2);
+    const bool small = all_small<V>(k2);
     for (int turn = 0; at < tiles; turn ^= 1) {
         const auto& P = argument<RecFwd>();
         int lane = threadIdx.x & 63;
@@ -555,7 +569,11 @@ struct RecBwd {
 };
 
 // The same from the last tile to the first.  With q = g / log 2, w = a q and b2 = 1 - a^2:
-//   e = dh (s x a w / beta - w h_before), in units of log 2;  what 1 / beta multiplies goes to 0 with it
+//   e = dh (s x a w / beta - w h_before), in units of log 2
+// (where beta goes to 0 so does w, faster).  Tiles of 64 tokens, 8 a wave: four values an element have to
+// stay in registers over the wait.  16384 x 2048 bf16 (470 MB) 150 us, 123 in a copy that does not wait, 93
+// at a copy's rate; vector units busy for 49 % of the clocks (77 instructions a place, 9 of them of the slow
+// kind).  f32 199 us, floor 185.
 template <int DT, int V, int R>
 __global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_bwd_kernel(RecBwd arg) {
     constexpr int WAVES = kKept / R, NT = 64 * WAVES;
@@ -567,12 +585,16 @@ __global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_b
         s_m[WAVES][64 * V];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles = (int)((arg.T - 1) / kKept + 1), block = my_block((arg.D - 1) / (64 * V) + 1);
+    // (ticket, rates and bounds on their way at once)
+    int first = 0;
+    if (threadIdx.x == 0 && arg.sh.ticket) first = (int)atomicAdd(arg.sh.ticket + block * 16, 1u);
+    float k2[V];
+    decay_rates<V>(arg, block, k2);
     stage_bounds<NT>(arg.cu, arg.S, s_cu);
-    if (threadIdx.x == 0) s_next = arg.sh.ticket ? (int)atomicAdd(arg.sh.ticket + block * 16, 1u) : 0;
+    if (threadIdx.x == 0) s_next = first;
     __syncthreads();
     int at = __builtin_amdgcn_readfirstlane(s_next);
-    float k2[V];
-    const bool small = decay_rates<V>(arg, block, k2);
+    const bool small = all_small<V>(k2);
     while (at < tiles) {
         const auto& P = argument<RecBwd>();
         int lane = threadIdx.x & 63;
@@ -641,12 +663,17 @@ __global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_b
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     M[k] = out ? 0.0f : a[j][k] * (d[j].get(k) + M[k]);
-                    B[k] = end || out ? 0.0f : B[k] * a[j][k];
+                    if (BORDERS) B[k] = end || out ? 0.0f : B[k] * a[j][k];
                 }
             }
         };
-        if (plain) local(std::false_type{});
-        else local(std::true_type{});
+        if (plain) {
+            local(std::false_type{});
+#pragma unroll
+            for (int k = 0; k < V; ++k) B[k] = A[k];
+        } else {
+            local(std::true_type{});
+        }
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             s_a[wave][lane * V + k] = A[k], s_h[wave][lane * V + k] = H[k];
@@ -751,7 +778,8 @@ __global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_b
 }
 
 // dlam = sigmoid(lam) / softplus(lam) * sum_t e, e in units of log 2: the tiles' sums in a fixed order (16
-// channels a workgroup, 64 runs of tiles: a short chain of loads, as the sums are few).
+// channels a workgroup, 64 runs of tiles: a short chain of loads, as the sums are few).  256 tiles x 2048
+// channels 4 us, with 64 channels a workgroup 8.
 __global__ __launch_bounds__(1024) void recurrence_dlam_kernel(const float* __restrict__ part, int tiles,
                                                                int D, const float* __restrict__ lam,
                                                                float* __restrict__ dlam) {
@@ -775,7 +803,9 @@ __global__ __launch_bounds__(1024) void recurrence_dlam_kernel(const float* __re
     dlam[c] = sum * kLn2 * (sp == 0.0f ? 1.0f : sig / sp);
 }
 
-// One token per row: a thread per channel and run of kStepRows rows.
+// One token per row: a thread per channel and run of kStepRows rows, which share the channel's decay rate (a
+// logarithm and two exponentials).  Bound by the launch (8 x 2048) or by memory: 1000 x 2559 f32, 61 MB, in
+// a call of 11.5 us, 12 at a copy's rate (part of it stays in the 256 MB cache).
 constexpr int kStepRows = 4;
 
 template <int DT>
@@ -868,7 +898,8 @@ static unsigned rec_grid(int64_t tiles, int D, int V, int resident) {
 }
 
 // bf16: two channels a lane, f32 one (64 channels are a full line there, and the registers carry more
-// workgroups: 16384 x 2048 f32 121 us and 208 back, with two 167 and 273).
+// workgroups: 16384 x 2048 f32 119 us and 199 back, with two 167 and 273; bf16 76 and 151, with one 82 and
+// 148).
 template <int DT, int V>
 static void launch_recurrence(const RecFwd& p, hipStream_t st) {
     hipLaunchKernelGGL((recurrence_kernel<DT, V, 16>), dim3(rec_grid(rec_tiles(p.T, kTile), p.D, V, 512)),
