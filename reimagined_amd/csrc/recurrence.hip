@@ -51,19 +51,6 @@ template <> struct Pair<NSOSX_BF16, 2> {
         __builtin_amdgcn_raw_buffer_store_b32(pack_bf16x2(f[0], f[1]), v.r, lane, row * v.row, 0);
     }
 };
-template <> struct Pair<NSOSX_F32, 2> {
-    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-    u32x2 w;
-    __device__ __forceinline__ void load(const Rows& v, uint32_t lane, int row) {
-        w = __builtin_amdgcn_raw_buffer_load_b64(v.r, lane, row * v.row, 0);
-    }
-    __device__ __forceinline__ void forget() { asm volatile("" : "+v"(w)); }
-    __device__ __forceinline__ float get(int k) const { return __uint_as_float(k ? w.y : w.x); }
-    static __device__ __forceinline__ void store(const Rows& v, uint32_t lane, int row, const float (&f)[2]) {
-        const u32x2 w = {__float_as_uint(f[0]), __float_as_uint(f[1])};
-        __builtin_amdgcn_raw_buffer_store_b64(w, v.r, lane, row * v.row, 0);
-    }
-};
 template <int DT> struct Pair<DT, 1> {
     float v;
     __device__ __forceinline__ void load(const Rows& p, uint32_t lane, int row) {
@@ -120,8 +107,8 @@ struct Tokens {
 };
 
 // cu holds S + 1 bounds: a search per lane, in LDS but for thousands of sequences.  seqs: the wave's R.
-template <int R>
-__device__ __forceinline__ Tokens find_tokens(const int32_t* cu, int S, int lane, int64_t first, int64_t T,
+template <int R, typename Bounds>
+__device__ __forceinline__ Tokens find_tokens(const Bounds& cu, int S, int lane, int64_t first, int64_t T,
                                               int32_t* seqs) {
     const int i = min(lane, R - 1);
     const int64_t t = first + i;
@@ -378,7 +365,7 @@ __device__ __forceinline__ const __attribute__((address_space(4))) T& argument()
 
 // The workgroup's block of channels.  Tiles of a block end in the order of the scan, so its workgroups move
 // in step; each XCD and each CU holds workgroups of different blocks, whose steps differ, so that some
-// compute while others load (65536 x 1024: 215 us with a block on one XCD, 165 so).
+// compute while others load (65536 x 1024 took 215 us with a block on one XCD when it took 165 so).
 __device__ __forceinline__ int my_block(int blocks) {
     // (up to 32 blocks are all named by the first 256 workgroups)
     return (blocks <= 32 && gridDim.x >= 256 ? blockIdx.x / 8 + blockIdx.x / 256 : blockIdx.x) % blocks;
@@ -424,12 +411,29 @@ __device__ __forceinline__ void look_back(const Shared& sh, int order, int tiles
                           : 0.0f;
 }
 
+// (A, H) of the lane's channels over the waves from `first`, `n` of them, in steps of `step`.
+template <int V, int WAVES>
+__device__ __forceinline__ void through_waves(const float (&s_a)[WAVES][64 * V], const float (&s_h)[WAVES][64 * V],
+                                              int lane, int first, int n, int step, float (&A)[V], float (&H)[V]) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) A[k] = 1.0f, H[k] = 0.0f;
+    for (int i = 0; i < n; ++i) {
+        const int w = first + i * step;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float a = s_a[w][lane * V + k];
+            H[k] = through(a, s_h[w][lane * V + k], H[k]);
+            A[k] = a == 0.0f ? 0.0f : A[k] * a;
+        }
+    }
+}
+
 // Workgroups take tiles of kTile tokens and 64 V channels, V a lane, in the order of the scan; each wave
-// takes R of the tile's tokens.  Bound by waiting for the tiles before: 65536 x 1024 bf16 (537 MB) 146 us,
-// 115 in a copy that does not wait, 106 at a copy's rate; vector units busy for 36 % of the clocks (29
-// instructions a place, 6 of them exponentials, roots or reciprocals).  As fast: 16 tokens a wave and two
-// workgroups a CU, 8 tokens and three.  Slower: the next tiles' inputs on their way and their pair left before
-// a tile's state is looked up (that takes 256 registers, two waves a SIMD: 220 us).
+// takes R of the tile's tokens.  Bound by waiting for the tiles before: 65536 x 1024 bf16 (537 MB) 135 us,
+// 108 in a copy that does not wait, 106 at a copy's rate; 40796 x 2048 153, 132 and 132.  As fast: 16 tokens
+// a wave and two workgroups a CU, 8 tokens and three.  Slower: the next tile's inputs on their way and its
+// pair left before this tile's state is looked up (that takes 256 registers, two waves a SIMD: 220 us); a
+// ticket taken before the wait (168), as it then lies with a workgroup that waits and holds all later tiles up.
 template <int DT, int V, int R>
 __global__ __launch_bounds__(64 * (kTile / R), 4) void recurrence_kernel(RecFwd arg) {
     constexpr int WAVES = kTile / R, NT = 64 * WAVES;
@@ -469,7 +473,9 @@ __global__ __launch_bounds__(64 * (kTile / R), 4) void recurrence_kernel(RecFwd 
                 x[j].load(vx, off, t);
             }
         }
-        const Tokens tok = find_tokens<R>(P.S < kCuLds ? s_cu : P.cu, P.S, lane, p.t0 + wave * R, P.T, s_seq + wave * R);
+        Tokens tok;  // (a search of its own for either memory: one through a flat address would wait for the inputs)
+        if (P.S < kCuLds) tok = find_tokens<R>(s_cu, P.S, lane, p.t0 + wave * R, P.T, s_seq + wave * R);
+        else tok = find_tokens<R>(P.cu, P.S, lane, p.t0 + wave * R, P.T, s_seq + wave * R);
         const bool plain = tok.template plain<R>();
         float a[R][V], u[R][V];
         auto gates = [&](auto fits) {
@@ -512,16 +518,12 @@ __global__ __launch_bounds__(64 * (kTile / R), 4) void recurrence_kernel(RecFwd 
         for (int k = 0; k < V; ++k) s_a[turn][wave][lane * V + k] = A[k], s_h[turn][wave][lane * V + k] = H[k];
         __syncthreads();
         if (wave < V) look_back<V, WAVES>(P.sh, p.order, tiles, p.c0, P.D, false, wave * 64 + lane, s_a[turn], s_h[turn], s_c, s_w);
+        // (the waves before this one in the tile, meanwhile)
+        through_waves<V>(s_a[turn], s_h[turn], lane, 0, wave, 1, A, H);
         __syncthreads();
-        int next = tiles;  // (taken no earlier: a ticket that lies with a waiting workgroup holds all later ones up)
-        if (threadIdx.x == 0 && P.sh.ticket) next = (int)atomicAdd(P.sh.ticket + block * 16, 1u);
         float h[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) h[k] = s_c[lane * V + k];
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-            for (int w = 0; w < wave; ++w)
-                h[k] = through(s_a[turn][w][lane * V + k], s_h[turn][w][lane * V + k], h[k]);
+        for (int k = 0; k < V; ++k) h[k] = through(A[k], H[k], s_c[lane * V + k]);
         if (wave * R % kKept == 0 && P.carry && wave * R < p.real && p.act)
             put_state<V>(P.carry, (int)((p.t0 + wave * R) / kKept), P.D, ch, h);
         const Rows vy = tile_rows<DT>(P.y, P.ys, p.t0);
@@ -547,7 +549,7 @@ __global__ __launch_bounds__(64 * (kTile / R), 4) void recurrence_kernel(RecFwd 
         };
         if (plain) apply(std::false_type{});
         else apply(std::true_type{});
-        if (threadIdx.x == 0) s_next = next;
+        if (threadIdx.x == 0) s_next = P.sh.ticket ? (int)atomicAdd(P.sh.ticket + block * 16, 1u) : tiles;
         __syncthreads();
         at = __builtin_amdgcn_readfirstlane(s_next);
         if (p.order == 0 && P.final) empty_states<V, NT>(P.cu, P.S, P.D, ch, p.act, P.initial, P.final);
@@ -571,9 +573,9 @@ struct RecBwd {
 // The same from the last tile to the first.  With q = g / log 2, w = a q and b2 = 1 - a^2:
 //   e = dh (s x a w / beta - w h_before), in units of log 2
 // (where beta goes to 0 so does w, faster).  Tiles of 64 tokens, 8 a wave: four values an element have to
-// stay in registers over the wait.  16384 x 2048 bf16 (470 MB) 150 us, 123 in a copy that does not wait, 93
-// at a copy's rate; vector units busy for 49 % of the clocks (77 instructions a place, 9 of them of the slow
-// kind).  f32 199 us, floor 185.
+// stay in registers over the wait.  16384 x 2048 bf16 (470 MB) 137 us, 111 in a copy that does not wait, 93
+// at a copy's rate (77 vector instructions a place, 9 of them exponentials, roots and reciprocals); with
+// 1 - a^2 kept too, which spills, 159.  f32 191 us, floor 185.
 template <int DT, int V, int R>
 __global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_bwd_kernel(RecBwd arg) {
     constexpr int WAVES = kKept / R, NT = 64 * WAVES;
@@ -626,7 +628,9 @@ __global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_b
                     eg[j][k] = exp_neg(g[j].get(k));
                 }
         }
-        const Tokens tok = find_tokens<R>(P.S < kCuLds ? s_cu : P.cu, P.S, lane, p.t0 + wave * R, P.T, s_seq + wave * R);
+        Tokens tok;  // (a search of its own for either memory: one through a flat address would wait for the inputs)
+        if (P.S < kCuLds) tok = find_tokens<R>(s_cu, P.S, lane, p.t0 + wave * R, P.T, s_seq + wave * R);
+        else tok = find_tokens<R>(P.cu, P.S, lane, p.t0 + wave * R, P.T, s_seq + wave * R);
         const bool plain = tok.template plain<R>();
         auto gates = [&](auto fits) {
 #pragma unroll
@@ -680,10 +684,12 @@ __global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_b
             s_b[wave][lane * V + k] = B[k], s_m[wave][lane * V + k] = M[k];
         }
         __syncthreads();
-        if (wave < V) look_back<V, WAVES>(P.sh, p.order, tiles, p.c0, P.D, true, wave * 64 + lane, s_b, s_m, s_c, s_w);
+        if (wave >= WAVES - V)
+            look_back<V, WAVES>(P.sh, p.order, tiles, p.c0, P.D, true, (wave - (WAVES - V)) * 64 + lane, s_b, s_m, s_c, s_w);
+        through_waves<V>(s_a, s_h, lane, 0, wave, 1, A, H);
+        through_waves<V>(s_b, s_m, lane, WAVES - 1, WAVES - 1 - wave, -1, B, M);
 #pragma unroll
-        for (int k = 0; k < V; ++k)
-            for (int w = 0; w < wave; ++w) h[k] = through(s_a[w][lane * V + k], s_h[w][lane * V + k], h[k]);
+        for (int k = 0; k < V; ++k) h[k] = through(A[k], H[k], h[k]);
         // u becomes the state before each token
         auto states = [&](auto borders) {
 #pragma unroll
@@ -701,13 +707,10 @@ __global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_b
         if (plain) states(std::false_type{});
         else states(std::true_type{});
         __syncthreads();
-        int next = tiles;  // (taken no earlier: a ticket that lies with a waiting workgroup holds all later ones up)
-        if (threadIdx.x == 0 && P.sh.ticket) next = (int)atomicAdd(P.sh.ticket + block * 16, 1u);
         float m[V], e[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            m[k] = s_c[lane * V + k];
-            for (int w = WAVES - 1; w > wave; --w) m[k] = through(s_b[w][lane * V + k], s_m[w][lane * V + k], m[k]);
+            m[k] = through(B[k], M[k], s_c[lane * V + k]);
             e[k] = 0.0f;
         }
         // (the compiler would keep the gates since their first use, in registers that are not there)
@@ -764,7 +767,7 @@ __global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_b
         __syncthreads();  // (s_a is read by now)
 #pragma unroll
         for (int k = 0; k < V; ++k) s_a[wave][lane * V + k] = e[k];
-        if (threadIdx.x == 0) s_next = next;
+        if (threadIdx.x == 0) s_next = P.sh.ticket ? (int)atomicAdd(P.sh.ticket + block * 16, 1u) : tiles;
         __syncthreads();
         at = __builtin_amdgcn_readfirstlane(s_next);
         if (wave == 0 && p.act) {
@@ -898,8 +901,8 @@ static unsigned rec_grid(int64_t tiles, int D, int V, int resident) {
 }
 
 // bf16: two channels a lane, f32 one (64 channels are a full line there, and the registers carry more
-// workgroups: 16384 x 2048 f32 119 us and 199 back, with two 167 and 273; bf16 76 and 151, with one 82 and
-// 148).
+// workgroups: 16384 x 2048 f32 113 us and 191 back, with two 167 and 273; bf16 67 and 137, with one 82 and
+// 136).
 template <int DT, int V>
 static void launch_recurrence(const RecFwd& p, hipStream_t st) {
     hipLaunchKernelGGL((recurrence_kernel<DT, V, 16>), dim3(rec_grid(rec_tiles(p.T, kTile), p.D, V, 512)),

@@ -101,6 +101,20 @@ def test_wide(dev, d, dtype):
             assert torch.equal(got[k][..., lo:hi], want[k]), k
 
 
+@pytest.mark.parametrize("seqs", [2046, 2047, 2048, 5000])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_sequences(dev, seqs, dtype):
+    """More bounds than the kernels keep on the chip."""
+    c, n = make(dev, [(7 * i) % 4 for i in range(seqs)], 20, dtype, True)
+    want = ref.Recurrence(n["x"], n["rg"], n["ig"], n["lam"], n["cu"], 8.0, n["h0"])
+    y, final, carry = forward(c)
+    near(y, want.h, want.eh, dtype, "y")
+    near(final, want.final, want.efinal, what="final")
+    grads = want.backward(n["dy"], n["dfinal"])
+    for name, g in backward(c, carry).items():
+        near(g, *grads[name], dtype=dtype if name in ("dx", "drg", "dig") else "f32", what=name)
+
+
 def test_long_sequence(dev):
     """Many tiles behind one another (a state that crosses hundreds of them)."""
     c, n = make(dev, [40000, 7], 6, "f32", True)
