@@ -363,12 +363,15 @@ __device__ __forceinline__ const __attribute__((address_space(4))) T& argument()
     return *p;
 }
 
-// The workgroup's block of channels.  Tiles of a block end in the order of the scan, so its workgroups move
-// in step; each XCD and each CU holds workgroups of different blocks, whose steps differ, so that some
-// compute while others load (65536 x 1024 took 215 us with a block on one XCD when it took 165 so).
+// The workgroup's block of channels, as many workgroups for each.  Tiles of a block end in the order of the
+// scan, so its workgroups move in step; each XCD and each CU holds workgroups of different blocks, whose steps
+// differ, so that some compute while others load (65536 x 1024 took 215 us with a block on one XCD when it
+// took 165 so).
 __device__ __forceinline__ int my_block(int blocks) {
-    // (up to 32 blocks are all named by the first 256 workgroups)
-    return (blocks <= 32 && gridDim.x >= 256 ? blockIdx.x / 8 + blockIdx.x / 256 : blockIdx.x) % blocks;
+    // Workgroups go to the 8 XCDs in turn, and there to 32 CUs: `at` numbers them XCD by XCD, and a shift
+    // after every 32 or more (whole turns of the blocks) keeps a CU's next one off the same block.
+    const int n = gridDim.x, xcd = blockIdx.x % 8, at = xcd * (n / 8) + min(xcd, n % 8) + blockIdx.x / 8;
+    return (at + at / ((31 / blocks + 1) * blocks)) % blocks;
 }
 
 // The lane's decay rates.
@@ -454,6 +457,7 @@ __global__ __launch_bounds__(64 * (kTile / R), 4) void recurrence_kernel(RecFwd 
     __syncthreads();
     int at = __builtin_amdgcn_readfirstlane(s_next);
     const bool small = all_small<V>(k2);
+    const bool again = (int64_t)gridDim.x < (int64_t)tiles * ((arg.D - 1) / (64 * V) + 1);  // (else a tile each)
     for (int turn = 0; at < tiles; turn ^= 1) {
         const auto& P = argument<RecFwd>();
         int lane = threadIdx.x & 63;
@@ -549,7 +553,7 @@ __global__ __launch_bounds__(64 * (kTile / R), 4) void recurrence_kernel(RecFwd 
         };
         if (plain) apply(std::false_type{});
         else apply(std::true_type{});
-        if (threadIdx.x == 0) s_next = P.sh.ticket ? (int)atomicAdd(P.sh.ticket + block * 16, 1u) : tiles;
+        if (threadIdx.x == 0) s_next = again ? (int)atomicAdd(P.sh.ticket + block * 16, 1u) : tiles;
         __syncthreads();
         at = __builtin_amdgcn_readfirstlane(s_next);
         if (p.order == 0 && P.final) empty_states<V, NT>(P.cu, P.S, P.D, ch, p.act, P.initial, P.final);
@@ -597,6 +601,7 @@ __global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_b
     __syncthreads();
     int at = __builtin_amdgcn_readfirstlane(s_next);
     const bool small = all_small<V>(k2);
+    const bool again = (int64_t)gridDim.x < (int64_t)tiles * ((arg.D - 1) / (64 * V) + 1);  // (else a tile each)
     while (at < tiles) {
         const auto& P = argument<RecBwd>();
         int lane = threadIdx.x & 63;
@@ -767,7 +772,7 @@ __global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_b
         __syncthreads();  // (s_a is read by now)
 #pragma unroll
         for (int k = 0; k < V; ++k) s_a[wave][lane * V + k] = e[k];
-        if (threadIdx.x == 0) s_next = P.sh.ticket ? (int)atomicAdd(P.sh.ticket + block * 16, 1u) : tiles;
+        if (threadIdx.x == 0) s_next = again ? (int)atomicAdd(P.sh.ticket + block * 16, 1u) : tiles;
         __syncthreads();
         at = __builtin_amdgcn_readfirstlane(s_next);
         if (wave == 0 && p.act) {

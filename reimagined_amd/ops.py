@@ -870,7 +870,7 @@ def moe_balance_loss(logits: torch.Tensor, selected: torch.Tensor, score: str = 
     # (the workspace in front: its sums of 64 bits are aligned)
     ws = (int(lib().nsosx_moe_balance_loss_workspace(rows, e, s)) + 7) // 8 * 2
     buf = torch.empty(ws + 1 + 2 * s * e + s, dtype=torch.float32, device=logits.device)
-    ws, loss, mean, counts, tokens = buf.split((ws, 1, s * e, s * e, s))
+    ws, loss, mean, counts, tokens = buf.split_with_sizes((ws, 1, s * e, s * e, s))
     counts, tokens = counts.view(torch.int32).view(s, e), tokens.view(torch.int32)
     call("nsosx_moe_balance_loss", _p(logits), _dt(logits), stride, _p(selected), _p(mask), rows, e, k,
          sig, _p(cu_seqlens), s, _p(loss), _p(counts), _p(tokens), _p(mean), _p(ws), _stream_on(dev))
@@ -1127,7 +1127,7 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rs
     dw = db = ws = None
     if want_params:
         n = int(lib().nsosx_layernorm_backward_workspace(rows, dim)) // 4
-        dw, db, ws = x.new_empty(2 * dim + n, dtype=torch.float32).split((dim, dim, n))
+        dw, db, ws = x.new_empty(2 * dim + n, dtype=torch.float32).split_with_sizes((dim, dim, n))
     call("nsosx_layernorm_backward", _p(dy), _dt(dy), _p(x), _p(mean), _p(rstd), _p(weight),
          _p(dresidual), rows, dim, _dt(x), _p(dx), _p(dw), _p(db), _p(ws), _stream_on(dev))
     return {"dx": dx, "dweight": dw, "dbias": db} if want_params else {"dx": dx}
@@ -1153,16 +1153,19 @@ def _rec_view(fn: str, dev: int, name: str, t: torch.Tensor, dtype, shape) -> in
     return t.stride(0) if rows > 1 else d
 
 
-def _rec_inputs(fn: str, x, rg, ig, lam) -> tuple:
+def _rec_inputs(fn: str, x, rg, ig, lam, *more) -> tuple:
+    """Checks the recurrence's inputs and `more` as _on takes it; device, type and row strides."""
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"{fn}: x must be [tokens, dim], got {tuple(x.shape)}")
     dt = _dt(x)
     if not x.is_cuda:
         raise ValueError("x must be a device tensor")
     dev = x.get_device()
-    strides = [_rec_view(fn, dev, n, t, x.dtype, x.shape) for n, t in (("x", x), ("rg", rg), ("ig", ig))]
-    _on(fn, dev, ("lam", lam, torch.float32, (x.shape[1],)))
-    return dev, dt, *strides
+    dtype, shape = x.dtype, x.shape
+    xs, rs = _rec_view(fn, dev, "x", x, dtype, shape), _rec_view(fn, dev, "rg", rg, dtype, shape)
+    igs = _rec_view(fn, dev, "ig", ig, dtype, shape)
+    _on(fn, dev, ("lam", lam, torch.float32, shape[1:]), *more)
+    return dev, dt, xs, rs, igs
 
 
 def gated_recurrence(x: torch.Tensor, rg: torch.Tensor, ig: torch.Tensor, lam: torch.Tensor,
@@ -1239,11 +1242,12 @@ def gated_recurrence_step(x: torch.Tensor, rg: torch.Tensor, ig: torch.Tensor, l
     """One token per row through gated_recurrence (nsosx_gated_recurrence_step): x, rg, ig [R, D],
     state f32 [R, D], updated in place or written to state_out.  -> y [R, D] in x's dtype."""
     fn = "gated_recurrence_step"
-    dev, dt, xs, rs, igs = _rec_inputs(fn, x, rg, ig, lam)
+    f32 = torch.float32
+    dev, dt, xs, rs, igs = _rec_inputs(fn, x, rg, ig, lam, ("state", state, f32, x.shape),
+                                       ("state_out", state_out, f32, x.shape))
     r, d = x.shape
     if state_out is None:
         state_out = state
-    _on(fn, dev, ("state", state, torch.float32, (r, d)), ("state_out", state_out, torch.float32, (r, d)))
     y = x.new_empty((r, d))
     call("nsosx_gated_recurrence_step", _p(x), xs, _p(rg), rs, _p(ig), igs, _p(lam), rate, r, d, dt,
          _p(state), _p(state_out), _p(y), d, _stream_on(dev))
