@@ -361,6 +361,7 @@ __global__ __launch_bounds__(256) void layernorm_cols_kernel(
     part[((int64_t)gridDim.y + blockIdx.y) * dim + e] = ab;
 }
 
+// out0[c], out1[c] = the sums over n rows of part[0], part[1] (a NULL out is skipped), in a fixed order.
 // 16 columns a workgroup (64 B of a row), a row of partial sums per 16 lanes: enough workgroups for
 // every load to be on its way at once.  Each thread adds its rows in order, the threads as a tree.
 __global__ __launch_bounds__(1024) void column_sums_kernel(const float* __restrict__ part, int n,
@@ -382,12 +383,6 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const float* __restri
         for (int w = 1; w < 16; ++w) sum += s[w][lane];
         out[c] = sum;
     }
-}
-
-void launch_column_sums(const float* part, int arrays, int n, int cols, float* out0, float* out1,
-                        hipStream_t st) {
-    hipLaunchKernelGGL(column_sums_kernel, dim3((cols + 15) / 16, arrays), dim3(1024), 0, st, part,
-                       n, cols, out0, out1);
 }
 
 // Threads a row and elements a thread (8 CH): as few threads as hold the row in registers.  Add and norm
@@ -582,6 +577,8 @@ extern "C" int nsosx_layernorm_backward(const void* dy, int dy_dtype, const void
         }
     }
 #undef NSOSX_LN_GO
-    if (cols) launch_column_sums(part, 2, ln_bwd_workgroups(rows, dim), dim, dweight, dbias, st);
+    if (cols)
+        hipLaunchKernelGGL(column_sums_kernel, dim3((dim + 15) / 16, 2), dim3(1024), 0, st, part,
+                           ln_bwd_workgroups(rows, dim), dim, dweight, dbias);
     return check_launch("layernorm_backward");
 }

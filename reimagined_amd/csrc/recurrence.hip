@@ -10,7 +10,7 @@
 // registers, from there, so every input is read once.
 // Backwards the same stream runs the other way in m_t = a_t dh_t, dh_t = dy_t + m_(t+1): a sequence's
 // last token takes dfinal in place of m_(t+1), its first token's m is dinitial.  h is formed again
-// from the forward's states at the tiles' borders (f32, one per kTile tokens), so y is not read.
+// from the forward's states before every kKept-th token (f32), so y is not read.
 #include "train.hpp"
 
 #include <type_traits>

@@ -1,5 +1,5 @@
 // Shared pieces of the operators a block is trained with (layer norm, gated recurrence, balance
-// loss): vectors at any alignment, sums over partial columns.
+// loss): vectors at any alignment, checks of buffers.
 #pragma once
 
 #include "common.hpp"
@@ -68,10 +68,6 @@ template <> struct Raw8<NSOSX_F32> {
         for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(v.v[j])::"memory");
     }
 };
-
-// out_a[c] = sum_n part[a][n][c] for a < arrays (1 or 2; a NULL out is skipped), in a fixed order.
-void launch_column_sums(const float* part, int arrays, int n, int cols, float* out0, float* out1,
-                        hipStream_t st);
 
 // whether [a, a + a_bytes) and [b, b + b_bytes) share a byte but are not the same buffer
 inline bool crosses(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {

@@ -835,14 +835,21 @@ def moe_route_scored_backward(logits: torch.Tensor, selected: torch.Tensor, dwei
     return out
 
 
+def _sequences(fn: str, cu_seqlens) -> int:
+    """Sequences of a packed batch's bounds [S + 1]."""
+    shape = () if cu_seqlens is None else cu_seqlens.shape
+    if len(shape) != 1 or shape[0] < 1:
+        raise ValueError(f"{fn}: cu_seqlens must be [sequences + 1], got {tuple(shape)}")
+    return shape[0] - 1
+
+
 def _segments(fn: str, cu_seqlens, dev: int) -> int:
     """Sequences of a packed batch's bounds int32 [S + 1] (None: the batch is one)."""
     if cu_seqlens is None:
         return 1
-    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
-        raise ValueError(f"{fn}: cu_seqlens must be [sequences + 1], got {tuple(cu_seqlens.shape)}")
+    s = _sequences(fn, cu_seqlens)
     _on(fn, dev, ("cu_seqlens", cu_seqlens, torch.int32, None))
-    return cu_seqlens.numel() - 1
+    return s
 
 
 def moe_balance_loss(logits: torch.Tensor, selected: torch.Tensor, score: str = "softmax",
@@ -1182,10 +1189,10 @@ def gated_recurrence(x: torch.Tensor, rg: torch.Tensor, ig: torch.Tensor, lam: t
     gated_recurrence_backward takes.  out: a [T, D] view to write y into.  zero_rest: rows of no
     sequence become zeros (a fresh y's by default) or stay as they were (out's).  No autograd."""
     fn = "gated_recurrence"
-    dev, dt, xs, rs, igs = _rec_inputs(fn, x, rg, ig, lam)
+    s = _sequences(fn, cu_seqlens)
+    dev, dt, xs, rs, igs = _rec_inputs(fn, x, rg, ig, lam, ("cu_seqlens", cu_seqlens, torch.int32, None),
+                                       ("initial_state", initial_state, torch.float32, (s, *x.shape[1:])))
     t, d = x.shape
-    s = _segments(fn, cu_seqlens, dev)
-    _on(fn, dev, ("initial_state", initial_state, torch.float32, (s, d)))
     y = x.new_empty((t, d)) if out is None else out
     ys = d if out is None else _rec_view(fn, dev, "out", out, x.dtype, (t, d))
     final = x.new_empty((s, d), dtype=torch.float32) if want_final else None
@@ -1208,13 +1215,13 @@ def gated_recurrence_backward(dy: torch.Tensor, x: torch.Tensor, rg: torch.Tenso
     [S, D].  out: three [T, D] views (dx, drg, dig) to write into, side by side in one buffer for
     one.  zero_rest as in gated_recurrence."""
     fn = "gated_recurrence_backward"
-    dev, dt, xs, rs, igs = _rec_inputs(fn, x, rg, ig, lam)
-    t, d = x.shape
-    s = _segments(fn, cu_seqlens, dev)
-    dys = _rec_view(fn, dev, "dy", dy, x.dtype, (t, d))
+    s, f32 = _sequences(fn, cu_seqlens), torch.float32
+    t, d = x.shape if x.dim() == 2 else (0, 0)
     tiles = -(-t // lib().nsosx_gated_recurrence_tile())
-    _on(fn, dev, ("carry", carry, torch.float32, (tiles, d)),
-        ("initial_state", initial_state, torch.float32, (s, d)), ("dfinal", dfinal, torch.float32, (s, d)))
+    dev, dt, xs, rs, igs = _rec_inputs(fn, x, rg, ig, lam, ("cu_seqlens", cu_seqlens, torch.int32, None),
+                                       ("carry", carry, f32, (tiles, d)),
+                                       ("initial_state", initial_state, f32, (s, d)), ("dfinal", dfinal, f32, (s, d)))
+    dys = _rec_view(fn, dev, "dy", dy, x.dtype, x.shape)
     if out is None:
         grads, gs = x.new_empty((3, t, d)).unbind(0), (d, d, d)
     else:

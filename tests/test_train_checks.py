@@ -189,6 +189,21 @@ def test_balance_wrappers():
         ops.moe_balance_loss_backward(x, sel, sel, 2)
 
 
+def test_recurrence_bounds():
+    x, lam = torch.zeros(4, 8), torch.zeros(8)
+    for cu in (None, torch.zeros((2, 2), dtype=torch.int32), torch.zeros(0, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="cu_seqlens must be"):
+            ops.gated_recurrence(x, x, x, lam, cu)
+        with pytest.raises(ValueError, match="cu_seqlens must be"):
+            ops.gated_recurrence_backward(x, x, x, x, lam, cu, torch.zeros(1, 8))
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    for bad in (torch.zeros(()), torch.zeros(4), torch.zeros(2, 2, 8), torch.zeros(4, 0)):
+        with pytest.raises(ValueError, match="tokens, dim"):
+            ops.gated_recurrence(bad, x, x, lam, cu)
+        with pytest.raises(ValueError, match="tokens, dim"):
+            ops.gated_recurrence_backward(x, bad, x, x, lam, cu, torch.zeros(1, 8))
+
+
 def test_layer_refusals():
     from reimagined_amd.layers import RecurrentLayer
     p = lambda **kw: {"w_in": torch.zeros(96, 48), "w_out": torch.zeros(48, 32), "lam": torch.zeros(32), **kw}
