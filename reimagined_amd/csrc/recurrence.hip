@@ -577,7 +577,7 @@ struct RecBwd {
 // The same from the last tile to the first.  With q = g / log 2, w = a q and b2 = 1 - a^2:
 //   e = dh (s x a w / beta - w h_before), in units of log 2
 // (where beta goes to 0 so does w, faster).  Tiles of 64 tokens, 8 a wave: four values an element have to
-// stay in registers over the wait.  16384 x 2048 bf16 (470 MB) 137 us, 111 in a copy that does not wait, 93
+// stay in registers over the wait.  16384 x 2048 bf16 (470 MB) 134 us, 111 in a copy that does not wait, 93
 // at a copy's rate (77 vector instructions a place, 9 of them exponentials, roots and reciprocals); with
 // 1 - a^2 kept too, which spills, 159.  f32 191 us, floor 185.
 template <int DT, int V, int R>
@@ -588,7 +588,7 @@ __global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_b
     __shared__ int32_t s_seq[kKept];
     __shared__ int s_next;
     __shared__ float s_c[64 * V], s_a[WAVES][64 * V], s_h[WAVES][64 * V], s_b[WAVES][64 * V],
-        s_m[WAVES][64 * V];
+        s_m[WAVES][64 * V], s_e[WAVES][64 * V];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles = (int)((arg.T - 1) / kKept + 1), block = my_block((arg.D - 1) / (64 * V) + 1);
     // (ticket, rates and bounds on their way at once)
@@ -769,16 +769,15 @@ __global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_b
         if (!plain) apply(std::true_type{}, std::false_type{});
         else if (small) apply(std::false_type{}, std::true_type{});
         else apply(std::false_type{}, std::false_type{});
-        __syncthreads();  // (s_a is read by now)
 #pragma unroll
-        for (int k = 0; k < V; ++k) s_a[wave][lane * V + k] = e[k];
+        for (int k = 0; k < V; ++k) s_e[wave][lane * V + k] = e[k];
         if (threadIdx.x == 0) s_next = again ? (int)atomicAdd(P.sh.ticket + block * 16, 1u) : tiles;
         __syncthreads();
         at = __builtin_amdgcn_readfirstlane(s_next);
         if (wave == 0 && p.act) {
 #pragma unroll
             for (int k = 0; k < V; ++k)
-                for (int w = 1; w < WAVES; ++w) e[k] += s_a[w][lane * V + k];
+                for (int w = 1; w < WAVES; ++w) e[k] += s_e[w][lane * V + k];  // (next written two barriers on)
             put_state<V>(P.dlam_part, (int)(p.t0 / kKept), P.D, ch, e);
         }
         if (p.order == 0 && P.dinitial) empty_states<V, NT>(P.cu, P.S, P.D, ch, p.act, P.dfinal, P.dinitial);
