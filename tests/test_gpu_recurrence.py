@@ -302,3 +302,32 @@ def test_streams_and_graphs(dev):
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_two_full_cards_at_once(dev):
+    """Calls that could each fill the card, on two streams: their workgroups wait for started ones only."""
+    torch.manual_seed(8)
+    t, d = 20011, 1024
+    sets = []
+    for i in range(2):
+        c = {k: torch.randn((t, d), device=dev).to(torch.bfloat16) for k in ("x", "rg", "ig", "dy")}
+        c["lam"] = torch.randn(d, device=dev) - 4.0
+        c["cu"] = torch.tensor([0, 9000 + i, 9000 + i, t - 5 * i], dtype=torch.int32, device=dev)
+        c["h0"], c["dfinal"] = (torch.randn((3, d), device=dev) for _ in range(2))
+        sets.append(c)
+
+    def both(c):
+        y, final, carry = forward(c)
+        return [y, final, *backward(c, carry).values()]
+
+    want = [both(c) for c in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, both(sets[i])))
+    torch.cuda.synchronize()
+    for i, r in got:
+        assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
