@@ -12,8 +12,10 @@
 
 namespace nsosx {
 
-constexpr int kBalRows = 64;  // of a block of the forward pass: all of them in flight at once
+constexpr int kBalRows = 64;  // of a step of the forward pass: all of them in flight at once
+constexpr int kBalBlocks = 512;  // two a CU; more rows take more steps each (1000000 x 64: 201 us without, 76 so)
 constexpr int kBalMaxE = 512, kBalMaxK = 16;
+constexpr int64_t kBalArrivals = 64;  // more parts of the loss are added by a launch of its own
 constexpr int kBalCols = 16;  // columns of a workgroup that adds the blocks' sums
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -141,22 +143,29 @@ __device__ __forceinline__ void row_probs(const Lane<NV, V>& ln, float (&p)[NV][
 // One block of rows, a row per sixteen lanes: for each sequence in it, the sums of p and the counts, left
 // in slot block + sequence (no two pairs share one: along the rows each step raises one of them or both).
 template <int DT, int NV, int V, bool SIG>
-__global__ __launch_bounds__(1024) void balance_sums_kernel(Balance P, float* __restrict__ part,
+__global__ __launch_bounds__(1024) void balance_sums_kernel(Balance P, int steps, float* __restrict__ part,
                                                             int32_t* __restrict__ counts,
                                                             int32_t* __restrict__ tokens,
                                                             uint32_t* __restrict__ arrived) {
     __shared__ float s_sum[16][NV * 16 * V];
     __shared__ int32_t s_count[NV * 16 * V], s_tokens, s_first, s_last;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = threadIdx.x & 15;
-    const int64_t r0 = (int64_t)blockIdx.x * kBalRows, r1 = min(r0 + kBalRows, (int64_t)P.rows);
+    const int64_t r0 = (int64_t)blockIdx.x * kBalRows * steps, r1 = min(r0 + kBalRows * steps, (int64_t)P.rows);
     const Lane<NV, V> ln(l, P.E);
-    const int64_t r = r0 + (threadIdx.x >> 4), rr = min(r, r1 - 1);
-    const bool valid = r < r1 && (!P.valid || P.valid[rr]);
     float p[NV][V], rest[NV][V];
-    load_row<DT, NV, V>(P.logits, rr * P.stride, ln, p);
-    const int chosen = valid && l < P.k ? P.selected[rr * P.k + l] : -1;
+    int64_t r = 0;
+    int chosen = -1;
+    bool valid = false;
+    auto take = [&](int64_t at) {
+        r = at + (threadIdx.x >> 4);
+        const int64_t rr = min(r, r1 - 1);
+        valid = r < r1 && (!P.valid || P.valid[rr]);
+        load_row<DT, NV, V>(P.logits, rr * P.stride, ln, p);
+        chosen = valid && l < P.k ? P.selected[rr * P.k + l] : -1;
+        row_probs<NV, V, SIG, false>(ln, p, rest);
+    };
+    if (steps == 1) take(r0);
     if (blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;  // of the next launch
-    row_probs<NV, V, SIG, false>(ln, p, rest);
     int first = 0, last = 0;
     if (P.cu) {
         if (threadIdx.x == 0) s_first = P.S, s_last = -1;
@@ -175,14 +184,22 @@ __global__ __launch_bounds__(1024) void balance_sums_kernel(Balance P, float* __
         for (int e = threadIdx.x; e < P.E; e += 1024) s_count[e] = 0;
         if (threadIdx.x == 0) s_tokens = 0;
         __syncthreads();
-        const bool in = valid && r >= lo && r < hi;
-        if (in && chosen >= 0 && chosen < P.E) atomicAdd(&s_count[chosen], 1);
-        if (in && l == 0) atomicAdd(&s_tokens, 1);
+        float sums[NV][V] = {};
+        for (int64_t at = r0 + (lo - r0) / kBalRows * kBalRows; at < hi; at += kBalRows) {
+            if (steps > 1) take(at);
+            const bool in = valid && r >= lo && r < hi;
+            if (in && chosen >= 0 && chosen < P.E) atomicAdd(&s_count[chosen], 1);
+            if (in && l == 0) atomicAdd(&s_tokens, 1);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int v = 0; v < V; ++v) sums[i][v] += in ? p[i][v] : 0.0f;
+        }
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                float sum = in ? p[i][v] : 0.0f;
+                float sum = sums[i][v];
                 sum += lane_xor<16>(sum);
                 sum += lane_xor<32>(sum);
                 if (lane < 16) s_sum[wave][ln.at[i] + v] = sum;  // (what two lanes hold is the same)
@@ -201,9 +218,34 @@ __global__ __launch_bounds__(1024) void balance_sums_kernel(Balance P, float* __
     }
 }
 
+// The loss of its parts, in a fixed order, by one workgroup.
+template <int NT>
+__device__ __forceinline__ void add_loss(int64_t parts, int S, const double* loss_part, const int32_t* tokens,
+                                         float* __restrict__ loss) {
+    __shared__ double s_loss[NT];
+    __shared__ int32_t s_some[NT];
+    double f = 0.0;
+    int32_t some = 0;
+    for (int64_t i = threadIdx.x; i < parts; i += NT)
+        f += __hip_atomic_load(loss_part + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int i = threadIdx.x; i < S; i += NT)
+        some += __hip_atomic_load(tokens + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) > 0;
+    s_loss[threadIdx.x] = f;
+    s_some[threadIdx.x] = some;
+    __syncthreads();
+    for (int o = NT / 2; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) {
+            s_loss[threadIdx.x] += s_loss[threadIdx.x + o];
+            s_some[threadIdx.x] += s_some[threadIdx.x + o];
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *loss = s_some[0] ? (float)(s_loss[0] / s_some[0]) : 0.0f;
+}
+
 // kBalCols columns of a sequence: its blocks' sums, sixteen runs of them side by side.  The workgroup that
-// arrives last adds the loss's parts in their order.
-__global__ __launch_bounds__(256) void balance_finish_kernel(Balance P, const float* __restrict__ part,
+// arrives last adds the loss's parts, where `arrived` counts them.
+__global__ __launch_bounds__(256) void balance_finish_kernel(Balance P, int64_t block_rows, const float* __restrict__ part,
                                                              const int32_t* __restrict__ pcounts,
                                                              const int32_t* __restrict__ ptokens,
                                                              int32_t* __restrict__ counts, int32_t* tokens,
@@ -211,11 +253,9 @@ __global__ __launch_bounds__(256) void balance_finish_kernel(Balance P, const fl
                                                              uint32_t* arrived, float* __restrict__ loss) {
     __shared__ float s_sum[16][kBalCols];
     __shared__ int32_t s_count[16][kBalCols], s_tokens, s_last;
-    __shared__ double s_loss[256];
-    __shared__ int32_t s_some[256];
     const int s = blockIdx.y;
     const int64_t lo = P.cu ? max(0, P.cu[s]) : 0, hi = P.cu ? min(P.rows, P.cu[s + 1]) : P.rows;
-    const int64_t b0 = lo / kBalRows, b1 = hi > lo ? (hi - 1) / kBalRows + 1 : b0;
+    const int64_t b0 = lo / block_rows, b1 = hi > lo ? (hi - 1) / block_rows + 1 : b0;
     const int l = threadIdx.x % kBalCols, run = threadIdx.x / kBalCols, e = blockIdx.x * kBalCols + l;
     float sum = 0.0f;
     int32_t count = 0, n = 0;
@@ -251,31 +291,20 @@ __global__ __launch_bounds__(256) void balance_finish_kernel(Balance P, const fl
             const int64_t at = (int64_t)s * gridDim.x + blockIdx.x;
             __hip_atomic_store(loss_part + at, f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             if (blockIdx.x == 0) __hip_atomic_store(tokens + s, total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const uint32_t before =
-                __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-            s_last = before == gridDim.x * gridDim.y - 1;
+            s_last = arrived && __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
+                                    gridDim.x * gridDim.y - 1;
         }
     }
     __syncthreads();
-    if (!s_last) return;
-    double f = 0.0;
-    int32_t some = 0;
-    const int64_t parts = (int64_t)gridDim.x * gridDim.y;
-    for (int64_t i = threadIdx.x; i < parts; i += 256)
-        f += __hip_atomic_load(loss_part + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int i = threadIdx.x; i < P.S; i += 256)
-        some += __hip_atomic_load(tokens + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) > 0;
-    s_loss[threadIdx.x] = f;
-    s_some[threadIdx.x] = some;
-    __syncthreads();
-    for (int o = 128; o > 0; o >>= 1) {
-        if ((int)threadIdx.x < o) {
-            s_loss[threadIdx.x] += s_loss[threadIdx.x + o];
-            s_some[threadIdx.x] += s_some[threadIdx.x + o];
-        }
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) *loss = s_some[0] ? (float)(s_loss[0] / s_some[0]) : 0.0f;
+    if (s_last) add_loss<256>((int64_t)gridDim.x * gridDim.y, P.S, loss_part, tokens, loss);
+}
+
+// The loss's parts where they are many: 25 ns and a write-back of an L2 for each arrival cost more than a
+// launch (the forward pass of 65536 x 64 in 1500 sequences, 6000 parts: 157 us with arrivals, 31 so; 16384 x
+// 256 in one, 16 parts: 15.3 and 16.1).
+__global__ __launch_bounds__(1024) void balance_loss_kernel(int64_t parts, int S, const double* loss_part,
+                                                            const int32_t* tokens, float* __restrict__ loss) {
+    add_loss<1024>(parts, S, loss_part, tokens, loss);
 }
 
 // Nothing to add up: no row, or no sequence.
@@ -357,7 +386,9 @@ __global__ __launch_bounds__(256) void balance_bwd_kernel(Balance P, const int32
     }
 }
 
-static int64_t bal_blocks(int rows) { return ((int64_t)rows + kBalRows - 1) / kBalRows; }
+static int64_t bal_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
+static int bal_steps(int rows) { return (int)bal_ceil(bal_ceil(rows, kBalRows), kBalBlocks); }
+static int64_t bal_blocks(int rows) { return rows > 0 ? bal_ceil(rows, (int64_t)kBalRows * bal_steps(rows)) : 0; }
 
 #define NSOSX_BAL_NV(GO, DT, SIG)                 \
     do {                                          \
@@ -422,20 +453,25 @@ extern "C" int nsosx_moe_balance_loss(const void* logits, int logits_dtype, int6
                            0, st, S, experts, loss, counts, tokens, mean_prob);
         return check_launch("moe_balance_loss");
     }
+    const int steps = bal_steps(rows);
     const int64_t blocks = bal_blocks(rows), slots = blocks + S;
     const dim3 grid((experts + kBalCols - 1) / kBalCols, S);
+    const int64_t parts = (int64_t)grid.x * S;
+    const bool few = parts <= kBalArrivals;
     double* loss_part = static_cast<double*>(workspace);
-    uint32_t* arrived = reinterpret_cast<uint32_t*>(loss_part + (int64_t)grid.x * S);
+    uint32_t* arrived = reinterpret_cast<uint32_t*>(loss_part + parts);
     float* part = reinterpret_cast<float*>(arrived + 4);
     int32_t* pcounts = reinterpret_cast<int32_t*>(part + slots * experts);
     int32_t* ptokens = pcounts + slots * experts;
 #define NSOSX_BAL_GO(DT, NV, V, SIG)                                                                     \
     hipLaunchKernelGGL((balance_sums_kernel<DT, NV, V, SIG>), dim3((unsigned)blocks), dim3(1024), 0, st, p, \
-                       part, pcounts, ptokens, arrived)
+                       steps, part, pcounts, ptokens, arrived)
     NSOSX_BAL(NSOSX_BAL_GO, logits_dtype, sigmoid);
 #undef NSOSX_BAL_GO
-    hipLaunchKernelGGL(balance_finish_kernel, grid, dim3(256), 0, st, p, part, pcounts, ptokens, counts, tokens,
-                       mean_prob, loss_part, arrived, loss);
+    hipLaunchKernelGGL(balance_finish_kernel, grid, dim3(256), 0, st, p, (int64_t)kBalRows * steps, part, pcounts, ptokens,
+                       counts, tokens, mean_prob, loss_part, few ? arrived : nullptr, loss);
+    if (!few)
+        hipLaunchKernelGGL(balance_loss_kernel, dim3(1), dim3(1024), 0, st, parts, S, loss_part, tokens, loss);
     return check_launch("moe_balance_loss");
 }
 

@@ -198,3 +198,14 @@ def test_far_logits(dev, dtype, score, e):
     near(f["loss"], np.array([loss]), np.array([(rel + 4 * ref.U) * loss]), "loss")
     d = ops.moe_balance_loss_backward(t, f["counts"], f["tokens"], k, score=score)
     near(d, dx, lim + ref.HALF_STEP[dtype] * np.abs(dx) * (1 + 2.0**-7), "dlogits")
+
+
+@pytest.mark.parametrize("lens", [None, [30000, 0, 33, 100] + [1] * 200 + [39700], [10] * 6500 + [7], [70001]],
+                         ids=["batch", "mixed", "many", "one"])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("pad", [False, True])
+def test_many_rows(dev, lens, score, pad):
+    """Blocks of several steps, borders inside and between them, loss parts in the thousands."""
+    rows = 70001 if lens is None else sum(lens)
+    check(dev, rows, 20, 2, "f32", score, pad, lens)
+    check(dev, rows, 37, 3, "bf16", score, pad, lens)
