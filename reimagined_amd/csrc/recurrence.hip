@@ -146,6 +146,14 @@ __device__ __forceinline__ void empty_states(const int32_t* __restrict__ cu, int
     }
 }
 
+// The product of decays, and never 0 but for a border, however strong they are: what is not finite goes on to
+// the end of its sequence (a finite state's 1e-38th part is nothing).
+constexpr float kLeast = 1.17549435e-38f;
+
+__device__ __forceinline__ float joined(float A, float a) {
+    return A == 0.0f || a == 0.0f ? 0.0f : fmaxf(A * a, kLeast);
+}
+
 // h -> A h + H; A = 0 passes nothing on, whatever h holds (it may be another sequence's infinity)
 __device__ __forceinline__ float through(float A, float H, float h) {
     return A == 0.0f ? H : __fmaf_rn(A, h, H);
@@ -242,7 +250,7 @@ __device__ __forceinline__ float state_before(const Shared& sh, int k, int tiles
         for (int i = 0; i < kGroup; ++i) {
             const float a = i < kGroup - 1 ? pair_a(s_w[i * step]) : A;
             Hg = through(a, i < kGroup - 1 ? pair_h(s_w[i * step]) : H, Hg);
-            Ag = a == 0.0f ? 0.0f : Ag * a;
+            Ag = joined(Ag, a);
         }
         // nothing enters the first group, and nothing passes a sequence's border
         const bool whole = g == 0 || Ag == 0.0f;
@@ -393,8 +401,8 @@ __device__ __forceinline__ bool all_small(const float (&k2)[V]) {
     return __all(small);
 }
 
-// The look back over the workgroup's 64 V slots (a lane's V channels side by side), a slot a lane of the
-// first V waves: the waves' pairs (s_a, s_h) in the scan's order make the tile's, and s_c gets the state
+// The look back over the workgroup's 64 V slots (a lane's V channels side by side), a slot a lane of
+// V waves: the waves' pairs (s_a, s_h) in the scan's order make the tile's, and s_c gets the state
 // before it.
 template <int V, int WAVES, typename Shared>
 __device__ __forceinline__ void look_back(const Shared& sh, int order, int tiles, int c0, int D, bool reverse, int slot,
@@ -407,7 +415,7 @@ __device__ __forceinline__ void look_back(const Shared& sh, int order, int tiles
         const int w = reverse ? WAVES - 1 - i : i;
         const float aw = s_a[w][slot];
         H = through(aw, s_h[w][slot], H);
-        A = aw == 0.0f ? 0.0f : A * aw;
+        A = joined(A, aw);
     }
     const int part = __builtin_amdgcn_readfirstlane((c0 + slot) / 64);
     s_c[slot] = sh.ticket ? state_before(sh, order, tiles, D, part, ch, A, H, s_w + slot, 64 * V)
@@ -426,7 +434,7 @@ __device__ __forceinline__ void through_waves(const float (&s_a)[WAVES][64 * V],
         for (int k = 0; k < V; ++k) {
             const float a = s_a[w][lane * V + k];
             H[k] = through(a, s_h[w][lane * V + k], H[k]);
-            A[k] = a == 0.0f ? 0.0f : A[k] * a;
+            A[k] = joined(A[k], a);
         }
     }
 }
@@ -518,6 +526,10 @@ __global__ __launch_bounds__(64 * (kTile / R), 4) void recurrence_kernel(RecFwd 
         };
         if (plain) local(std::false_type{});
         else local(std::true_type{});
+        if (!tok.starts) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) A[k] = fmaxf(A[k], kLeast);
+        }
 #pragma unroll
         for (int k = 0; k < V; ++k) s_a[turn][wave][lane * V + k] = A[k], s_h[turn][wave][lane * V + k] = H[k];
         __syncthreads();
@@ -676,12 +688,18 @@ __global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_b
                 }
             }
         };
+        if (plain) local(std::false_type{});
+        else local(std::true_type{});
+        if (!tok.starts) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) A[k] = fmaxf(A[k], kLeast);
+        }
         if (plain) {
-            local(std::false_type{});
 #pragma unroll
             for (int k = 0; k < V; ++k) B[k] = A[k];
-        } else {
-            local(std::true_type{});
+        } else if (!tok.ends && tok.inside == (1u << R) - 1) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) B[k] = fmaxf(B[k], kLeast);
         }
 #pragma unroll
         for (int k = 0; k < V; ++k) {

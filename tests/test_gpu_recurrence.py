@@ -331,3 +331,29 @@ def test_two_full_cards_at_once(dev):
     torch.cuda.synchronize()
     for i, r in got:
         assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lam", [-5.0, 0.0, 4.0])
+def test_nan_reaches_the_end(dev, dtype, lam):
+    """What is not a number stays one to the end of its sequence (backwards: to its start), however strong
+    the decays are, in its own channel and sequence only."""
+    torch.manual_seed(9)
+    d, cu = 70, [0, 300, 5000, 5200]
+    c = {k: torch.randn((5200, d), device=dev).to(DT[dtype]) for k in ("x", "rg", "ig", "dy")}
+    c["lam"] = torch.full((d,), lam, device=dev)
+    c["cu"] = torch.tensor(cu, dtype=torch.int32, device=dev)
+    c["h0"], c["dfinal"] = (torch.randn((3, d), device=dev) for _ in range(2))
+    c["x"][310, 5] = float("nan")
+    c["dy"][4990, 7] = float("nan")
+    y, final, carry = forward(c)
+    want = torch.zeros(5200, d, dtype=torch.bool, device=dev)
+    want[310:5000, 5] = True
+    assert torch.equal(y.isnan(), want) and final.isnan().nonzero().tolist() == [[1, 5]]
+    g = backward(c, carry)
+    # (the channel of the missing x: what lies before it has a gradient; its own x has none that meets it)
+    back = torch.zeros(5200, d, dtype=torch.bool, device=dev)
+    back[300:4991, 7] = True
+    assert torch.equal(g["dx"].isnan(), back)
+    assert g["dinitial"].isnan().nonzero().tolist() == [[1, 7]]
+    assert g["dlam"].isnan().nonzero().flatten().tolist() == [5, 7]
