@@ -15,7 +15,7 @@ namespace nsosx {
 constexpr int kBalRows = 64;  // of a step of the forward pass: all of them in flight at once
 constexpr int kBalBlocks = 512;  // two a CU; more rows take more steps each (1000000 x 64: 201 us without, 76 so)
 constexpr int kBalMaxE = 512, kBalMaxK = 16;
-constexpr int64_t kBalArrivals = 64;  // more parts of the loss are added by a launch of its own
+constexpr int64_t kBalArrivals = 128;  // more parts of the loss are added by a launch of its own
 constexpr int kBalCols = 16;  // columns of a workgroup that adds the blocks' sums
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(256) void balance_finish_kernel(Balance P, int64_t 
 
 // The loss's parts where they are many: 25 ns and a write-back of an L2 for each arrival cost more than a
 // launch (the forward pass of 65536 x 64 in 1500 sequences, 6000 parts: 157 us with arrivals, 31 so; 16384 x
-// 256 in one, 16 parts: 15.3 and 16.1).
+// 256 in one, 16 parts: 15.3 and 16.1; in eight, 128 parts: 16.4 and 15.0, and 3 of host time for the launch).
 __global__ __launch_bounds__(1024) void balance_loss_kernel(int64_t parts, int S, const double* loss_part,
                                                             const int32_t* tokens, float* __restrict__ loss) {
     add_loss<1024>(parts, S, loss_part, tokens, loss);
@@ -350,10 +350,13 @@ __global__ __launch_bounds__(256) void balance_bwd_kernel(Balance P, const int32
     float g[NV][V];
     if (n > 0 && !(P.valid && !P.valid[r])) {
         float dot = 0.0f;
+        // (the p sum to 1, so a part that all counts share changes nothing but the rounding: without it the
+        // difference of a balanced router's counts and their mean keeps its bits, and is 0 where they are equal)
+        const int even = (int)((int64_t)P.k * n / P.E);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int v = 0; v < V; ++v) g[i][v] = static_cast<float>(counts[(int64_t)s * P.E + ln.at[i] + v]);
+            for (int v = 0; v < V; ++v) g[i][v] = static_cast<float>(counts[(int64_t)s * P.E + ln.at[i] + v] - even);
         row_probs<NV, V, SIG, true>(ln, p, rest);
 #pragma unroll
         for (int i = 0; i < NV; ++i)

@@ -209,3 +209,32 @@ def test_many_rows(dev, lens, score, pad):
     rows = 70001 if lens is None else sum(lens)
     check(dev, rows, 20, 2, "f32", score, pad, lens)
     check(dev, rows, 37, 3, "bf16", score, pad, lens)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("e,k", [(4, 4), (7, 7), (48, 3)])
+def test_balanced(dev, dtype, score, e, k):
+    """Experts that all have the same load: the gradient is 0, not what rounding leaves of it; and one choice
+    more of one of them shows with all of its bits."""
+    rows = 48 * 20
+    x = torch.randn((rows, e), device=dev, generator=torch.Generator(dev).manual_seed(e)).to(DT[dtype])
+    sel = torch.stack([(torch.arange(rows, device=dev) + i * (e // k)) % e for i in range(k)], 1).int()
+    rows = rows if k < e else 7
+    x, sel = x[:rows], sel[:rows].contiguous()
+    f = ops.moe_balance_loss(x, sel, score=score)
+    assert (f["counts"] == rows * k // e).all()
+    back = lambda counts: ops.moe_balance_loss_backward(x, counts, f["tokens"], k, score=score)
+    assert not back(f["counts"]).any()
+    counts = f["counts"].clone()
+    counts[0, 1] += 1
+    xd = x.double()
+    p = torch.softmax(xd, 1) if score == "softmax" else torch.sigmoid(xd) / torch.sigmoid(xd).sum(1, keepdim=True)
+    one = torch.zeros(e, device=dev, dtype=torch.float64)
+    one[1] = 1.0
+    want = e / (k * float(rows) ** 2) * p * (one - p[:, 1:2])
+    if score == "sigmoid":
+        want = want * torch.sigmoid(-xd)
+    # a probability is off by 2 U a unit of the exponent (10 at most here) and 80 U, twice; twelve roundings
+    lim = e / (k * float(rows) ** 2) * p * (one + p[:, 1:2]) * (2 * (2 * 10 + 80) + 12) * ref.U
+    near(back(counts), want.cpu().numpy(), (lim + ref.HALF_STEP[dtype] * want.abs() * (1 + 2.0**-7)).cpu().numpy(), "dlogits")
