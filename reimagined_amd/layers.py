@@ -56,19 +56,32 @@ class BitLinear:
         """The prefill GEMM's copy of the weights (MFMA layout), when K % 128 == 0."""
         return ops.pack_mfma_layout(self.packed) if self.in_features % 128 == 0 else None
 
-    def gemm(self, q, s, m, y, st, magnitude=None, bias=None):
+    def load(self, w_float: np.ndarray) -> None:
+        """Other weights of the same shape, into the same device words: what holds them (a captured
+        call) reads the new ones."""
+        w_float = np.ascontiguousarray(w_float, dtype=np.float32)
+        if w_float.shape != (self.out_features, self.in_features):
+            raise ValueError(f"BitLinear: weights must be [{self.out_features}, {self.in_features}], "
+                             f"got {w_float.shape}")
+        packed, self.weight_scale = ops.pack_ternary(w_float)
+        self.packed.copy_(torch.from_numpy(packed.view(np.int32)))
+        if self.packed_mfma is not None:
+            self.packed_mfma.copy_(self._mfma_layout())
+
+    def gemm(self, q, s, m, y, st, magnitude=None, bias=None, weight_scale=None):
         """The ternary GEMM of m rows of codes into y: on the MFMA-layout words the MFMA GEMMs
         above 8 rows and at the skinny decode kernel's shapes, else the dispatching entry on
         the reference words (GEMV / small-M MFMA kernels; up to 128 rows also of a K past the
-        MFMA layout's sums)."""
+        MFMA layout's sums).  weight_scale: another one than the weights' own (1 where s holds it
+        already)."""
+        scale = self.weight_scale if weight_scale is None else weight_scale
         few = 8 if self.in_features <= ops.MFMA_LAYOUT_MAX_K else 128
         if self.packed_mfma is not None and (m > few or ops.skinny_shape(m, self.in_features,
                                                                           self.out_features)):
-            call("nsosx_ternary_gemm_mfma", _p(q), _p(s), _p(self.packed_mfma),
-                 self.weight_scale, m, self.in_features, self.out_features, _p(magnitude),
+            call("nsosx_ternary_gemm_mfma", _p(q), _p(s), _p(self.packed_mfma), scale, m, self.in_features, self.out_features, _p(magnitude),
                  _p(bias), _p(y), _DT[y.dtype], None, st)
         else:
-            call("nsosx_ternary_gemm", _p(q), _p(s), _p(self.packed), self.weight_scale, m,
+            call("nsosx_ternary_gemm", _p(q), _p(s), _p(self.packed), scale, m,
                  self.in_features, self.out_features, _p(magnitude), _p(bias), _p(y),
                  _DT[y.dtype], None, st)
 
@@ -446,8 +459,9 @@ class RecurrentLayer:
     optional b_in [3 inner], norm_w and norm_b [d_model], rate (8) and eps (1e-5).  d_model and inner
     are multiples of 16 (the packed words).  The latent weights w_in and w_out stay on the device in f32: the
     gradients are theirs (straight through the ternary and the int8 rounding), and repack() forms the
-    ternary ones again after an update.  Activations run in x's type.  Nothing is kept between calls
-    but the weights."""
+    ternary ones again after an update.  All of them are updated in place: captured calls hold their
+    addresses, and a replay after repack() runs on the new ones.  Activations run in x's type.  Nothing is
+    kept between calls but the weights."""
 
     def __init__(self, params: dict, device="cuda"):
         f32 = dict(dtype=torch.float32, device=device)
@@ -463,12 +477,17 @@ class RecurrentLayer:
         if self.b_in is not None and self.b_in.numel() != 3 * self.inner:
             raise ValueError("RecurrentLayer: b_in must be [3 inner]")
         self.device = device
-        self.repack()
+        linear = lambda w, b: BitLinear(w.cpu().numpy(), device, rms_input=False, bias=b)
+        self.in_proj, self.out_proj = linear(self.w_in, self.b_in), linear(self.w_out, None)
+        # their scales, as captured calls read them
+        self.in_scale, self.out_scale = (torch.full((1,), p.weight_scale, **f32) for p in (self.in_proj, self.out_proj))
 
     def repack(self) -> None:
-        """The ternary weights of the latent ones as they are now (through the host)."""
-        linear = lambda w, b: BitLinear(w.cpu().numpy(), self.device, rms_input=False, bias=b)
-        self.in_proj, self.out_proj = linear(self.w_in, self.b_in), linear(self.w_out, None)
+        """The ternary weights of the latent ones as they are now, into the words that are there: captured
+        calls have them from their next replay on.  Packed on the host, so not for a capture."""
+        for linear, scale, w in ((self.in_proj, self.in_scale, self.w_in), (self.out_proj, self.out_scale, self.w_out)):
+            linear.load(w.cpu().numpy())
+            scale.fill_(linear.weight_scale)
 
     def _norm(self, x, delta, want_stats: bool):
         """-> r, f and with want_stats the norm's mean and rstd."""
@@ -477,14 +496,31 @@ class RecurrentLayer:
             return (x, *f) if want_stats else (x, f)
         return ops.add_layernorm(x, delta, self.norm_w, self.norm_b, eps=self.eps, want_stats=want_stats)
 
+    # The kernels take the ternary weights' scale as an argument, which a captured call would keep: there it
+    # comes from the device instead, in a launch of its own on the one factor and 1 as the other: the same bits.
+
     @staticmethod
-    def _project(linear: BitLinear, x: torch.Tensor):
+    def _project(linear: BitLinear, scale: torch.Tensor, x: torch.Tensor):
         """-> x's product, and the codes and scales that it was formed from."""
         m = x.shape[0]
         y = x.new_empty((m, linear.out_features))
         q, s = ops.quantize_activations_bitnet(x, rms_input=False)
-        linear.gemm(q, s, m, y, _stream(), linear.magnitude, linear.bias)
+        if torch.cuda.is_current_stream_capturing():
+            linear.gemm(q, s * scale, m, y, _stream(), linear.magnitude, linear.bias, 1.0)
+        else:
+            linear.gemm(q, s, m, y, _stream(), linear.magnitude, linear.bias)
         return y, q, s
+
+    @staticmethod
+    def _project_backward(linear: BitLinear, scale: torch.Tensor, w: torch.Tensor, q, s, grad, want_dbias=False) -> dict:
+        if not torch.cuda.is_current_stream_capturing():
+            return ops.bitlinear_ste_backward(None, q, s, w, linear.packed, linear.weight_scale, grad, rms_input=False,
+                                              want_dbias=want_dbias)
+        # (the clip divides by scale + 1e-8 in f32, which is 1 for a scale of 1)
+        g = ops.bitlinear_ste_backward(None, q, s, w / (scale + 1e-8), linear.packed, 1.0, grad, rms_input=False,
+                                       want_dbias=want_dbias)
+        g["dx"].mul_(scale)
+        return g
 
     def _split(self, p: torch.Tensor):
         return p[:, :self.inner], p[:, self.inner:2 * self.inner], p[:, 2 * self.inner:]
@@ -494,10 +530,10 @@ class RecurrentLayer:
         """x (and delta) [T, d_model] f32 or bf16 over the packed batch -> {"residual", "out",
         "final_state" f32 [S, inner]}; with train what backward() takes as well."""
         r, f, *stats = self._norm(x, delta, train)
-        p, fq, fs = self._project(self.in_proj, f)
+        p, fq, fs = self._project(self.in_proj, self.in_scale, f)
         y, final, *carry = ops.gated_recurrence(*self._split(p), self.lam, cu_seqlens, rate=self.rate,
                                                 initial_state=initial_state, want_carry=train)
-        out, yq, ys = self._project(self.out_proj, y)
+        out, yq, ys = self._project(self.out_proj, self.out_scale, y)
         fwd = {"residual": r, "out": out, "final_state": final}
         if train:
             fwd.update(f=f, mean=stats[0], rstd=stats[1], p=p, fq=fq, fs=fs, y=y, yq=yq, ys=ys, carry=carry[0],
@@ -512,16 +548,14 @@ class RecurrentLayer:
         if "carry" not in fwd:
             raise ValueError("RecurrentLayer: backward() needs what forward(train=True) gave")
         p, r = fwd["p"], fwd["residual"]
-        o = ops.bitlinear_ste_backward(None, fwd["yq"], fwd["ys"], self.w_out, self.out_proj.packed,
-                                       self.out_proj.weight_scale, dout.float(), rms_input=False)
+        o = self._project_backward(self.out_proj, self.out_scale, self.w_out, fwd["yq"], fwd["ys"], dout.float())
         dy = o["dx"].to(p.dtype)
         dp = torch.empty_like(p)
         g = ops.gated_recurrence_backward(dy, *self._split(p), self.lam, fwd["cu_seqlens"], fwd["carry"],
                                           rate=self.rate, initial_state=fwd["initial_state"], dfinal=dfinal,
                                           out=self._split(dp), zero_rest=True)
-        i = ops.bitlinear_ste_backward(None, fwd["fq"], fwd["fs"], self.w_in, self.in_proj.packed,
-                                       self.in_proj.weight_scale, dp.float(), rms_input=False,
-                                       want_dbias=self.b_in is not None)
+        i = self._project_backward(self.in_proj, self.in_scale, self.w_in, fwd["fq"], fwd["fs"], dp.float(),
+                                   self.b_in is not None)
         n = ops.layernorm_backward(i["dx"], r, fwd["mean"], fwd["rstd"], self.norm_w, dresidual=dresidual)
         grads = {"dx": n["dx"], "dw_in": i["dW"], "dw_out": o["dW"], "dlam": g["dlam"], "dnorm_w": n["dweight"],
                  "dnorm_b": n["dbias"], "dy": dy, "dp": dp}
@@ -538,9 +572,9 @@ class RecurrentLayer:
         """One token per row, x (and delta) [R, d_model]; state f32 [R, inner] is updated in place.
         -> (residual, out)."""
         r, f = self._norm(x, delta, False)
-        p, _, _ = self._project(self.in_proj, f)
+        p, _, _ = self._project(self.in_proj, self.in_scale, f)
         y = ops.gated_recurrence_step(*self._split(p), self.lam, state, rate=self.rate)
-        return r, self._project(self.out_proj, y)[0]
+        return r, self._project(self.out_proj, self.out_scale, y)[0]
 
 
 class HybridBlock:
