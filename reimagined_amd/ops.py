@@ -874,14 +874,13 @@ def moe_balance_loss(logits: torch.Tensor, selected: torch.Tensor, score: str = 
     mask = valid_rows_mask(valid_rows, rows, logits.device)
     _on(fn, dev, ("selected", selected, torch.int32, None), ("valid_rows", mask, torch.uint8, None))
     s = _segments(fn, cu_seqlens, dev)
-    # (the workspace in front: its sums of 64 bits are aligned)
-    ws = (int(lib().nsosx_moe_balance_loss_workspace(rows, e, s)) + 7) // 8 * 2
-    buf = torch.empty(ws + 1 + 2 * s * e + s, dtype=torch.float32, device=logits.device)
-    ws, loss, mean, counts, tokens = buf.split_with_sizes((ws, 1, s * e, s * e, s))
-    counts, tokens = counts.view(torch.int32).view(s, e), tokens.view(torch.int32)
+    # (tensors of their own: a loss that is kept keeps nothing else, no workspace above all)
+    loss = logits.new_empty(1, dtype=torch.float32)
+    mean, counts, tokens = loss.new_empty((s, e)), selected.new_empty((s, e)), selected.new_empty(s)
+    ws = selected.new_empty((lib().nsosx_moe_balance_loss_workspace(rows, e, s) + 3) // 4)
     call("nsosx_moe_balance_loss", _p(logits), _dt(logits), stride, _p(selected), _p(mask), rows, e, k,
          sig, _p(cu_seqlens), s, _p(loss), _p(counts), _p(tokens), _p(mean), _p(ws), _stream_on(dev))
-    return {"loss": loss, "counts": counts, "tokens": tokens, "mean_prob": mean.view(s, e)}
+    return {"loss": loss, "counts": counts, "tokens": tokens, "mean_prob": mean}
 
 
 def moe_balance_loss_backward(logits: torch.Tensor, counts: torch.Tensor, tokens: torch.Tensor, k: int,
@@ -1133,8 +1132,9 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rs
     dx = torch.empty_like(x)
     dw = db = ws = None
     if want_params:
-        n = int(lib().nsosx_layernorm_backward_workspace(rows, dim)) // 4
-        dw, db, ws = x.new_empty(2 * dim + n, dtype=torch.float32).split_with_sizes((dim, dim, n))
+        # (f32 tensors of their own: a gradient that is kept keeps no partial sums)
+        dw, db = mean.new_empty(dim), mean.new_empty(dim)
+        ws = mean.new_empty(lib().nsosx_layernorm_backward_workspace(rows, dim) // 4)
     call("nsosx_layernorm_backward", _p(dy), _dt(dy), _p(x), _p(mean), _p(rstd), _p(weight),
          _p(dresidual), rows, dim, _dt(x), _p(dx), _p(dw), _p(db), _p(ws), _stream_on(dev))
     return {"dx": dx, "dweight": dw, "dbias": db} if want_params else {"dx": dx}
