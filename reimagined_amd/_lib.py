@@ -106,6 +106,7 @@ SIGNATURES = {
     "nsosx_layernorm_backward": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp,
                                       _vp, _vp]),
     "nsosx_gated_recurrence_tile": (_i, []),
+    "nsosx_gated_recurrence_looks": (_i, [_i]),
     "nsosx_gated_recurrence_workspace": (_i64, [_i, _i]),
     "nsosx_gated_recurrence": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _f, _vp, _i, _i, _i, _i,
                                     _vp, _i, _vp, _i64, _vp, _vp, _vp, _vp]),

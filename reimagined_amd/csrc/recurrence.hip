@@ -13,6 +13,7 @@
 // from the forward's states before every kKept-th token (f32), so y is not read.
 #include "train.hpp"
 
+#include <atomic>
 #include <type_traits>
 
 namespace nsosx {
@@ -172,16 +173,20 @@ __device__ __forceinline__ float through(float A, float H, float h) {
 // everything else.  The flags are hints, the words' own tags decide.
 // Every wait ends: workgroups take their tiles by a ticket, in the order of the scan, and leave a tile's
 // pair before they wait for another's, so whoever waits waits for tiles that a started workgroup has
-// left or will leave without waiting for a later one.
+// left or will leave without waiting for a later one.  One that has looked kLooks times all the same
+// gives up: it takes what it has not seen for NaN, also in the words that it leaves, so what a later tile
+// makes of them is right or NaN.
 constexpr uint32_t kWhole = 1;
-constexpr int kGroup = 4;           // tiles
-constexpr int kMaxPolls = 1 << 22;  // seconds; then the state is NaN and the kernel ends
+constexpr int kGroup = 4;        // tiles
+constexpr int kLooks = 1 << 22;  // seconds
+constexpr uint64_t kLost = 0xbf8000007fc00000ull;  // the pair (1, NaN)
 
 struct RecShared {
     uint32_t* ticket;           // NULL where there is one tile in time: no tile waits for another
     uint64_t *words, *groups;   // [tiles, D], [groups, D]
     uint32_t *flags, *gflags;   // [D / 64 up, tiles], [D / 64 up, groups]
     float* k2;                  // [D]: the channels' decay rates, formed once
+    int spent;                  // looks that a tile starts with (kLooks: it waits for nothing)
 };
 
 __device__ __forceinline__ void leave(uint64_t* word, uint32_t tag, float v) {
@@ -219,13 +224,12 @@ __device__ __forceinline__ float state_before(const Shared& sh, int k, int tiles
     uint64_t* behind = sh.groups + g * D + ch;
     leave(sh.words + k * D + ch, __float_as_uint(A) | 0x80000000u, H);
     raise_flag(flags + k, 1);
-    int polls = 0;
+    int polls = sh.spent;
     if (pos > 0) {  // the pairs of the tiles before this one in its group
         const uint64_t* row = sh.words + (int64_t)g * kGroup * D;
-        bool all = false;
 #pragma unroll 1
-        while (!all && polls <= kMaxPolls) {
-            while (!__all(see_flag(flags + g * kGroup + min(lane, pos - 1)) != 0) && ++polls <= kMaxPolls)
+        for (bool all = false; !all && polls <= kLooks;) {
+            while (!__all(see_flag(flags + g * kGroup + min(lane, pos - 1)) != 0) && ++polls <= kLooks)
                 __builtin_amdgcn_s_sleep(4);
             uint64_t w[kGroup - 1];
             uint32_t at = ch * 8;
@@ -238,7 +242,7 @@ __device__ __forceinline__ float state_before(const Shared& sh, int k, int tiles
             for (int i = 0; i < kGroup - 1; ++i)
                 if (i < pos) {
                     all = all & (tag_of(w[i]) != 0);
-                    s_w[i * step] = w[i];
+                    s_w[i * step] = tag_of(w[i]) != 0 ? w[i] : kLost;
                 }
             all = __all(all);
             ++polls;
@@ -260,14 +264,14 @@ __device__ __forceinline__ float state_before(const Shared& sh, int k, int tiles
     if (g > 0) {
         bool all = false;
 #pragma unroll 1
-        while (!all && polls <= kMaxPolls) {
+        while (!all && polls <= kLooks) {
             int far;  // the nearest group whose state is known, with pairs of all groups between
             for (;; __builtin_amdgcn_s_sleep(4)) {
                 const uint32_t f = lane < g ? see_flag(gflags + g - 1 - lane) : 0;
                 const uint64_t whole = __ballot(f == 2), some = __ballot(f != 0);
                 far = whole ? __builtin_ctzll(whole) : 64;
                 const uint64_t between = far < 64 ? (1ull << far) - 1 : ~0ull;
-                if ((far < 64 && (some & between) == between) || ++polls > kMaxPolls) break;
+                if ((far < 64 && (some & between) == between) || ++polls > kLooks) break;
             }
             // (a word may say less than its flag, for a moment, or more: any P on the way is as good)
             all = far < 64;
@@ -290,13 +294,14 @@ __device__ __forceinline__ float state_before(const Shared& sh, int k, int tiles
             all = __all(known) && all;
             ++polls;
         }
+        if (!all) c = __builtin_nanf("");
         if (pos == kGroup - 1) {
             if (Ag != 0.0f) leave(behind, kWhole, __fmaf_rn(Ag, c, Hg));
             raise_flag(gflags + g, 2);
         }
     }
     for (int i = 0; i < pos; ++i) c = through(pair_a(s_w[i * step]), pair_h(s_w[i * step]), c);
-    return polls > kMaxPolls ? __builtin_nanf("") : c;
+    return c;
 }
 
 // Words and flags to 0, the decay rates: 2.5 us, most of it the launch.
@@ -876,6 +881,8 @@ static const char* rec_check(int S, int64_t T, int D, int dtype, float rate) {
     return nullptr;
 }
 
+static std::atomic<int> g_looks{kLooks};
+
 // What the tiles share, in the workspace: ticket (16 bytes), words, flags, decay rates; nothing for one
 // tile in time.
 static RecShared rec_shared(int64_t tiles, int D, void* workspace, int64_t* clear, int64_t* bytes) {
@@ -896,6 +903,7 @@ static RecShared rec_shared(int64_t tiles, int D, void* workspace, int64_t* clea
     n = (n + parts * groups * 4 + 15) / 16 * 16;
     *clear = n / 16;
     s.k2 = reinterpret_cast<float*>(at + n);
+    s.spent = kLooks - g_looks.load(std::memory_order_relaxed);
     *bytes = n + ((int64_t)D * 4 + 15) / 16 * 16;
     return s;
 }
@@ -956,6 +964,11 @@ static void launch_empty(const float* from, int64_t n, float* to, hipStream_t st
 using namespace nsosx;
 
 extern "C" int nsosx_gated_recurrence_tile(void) { return kKept; }
+
+extern "C" int nsosx_gated_recurrence_looks(int looks) {
+    if (looks < 0) return g_looks.load(std::memory_order_relaxed);
+    return g_looks.exchange(looks < kLooks ? looks : kLooks, std::memory_order_relaxed);
+}
 
 extern "C" int64_t nsosx_gated_recurrence_workspace(int T, int D) {
     if (T <= 0 || D <= 0) return 0;
