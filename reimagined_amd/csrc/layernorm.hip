@@ -362,26 +362,31 @@ __global__ __launch_bounds__(256) void layernorm_cols_kernel(
 }
 
 // out0[c], out1[c] = the sums over n rows of part[0], part[1] (a NULL out is skipped), in a fixed order.
-// 16 columns a workgroup (64 B of a row), a row of partial sums per 16 lanes: enough workgroups for
+// 16 columns a workgroup (64 B of a row) at a time, a row of partial sums per 16 lanes: enough workgroups for
 // every load to be on its way at once.  Each thread adds its rows in order, the threads as a tree.
+constexpr int kLnSumWorkgroups = 1 << 16;  // past a million columns each takes several sixteens: a launch ends at 2^32 threads
+
 __global__ __launch_bounds__(1024) void column_sums_kernel(const float* __restrict__ part, int n,
                                                            int cols, float* out0, float* out1) {
     float* out = blockIdx.y ? out1 : out0;
     if (!out) return;
     __shared__ float s[16][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 16 + (lane & 15);
-    const float* p = part + (int64_t)blockIdx.y * n * cols + min(c, (int64_t)cols - 1);
-    float sum = 0.0f;
+    for (int64_t c0 = (int64_t)blockIdx.x * 16; c0 < cols; c0 += (int64_t)gridDim.x * 16) {
+        const int64_t c = c0 + (lane & 15);
+        const float* p = part + (int64_t)blockIdx.y * n * cols + min(c, (int64_t)cols - 1);
+        float sum = 0.0f;
 #pragma unroll 8
-    for (int r = threadIdx.x >> 4; r < n; r += 64) sum += p[(int64_t)r * cols];
-    sum += lane_xor<16>(sum);
-    sum += lane_xor<32>(sum);
-    if (lane < 16) s[wave][lane] = sum;
-    __syncthreads();
-    if (threadIdx.x < 16 && c < cols) {
-        for (int w = 1; w < 16; ++w) sum += s[w][lane];
-        out[c] = sum;
+        for (int r = threadIdx.x >> 4; r < n; r += 64) sum += p[(int64_t)r * cols];
+        sum += lane_xor<16>(sum);
+        sum += lane_xor<32>(sum);
+        if (lane < 16) s[wave][lane] = sum;
+        __syncthreads();
+        if (threadIdx.x < 16 && c < cols) {
+            for (int w = 1; w < 16; ++w) sum += s[w][lane];
+            out[c] = sum;
+        }
+        __syncthreads();
     }
 }
 
@@ -577,8 +582,10 @@ extern "C" int nsosx_layernorm_backward(const void* dy, int dy_dtype, const void
         }
     }
 #undef NSOSX_LN_GO
-    if (cols)
-        hipLaunchKernelGGL(column_sums_kernel, dim3((dim + 15) / 16, 2), dim3(1024), 0, st, part,
-                           ln_bwd_workgroups(rows, dim), dim, dweight, dbias);
+    if (cols) {
+        const int wgs = (dim - 1) / 16 + 1;
+        hipLaunchKernelGGL(column_sums_kernel, dim3(wgs < kLnSumWorkgroups ? wgs : kLnSumWorkgroups, 2), dim3(1024), 0, st,
+                           part, ln_bwd_workgroups(rows, dim), dim, dweight, dbias);
+    }
     return check_launch("layernorm_backward");
 }
