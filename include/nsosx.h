@@ -757,8 +757,10 @@ int nsosx_conv_step(const void* x, int x_dtype, int64_t x_stride, int rows, int 
  * is its initial state).  Rows of no sequence (before cu_seqlens[0], past cu_seqlens[S]) are left as
  * they were, or with zero_rest != 0 written as zeros.  carry f32 [ceil(T / tile), D] or NULL: the states between
  * tiles of nsosx_gated_recurrence_tile() tokens, which the gradients start from.  The state is f32
- * throughout; the same inputs give the same bits.  workspace: device, 16-byte aligned,
- * nsosx_gated_recurrence_workspace bytes, one for each call that may run at the same time.
+ * throughout; the same inputs give the same bits.  A token's decay below 2^-126 counts as 0, and where those
+ * of several tokens multiply to less, what is left of a state is off by up to its 2^-143rd part.
+ * workspace: device, 16-byte aligned, nsosx_gated_recurrence_workspace bytes, one for each call that may run at
+ * the same time.
  * nsosx_gated_recurrence_looks() sets how often (of launches from then on, in the whole process) a tile looks
  * for the state that the tiles before it leave, until it goes on without: 2^22 times at the start and at most,
  * some seconds, which only a held up GPU takes.  Values that would need a state not seen are NaN then, never

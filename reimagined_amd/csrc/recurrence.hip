@@ -148,8 +148,9 @@ __device__ __forceinline__ void empty_states(const int32_t* __restrict__ cu, int
 }
 
 // The product of decays, and never 0 but for a border, however strong they are: what is not finite goes on to
-// the end of its sequence (a finite state's 1e-38th part is nothing).
-constexpr float kLeast = 1.17549435e-38f;
+// the end of its sequence.  The least is 2^-149: products below 2^-126 keep the bits that they can, and of a
+// finite state its 2^-149th part, 5e-7 at most, is what goes on too far.
+constexpr float kLeast = 1.40129846e-45f;
 
 __device__ __forceinline__ float joined(float A, float a) {
     return A == 0.0f || a == 0.0f ? 0.0f : fmaxf(A * a, kLeast);
