@@ -751,8 +751,16 @@ def _stream_on(dev: int):
     return _stream() if _raw_stream is None else _raw_stream(dev)
 
 
+def _counts(fn: str, name: str, rows: int, cols: int = 0) -> None:
+    """Refuses what the C entries' int cannot hold (ctypes would pass its lowest 32 bits)."""
+    if (rows | cols) >> 31:
+        raise ValueError(f"{fn}: {name} must have less than 2^31 rows and columns, got {rows} x {cols}")
+
+
 def _logit_rows(fn: str, logits: torch.Tensor) -> int:
     """Checks router logits [rows, E] (a column slice of a wider tensor is fine); row stride."""
+    if logits.dim() == 2:
+        _counts(fn, "logits", *logits.shape)
     if not logits.is_cuda:
         raise ValueError("logits must be a device tensor")
     if logits.dim() != 2 or 0 in logits.shape:
@@ -840,6 +848,7 @@ def _sequences(fn: str, cu_seqlens) -> int:
     shape = () if cu_seqlens is None else cu_seqlens.shape
     if len(shape) != 1 or shape[0] < 1:
         raise ValueError(f"{fn}: cu_seqlens must be [sequences + 1], got {tuple(shape)}")
+    _counts(fn, "cu_seqlens", shape[0])
     return shape[0] - 1
 
 
@@ -1072,6 +1081,7 @@ def add_rmsnorm(x: torch.Tensor, delta: torch.Tensor, gamma=None, eps: float = 1
 def _norm_rows(fn: str, x: torch.Tensor, name: str = "x") -> tuple:
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"{fn}: {name} must be [rows, dim], got {tuple(x.shape)}")
+    _counts(fn, name, *x.shape)
     _dt(x)
     return x.shape
 
@@ -1164,6 +1174,7 @@ def _rec_inputs(fn: str, x, rg, ig, lam, *more) -> tuple:
     """Checks the recurrence's inputs and `more` as _on takes it; device, type and row strides."""
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"{fn}: x must be [tokens, dim], got {tuple(x.shape)}")
+    _counts(fn, "x", *x.shape)
     dt = _dt(x)
     if not x.is_cuda:
         raise ValueError("x must be a device tensor")
