@@ -754,7 +754,7 @@ int nsosx_conv_step(const void* x, int x_dtype, int64_t x_stride, int rows, int 
  * fine) of at most 2^22; lam f32 [D]; cu_seqlens int32 [S + 1], not decreasing, within [0, T], empty
  * sequences allowed.
  * initial_state f32 [S, D] or NULL (zeros); final_state f32 [S, D] or NULL (an empty sequence's
- * is its initial state).  Rows of no sequence (before cu_seqlens[0], past cu_seqlens[S]) are left as
+ * is its initial state).  y must not overlap an input.  Rows of no sequence (before cu_seqlens[0], past cu_seqlens[S]) are left as
  * they were, or with zero_rest != 0 written as zeros.  carry f32 [ceil(T / tile), D] or NULL: the states between
  * tiles of nsosx_gated_recurrence_tile() tokens, which the gradients start from.  The state is f32
  * throughout; the same inputs give the same bits.  A token's decay below 2^-126 counts as 0, and where those
@@ -792,8 +792,8 @@ int nsosx_gated_recurrence_backward(const void* dy, int64_t dy_stride, const voi
                                     void* workspace, void* stream);
 
 /* One token per row: state_out = a state + sqrt(1 - a^2) sigmoid(ig) x, y = state_out rounded to
- * act_dtype.  state, state_out f32 [rows, D] (the same buffer for an update in place); the rest as
- * above with rows in place of T, at most 262140. */
+ * act_dtype.  state, state_out f32 [rows, D] (the same buffer for an update in place; they must not
+ * cross the views); the rest as above with rows in place of T, at most 262140. */
 int nsosx_gated_recurrence_step(const void* x, int64_t x_stride, const void* rg,
                                 int64_t rg_stride, const void* ig, int64_t ig_stride,
                                 const float* lam, float rate, int rows, int D, int act_dtype,

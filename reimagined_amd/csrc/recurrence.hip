@@ -875,6 +875,16 @@ static bool views_cross(const void* a, int64_t as, const void* b, int64_t bs, in
     return off < D * size || off + D * size > row;
 }
 
+// Whether a block of n bytes (states, rates) and a view's rows share an element.
+static bool block_meets(const void* b, int64_t n, const void* v, int64_t vs, int64_t rows, int64_t D, int64_t size) {
+    if (!b || !v || rows <= 0 || n <= 0 || !overlaps(b, n, v, ((rows - 1) * vs + D) * size)) return false;
+    if (rows == 1) return true;
+    const int64_t row = vs * size;
+    int64_t off = (static_cast<const char*>(b) - static_cast<const char*>(v)) % row;
+    if (off < 0) off += row;
+    return off < D * size || off + n > row;
+}
+
 static const char* rec_check(int S, int64_t T, int D, int dtype, float rate) {
     if (S < 0 || T < 0 || D <= 0) return "need sequences >= 0, tokens >= 0 and dim > 0";
     if (!valid_dtype(dtype)) return "bad dtype";
@@ -1010,6 +1020,8 @@ extern "C" int nsosx_gated_recurrence(const void* x, int64_t x_stride, const voi
         return fail(NSOSX_ERR_INVALID, "gated_recurrence: y overlaps an input");
     if (final_state && initial_state && overlaps(final_state, sd * 4, initial_state, sd * 4))
         return fail(NSOSX_ERR_INVALID, "gated_recurrence: final_state overlaps initial_state");
+    if (block_meets(initial_state, sd * 4, y, y_stride, T, D, size) || block_meets(lam, (int64_t)D * 4, y, y_stride, T, D, size))
+        return fail(NSOSX_ERR_INVALID, "gated_recurrence: y overlaps an input");
     RecFwd p{x, rg, ig, x_stride, rg_stride, ig_stride, lam, rate, cu_seqlens, S, T, D, zero_rest,
              initial_state, y, y_stride, final_state, carry,
              start_shared(rec_tiles(T, kTile), D, lam, rate, workspace, st)};
@@ -1066,6 +1078,11 @@ extern "C" int nsosx_gated_recurrence_backward(
         for (int i = 0; i < 4; ++i)
             if (views_cross(out[o], out_s[o], in[i], in_s[i], T, D, size))
                 return fail(NSOSX_ERR_INVALID, "gated_recurrence_backward: a gradient overlaps an input");
+        if (block_meets(initial_state, sd * 4, out[o], out_s[o], T, D, size) ||
+            block_meets(dfinal, sd * 4, out[o], out_s[o], T, D, size) ||
+            block_meets(carry, rec_tiles(T, kKept) * D * 4, out[o], out_s[o], T, D, size) ||
+            block_meets(lam, (int64_t)D * 4, out[o], out_s[o], T, D, size))
+            return fail(NSOSX_ERR_INVALID, "gated_recurrence_backward: a gradient overlaps an input");
         for (int i = 0; i < o; ++i)
             if (views_cross(out[o], out_s[o], out[i], out_s[i], T, D, size))
                 return fail(NSOSX_ERR_INVALID, "gated_recurrence_backward: the gradients overlap");
@@ -1107,6 +1124,16 @@ extern "C" int nsosx_gated_recurrence_step(const void* x, int64_t x_stride, cons
         views_cross(y, y_stride, rg, rg_stride, rows, D, size) ||
         views_cross(y, y_stride, ig, ig_stride, rows, D, size))
         return fail(NSOSX_ERR_INVALID, "gated_recurrence_step: y overlaps an input");
+    // (element for element the states may lie over f32 views: a thread reads its own before it writes it)
+    const void* seen[4] = {x, rg, ig, y};
+    const int64_t seen_s[4] = {x_stride, rg_stride, ig_stride, y_stride};
+    for (int i = 0; i < 4; ++i) {
+        const bool dense = size == 4 && (rows == 1 || seen_s[i] == D);
+        if (!(dense && seen[i] == state_out) && block_meets(state_out, n, seen[i], seen_s[i], rows, D, size))
+            return fail(NSOSX_ERR_INVALID, "gated_recurrence_step: state_out overlaps an input or y");
+    }
+    if (!(size == 4 && (rows == 1 || y_stride == D) && y == state) && block_meets(state, n, y, y_stride, rows, D, size))
+        return fail(NSOSX_ERR_INVALID, "gated_recurrence_step: y overlaps state");
     const int64_t gx = (D - 1) / 256 + 1, gy = ((int64_t)rows + kStepRows - 1) / kStepRows;
     if (D > kRecMaxStride || gy > 65535 || gx * gy > 0xffffffffLL / 256)
         return fail(NSOSX_ERR_OVERFLOW, "gated_recurrence_step: rows or dim too large");
