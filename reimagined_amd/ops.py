@@ -751,22 +751,22 @@ def _stream_on(dev: int):
     return _stream() if _raw_stream is None else _raw_stream(dev)
 
 
-def _counts(fn: str, name: str, rows: int, cols: int = 0) -> None:
-    """Refuses what the C entries' int cannot hold (ctypes would pass its lowest 32 bits)."""
-    if (rows | cols) >> 31:
-        raise ValueError(f"{fn}: {name} must have less than 2^31 rows and columns, got {rows} x {cols}")
+def _too_many(fn: str, name: str, shape) -> ValueError:
+    """For sizes that the C entries' int cannot hold (ctypes would pass their lowest 32 bits)."""
+    return ValueError(f"{fn}: {name} must have less than 2^31 rows and columns, got {tuple(shape)}")
 
 
 def _logit_rows(fn: str, logits: torch.Tensor) -> int:
     """Checks router logits [rows, E] (a column slice of a wider tensor is fine); row stride."""
-    if logits.dim() == 2:
-        _counts(fn, "logits", *logits.shape)
+    shape = logits.shape
+    if len(shape) == 2 and (shape[0] | shape[1]) >> 31:
+        raise _too_many(fn, "logits", shape)
     if not logits.is_cuda:
         raise ValueError("logits must be a device tensor")
-    if logits.dim() != 2 or 0 in logits.shape:
-        raise ValueError(f"{fn}: logits must be [rows, experts], got {tuple(logits.shape)}")
+    if len(shape) != 2 or 0 in shape:
+        raise ValueError(f"{fn}: logits must be [rows, experts], got {tuple(shape)}")
     _dt(logits)
-    rows, e = logits.shape
+    rows, e = shape
     if (e > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < e):
         raise ValueError(f"{fn}: logits need unit column stride and rows that do not overlap")
     return logits.stride(0) if rows > 1 else e
@@ -848,7 +848,8 @@ def _sequences(fn: str, cu_seqlens) -> int:
     shape = () if cu_seqlens is None else cu_seqlens.shape
     if len(shape) != 1 or shape[0] < 1:
         raise ValueError(f"{fn}: cu_seqlens must be [sequences + 1], got {tuple(shape)}")
-    _counts(fn, "cu_seqlens", shape[0])
+    if shape[0] >> 31:
+        raise _too_many(fn, "cu_seqlens", shape)
     return shape[0] - 1
 
 
@@ -875,9 +876,10 @@ def moe_balance_loss(logits: torch.Tensor, selected: torch.Tensor, score: str = 
     fn = "moe_balance_loss"
     stride = _logit_rows(fn, logits)
     rows, e = logits.shape
-    if selected.dim() != 2 or selected.shape[0] != rows or selected.shape[1] < 1:
-        raise ValueError(f"{fn}: selected must be [rows, k], got {tuple(selected.shape)}")
-    k = selected.shape[1]
+    shape = selected.shape
+    if len(shape) != 2 or shape[0] != rows or shape[1] < 1:
+        raise ValueError(f"{fn}: selected must be [rows, k], got {tuple(shape)}")
+    k = shape[1]
     sig = _score_mode(fn, score)
     dev = logits.get_device()
     mask = valid_rows_mask(valid_rows, rows, logits.device)
@@ -1078,12 +1080,15 @@ def add_rmsnorm(x: torch.Tensor, delta: torch.Tensor, gamma=None, eps: float = 1
 
 # ---- layer norm and its gradients -------------------------------------------------
 
-def _norm_rows(fn: str, x: torch.Tensor, name: str = "x") -> tuple:
-    if x.dim() != 2 or x.shape[1] == 0:
-        raise ValueError(f"{fn}: {name} must be [rows, dim], got {tuple(x.shape)}")
-    _counts(fn, name, *x.shape)
-    _dt(x)
-    return x.shape
+def _norm_rows(fn: str, x: torch.Tensor) -> tuple:
+    """Rows, dim and type of x."""
+    shape = x.shape
+    if len(shape) != 2 or shape[1] == 0:
+        raise ValueError(f"{fn}: x must be [rows, dim], got {tuple(shape)}")
+    rows, dim = shape
+    if (rows | dim) >> 31:
+        raise _too_many(fn, "x", shape)
+    return rows, dim, _dt(x)
 
 
 def layernorm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out_dtype=None,
@@ -1092,7 +1097,7 @@ def layernorm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out_dt
     bf16 [rows, dim], weight and bias f32 [dim] or None.  -> y, or with want_stats (y, mean, rstd),
     f32 [rows] each, which layernorm_backward takes.  No autograd."""
     fn = "layernorm"
-    rows, dim = _norm_rows(fn, x)
+    rows, dim, dt = _norm_rows(fn, x)
     odt = out_dtype or x.dtype
     if odt not in _DT:
         raise ValueError(f"{fn}: out_dtype must be float32 or bfloat16")
@@ -1103,7 +1108,7 @@ def layernorm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, out_dt
     mean = rstd = None
     if want_stats:
         mean, rstd = x.new_empty((2, rows), dtype=torch.float32).unbind(0)
-    call("nsosx_layernorm", _p(x), None, _p(weight), _p(bias), rows, dim, eps, _dt(x), None, _p(y),
+    call("nsosx_layernorm", _p(x), None, _p(weight), _p(bias), rows, dim, eps, dt, None, _p(y),
          _DT[odt], _p(mean), _p(rstd), _stream_on(dev))
     return (y, mean, rstd) if want_stats else y
 
@@ -1113,7 +1118,7 @@ def add_layernorm(x: torch.Tensor, delta: torch.Tensor, weight=None, bias=None, 
     """residual = x + delta, y = layernorm(residual as stored), in one pass (nsosx_layernorm).
     -> (residual, y), or with want_stats (residual, y, mean, rstd)."""
     fn = "add_layernorm"
-    rows, dim = _norm_rows(fn, x)
+    rows, dim, dt = _norm_rows(fn, x)
     dev = x.get_device()
     _on(fn, dev, ("x", x, None, None), ("delta", delta, x.dtype, (rows, dim)),
         ("weight", weight, torch.float32, (dim,)), ("bias", bias, torch.float32, (dim,)))
@@ -1121,8 +1126,8 @@ def add_layernorm(x: torch.Tensor, delta: torch.Tensor, weight=None, bias=None, 
     mean = rstd = None
     if want_stats:
         mean, rstd = x.new_empty((2, rows), dtype=torch.float32).unbind(0)
-    call("nsosx_layernorm", _p(x), _p(delta), _p(weight), _p(bias), rows, dim, eps, _dt(x), _p(res),
-         _p(y), _dt(x), _p(mean), _p(rstd), _stream_on(dev))
+    call("nsosx_layernorm", _p(x), _p(delta), _p(weight), _p(bias), rows, dim, eps, dt, _p(res),
+         _p(y), dt, _p(mean), _p(rstd), _stream_on(dev))
     return (res, y, mean, rstd) if want_stats else (res, y)
 
 
@@ -1133,8 +1138,8 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rs
     of both x and delta of an add) and, with want_params, dweight and dbias f32 [dim].  dresidual:
     the gradient that reached the residual by another way, added to dx."""
     fn = "layernorm_backward"
-    rows, dim = _norm_rows(fn, x)
-    _dt(dy)
+    rows, dim, dt = _norm_rows(fn, x)
+    gdt = _dt(dy)
     dev = x.get_device()
     _on(fn, dev, ("x", x, None, None), ("dy", dy, None, (rows, dim)),
         ("mean", mean, torch.float32, (rows,)), ("rstd", rstd, torch.float32, (rows,)),
@@ -1145,8 +1150,8 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rs
         # (f32 tensors of their own: a gradient that is kept keeps no partial sums)
         dw, db = mean.new_empty(dim), mean.new_empty(dim)
         ws = mean.new_empty(lib().nsosx_layernorm_backward_workspace(rows, dim) // 4)
-    call("nsosx_layernorm_backward", _p(dy), _dt(dy), _p(x), _p(mean), _p(rstd), _p(weight),
-         _p(dresidual), rows, dim, _dt(x), _p(dx), _p(dw), _p(db), _p(ws), _stream_on(dev))
+    call("nsosx_layernorm_backward", _p(dy), gdt, _p(x), _p(mean), _p(rstd), _p(weight),
+         _p(dresidual), rows, dim, dt, _p(dx), _p(dw), _p(db), _p(ws), _stream_on(dev))
     return {"dx": dx, "dweight": dw, "dbias": db} if want_params else {"dx": dx}
 
 
@@ -1172,14 +1177,16 @@ def _rec_view(fn: str, dev: int, name: str, t: torch.Tensor, dtype, shape) -> in
 
 def _rec_inputs(fn: str, x, rg, ig, lam, *more) -> tuple:
     """Checks the recurrence's inputs and `more` as _on takes it; device, type and row strides."""
-    if x.dim() != 2 or x.shape[1] == 0:
-        raise ValueError(f"{fn}: x must be [tokens, dim], got {tuple(x.shape)}")
-    _counts(fn, "x", *x.shape)
+    shape = x.shape
+    if len(shape) != 2 or shape[1] == 0:
+        raise ValueError(f"{fn}: x must be [tokens, dim], got {tuple(shape)}")
+    if (shape[0] | shape[1]) >> 31:
+        raise _too_many(fn, "x", shape)
     dt = _dt(x)
     if not x.is_cuda:
         raise ValueError("x must be a device tensor")
     dev = x.get_device()
-    dtype, shape = x.dtype, x.shape
+    dtype = x.dtype
     xs, rs = _rec_view(fn, dev, "x", x, dtype, shape), _rec_view(fn, dev, "rg", rg, dtype, shape)
     igs = _rec_view(fn, dev, "ig", ig, dtype, shape)
     _on(fn, dev, ("lam", lam, torch.float32, shape[1:]), *more)
