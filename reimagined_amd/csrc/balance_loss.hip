@@ -5,9 +5,11 @@
 //   dloss/dx_rj = E / (M k N_s^2) p_rj (count_sj - sum_e count_se p_re)  [(1 - sigmoid) for sigmoids]
 // Sixteen lanes per row, as in the scored routing, four neighbouring columns a load: the row's sums are
 // four lane exchanges, and one read of the logits is all either pass does.  Both are bound by latency up
-// to some ten thousand rows: 16384 x 256 f32 sigmoids, k 8, take 7 us for the blocks' sums, 8 to add
-// them up (a chain of loads, barriers and one atomic) and 9 back (17 MB read and written: 3.8 TB/s).
+// to some ten thousand rows: 16384 x 256 f32 sigmoids, k 8, take 8.6 us for the blocks' sums, 7.6 to add
+// them up (a chain of loads, barriers and one atomic) and 10.7 back (34 MB read and written: 3.1 TB/s).
 // With a scalar load a column they took 13, 14 and 15, with one workgroup a sequence to add them up 14.
+// Both passes look through all sequences' bounds in each of their workgroups (512 and rows / 16 of them): for
+// batches of up to some thousand sequences.
 #include "train.hpp"
 
 namespace nsosx {

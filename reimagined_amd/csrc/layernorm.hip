@@ -7,7 +7,7 @@
 // TPR threads of 8 CH elements each, and its sums are f32, the variance from the centred row.
 // 67 million bf16 places, add and norm (537 MB): 92 us at rows of 64 to 256 and of 1024 (5.8 TB/s), 94 to
 // 100 at 2048 to 16384, 110 at 777, 121 at 32; the gradients with a residual (as much): 101 to 108 at
-// 128 to 8192, 114 at 64, 179 at 16384.
+// 128 to 8192, 114 at 64, 181 at 16384.
 #include "train.hpp"
 
 namespace nsosx {
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(NT) void layernorm_long_kernel(
 // Threads of a workgroup of the gradients (a longer row takes 1024): eight waves share one row of partial
 // sums.  16384 x 2048 bf16 with a residual: 8 elements a thread in 128 registers 49 us, 16 elements 54 - 58
 // (they spill), workgroups of 256 51.  Rows past 8192 have no more threads to give and take 16 each; with the
-// weights held too 4096 x 16384 took 215 us, without 179, reading the rows twice 308.
+// weights held too 4096 x 16384 took 215 us, without 181 (16 to 24 registers spilled), reading the rows twice 308.
 constexpr int kLnBwdThreads = 512;
 
 template <int TPR> constexpr int ln_bwd_threads() { return TPR > kLnBwdThreads ? TPR : kLnBwdThreads; }

@@ -305,7 +305,8 @@ __device__ __forceinline__ float state_before(const Shared& sh, int k, int tiles
     return c;
 }
 
-// Words and flags to 0, the decay rates: 2.5 us, most of it the launch.
+// Words and flags to 0, the decay rates: 2.5 us for a small batch, most of it the launch, 5 to 6 for the 5 MB of
+// 16384 x 2048 or 65536 x 1024.
 __global__ __launch_bounds__(256) void recurrence_clear_kernel(RecShared s, int64_t n16, int D,
                                                                const float* __restrict__ lam, float rate) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -398,7 +399,8 @@ __device__ __forceinline__ void decay_rates(const Args& arg, int block, float (&
     }
 }
 
-// Whether they all stay below kSmall, as most do: those take fewer steps.
+// Whether they all stay below kSmall (decays above 0.88 even at open gates): those take fewer instructions, which
+// the waits hide.  16384 x 2048 bf16 with rates below it 73 us and 116 back, past it 74 and 120.
 template <int V>
 __device__ __forceinline__ bool all_small(const float (&k2)[V]) {
     bool small = true;
@@ -446,11 +448,12 @@ __device__ __forceinline__ void through_waves(const float (&s_a)[WAVES][64 * V],
 }
 
 // Workgroups take tiles of kTile tokens and 64 V channels, V a lane, in the order of the scan; each wave
-// takes R of the tile's tokens.  Bound by waiting for the tiles before: 65536 x 1024 bf16 (537 MB) 135 us,
-// 108 in a copy that does not wait, 106 at a copy's rate; 40796 x 2048 153, 132 and 132.  As fast: 16 tokens
-// a wave and two workgroups a CU, 8 tokens and three.  Slower: the next tile's inputs on their way and its
-// pair left before this tile's state is looked up (that takes 256 registers, two waves a SIMD: 220 us); a
-// ticket taken before the wait (168), as it then lies with a workgroup that waits and holds all later tiles up.
+// takes R of the tile's tokens.  Bound by waiting for the tiles before: 65536 x 1024 bf16 (537 MB) 134 us, 112
+// in a copy that does not wait, 106 at a copy's rate; 40796 x 2048 150, 127 and 132; 16384 x 2048 73, 63 and 53, f32
+// 118, 111 and 106.  As fast: 16 tokens a wave and two workgroups a CU, 8 tokens and three.  Slower: the next
+// tile's inputs on their way and its pair left before this tile's state is looked up (that takes 256 registers, two
+// waves a SIMD: 220 us where this took 150); a ticket taken before the wait (168 for 136), as it then lies with a
+// workgroup that waits and holds all later tiles up.  The bf16 form spills 3 of its 128 registers.
 template <int DT, int V, int R>
 __global__ __launch_bounds__(64 * (kTile / R), 4) void recurrence_kernel(RecFwd arg) {
     constexpr int WAVES = kTile / R, NT = 64 * WAVES;
@@ -512,7 +515,6 @@ __global__ __launch_bounds__(64 * (kTile / R), 4) void recurrence_kernel(RecFwd 
                 __builtin_amdgcn_sched_barrier(0);  // token after token, or all of them are half done at once
             }
         };
-        // (decays that stay above 0.88 even at open gates, as most do, take fewer steps)
         if (small) gates(std::true_type{});
         else gates(std::false_type{});
         float A[V], H[V];
@@ -595,9 +597,10 @@ struct RecBwd {
 // The same from the last tile to the first.  With q = g / log 2, w = a q and b2 = 1 - a^2:
 //   e = dh (s x a w / beta - w h_before), in units of log 2
 // (where beta goes to 0 so does w, faster).  Tiles of 64 tokens, 8 a wave: four values an element have to
-// stay in registers over the wait.  16384 x 2048 bf16 (470 MB) 134 us, 111 in a copy that does not wait, 93
-// at a copy's rate (77 vector instructions a place, 9 of them exponentials, roots and reciprocals); with
-// 1 - a^2 kept too, which spills, 159.  f32 191 us, floor 185.
+// stay in registers over the wait.  16384 x 2048 bf16 (470 MB) 116 us, 98 in a copy that does not wait, 93
+// at a copy's rate (77 vector instructions a place, 9 of them exponentials, roots and reciprocals); f32 172 and
+// 161, at a copy's rate 185 (part of it stays in the 256 MB cache).  2 or 3 registers are spilled; with 1 - a^2 kept
+// too 31, and 159 us where this took 134.
 template <int DT, int V, int R>
 __global__ __launch_bounds__(64 * (kKept / R), V == 1 ? 6 : 4) void recurrence_bwd_kernel(RecBwd arg) {
     constexpr int WAVES = kKept / R, NT = 64 * WAVES;
@@ -942,8 +945,8 @@ static unsigned rec_grid(int64_t tiles, int D, int V, int resident) {
 }
 
 // bf16: two channels a lane, f32 one (64 channels are a full line there, and the registers carry more
-// workgroups: 16384 x 2048 f32 113 us and 191 back, with two 167 and 273; bf16 67 and 137, with one 82 and
-// 136).
+// workgroups).  16384 x 2048 f32 with one 118 us and 172 back, with two 1.45 times as long when both were there; bf16
+// with two 73 and 116, with one 79 and 120 (65536 x 1024: 134 and 153).
 template <int DT, int V>
 static void launch_recurrence(const RecFwd& p, hipStream_t st) {
     hipLaunchKernelGGL((recurrence_kernel<DT, V, 16>), dim3(rec_grid(rec_tiles(p.T, kTile), p.D, V, 512)),

@@ -461,7 +461,9 @@ class RecurrentLayer:
     gradients are theirs (straight through the ternary and the int8 rounding), and repack() forms the
     ternary ones again after an update.  All of them are updated in place: captured calls hold their
     addresses, and a replay after repack() runs on the new ones.  Activations run in x's type.  Nothing is
-    kept between calls but the weights."""
+    kept between calls but the weights.  Rows of no sequence come out as their residual and zeros; backward()
+    gives them no weight in the parameters' gradients, but they have to hold finite values there, as do those of
+    dout and dresidual."""
 
     def __init__(self, params: dict, device="cuda"):
         f32 = dict(dtype=torch.float32, device=device)
@@ -484,7 +486,8 @@ class RecurrentLayer:
 
     def repack(self) -> None:
         """The ternary weights of the latent ones as they are now, into the words that are there: captured
-        calls have them from their next replay on.  Packed on the host, so not for a capture."""
+        calls have them from their next replay on.  Packed on the host (8 million weights: 45 ms), so not for a
+        capture."""
         for linear, scale, w in ((self.in_proj, self.in_scale, self.w_in), (self.out_proj, self.out_scale, self.w_out)):
             linear.load(w.cpu().numpy())
             scale.fill_(linear.weight_scale)
